@@ -365,6 +365,91 @@ MLA_API mla_status_t mla_cache_append(const mla_config_t* cfg, mla_dtype_t dtype
                               int page_rows, int max_pages, int* seq_lens, int max_seq_len, int* status,
                               mla_stream_t stream);
 
+/* Device-side append of a ragged batch of new tokens (whole prompts and single tokens), with the
+ * latent's RMS norm and the rotary rotation applied on the way. Sequence b's new tokens are
+ * [cu_tokens[b], cu_tokens[b + 1]); its i-th one goes to position p = seq_lens[b] + i:
+ *   row(b, p)[0 : d_c]         = c[t] * rsqrt(mean(c[t]^2) + norm_eps) * norm_weight   (NULL: c[t])
+ *   row(b, p)[d_c : d_c + d_R] = rot(k_rope[t], p);   q_out[t, h] = rot(q_rope[t, h], p)
+ * with the rotate-half pairing (i, i + d_R/2) of mla_decode. fp32 arithmetic, one rounding. The
+ * cache then holds ROTATED keys: mla_prefix_decode reads it as it is (mla_decode, which rotates
+ * what it reads, takes mla_cache_append's unrotated rows). No reference counterpart beyond
+ * LatentKVCache::append_host (src/mla_config.cuh:58-72). seq_lens is only read: new_lens receives
+ * the lengths after the call.
+ * - A token at or past max_seq_len (or of a negative length) is dropped and sets bit 0 of *status;
+ *   one whose page or offset lies outside kv_total_rows is not written and sets bit 1. */
+typedef struct mla_append_rope_args {
+  mla_dtype_t dtype;            /* of the cache, c, k_rope, norm_weight, q_rope, q_out: F16 or BF16 */
+  int batch;                    /* B >= 1 sequences */
+  int tokens;                   /* rows of c and k_rope (0: only new_lens is written) */
+  void* kv_cache;
+  int64_t kv_row_stride;        /* elements, 0: d_c + d_R */
+  int64_t kv_total_rows;        /* rows of kv_cache (> 0) */
+  const void* c;                /* (tokens, d_c) */
+  int64_t c_stride;             /* elements between tokens, 0: d_c */
+  const void* k_rope;           /* (tokens, d_R) unrotated */
+  int64_t k_stride;             /* 0: d_R */
+  const int* cu_tokens;         /* device (B + 1,), non-decreasing */
+  const int* seq_lens;          /* device (B,) rows already held */
+  int max_seq_len;
+  const int64_t* kv_offsets;    /* device (B,) or NULL: b * max_seq_len */
+  const int* page_table;        /* device (B, max_pages) or NULL; excludes kv_offsets */
+  int page_rows;                /* > 0 with page_table */
+  int max_pages;                /* max_pages * page_rows >= max_seq_len */
+  const void* norm_weight;      /* (d_c,) or NULL */
+  float norm_eps;
+  const float* rope_cos;        /* (>= max_seq_len, d_R / 2) fp32, or both NULL: computed from rope_theta */
+  const float* rope_sin;
+  float rope_theta;             /* 0: 10000; as in mla_decode_args_t (d_R <= 128) */
+  const void* q_rope;           /* (tokens, H, d_R) with the strides below, or NULL */
+  int64_t q_token_stride, q_head_stride;         /* elements, 0: H * d_R and d_R */
+  void* q_out;                  /* with q_rope; may be q_rope itself (same strides), else disjoint */
+  int64_t q_out_token_stride, q_out_head_stride;
+  int* new_lens;                /* device (B,) or NULL; not seq_lens */
+  int* status;                  /* device int or NULL */
+} mla_append_rope_args_t;
+MLA_API mla_status_t mla_cache_append_rope(const mla_config_t* cfg, const mla_append_rope_args_t* args,
+                                           mla_stream_t stream);
+
+/* Decode attention of a batch whose requests share prefixes. Request b of group g (group_starts[g]
+ * <= b < group_starts[g + 1]) attends to the group's prefix_lens[g] prefix rows and its own
+ * seq_lens[b] rows, all in one cache of rotated rows (mla_cache_append_rope):
+ *   s_j = softmax_scale (q_absorbed[b, h] . c_j + q_rope[b, h] . k_j),  out[b, h] = softmax(s) . c
+ * in latent space (no W_UV), 0 for a request without rows. Each prefix is read once for all the
+ * query rows of its group, not once a request; partial results are merged in fp32-weighted form.
+ * No reference counterpart (its batched op, src/fused_mla_batched.cuh:5-11, shares the whole cache).
+ * Lengths are clamped to [0, max]. A page id or offset outside the cache reads nothing and makes
+ * the outputs of the requests that use it NaN. */
+typedef struct mla_prefix_args {
+  mla_dtype_t dtype;            /* of everything below: F16 or BF16 */
+  int batch;                    /* B >= 1 requests, ordered by group */
+  int num_groups;               /* >= 1 */
+  const void* kv_cache;
+  int64_t kv_row_stride;        /* elements, 0: d_c + d_R */
+  int64_t kv_total_rows;        /* > 0 */
+  const void* q_absorbed;       /* (B, H, d_c) */
+  const void* q_rope;           /* (B, H, d_R), rotated to the token's position */
+  const int* group_starts;      /* device (num_groups + 1,): requests outside every group have no prefix */
+  const int* prefix_lens;       /* device (num_groups,) */
+  int max_prefix_len;           /* upper bound, >= 0 */
+  const int* seq_lens;          /* device (B,) */
+  int max_seq_len;              /* upper bound, >= 0 */
+  const int64_t* prefix_offsets;  /* contiguous: device (num_groups,) first row of each prefix */
+  const int64_t* kv_offsets;      /* contiguous: device (B,) first own row of each request */
+  const int* prefix_table;      /* paged: device (num_groups, max_prefix_pages) */
+  int max_prefix_pages;
+  const int* page_table;        /* paged: device (B, max_pages) */
+  int max_pages;
+  int page_rows;                /* paged: rows a page, a multiple of 64; 0 selects the contiguous layout */
+  float softmax_scale;          /* 0: 1 / sqrt(dn + d_R) */
+  void* output;                 /* (B, H, d_c) */
+  int kernel;                   /* MLA_KERNEL_AUTO, _TENSOR_CORE (d_c 512, d_R 64) or _CUDA_CORE */
+} mla_prefix_args_t;
+MLA_API mla_status_t mla_prefix_decode_workspace_size(const mla_config_t* cfg, const mla_prefix_args_t* args,
+                                                      size_t* bytes);
+/* workspace: 256-byte aligned, uninitialised; calls that may overlap need one each. */
+MLA_API mla_status_t mla_prefix_decode(const mla_config_t* cfg, const mla_prefix_args_t* args, void* workspace,
+                                       size_t workspace_bytes, mla_stream_t stream);
+
 /* Kernel timing for benchmarks: a timer passed in mla_decode_args_t.timer gets
  * CUDA events recorded on the call's stream immediately before and after the
  * split-KV decode kernel. mla_timer_decode_ms waits for the second event and

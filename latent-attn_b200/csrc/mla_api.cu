@@ -19,6 +19,7 @@
 
 #include "latent_attn_b200/mla.h"
 #include "mla_internal.cuh"
+#include "ops.cuh"
 #include "peer.cuh"
 
 struct mla_timer_st {
@@ -469,6 +470,31 @@ mla_status_t peer_sig(const mla_peer_signal_t* in, mla::PeerSig* out) {
     return MLA_OK;
 }
 }  // namespace
+
+// ---- for the other files with C entry points (ops.cuh)
+namespace mla {
+mla_status_t api_fail(mla_status_t st, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    return fail(st, "%s", buf);
+}
+mla_status_t api_cuda_fail(cudaError_t e, const char* what) {
+    if (e == cudaErrorNoKernelImageForDevice || e == cudaErrorInvalidDeviceFunction)
+        return fail(MLA_ERR_NO_DEVICE_CODE, "%s: %s (library is built for sm_100a)", what, cudaGetErrorString(e));
+    return cuda_fail(e, what);
+}
+mla_status_t api_check_config(const mla_config_t* cfg) { return validate_cfg(cfg); }
+bool api_device(int* sms, int* major) {
+    DeviceInfo d;
+    if (!device_info(&d)) return false;
+    *sms = d.sms;
+    *major = d.major;
+    return true;
+}
+}  // namespace mla
 
 extern "C" {
 

@@ -1,0 +1,135 @@
+// Shared-prefix decode attention, CUDA-core form: any latent width that is a multiple of 32 (up to
+// 1024) and any even rope width (up to 256).
+//
+// One block attends one query row (b, h) to the concatenation of its group's prefix and the
+// request's own rows. Its warps take positions in turn, each with its own online softmax (running
+// maximum m, sum l and latent sum o, all fp32, rescaled when m moves), merged through shared memory
+// at the end. It reads a prefix once per query row, through L2: it serves the shapes outside the
+// tensor-core kernel's, and checks that kernel.
+#include "mla_internal.cuh"
+#include "ops.cuh"
+
+namespace mla {
+namespace {
+
+constexpr int kSimtWarps = 8;
+constexpr int kMaxLane = 32;   // latent elements per lane: dc <= 1024
+constexpr int kMaxRope = 8;    // rope elements per lane: dR <= 256
+
+template <typename T>
+__global__ void __launch_bounds__(32 * kSimtWarps) prefix_simt_kernel(const __grid_constant__ PrefixArgs A) {
+    extern __shared__ float sh[];   // [warps][dc] latent sums, then m, l, bad per warp
+    float* sh_m = sh + kSimtWarps * A.dc;
+    float* sh_l = sh_m + kSimtWarps;
+    int* sh_bad = reinterpret_cast<int*>(sh_l + kSimtWarps);
+    const int b = blockIdx.x / A.H;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    const T* qa = static_cast<const T*>(A.qa) + static_cast<long long>(blockIdx.x) * A.dc;
+    const T* qr = static_cast<const T*>(A.qr) + static_cast<long long>(blockIdx.x) * A.dR;
+    const T* kv = static_cast<const T*>(A.kv);
+    int lo = 0, hi = A.P;   // last group whose start is at or before b
+    while (lo + 1 < hi) {
+        const int mid = (lo + hi) / 2;
+        if (A.starts[mid] <= b) lo = mid; else hi = mid;
+    }
+    const bool grouped = A.starts[lo] <= b && b < A.starts[lo + 1];
+    const int np = grouped ? min(max(A.plens[lo], 0), A.max_plen) : 0;
+    const int n = np + min(max(A.lens[b], 0), A.max_len);
+    const int ne = A.dc / 32, nr = (A.dR + 31) / 32;
+    float q[kMaxLane], k[kMaxLane], o[kMaxLane], r[kMaxRope];
+#pragma unroll
+    for (int j = 0; j < kMaxLane; ++j) {
+        q[j] = j < ne ? ElemTraits<T>::to_f(qa[lane + 32 * j]) : 0.f;
+        o[j] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < kMaxRope; ++j)
+        r[j] = j < nr && lane + 32 * j < A.dR ? ElemTraits<T>::to_f(qr[lane + 32 * j]) : 0.f;
+    float m = -INFINITY, l = 0.f;
+    int bad = 0;
+    for (int p = warp; p < n; p += kSimtWarps) {
+        const bool own = p >= np;
+        const int pos = own ? p - np : p;
+        long long row;
+        if (A.page_rows) {
+            const int pg = own ? A.table[static_cast<long long>(b) * A.max_pages + pos / A.page_rows]
+                               : A.ptable[static_cast<long long>(lo) * A.max_ppages + pos / A.page_rows];
+            row = pg < 0 ? -1 : static_cast<long long>(pg) * A.page_rows + pos % A.page_rows;
+        } else {
+            row = (own ? A.offs[b] : A.poffs[lo]) + pos;
+        }
+        if (row < 0 || row >= A.kv_rows) {
+            bad = 1;
+            continue;
+        }
+        const T* key = kv + row * A.stride;
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < kMaxLane; ++j)
+            if (j < ne) {
+                k[j] = ElemTraits<T>::to_f(key[lane + 32 * j]);
+                s += q[j] * k[j];
+            }
+#pragma unroll
+        for (int j = 0; j < kMaxRope; ++j)
+            if (j < nr && lane + 32 * j < A.dR) s += r[j] * ElemTraits<T>::to_f(key[A.dc + lane + 32 * j]);
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+        s *= A.scale;
+        if (s > m) {
+            const float a = __expf(m - s);   // 0 at the first position
+            m = s;
+            l *= a;
+#pragma unroll
+            for (int j = 0; j < kMaxLane; ++j) o[j] *= a;
+        }
+        const float e = s == -INFINITY ? 0.f : __expf(s - m);   // a NaN score stays one
+        l += e;
+#pragma unroll
+        for (int j = 0; j < kMaxLane; ++j)
+            if (j < ne) o[j] += e * k[j];
+    }
+#pragma unroll
+    for (int j = 0; j < kMaxLane; ++j)
+        if (j < ne) sh[warp * A.dc + lane + 32 * j] = o[j];
+    if (lane == 0) {
+        sh_m[warp] = m;
+        sh_l[warp] = l;
+        sh_bad[warp] = bad;
+    }
+    __syncthreads();
+    float top = -INFINITY, total = 0.f;
+    int any_bad = 0;
+#pragma unroll
+    for (int w = 0; w < kSimtWarps; ++w) {
+        top = fmaxf(top, sh_m[w]);
+        any_bad |= sh_bad[w];
+    }
+    float f[kSimtWarps];
+#pragma unroll
+    for (int w = 0; w < kSimtWarps; ++w) {
+        f[w] = sh_m[w] == -INFINITY ? 0.f : __expf(sh_m[w] - top);
+        total += sh_l[w] * f[w];
+    }
+    T* out = static_cast<T*>(A.out) + static_cast<long long>(blockIdx.x) * A.dc;
+    for (int i = threadIdx.x; i < A.dc; i += 32 * kSimtWarps) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kSimtWarps; ++w) v += sh[w * A.dc + i] * f[w];
+        v = any_bad ? NAN : (total == 0.f ? 0.f : v / total);
+        out[i] = ElemTraits<T>::from_f(v);
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_prefix_simt(const PrefixArgs& A, bool bf16, cudaStream_t s) {
+    const size_t smem = (static_cast<size_t>(kSimtWarps) * A.dc + 3 * kSimtWarps) * sizeof(float);
+    const dim3 grid(static_cast<unsigned>(A.B) * static_cast<unsigned>(A.H));
+    if (bf16) prefix_simt_kernel<__nv_bfloat16><<<grid, 32 * kSimtWarps, smem, s>>>(A);
+    else prefix_simt_kernel<__half><<<grid, 32 * kSimtWarps, smem, s>>>(A);
+    count_launches(1);
+    return cudaGetLastError();
+}
+
+}  // namespace mla

@@ -682,6 +682,180 @@ def mla_cache_append(kv_cache: torch.Tensor, c_t: torch.Tensor, k_rope: torch.Te
                                     C.c_void_p(_ptr(status)), C.c_void_p(_stream(kv_cache.device))))
 
 
+# ---------------------------------------------------------------------------
+# serving operators: append with rotation, shared-prefix decode (no reference counterpart)
+# ---------------------------------------------------------------------------
+
+def _check_ints(t: Optional[torch.Tensor], name: str, shape, device, dtype=torch.int32) -> None:
+    if t is None:
+        return
+    if t.dtype != dtype or t.device != device or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
+
+
+def _check_table(t: Optional[torch.Tensor], name: str, rows: int, device) -> None:
+    if t is not None and (t.dtype != torch.int32 or t.device != device or t.dim() != 2 or t.size(0) != rows
+                          or not t.is_contiguous()):
+        raise RuntimeError(f"{name} must be a contiguous int32 tensor of shape ({rows}, pages) on {device}")
+
+
+def _check_rows(t: torch.Tensor, name: str, shape, like: torch.Tensor) -> None:
+    """A 16-bit tensor of the cache's type with unit inner stride."""
+    if t.dtype != like.dtype or t.device != like.device:
+        raise RuntimeError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+    if tuple(t.shape) != tuple(shape):
+        raise RuntimeError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    if t.numel() and t.size(-1) > 1 and t.stride(-1) != 1:
+        raise RuntimeError(f"{name} must have unit inner stride")
+
+
+def _unexpanded(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """`t`, copied if a dimension of it is broadcast: a stride of 0 means the default in the C structs."""
+    return t.contiguous() if t is not None and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)) else t
+
+
+def _check_cache(kv_cache: torch.Tensor, width: int) -> None:
+    if kv_cache.dtype not in _DT or not kv_cache.is_cuda or kv_cache.dim() != 2 or kv_cache.size(1) != width \
+            or kv_cache.stride(1) != 1:
+        raise RuntimeError(f"kv_cache must be a CUDA fp16/bf16 (rows, {width}) tensor with unit inner stride")
+
+
+def mla_cache_append_rope(kv_cache: torch.Tensor, c: torch.Tensor, k_rope: torch.Tensor, cu_tokens: torch.Tensor,
+                          seq_lens: torch.Tensor, max_seq_len: int, d_model, kv_lora_rank, qk_nope_head_dim,
+                          qk_rope_head_dim, num_heads, v_head_dim, *, rope_cos: Optional[torch.Tensor] = None,
+                          rope_sin: Optional[torch.Tensor] = None, rope_theta: float = 0.0,
+                          norm_weight: Optional[torch.Tensor] = None, norm_eps: float = 1e-6,
+                          kv_offsets: Optional[torch.Tensor] = None, page_table: Optional[torch.Tensor] = None,
+                          page_rows: int = 0, q_rope: Optional[torch.Tensor] = None,
+                          q_out: Optional[torch.Tensor] = None, new_lens: Optional[torch.Tensor] = None,
+                          status: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Append a ragged batch of new tokens to the cache on the device, normalised and rotated.
+
+    Sequence b's new tokens are rows ``cu_tokens[b] .. cu_tokens[b + 1]`` of ``c`` (T, d_c) and
+    ``k_rope`` (T, d_R); the i-th goes to position ``p = seq_lens[b] + i`` of its sequence (at
+    ``kv_offsets[b] + p``, ``b * max_seq_len + p``, or through ``page_table`` (B, max_pages)) as
+    ``[c * rsqrt(mean(c^2) + norm_eps) * norm_weight | rot(k_rope, p)]`` (no norm without
+    ``norm_weight``). The rotation is that of ``mla_decode`` (pairs i, i + d_R / 2), from the tables
+    (max_seq_len rows at least) or computed from ``rope_theta``. The rows hold rotated keys, as
+    ``mla_prefix_decode`` reads them. With ``q_rope`` (T, H, d_R) the queries are rotated by the same
+    angles into ``q_out`` (may be ``q_rope`` itself; a new tensor without it), which is returned.
+    ``seq_lens`` is only read; ``new_lens`` (B,) receives the lengths after the call. ``status`` (CUDA
+    int32): bit 0, a token past ``max_seq_len`` was dropped; bit 1, a row lay outside the cache."""
+    cfg = _cfg(d_model, kv_lora_rank, qk_nope_head_dim, qk_rope_head_dim, num_heads, v_head_dim)
+    dc, dR, H = int(kv_lora_rank), int(qk_rope_head_dim), int(num_heads)
+    _check_cache(kv_cache, dc + dR)
+    dev = kv_cache.device
+    T, B = c.size(0), seq_lens.numel()
+    _check_rows(c, "c", (T, dc), kv_cache)
+    _check_rows(k_rope, "k_rope", (T, dR), kv_cache)
+    _check_ints(cu_tokens, "cu_tokens", (B + 1,), dev)
+    _check_ints(seq_lens, "seq_lens", (B,), dev)
+    _check_ints(new_lens, "new_lens", (B,), dev)
+    _check_ints(kv_offsets, "kv_offsets", (B,), dev, torch.int64)
+    _check_table(page_table, "page_table", B, dev)
+    if status is not None and (status.dtype != torch.int32 or status.device != dev):
+        raise RuntimeError("status must be a CUDA int32 tensor")
+    _check_tables(rope_cos, rope_sin)
+    if rope_cos is not None:
+        for t, n in ((rope_cos, "rope_cos"), (rope_sin, "rope_sin")):
+            if t.dim() != 2 or t.size(1) != dR // 2 or t.size(0) < max_seq_len or t.device != dev:
+                raise RuntimeError(f"{n} must be (>= {max_seq_len}, {dR // 2}) on {dev}")
+    if norm_weight is not None:
+        _check_rows(norm_weight, "norm_weight", (dc,), kv_cache)
+    if q_rope is None and q_out is not None:
+        raise RuntimeError("q_out needs q_rope")
+    if q_out is not None and _unexpanded(q_out) is not q_out:
+        raise RuntimeError("q_out's rows overlap")
+    c, k_rope, q_rope = _unexpanded(c), _unexpanded(k_rope), _unexpanded(q_rope)
+    if q_rope is not None:
+        _check_rows(q_rope, "q_rope", (T, H, dR), kv_cache)
+        if q_out is None:
+            q_out = torch.empty(T, H, dR, dtype=q_rope.dtype, device=dev)
+        _check_rows(q_out, "q_out", (T, H, dR), kv_cache)
+    a = _lib.MlaAppendRopeArgs()
+    a.dtype = _DT[kv_cache.dtype]
+    a.batch, a.tokens = B, T
+    a.kv_cache, a.kv_row_stride, a.kv_total_rows = kv_cache.data_ptr(), kv_cache.stride(0), kv_cache.size(0)
+    a.c, a.c_stride = c.data_ptr(), c.stride(0)
+    a.k_rope, a.k_stride = k_rope.data_ptr(), k_rope.stride(0)
+    a.cu_tokens, a.seq_lens, a.max_seq_len = cu_tokens.data_ptr(), seq_lens.data_ptr(), int(max_seq_len)
+    a.kv_offsets, a.page_table, a.page_rows = _ptr(kv_offsets), _ptr(page_table), int(page_rows)
+    a.max_pages = int(page_table.size(1)) if page_table is not None else 0
+    a.norm_weight, a.norm_eps = _ptr(norm_weight), float(norm_eps)
+    a.rope_cos, a.rope_sin, a.rope_theta = _ptr(rope_cos), _ptr(rope_sin), float(rope_theta)
+    if q_rope is not None and T:
+        a.q_rope, a.q_token_stride, a.q_head_stride = q_rope.data_ptr(), q_rope.stride(0), q_rope.stride(1)
+        a.q_out, a.q_out_token_stride, a.q_out_head_stride = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
+    a.new_lens, a.status = _ptr(new_lens), _ptr(status)
+    _lib.check(_lib.load().mla_cache_append_rope(C.byref(cfg), C.byref(a), C.c_void_p(_stream(dev))))
+    return q_out
+
+
+def mla_prefix_decode(kv_cache: torch.Tensor, q_absorbed: torch.Tensor, q_rope: torch.Tensor, d_model, kv_lora_rank,
+                      qk_nope_head_dim, qk_rope_head_dim, num_heads, v_head_dim, *, group_starts: torch.Tensor,
+                      prefix_lens: torch.Tensor, max_prefix_len: int, seq_lens: torch.Tensor, max_seq_len: int,
+                      prefix_offsets: Optional[torch.Tensor] = None, kv_offsets: Optional[torch.Tensor] = None,
+                      prefix_table: Optional[torch.Tensor] = None, page_table: Optional[torch.Tensor] = None,
+                      page_rows: int = 0, softmax_scale: float = 0.0, out: Optional[torch.Tensor] = None,
+                      workspace: Optional[torch.Tensor] = None, kernel: int = 0) -> torch.Tensor:
+    """Decode attention of B requests whose groups share prefixes: (B, H, d_c) latent outputs in the
+    cache's type.
+
+    Request b of group g (``group_starts[g] <= b < group_starts[g + 1]``) attends to the
+    ``prefix_lens[g]`` rows of its group's prefix and its own ``seq_lens[b]`` rows of ``kv_cache``,
+    whose keys are rotated already (``mla_cache_append_rope``); a request without rows gives zeros.
+    ``q_absorbed`` (B, H, d_c) and ``q_rope`` (B, H, d_R, rotated) have the cache's type. Contiguous
+    layout: ``prefix_offsets`` (groups,) and ``kv_offsets`` (B,) int64 first rows. Paged: ``page_rows``
+    (a multiple of 64) with ``prefix_table`` (groups, pages) and ``page_table`` (B, pages) int32. All
+    index tensors are on the device; ``max_prefix_len`` and ``max_seq_len`` bound the lengths (longer
+    ones are cut). ``workspace``: uint8, kept by callers that must not allocate."""
+    cfg = _cfg(d_model, kv_lora_rank, qk_nope_head_dim, qk_rope_head_dim, num_heads, v_head_dim)
+    dc, dR, H = int(kv_lora_rank), int(qk_rope_head_dim), int(num_heads)
+    _check_cache(kv_cache, dc + dR)
+    dev = kv_cache.device
+    if q_absorbed.dim() != 3:
+        raise RuntimeError("q_absorbed must be 3D (batch, num_heads, kv_lora_rank)")
+    B, P = q_absorbed.size(0), prefix_lens.numel()
+    _check_rows(q_absorbed, "q_absorbed", (B, H, dc), kv_cache)
+    _check_rows(q_rope, "q_rope", (B, H, dR), kv_cache)
+    if not q_absorbed.is_contiguous() or not q_rope.is_contiguous():
+        raise RuntimeError("q_absorbed and q_rope must be contiguous")
+    _check_ints(group_starts, "group_starts", (P + 1,), dev)
+    _check_ints(prefix_lens, "prefix_lens", (P,), dev)
+    _check_ints(seq_lens, "seq_lens", (B,), dev)
+    _check_ints(prefix_offsets, "prefix_offsets", (P,), dev, torch.int64)
+    _check_ints(kv_offsets, "kv_offsets", (B,), dev, torch.int64)
+    _check_table(prefix_table, "prefix_table", P, dev)
+    _check_table(page_table, "page_table", B, dev)
+    if out is None:
+        out = torch.empty(B, H, dc, dtype=kv_cache.dtype, device=dev)
+    else:
+        _check_rows(out, "out", (B, H, dc), kv_cache)
+        if not out.is_contiguous():
+            raise RuntimeError("out must be contiguous")
+    a = _lib.MlaPrefixArgs()
+    a.dtype = _DT[kv_cache.dtype]
+    a.batch, a.num_groups = B, P
+    a.kv_cache, a.kv_row_stride, a.kv_total_rows = kv_cache.data_ptr(), kv_cache.stride(0), kv_cache.size(0)
+    a.q_absorbed, a.q_rope, a.group_starts = q_absorbed.data_ptr(), q_rope.data_ptr(), group_starts.data_ptr()
+    a.prefix_lens, a.max_prefix_len = prefix_lens.data_ptr(), int(max_prefix_len)
+    a.seq_lens, a.max_seq_len = seq_lens.data_ptr(), int(max_seq_len)
+    a.prefix_offsets, a.kv_offsets = _ptr(prefix_offsets), _ptr(kv_offsets)
+    if prefix_table is not None:
+        a.prefix_table, a.max_prefix_pages = prefix_table.data_ptr(), int(prefix_table.size(1))
+    if page_table is not None:
+        a.page_table, a.max_pages = page_table.data_ptr(), int(page_table.size(1))
+    a.page_rows, a.softmax_scale, a.output, a.kernel = int(page_rows), float(softmax_scale), out.data_ptr(), int(kernel)
+    lib = _lib.load()
+    n = C.c_size_t(0)
+    _lib.check(lib.mla_prefix_decode_workspace_size(C.byref(cfg), C.byref(a), C.byref(n)))
+    if workspace is None or workspace.numel() * workspace.element_size() < n.value or workspace.data_ptr() % 256:
+        workspace = torch.empty(max(int(n.value), 1), dtype=torch.uint8, device=dev)
+    _lib.check(lib.mla_prefix_decode(C.byref(cfg), C.byref(a), C.c_void_p(workspace.data_ptr()), n,
+                                     C.c_void_p(_stream(dev))))
+    return out
+
+
 # ---- peer memory for the multi-GPU exchange (mla_ipc_* / mla_peer_*)
 
 class IpcBuffer:

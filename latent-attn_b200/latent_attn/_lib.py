@@ -63,6 +63,29 @@ class MlaDecodeArgs(C.Structure):
                 ("page_table", C.c_void_p), ("page_rows", C.c_int), ("max_pages", C.c_int),
                 ("rope_theta", C.c_float)]
 
+
+class MlaAppendRopeArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("batch", C.c_int), ("tokens", C.c_int), ("kv_cache", C.c_void_p),
+                ("kv_row_stride", C.c_int64), ("kv_total_rows", C.c_int64), ("c", C.c_void_p), ("c_stride", C.c_int64),
+                ("k_rope", C.c_void_p), ("k_stride", C.c_int64), ("cu_tokens", C.c_void_p), ("seq_lens", C.c_void_p),
+                ("max_seq_len", C.c_int), ("kv_offsets", C.c_void_p), ("page_table", C.c_void_p),
+                ("page_rows", C.c_int), ("max_pages", C.c_int), ("norm_weight", C.c_void_p), ("norm_eps", C.c_float),
+                ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p), ("rope_theta", C.c_float), ("q_rope", C.c_void_p),
+                ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64), ("q_out", C.c_void_p),
+                ("q_out_token_stride", C.c_int64), ("q_out_head_stride", C.c_int64), ("new_lens", C.c_void_p),
+                ("status", C.c_void_p)]
+
+
+class MlaPrefixArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("batch", C.c_int), ("num_groups", C.c_int), ("kv_cache", C.c_void_p),
+                ("kv_row_stride", C.c_int64), ("kv_total_rows", C.c_int64), ("q_absorbed", C.c_void_p),
+                ("q_rope", C.c_void_p), ("group_starts", C.c_void_p), ("prefix_lens", C.c_void_p),
+                ("max_prefix_len", C.c_int), ("seq_lens", C.c_void_p), ("max_seq_len", C.c_int),
+                ("prefix_offsets", C.c_void_p), ("kv_offsets", C.c_void_p), ("prefix_table", C.c_void_p),
+                ("max_prefix_pages", C.c_int), ("page_table", C.c_void_p), ("max_pages", C.c_int),
+                ("page_rows", C.c_int), ("softmax_scale", C.c_float), ("output", C.c_void_p), ("kernel", C.c_int)]
+
+
 class MlaPeerSignal(C.Structure):
     _fields_ = [("flags", C.c_void_p), ("flag_index", C.c_int), ("epoch", C.c_void_p), ("counters", C.c_void_p)]
 
@@ -95,6 +118,10 @@ SIGNATURES = {
     "mla_cache_append": (C.c_int, [C.POINTER(MlaConfig), C.c_int, C.c_void_p, C.c_int64, C.c_int64, C.c_int,
                                    C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
                                    C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]),
+    "mla_cache_append_rope": (C.c_int, [C.POINTER(MlaConfig), C.POINTER(MlaAppendRopeArgs), C.c_void_p]),
+    "mla_prefix_decode_workspace_size": (C.c_int, [C.POINTER(MlaConfig), C.POINTER(MlaPrefixArgs),
+                                                   C.POINTER(C.c_size_t)]),
+    "mla_prefix_decode": (C.c_int, [C.POINTER(MlaConfig), C.POINTER(MlaPrefixArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
     "mla_linear": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "mla_ipc_alloc": (C.c_int, [C.c_size_t, C.POINTER(C.c_void_p), C.c_void_p]),
     "mla_ipc_free": (C.c_int, [C.c_void_p]),

@@ -88,3 +88,17 @@ def mla_decode(kv_cache: torch.Tensor, q_rope: torch.Tensor, W_UV: torch.Tensor,
                                   kv_row_stride=kv_row_stride, kernel=kernel, out=out, workspace=workspace,
                                   timer=timer, page_table=page_table, page_rows=page_rows,
                                   rope_theta=rope_theta)
+
+
+def mla_cache_append_rope(kv_cache: torch.Tensor, c: torch.Tensor, k_rope: torch.Tensor, cu_tokens: torch.Tensor,
+                          seq_lens: torch.Tensor, max_seq_len: int, cfg: "MLAConfig", **kw) -> Optional[torch.Tensor]:
+    """Append a ragged batch of new tokens, normalised and rotated, and rotate their queries; see
+    ``_C.mla_cache_append_rope`` for the keyword arguments. Returns the rotated queries, if any."""
+    return _load_ext().mla_cache_append_rope(kv_cache, c, k_rope, cu_tokens, seq_lens, max_seq_len, *_dims(cfg), **kw)
+
+
+def mla_prefix_decode(kv_cache: torch.Tensor, q_absorbed: torch.Tensor, q_rope: torch.Tensor, cfg: "MLAConfig",
+                      **kw) -> torch.Tensor:
+    """Decode attention of a batch whose requests share prefixes, over rotated cache rows; see
+    ``_C.mla_prefix_decode`` for the keyword arguments. Returns (B, H, d_c) in the cache's type."""
+    return _load_ext().mla_prefix_decode(kv_cache, q_absorbed, q_rope, *_dims(cfg), **kw)
