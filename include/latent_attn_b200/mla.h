@@ -450,6 +450,32 @@ MLA_API mla_status_t mla_prefix_decode_workspace_size(const mla_config_t* cfg, c
 MLA_API mla_status_t mla_prefix_decode(const mla_config_t* cfg, const mla_prefix_args_t* args, void* workspace,
                                        size_t workspace_bytes, mla_stream_t stream);
 
+/* A shared projection with the requests' low-rank adapters beside it:
+ *   Y[m] = W X[m] + scales[a] B_a (A_a X[m]),  a = adapter_ids[m]
+ * an id outside [0, num_adapters) means no adapter. Any mix of adapters in any order; only those
+ * that occur are read. Replaces, like mla_linear, the torch matmuls of LatentAttentionLayer.forward
+ * (latent_attn/__init__.py:126, :128, :145), for requests with adapters; no reference counterpart.
+ * tcgen05 kernel; the same call gives the same bits every time. Products and sums in fp32,
+ * A_a X[m] and Y rounded once to the operands' type. */
+typedef struct mla_lora_args {
+  mla_dtype_t dtype;            /* of X, W, A, B, Y: F16 or BF16 */
+  int M, N, K;                  /* tokens >= 1, outputs, inputs (a multiple of 8) */
+  const void* X;                /* (M, K) */
+  int64_t x_stride;             /* elements between tokens, a multiple of 8; 0: K */
+  const void* W;                /* (N, K) */
+  int num_adapters;             /* >= 1 */
+  int rank;                     /* a multiple of 8, <= 256 */
+  const void* lora_a;           /* (num_adapters, rank, K) */
+  const void* lora_b;           /* (num_adapters, N, rank) */
+  const int* adapter_ids;       /* device (M,) */
+  const float* scales;          /* device (num_adapters,) or NULL: 1 */
+  void* Y;                      /* (M, N) */
+} mla_lora_args_t;
+MLA_API mla_status_t mla_linear_lora_workspace_size(const mla_lora_args_t* args, size_t* bytes);
+/* workspace: 256-byte aligned, uninitialised; calls that may overlap need one each. */
+MLA_API mla_status_t mla_linear_lora(const mla_lora_args_t* args, void* workspace, size_t workspace_bytes,
+                                     mla_stream_t stream);
+
 /* Kernel timing for benchmarks: a timer passed in mla_decode_args_t.timer gets
  * CUDA events recorded on the call's stream immediately before and after the
  * split-KV decode kernel. mla_timer_decode_ms waits for the second event and

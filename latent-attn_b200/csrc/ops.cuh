@@ -62,6 +62,22 @@ struct PrefixArgs {
 // CUDA cores, any dimensions: no workspace
 cudaError_t launch_prefix_simt(const PrefixArgs& A, bool bf16, cudaStream_t s);
 
+// lora.cu: Y = X W^T + scale_a (X A_a^T) B_a^T, a the token's adapter
+struct LoraArgs {
+    int M, N, K;
+    const void* x;            // (M, K)
+    long long x_stride;
+    const void* w;            // (N, K)
+    int adapters, rank;
+    const void* a;            // (adapters, rank, K)
+    const void* b;            // (adapters, N, rank)
+    const int* ids;           // (M,) adapter of each token; outside [0, adapters): none
+    const float* scales;      // (adapters,) or null: 1
+    void* y;                  // (M, N)
+};
+size_t lora_workspace(int M, int N, int K, int adapters, int rank, int sms);
+cudaError_t launch_lora(const LoraArgs& A, bool bf16, void* workspace, int sms, cudaStream_t s);
+
 // ---- shared with mla_api.cu: the thread's error message and the device's properties
 mla_status_t api_fail(mla_status_t s, const char* fmt, ...);
 mla_status_t api_cuda_fail(cudaError_t e, const char* what);   // NO_DEVICE_CODE or CUDA

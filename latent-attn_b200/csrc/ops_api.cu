@@ -163,4 +163,53 @@ mla_status_t mla_prefix_decode(const mla_config_t* cfg, const mla_prefix_args_t*
     return e == cudaSuccess ? MLA_OK : api_cuda_fail(e, "prefix decode kernel launch");
 }
 
+static mla_status_t make_lora(const mla_lora_args_t* a, mla::LoraArgs* A, int* sms) {
+    if (!a) return api_fail(MLA_ERR_INVALID_ARGUMENT, "args is null");
+    const mla_status_t st = check_dtype(a->dtype);
+    if (st != MLA_OK) return st;
+    if (a->M <= 0 || a->N <= 0 || a->K <= 0)
+        return api_fail(MLA_ERR_INVALID_ARGUMENT, "M, N and K must be positive (M=%d, N=%d, K=%d)", a->M, a->N, a->K);
+    if (a->num_adapters <= 0) return api_fail(MLA_ERR_INVALID_ARGUMENT, "num_adapters must be positive, got %d", a->num_adapters);
+    if (a->K % 8 != 0 || a->x_stride % 8 != 0)
+        return api_fail(MLA_ERR_UNSUPPORTED, "K and x_stride must be multiples of 8 (K=%d, x_stride=%lld)", a->K, (long long)a->x_stride);
+    if (a->rank <= 0 || a->rank % 8 != 0 || a->rank > 256)
+        return api_fail(MLA_ERR_UNSUPPORTED, "rank must be a multiple of 8 and <= 256 (got %d)", a->rank);
+    if (a->M > (1 << 23) || a->N > (1 << 28)) return api_fail(MLA_ERR_UNSUPPORTED, "M must be <= 2^23 and N <= 2^28");
+    if (!a->X || !a->W || !a->lora_a || !a->lora_b || !a->adapter_ids || !a->Y)
+        return api_fail(MLA_ERR_INVALID_ARGUMENT, "null pointer");
+    if (a->x_stride != 0 && a->x_stride < a->K) return api_fail(MLA_ERR_INVALID_ARGUMENT, "x_stride %lld < K", (long long)a->x_stride);
+    if ((reinterpret_cast<uintptr_t>(a->X) | reinterpret_cast<uintptr_t>(a->W) | reinterpret_cast<uintptr_t>(a->lora_a) |
+         reinterpret_cast<uintptr_t>(a->lora_b)) % 16 != 0)
+        return api_fail(MLA_ERR_INVALID_ARGUMENT, "X, W, lora_a and lora_b must be 16-byte aligned");
+    int major = 0;
+    if (!mla::api_device(sms, &major)) return api_fail(MLA_ERR_CUDA, "no CUDA device");
+    if (major != 10) return api_fail(MLA_ERR_NO_DEVICE_CODE, "mla_linear_lora needs an sm_100 GPU");
+    *A = {a->M, a->N, a->K, a->X, a->x_stride ? a->x_stride : a->K, a->W, a->num_adapters, a->rank,
+          a->lora_a, a->lora_b, a->adapter_ids, a->scales, a->Y};
+    return MLA_OK;
+}
+
+mla_status_t mla_linear_lora_workspace_size(const mla_lora_args_t* a, size_t* bytes) {
+    mla::LoraArgs A;
+    int sms = 0;
+    const mla_status_t st = make_lora(a, &A, &sms);
+    if (st != MLA_OK) return st;
+    if (!bytes) return api_fail(MLA_ERR_INVALID_ARGUMENT, "bytes is null");
+    *bytes = mla::lora_workspace(A.M, A.N, A.K, A.adapters, A.rank, sms);
+    return MLA_OK;
+}
+
+mla_status_t mla_linear_lora(const mla_lora_args_t* a, void* workspace, size_t workspace_bytes, mla_stream_t stream) {
+    mla::LoraArgs A;
+    int sms = 0;
+    const mla_status_t st = make_lora(a, &A, &sms);
+    if (st != MLA_OK) return st;
+    const size_t need = mla::lora_workspace(A.M, A.N, A.K, A.adapters, A.rank, sms);
+    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
+        return api_fail(MLA_ERR_WORKSPACE, "workspace is null or not 256-byte aligned");
+    if (workspace_bytes < need) return api_fail(MLA_ERR_WORKSPACE, "workspace too small: %zu < %zu bytes", workspace_bytes, need);
+    const cudaError_t e = mla::launch_lora(A, a->dtype == MLA_DTYPE_BF16, workspace, sms, reinterpret_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? MLA_OK : api_cuda_fail(e, "projection with adapters: kernel launch");
+}
+
 }  // extern "C"

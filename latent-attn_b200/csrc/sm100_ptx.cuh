@@ -6,7 +6,7 @@
 //   shared-memory descriptor (64 bit):
 //     [0,14) start address >> 4   [16,30) leading byte offset >> 4
 //     [32,46) stride byte offset >> 4   [46,48) version = 1
-//     [49,52) base offset = 0   [52] LBO mode = 0   [61,64) layout (2 = 128-byte swizzle)
+//     [49,52) base offset = 0   [52] LBO mode = 0   [61,64) layout (2 = 128-byte swizzle, 6 = 32-byte)
 //   instruction descriptor, kind::f16 (32 bit):
 //     [4,6) D format (1 = f32)   [7,10) A format   [10,13) B format (0 = f16, 1 = bf16)
 //     [15] A major (0 = K, 1 = MN)   [16] B major   [17,23) N >> 3   [24,29) M >> 4
@@ -165,6 +165,15 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* tmap, uint
         : "memory");
 }
 
+// 3-D tiled load into this CTA's shared memory.
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
 // ---------------- TMEM / tcgen05 ----------------
 __device__ __forceinline__ void tmem_alloc(uint32_t dst_smem, uint32_t ncols) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem),
@@ -187,6 +196,12 @@ __device__ __forceinline__ void tc_fence_after() {
 __host__ __device__ constexpr uint64_t smem_desc_sw128(uint32_t addr, uint32_t lbo, uint32_t sbo) {
     return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16) |
            (static_cast<uint64_t>((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// K-major operand whose rows hold one K = 16 step (32 bytes, 32-byte swizzle): 8-row groups 256 bytes apart.
+__host__ __device__ constexpr uint64_t smem_desc_sw32(uint32_t addr) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (1ull << 16) | (static_cast<uint64_t>(256 >> 4) << 32) |
+           (1ull << 46) | (6ull << 61);
 }
 
 // No-swizzle K-major operand: core matrices of 8 rows x 16 bytes; lbo = byte distance between

@@ -856,6 +856,47 @@ def mla_prefix_decode(kv_cache: torch.Tensor, q_absorbed: torch.Tensor, q_rope: 
     return out
 
 
+def linear_lora(x: torch.Tensor, W: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
+                adapter_ids: torch.Tensor, *, scales: Optional[torch.Tensor] = None,
+                out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x (M, K) @ W (N, K)^T`` plus each token's own low-rank adapter: ``y[m] += scales[a] *
+    lora_b[a] @ (lora_a[a] @ x[m])`` with ``a = adapter_ids[m]`` (an id outside the loaded adapters:
+    none). ``lora_a`` (adapters, rank, K), ``lora_b`` (adapters, N, rank), rank a multiple of 8 up to
+    256, ``adapter_ids`` (M,) int32 in any order, ``scales`` (adapters,) fp32. All fp16 or bf16 of one
+    type, which the result (M, N) has too. K is a multiple of 8. ``workspace``: uint8, kept by callers
+    that must not allocate."""
+    for t, n, d in ((x, "x", 2), (W, "W", 2), (lora_a, "lora_a", 3), (lora_b, "lora_b", 3)):
+        if t.dtype not in _DT or not t.is_cuda or t.dim() != d:
+            raise RuntimeError(f"{n} must be a {d}D float16 or bfloat16 CUDA tensor")
+    (M, K), N, (adapters, rank, _) = x.shape, W.size(0), lora_a.shape
+    _check_rows(W, "W", (N, K), x)
+    _check_rows(lora_a, "lora_a", (adapters, rank, K), x)
+    _check_rows(lora_b, "lora_b", (adapters, N, rank), x)
+    if not W.is_contiguous() or not lora_a.is_contiguous() or not lora_b.is_contiguous():
+        raise RuntimeError("W, lora_a and lora_b must be contiguous")
+    _check_rows(x, "x", (M, K), x)
+    _check_ints(adapter_ids, "adapter_ids", (M,), x.device)
+    _check_ints(scales, "scales", (adapters,), x.device, torch.float32)
+    if out is None:
+        out = torch.empty(M, N, dtype=x.dtype, device=x.device)
+    else:
+        _check_rows(out, "out", (M, N), x)
+        if not out.is_contiguous():
+            raise RuntimeError("out must be contiguous")
+    if M == 0:
+        return out
+    x = _unexpanded(x)
+    a = _lib.MlaLoraArgs(_DT[x.dtype], M, N, K, x.data_ptr(), x.stride(0) if M > 1 else K, W.data_ptr(), adapters, rank,
+                         lora_a.data_ptr(), lora_b.data_ptr(), adapter_ids.data_ptr(), _ptr(scales), out.data_ptr())
+    lib = _lib.load()
+    n = C.c_size_t(0)
+    _lib.check(lib.mla_linear_lora_workspace_size(C.byref(a), C.byref(n)))
+    if workspace is None or workspace.numel() * workspace.element_size() < n.value or workspace.data_ptr() % 256:
+        workspace = torch.empty(int(n.value), dtype=torch.uint8, device=x.device)
+    _lib.check(lib.mla_linear_lora(C.byref(a), C.c_void_p(workspace.data_ptr()), n, C.c_void_p(_stream(x.device))))
+    return out
+
+
 # ---- peer memory for the multi-GPU exchange (mla_ipc_* / mla_peer_*)
 
 class IpcBuffer:

@@ -86,6 +86,13 @@ class MlaPrefixArgs(C.Structure):
                 ("page_rows", C.c_int), ("softmax_scale", C.c_float), ("output", C.c_void_p), ("kernel", C.c_int)]
 
 
+class MlaLoraArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("M", C.c_int), ("N", C.c_int), ("K", C.c_int), ("X", C.c_void_p),
+                ("x_stride", C.c_int64), ("W", C.c_void_p), ("num_adapters", C.c_int), ("rank", C.c_int),
+                ("lora_a", C.c_void_p), ("lora_b", C.c_void_p), ("adapter_ids", C.c_void_p), ("scales", C.c_void_p),
+                ("Y", C.c_void_p)]
+
+
 class MlaPeerSignal(C.Structure):
     _fields_ = [("flags", C.c_void_p), ("flag_index", C.c_int), ("epoch", C.c_void_p), ("counters", C.c_void_p)]
 
@@ -122,6 +129,8 @@ SIGNATURES = {
     "mla_prefix_decode_workspace_size": (C.c_int, [C.POINTER(MlaConfig), C.POINTER(MlaPrefixArgs),
                                                    C.POINTER(C.c_size_t)]),
     "mla_prefix_decode": (C.c_int, [C.POINTER(MlaConfig), C.POINTER(MlaPrefixArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "mla_linear_lora_workspace_size": (C.c_int, [C.POINTER(MlaLoraArgs), C.POINTER(C.c_size_t)]),
+    "mla_linear_lora": (C.c_int, [C.POINTER(MlaLoraArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
     "mla_linear": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "mla_ipc_alloc": (C.c_int, [C.c_size_t, C.POINTER(C.c_void_p), C.c_void_p]),
     "mla_ipc_free": (C.c_int, [C.c_void_p]),

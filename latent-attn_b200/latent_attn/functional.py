@@ -102,3 +102,10 @@ def mla_prefix_decode(kv_cache: torch.Tensor, q_absorbed: torch.Tensor, q_rope: 
     """Decode attention of a batch whose requests share prefixes, over rotated cache rows; see
     ``_C.mla_prefix_decode`` for the keyword arguments. Returns (B, H, d_c) in the cache's type."""
     return _load_ext().mla_prefix_decode(kv_cache, q_absorbed, q_rope, *_dims(cfg), **kw)
+
+
+def linear_lora(x: torch.Tensor, W: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
+                adapter_ids: torch.Tensor, *, scales: Optional[torch.Tensor] = None,
+                out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A shared projection with each token's own low-rank adapter beside it; see ``_C.linear_lora``."""
+    return _load_ext().linear_lora(x, W, lora_a, lora_b, adapter_ids, scales=scales, out=out, workspace=workspace)
