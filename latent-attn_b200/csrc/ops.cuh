@@ -61,6 +61,10 @@ struct PrefixArgs {
 };
 // CUDA cores, any dimensions: no workspace
 cudaError_t launch_prefix_simt(const PrefixArgs& A, bool bf16, cudaStream_t s);
+// tensor cores (sm_100): dc 512, dR 64, 16-byte rows and pointers
+bool prefix_sm100_supported(const PrefixArgs& A);
+size_t prefix_sm100_workspace(const PrefixArgs& A, int sms);
+cudaError_t launch_prefix_sm100(const PrefixArgs& A, bool bf16, void* workspace, int sms, cudaStream_t s);
 
 // lora.cu: Y = X W^T + scale_a (X A_a^T) B_a^T, a the token's adapter
 struct LoraArgs {

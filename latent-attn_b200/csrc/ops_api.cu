@@ -143,23 +143,50 @@ static mla_status_t make_prefix(const mla_config_t* cfg, const mla_prefix_args_t
     return MLA_OK;
 }
 
+// Which kernel serves the call: the tensor cores' wherever their shape and alignment rules hold.
+static mla_status_t choose_prefix(const mla_prefix_args_t* a, const mla::PrefixArgs& A, bool* tc, int* sms) {
+    int major = 0;
+    if (!mla::api_device(sms, &major)) return api_fail(MLA_ERR_CUDA, "no CUDA device");
+    const bool can = major == 10 && mla::prefix_sm100_supported(A);
+    if (a->kernel == MLA_KERNEL_TENSOR_CORE && !can)
+        return api_fail(MLA_ERR_UNSUPPORTED, "the tensor-core kernel needs sm_100, kv_lora_rank 512, qk_rope_head_dim 64 "
+                        "and 16-byte aligned rows");
+    *tc = can && a->kernel != MLA_KERNEL_CUDA_CORE;
+    return MLA_OK;
+}
+
 mla_status_t mla_prefix_decode_workspace_size(const mla_config_t* cfg, const mla_prefix_args_t* a, size_t* bytes) {
     mla::PrefixArgs A;
-    const mla_status_t st = make_prefix(cfg, a, &A);
+    bool tc = false;
+    int sms = 0;
+    mla_status_t st = make_prefix(cfg, a, &A);
+    if (st == MLA_OK) st = choose_prefix(a, A, &tc, &sms);
     if (st != MLA_OK) return st;
     if (!bytes) return api_fail(MLA_ERR_INVALID_ARGUMENT, "bytes is null");
-    *bytes = 0;
+    *bytes = tc ? mla::prefix_sm100_workspace(A, sms) : 0;
     return MLA_OK;
 }
 
 mla_status_t mla_prefix_decode(const mla_config_t* cfg, const mla_prefix_args_t* a, void* workspace,
                                size_t workspace_bytes, mla_stream_t stream) {
-    (void)workspace;
-    (void)workspace_bytes;
     mla::PrefixArgs A;
-    const mla_status_t st = make_prefix(cfg, a, &A);
+    bool tc = false;
+    int sms = 0;
+    mla_status_t st = make_prefix(cfg, a, &A);
+    if (st == MLA_OK) st = choose_prefix(a, A, &tc, &sms);
     if (st != MLA_OK) return st;
-    const cudaError_t e = mla::launch_prefix_simt(A, a->dtype == MLA_DTYPE_BF16, reinterpret_cast<cudaStream_t>(stream));
+    const bool bf16 = a->dtype == MLA_DTYPE_BF16;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    cudaError_t e;
+    if (tc) {
+        const size_t need = mla::prefix_sm100_workspace(A, sms);
+        if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
+            return api_fail(MLA_ERR_WORKSPACE, "workspace is null or not 256-byte aligned");
+        if (workspace_bytes < need) return api_fail(MLA_ERR_WORKSPACE, "workspace too small: %zu < %zu bytes", workspace_bytes, need);
+        e = mla::launch_prefix_sm100(A, bf16, workspace, sms, s);
+    } else {
+        e = mla::launch_prefix_simt(A, bf16, s);
+    }
     return e == cudaSuccess ? MLA_OK : api_cuda_fail(e, "prefix decode kernel launch");
 }
 

@@ -1,0 +1,986 @@
+// Shared-prefix decode attention on the tensor cores (tcgen05 + TMEM + TMA), d_c = 512, d_R = 64.
+//
+// Three kernels, chained by programmatic dependent launch:
+//   1. prefix_plan_kernel (one block) cuts the query rows into groups of up to 128 and counts their
+//      64-position tiles, from the lengths on the device.
+//   2. prefix_attend_kernel streams the tiles: one worker is a pair of CTAs, the tiles of all groups
+//      are laid end to end and cut evenly over the workers, and a worker writes one partial record
+//      (m, l, o) per group that it touches, at index group + worker (unique: walking the tiles in
+//      order, every step to the next (group, worker) piece advances one of the two).
+//   3. prefix_merge_kernel merges each output row's records by their maxima and sums.
+// Rounding: P is rounded to the cache's type for its MMA, and the row sums add the rounded values, so
+// that the weights of a row still add up to one; a record's o is stored in fp16 after an exact scaling
+// of each half row by a power of two (2^-11 relative, a quarter of the bytes of fp32's error budget
+// being unused); all sums, maxima and accumulators are fp32; the result is rounded once.
+// A group is the M = 128 tile of the MMAs. When 128 divides H it is 128 heads of one request, whose
+// positions are its prefix followed by its own rows. Otherwise the (request, head) rows of a prefix
+// group are packed across requests, so that one pass over the prefix serves 128 / H requests, and
+// each request's own rows are a group of their own.
+//
+// The pair splits both products evenly and reads every cache byte into shared memory once: CTA r
+// holds columns [256 r, 256 r + 256) of the latent and [32 r, 32 r + 32) of the rope key; it computes
+// the partial scores over them, and the output columns [256 r, + 256). TMEM per CTA: O 256 columns |
+// S 64 | Q latent 128 (two elements a column) | P 2 x 32. (The alternatives: a whole score in each CTA
+// costs 1.53 times the MMAs; splitting the rows instead needs every value column twice in shared
+// memory, and those MMAs with both operands there run at 1319 TFLOP/s at best, 868 with the loads.)
+// The two partial scores are exchanged in fp16 through distributed shared memory (in log2 units after
+// scaling: 2^-11 of a partial; fp32 would double what already takes 0.6 us a tile), and both CTAs add
+// the same two fp16 values, so their softmax is the same bit for bit.
+//
+// Warps (128 + 128 kSets threads): warp 0 loads, warp 1 issues the MMAs, warps 2-3 rest; softmax set i
+// takes the tiles j with j % kSets == i, thread = query row. A tile's way through the softmax (read S,
+// exchange, maximum, exponentials, write P) takes about 3 us of latency and little issue time, so the
+// number of sets, each on a tile of its own, sets the pace until the stages of the ring do.
+#include <cfloat>
+
+#include "mla_internal.cuh"
+#include "ops.cuh"
+#include "sm100_ptx.cuh"
+#include "tma_host.cuh"
+
+namespace mla {
+using namespace sm100;
+
+namespace {
+
+constexpr int kTile = 64;                            // positions per tile
+constexpr int kStages = 5;
+constexpr int kChunkBytes = kTile * 128;             // 64 rows x 64 latent columns, 128-byte swizzle
+constexpr int kRopeBoxBytes = kTile * 16;            // 64 rows x 8 rope columns, no swizzle
+constexpr int kRopeBytes = 4 * kRopeBoxBytes;
+constexpr int kStageBytes = kRopeBytes + 4 * kChunkBytes;
+constexpr int kXSlots = 2;                           // exchange slots, tile j in slot j & 1
+constexpr int kXBytes = 128 * 128;                   // 128 rows x 64 fp16 partial scores
+constexpr int kQRopeBoxBytes = 128 * 16;
+constexpr int kQRopeBytes = 4 * kQRopeBoxBytes;
+constexpr int kMSlots = 4;
+constexpr int kSets = 3;
+constexpr int kThreads = 128 + 128 * kSets;
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kColO = 0, kColS = 256, kColQ = 320, kColP = 448;
+constexpr float kRescale = 8.0f;                     // log2 units
+constexpr float kLowest = -1e37f;                    // reference of rows whose scores are all -inf
+
+enum : int { kWaitLoad = 1, kWaitMma = 3, kWaitS = 7, kWaitX = 8, kWaitPV = 9, kWaitTeardown = 10, kWaitDrain = 11,
+             kWaitRef = 12, kWaitCredit = 13, kWaitEpi = 14 };
+
+// A group of query rows and what it attends to.
+struct __align__(16) Group {
+    int q_row0, rows;         // flattened (request, head) rows
+    int pid, sid;             // prefix group and request whose rows it attends to (-1: none)
+    int plen, slen;
+    int tile0, ptiles;        // first tile, tiles of the prefix
+};
+struct Header {
+    int groups, tiles;
+    int workers;              // that have a tile: no worker between two others is without
+};
+struct Work {                 // workspace
+    int* status;
+    Header* head;
+    Group* group;
+    int* gbase;               // per prefix group: its first row group (num_groups + 1)
+    int* bad;                 // per group: it met a row outside the cache
+    float4* rec_ml;           // per record row: m, l, 2^-f of o's columns 0..255 and 256..511
+    uint16_t* rec_o;          // o 2^f in fp16
+    float2* rowsum;           // per CTA: [2 kSets][128] row sums and references handed between its sets
+    int W;                    // workers
+    int own;                  // groups of single requests, which come first (B * ceil(H / 128))
+    int fold;                 // 1: prefix and own rows in one group (128 divides H)
+};
+
+__device__ __forceinline__ int code(int site) { return kStatusTimeout | (site << 8); }
+__device__ __forceinline__ bool warp_ok(bool ok) { return __all_sync(0xffffffffu, ok); }
+__device__ __forceinline__ int clampi(int v, int hi) { return v < 0 ? 0 : (v > hi ? hi : v); }
+
+__device__ __forceinline__ int w_begin(int T, int W, int w) {
+    return static_cast<int>(static_cast<long long>(T) * w / W);
+}
+__device__ __forceinline__ int w_of(int T, int W, int t) {
+    return static_cast<int>(((static_cast<long long>(t) + 1) * W - 1) / T);
+}
+
+// Prefix group of request b, or -1: the last one that starts at or before b, if it holds b.
+__device__ __forceinline__ int prefix_of(const PrefixArgs& A, int b) {
+    int lo = 0, hi = A.P;
+    while (lo + 1 < hi) {
+        const int mid = (lo + hi) / 2;
+        if (A.starts[mid] <= b) lo = mid; else hi = mid;
+    }
+    return A.starts[lo] <= b && b < A.starts[lo + 1] ? lo : -1;
+}
+
+// ------------------------------------------------------------------------------------- plan
+
+constexpr int kPlanThreads = 1024;
+
+// Exclusive sums over the block's threads of v; *carry is advanced by their total.
+__device__ int block_scan(int v, int* sh, int* carry) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) sh[warp] = x;
+    __syncthreads();
+    if (warp == 0) {
+        int s = sh[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, s, o);
+            if (lane >= o) s += y;
+        }
+        sh[lane] = s;
+    }
+    __syncthreads();
+    const int at = *carry + x - v + (warp ? sh[warp - 1] : 0);
+    const int total = sh[31];
+    __syncthreads();
+    if (threadIdx.x == 0) *carry += total;
+    __syncthreads();
+    return at;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(const __grid_constant__ PrefixArgs A, const Work wk) {
+    __shared__ int sh[32], carry;
+    pdl_launch_dependents();
+    const int hb = ceil_div(A.H, 128), tid = threadIdx.x;
+    if (tid == 0) {
+        carry = 0;
+        *wk.status = 0;
+    }
+    __syncthreads();
+    int extra = 0;   // row groups of the prefixes
+    if (!wk.fold) {
+        for (int p0 = 0; p0 < A.P; p0 += kPlanThreads) {
+            const int p = p0 + tid;
+            int n = 0;
+            if (p < A.P) {
+                const int s0 = max(A.starts[p], 0), s1 = min(A.starts[p + 1], A.B);
+                n = s1 > s0 ? (static_cast<long long>(s1 - s0) * A.H + 127) / 128 : 0;
+            }
+            const int at = block_scan(n, sh, &carry);
+            if (p < A.P) wk.gbase[p] = at;
+        }
+        extra = carry;
+        __syncthreads();
+        if (tid == 0) {
+            wk.gbase[A.P] = extra;
+            carry = 0;
+        }
+        __syncthreads();
+    }
+    const int G = wk.own + extra;
+    for (int g0 = 0; g0 < G; g0 += kPlanThreads) {
+        const int g = g0 + tid;
+        Group d = {};
+        int tiles = 0;
+        if (g < wk.own) {
+            const int b = g / hb, k = g % hb;
+            d.q_row0 = b * A.H + 128 * k;
+            d.rows = min(128, A.H - 128 * k);
+            d.pid = wk.fold ? prefix_of(A, b) : -1;
+            d.sid = b;
+            d.plen = d.pid >= 0 ? clampi(A.plens[d.pid], A.max_plen) : 0;
+            d.slen = clampi(A.lens[b], A.max_len);
+        } else if (g < G) {
+            const int e = g - wk.own;
+            int lo = 0, hi = A.P;   // last prefix group that starts at or before e
+            while (lo + 1 < hi) {
+                const int mid = (lo + hi) / 2;
+                if (wk.gbase[mid] <= e) lo = mid; else hi = mid;
+            }
+            const int s0 = max(A.starts[lo], 0), s1 = min(A.starts[lo + 1], A.B);
+            const int at = (e - wk.gbase[lo]) * 128;
+            d.q_row0 = s0 * A.H + at;
+            d.rows = min(128, (s1 - s0) * A.H - at);
+            d.pid = lo;
+            d.sid = -1;
+            d.plen = clampi(A.plens[lo], A.max_plen);
+        }
+        if (g < G) {
+            d.ptiles = ceil_div(d.plen, kTile);
+            tiles = d.ptiles + ceil_div(d.slen, kTile);
+            wk.bad[g] = 0;
+        }
+        d.tile0 = block_scan(tiles, sh, &carry);
+        if (g < G) wk.group[g] = d;
+    }
+    if (tid == 0) {
+        *wk.head = {G, carry, min(wk.W, carry)};
+        wk.group[G].tile0 = carry;   // the end of the last group's tiles
+    }
+}
+
+// ------------------------------------------------------------------------------------- attend
+
+struct __align__(8) Barriers {
+    uint64_t kv_full[kStages], kv_empty[kStages];
+    uint64_t s_full[kSets];           // per set: the score of its next tile is done
+    uint64_t s_free;
+    uint64_t p_full[2], pv_done[2];   // per P buffer (tile parity)
+    uint64_t x_full[kXSlots];         // the peer's partial scores have arrived
+    uint64_t x_empty[kXSlots];        // credit: the peer has read what this CTA sent into that slot
+    uint64_t mref[kMSlots];           // m_pub slot j % kMSlots holds tile j's reference
+    uint64_t lpub[2 * kSets];         // rowsum slot j % (2 kSets) holds tile j's set's sums (near a segment's end)
+    uint64_t q_ready, o_free, drain, done, epi_go;
+    int epi_rec, epi_rows;
+    float epi_f[128];
+    uint32_t tmem;
+};
+
+constexpr size_t kSmemBytes = static_cast<size_t>(kStages) * kStageBytes + static_cast<size_t>(kXSlots) * kXBytes +
+                              kQRopeBytes + kMSlots * 128 * sizeof(float) + sizeof(Barriers) + 1024;
+static_assert(kSmemBytes <= 232448, "shared memory budget");
+
+// Walks a worker's tiles; every role walks an identical copy. A segment is the worker's run of tiles
+// of one group.
+struct Tiles {
+    int t, t_begin, t_end, g, seg0;
+    Group d;
+    int gend;
+    __device__ void load(const Work& wk) {
+        const int4* p = reinterpret_cast<const int4*>(wk.group + g);
+        const int4 a = p[0], b = p[1];
+        d.q_row0 = a.x; d.rows = a.y; d.pid = a.z; d.sid = a.w;
+        d.plen = b.x; d.slen = b.y; d.tile0 = b.z; d.ptiles = b.w;
+        gend = wk.group[g + 1].tile0;
+    }
+    __device__ void init(const Work& wk, int groups, int tb, int te) {
+        t = t_begin = seg0 = tb;
+        t_end = te;
+        int lo = 0, hi = groups;   // last group whose tiles start at or before tb and are not none
+        while (lo + 1 < hi) {
+            const int mid = (lo + hi) / 2;
+            if (wk.group[mid].tile0 <= tb) lo = mid; else hi = mid;
+        }
+        g = lo;
+        load(wk);
+    }
+    __device__ bool valid() const { return t < t_end; }
+    __device__ bool own() const { return t - d.tile0 >= d.ptiles; }
+    __device__ int pos0() const { return (t - d.tile0 - (own() ? d.ptiles : 0)) * kTile; }
+    __device__ int np() const { return min(kTile, (own() ? d.slen : d.plen) - pos0()); }
+    __device__ int seg_tile() const { return t - seg0; }
+    __device__ bool seg_first() const { return t == seg0; }
+    __device__ bool seg_last() const { return t + 1 == t_end || t + 1 == gend; }
+    __device__ void next(const Work& wk) {
+        ++t;
+        if (t >= gend && t < t_end) {
+            do { ++g; } while (wk.group[g + 1].tile0 <= t);   // groups without tiles
+            load(wk);
+            seg0 = t;
+        }
+    }
+    __device__ void skip(const Work& wk, int n) {
+        for (; n > 0 && valid(); --n) next(wk);
+    }
+};
+
+template <typename T> struct Fmt;
+template <> struct Fmt<__half> { static constexpr uint32_t v = 0; };
+template <> struct Fmt<__nv_bfloat16> { static constexpr uint32_t v = 1; };
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t half2_of(float a, float b) {
+    __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+template <typename T> __device__ __forceinline__ uint32_t pair_of(float a, float b);
+template <> __device__ __forceinline__ uint32_t pair_of<__half>(float a, float b) { return half2_of(a, b); }
+template <> __device__ __forceinline__ uint32_t pair_of<__nv_bfloat16>(float a, float b) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 floats_of(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+// two fp32 lanes in one instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+        "add.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+// 2^f that brings this thread's O row (256 TMEM columns) below 2^15, for the fp16 record; 1 for rows
+// of zeros and for infinities and NaN, which go into the record as they are. Warp-collective.
+__device__ __forceinline__ float record_scale(uint32_t tsrc) {
+    float top = 0.f;
+#pragma unroll 1
+    for (int c0 = 0; c0 < 256; c0 += 32) {
+        uint32_t o[32];
+        tmem_ld32_sync(tsrc + c0, o);
+        float mx[4] = {};
+#pragma unroll
+        for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], fabsf(__uint_as_float(o[i])));
+        top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+    }
+    // exponent field of 2^(14 - floor(log2 top)), kept where both 2^f and 2^-f are normal
+    const int e = static_cast<int>(__float_as_uint(top) >> 23);
+    return e > 0 && e < 255 ? __uint_as_float(static_cast<uint32_t>(min(max(268 - e, 1), 253)) << 23) : 1.f;
+}
+// ncols columns of this thread's O row (TMEM) times scale to a record row. Warp-collective.
+__device__ __forceinline__ void write_cols(uint32_t tsrc, uint16_t* orow, float scale, bool row_ok, int ncols) {
+#pragma unroll 1
+    for (int c0 = 0; c0 < ncols; c0 += 32) {
+        uint32_t o[32];
+        tmem_ld32_sync(tsrc + c0, o);
+        if (row_ok) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                uint32_t v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    v[i] = half2_of(__uint_as_float(o[16 * q + 2 * i]) * scale, __uint_as_float(o[16 * q + 2 * i + 1]) * scale);
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(orow + c0 + 16 * q),
+                             "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                             : "memory");
+            }
+        }
+    }
+}
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ CUtensorMap tmap_rope,
+                     const __grid_constant__ PrefixArgs A, const __grid_constant__ Work wk) {
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    unsigned char* stages = smem;
+    unsigned char* xbuf = stages + kStages * kStageBytes;
+    unsigned char* qrope = xbuf + kXSlots * kXBytes;
+    float* m_pub = reinterpret_cast<float*>(qrope + kQRopeBytes);              // [kMSlots][128]
+    Barriers* bars = reinterpret_cast<Barriers*>(m_pub + kMSlots * 128);
+    // the row sums that one set hands to another at a segment's end: in global memory, where shared
+    // memory has no room, and only for the segment's last tiles
+    volatile float2* l_pub = wk.rowsum + static_cast<long long>(blockIdx.x) * 2 * kSets * 128;
+    const uint32_t rank = cluster_ctarank(), peer = rank ^ 1u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int w = blockIdx.x >> 1;
+    volatile int* err = wk.status;
+
+    if (threadIdx.x == 0) {
+        pdl_launch_dependents();
+        tma_prefetch_desc(&tmap);
+        tma_prefetch_desc(&tmap_rope);
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(smem_u32(&bars->kv_full[s]), 1);
+            mbar_init(smem_u32(&bars->kv_empty[s]), 1);
+        }
+        for (int i = 0; i < kSets; ++i) mbar_init(smem_u32(&bars->s_full[i]), 1);
+        mbar_init(smem_u32(&bars->s_free), 128);
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(smem_u32(&bars->p_full[b]), 128);
+            mbar_init(smem_u32(&bars->pv_done[b]), 1);
+        }
+        for (int i = 0; i < kMSlots; ++i) mbar_init(smem_u32(&bars->mref[i]), 128);
+        for (int i = 0; i < 2 * kSets; ++i) mbar_init(smem_u32(&bars->lpub[i]), 128);
+        for (int s = 0; s < kXSlots; ++s) {
+            mbar_init(smem_u32(&bars->x_full[s]), 1);
+            mbar_init(smem_u32(&bars->x_empty[s]), 4);   // one arrival per warp of the reading set
+        }
+        mbar_init(smem_u32(&bars->q_ready), 128);
+        mbar_init(smem_u32(&bars->o_free), 128);
+        mbar_init(smem_u32(&bars->drain), 1);
+        mbar_init(smem_u32(&bars->done), 1);
+        mbar_init(smem_u32(&bars->epi_go), 128);
+        fence_mbar_init();
+        // each exchange slot is armed for its first tile here, and for the next one by the set that
+        // has seen it complete
+        for (int s = 0; s < kXSlots; ++s) mbar_arrive_expect_tx(smem_u32(&bars->x_full[s]), kXBytes);
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(&bars->tmem), kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tbase = bars->tmem;
+    pdl_wait();   // the plan
+    const Header head = *wk.head;
+    // identical in both CTAs of the pair; a pair without tiles goes straight to the teardown
+    const int tb = w < head.workers ? w_begin(head.tiles, head.workers, w) : 0;
+    const int te = w < head.workers ? w_begin(head.tiles, head.workers, w + 1) : 0;
+    const int n = te - tb;
+    const uint32_t stages_u32 = smem_u32(stages), xbuf_u32 = smem_u32(xbuf), qrope_u32 = smem_u32(qrope);
+
+    if (warp < 4) {
+        if (n > 0 && warp == 0 && lane == 0) {
+            // ------------------------------------------------------------ loads
+            Tiles it;
+            it.init(wk, head.groups, tb, te);
+            int issued = 0;
+            for (int i = 0; it.valid(); ++i, it.next(wk)) {
+                const int st = i % kStages;
+                const int pos = it.pos0(), np = it.np();
+                long long row;
+                if (A.page_rows) {
+                    const int pg = it.own() ? A.table[static_cast<long long>(it.d.sid) * A.max_pages + pos / A.page_rows]
+                                            : A.ptable[static_cast<long long>(it.d.pid) * A.max_ppages + pos / A.page_rows];
+                    row = pg < 0 ? -1 : static_cast<long long>(pg) * A.page_rows + pos % A.page_rows;
+                } else {
+                    row = (it.own() ? A.offs[it.d.sid] : A.poffs[it.d.pid]) + pos;
+                }
+                if (row < 0 || row + np > A.kv_rows) {
+                    wk.bad[it.g] = 1;
+                    row = -2 * kTile;   // outside the tensor: reads zeros
+                }
+                if (i >= kStages && !mbar_wait(smem_u32(&bars->kv_empty[st]), ((i / kStages) - 1) & 1, err, code(kWaitLoad))) break;
+                const uint32_t full = smem_u32(&bars->kv_full[st]), dst = stages_u32 + st * kStageBytes;
+                mbar_arrive_expect_tx(full, kStageBytes);
+                tma_load_3d(dst + kRopeBytes, &tmap, full, 0, static_cast<int>(row), 4 * static_cast<int>(rank));
+                tma_load_3d(dst, &tmap_rope, full, 0, static_cast<int>(row), 4 * static_cast<int>(rank));
+                issued = i + 1;
+            }
+            // the last loads land before shared memory is released
+            for (int i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
+                mbar_wait(smem_u32(&bars->kv_full[i % kStages]), (i / kStages) & 1, err, code(kWaitLoad), 100000000ull);
+        } else if (n > 0 && warp == 1 && lane == 0) {
+            // ------------------------------------------------------------ MMAs
+            constexpr uint32_t idesc_s = idesc_f16(128, kTile, Fmt<T>::v, false, false);
+            constexpr uint32_t idesc_pv = idesc_f16(128, 256, Fmt<T>::v, false, true);
+            const uint32_t tS = tbase + kColS, tQ = tbase + kColQ, tO = tbase + kColO;
+            const uint64_t dqr = smem_desc_noswz(qrope_u32, kQRopeBoxBytes, 128);
+            auto issue_score = [&](int i) {
+                const uint32_t sa = stages_u32 + (i % kStages) * kStageBytes;
+                const uint64_t dl = smem_desc_sw128(sa + kRopeBytes, 16, 1024);
+                mma_ts(tS, tQ, dl, idesc_s, 0u);
+#pragma unroll
+                for (int k = 1; k < 16; ++k)
+                    mma_ts(tS, tQ + 8 * k, dl + static_cast<uint64_t>(((k >> 2) * kChunkBytes + (k & 3) * 32) >> 4), idesc_s, 1u);
+                const uint64_t dr = smem_desc_noswz(sa, kRopeBoxBytes, 128);
+                mma_ss(tS, dqr, dr, idesc_s, 1u);
+                mma_ss(tS, dqr + static_cast<uint64_t>((2 * kQRopeBoxBytes) >> 4),
+                       dr + static_cast<uint64_t>((2 * kRopeBoxBytes) >> 4), idesc_s, 1u);
+                mma_commit(smem_u32(&bars->s_full[i % kSets]));
+            };
+            auto issue_pv = [&](int i, bool first) {
+                const uint64_t dc = smem_desc_sw128(stages_u32 + (i % kStages) * kStageBytes + kRopeBytes, kChunkBytes, 1024);
+                const uint32_t tP = tbase + kColP + 32 * (i & 1);
+                mma_ts(tO, tP, dc, idesc_pv, first ? 0u : 1u);
+#pragma unroll
+                for (int k = 1; k < kTile / 16; ++k)
+                    mma_ts(tO, tP + 8 * k, dc + static_cast<uint64_t>((2048 * k) >> 4), idesc_pv, 1u);
+                mma_commit(smem_u32(&bars->pv_done[i & 1]));
+                mma_commit(smem_u32(&bars->kv_empty[i % kStages]));
+            };
+            // Scores and value products go in tile order each, whichever is ready first: score(s) needs
+            // S read out, its stage, and at a segment's start the group's Q; PV(v) needs P(v) and at a
+            // segment's start the O of the one before read out.
+            Tiles its, itv;
+            its.init(wk, head.groups, tb, te);
+            itv = its;
+            int next_s = 0, next_v = 0, qseg = 0, vseg = 0;
+            bool ok = true;
+            long long t_last = clock64();
+            const long long budget = wait_budget_cycles(kDefaultWaitNs);
+            for (uint32_t spin = 0; ok && next_v < n; ++spin) {
+                bool progressed = false;
+                if (next_s < n && (next_s == 0 || mbar_test(smem_u32(&bars->s_free), (next_s - 1) & 1)) &&
+                    mbar_test(smem_u32(&bars->kv_full[next_s % kStages]), (next_s / kStages) & 1) &&
+                    (!its.seg_first() || mbar_test(smem_u32(&bars->q_ready), qseg & 1))) {
+                    tc_fence_after();
+                    issue_score(next_s);
+                    if (its.seg_last()) ++qseg;
+                    its.next(wk);
+                    ++next_s;
+                    progressed = true;
+                }
+                if (next_v < next_s && mbar_test(smem_u32(&bars->p_full[next_v & 1]), (next_v >> 1) & 1) &&
+                    (!itv.seg_first() || vseg == 0 || mbar_test(smem_u32(&bars->o_free), (vseg - 1) & 1))) {
+                    tc_fence_after();
+                    issue_pv(next_v, itv.seg_first());
+                    if (itv.seg_last()) ++vseg;
+                    itv.next(wk);
+                    ++next_v;
+                    progressed = true;
+                }
+                if (progressed) {
+                    t_last = clock64();
+                    continue;
+                }
+                if ((spin & 31u) == 0u) {
+                    const long long dt = clock64() - t_last;
+                    if ((dt > kErrPollCycles && *err != 0) || dt > budget) {
+                        atomicCAS(const_cast<int*>(err), 0, code(kWaitMma));
+                        ok = false;
+                    }
+                }
+            }
+            mma_commit(smem_u32(&bars->drain));   // every MMA is done before the teardown
+            mbar_wait(smem_u32(&bars->drain), 0, err, code(kWaitDrain));
+        }
+    } else {
+        // ---------------------------------------------------------------- softmax sets
+        const int sid = (warp - 4) >> 2;
+        const int t = (warp & 3) * 32 + lane;             // query row == TMEM lane
+        const uint32_t trow = tbase + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
+        const uint32_t x_local = xbuf_u32 + t * 16;       // 16-byte unit c of row t at c * 2048 + t * 16
+        const uint32_t x_remote = mapa(x_local, peer);
+        const float qscale = A.scale * 1.4426950408889634f;
+        auto load_q = [&](const Group& d) {
+            const long long row = d.q_row0 + t;
+            const uint4* lat = reinterpret_cast<const uint4*>(static_cast<const T*>(A.qa) + row * 512 + 256 * rank);
+            const uint4* rope = reinterpret_cast<const uint4*>(static_cast<const T*>(A.qr) + row * 64 + 32 * rank);
+            const bool have = t < d.rows;
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+                uint4 v[8], r;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = have ? __ldg(lat + 8 * c + k) : make_uint4(0, 0, 0, 0);
+                r = have ? __ldg(rope + c) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const uint32_t x[16] = {v[4 * q].x, v[4 * q].y, v[4 * q].z, v[4 * q].w,
+                                            v[4 * q + 1].x, v[4 * q + 1].y, v[4 * q + 1].z, v[4 * q + 1].w,
+                                            v[4 * q + 2].x, v[4 * q + 2].y, v[4 * q + 2].z, v[4 * q + 2].w,
+                                            v[4 * q + 3].x, v[4 * q + 3].y, v[4 * q + 3].z, v[4 * q + 3].w};
+                    tmem_st16(trow + kColQ + 32 * c + 16 * q, x);
+                }
+                *reinterpret_cast<uint4*>(qrope + c * kQRopeBoxBytes + t * 16) = r;
+            }
+            fence_proxy_async_smem();
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(smem_u32(&bars->q_ready));
+        };
+        Tiles it;
+        bool ok = true;
+        if (n > 0) {
+            it.init(wk, head.groups, tb, te);
+            if (sid == 0) load_q(it.d);   // the first tile belongs to set 0
+            it.skip(wk, sid);
+        } else {
+            it.t = it.t_end = 0;
+        }
+        float l_self = 0.f, m_l = 0.f;    // this set's row sum over its tiles of the segment, and its reference
+        for (int j = sid; ok && it.valid(); j += kSets, it.skip(wk, kSets)) {
+            const int slot = j % kXSlots;
+            const int np = it.np();
+            // ---- S_r(j) to registers, release S, send the fp16 partial
+            bool got = mbar_wait(smem_u32(&bars->s_full[sid]), (j / kSets) & 1, err, code(kWaitS));
+            if (!warp_ok(got)) break;
+            tc_fence_after();
+            uint32_t h[32];
+            {
+                uint32_t sr[32];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    tmem_ld32_sync(trow + kColS + 32 * half, sr);
+#pragma unroll
+                    for (int q = 0; q < 16; ++q)
+                        h[16 * half + q] = half2_of(__uint_as_float(sr[2 * q]) * qscale, __uint_as_float(sr[2 * q + 1]) * qscale);
+                }
+                tc_fence_before();
+                mbar_arrive(smem_u32(&bars->s_free));
+            }
+            // the peer has read its slot's tile j - 2
+            got = j < kXSlots || mbar_wait_cluster(smem_u32(&bars->x_empty[slot]), ((j / kXSlots) - 1) & 1, err, code(kWaitCredit));
+            if (!warp_ok(got)) break;
+            {
+                const uint32_t rbar = mapa(smem_u32(&bars->x_full[slot]), peer);
+                const uint32_t dst = x_remote + slot * kXBytes;
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    st_async_v4(dst + c * 2048, h[4 * c], h[4 * c + 1], h[4 * c + 2], h[4 * c + 3], rbar);
+            }
+            if (it.seg_last() && it.t + 1 < te) {
+                // the score of tile j was the last MMA to read this group's Q
+                Tiles nx = it;
+                nx.next(wk);
+                load_q(nx.d);
+            }
+            if (np < kTile) {
+                // rows past the end: their weights are zero, but zero times what lies there need not be
+                unsigned char* sp = stages + (j % kStages) * kStageBytes + kRopeBytes;
+                const int units = (kTile - np) * 8;
+                for (int v = t; v < 4 * units; v += 128)
+                    *reinterpret_cast<uint4*>(sp + (v / units) * kChunkBytes + (np + (v % units) / 8) * 128 + (v % 8) * 16) =
+                        make_uint4(0, 0, 0, 0);
+                fence_proxy_async_smem();
+            }
+            // ---- the whole score, its reference, P into TMEM buffer j & 1
+            got = mbar_wait_cluster(smem_u32(&bars->x_full[slot]), (j / kXSlots) & 1, err, code(kWaitX));
+            if (!warp_ok(got)) break;
+            if (t == 0) mbar_arrive_expect_tx(smem_u32(&bars->x_full[slot]), kXBytes);   // for tile j + 2
+            float s[64];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                uint4 v;
+                asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                             : "r"(x_local + slot * kXBytes + c * 2048));
+                const uint32_t pv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float2 r = add2(floats_of(h[4 * c + q]), floats_of(pv[q]));
+                    s[8 * c + 2 * q] = r.x;
+                    s[8 * c + 2 * q + 1] = r.y;
+                }
+            }
+            // credit for the peer, relaxed: it only has to follow the reads above
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote_relaxed(mapa(smem_u32(&bars->x_empty[slot]), peer));
+            if (np < kTile) {
+#pragma unroll
+                for (int k = 0; k < kTile; ++k)
+                    if (k >= np) s[k] = -INFINITY;
+            }
+            float mx[32];
+#pragma unroll
+            for (int k = 0; k < 32; ++k) mx[k] = fmaxf(s[k], s[k + 32]);
+#pragma unroll
+            for (int w2 = 16; w2 > 0; w2 >>= 1)
+#pragma unroll
+                for (int k = 0; k < w2; ++k) mx[k] = fmaxf(mx[k], mx[k + w2]);
+            const float mt = fmaxf(mx[0], kLowest);
+            // the reference of the tile before, unless this one exceeds it by more than the threshold
+            float m = mt, alpha = 1.f;
+            bool need = false;
+            if (!it.seg_first()) {
+                got = mbar_wait(smem_u32(&bars->mref[(j - 1) % kMSlots]), ((j - 1) / kMSlots) & 1, err, code(kWaitRef));
+                if (!warp_ok(got)) break;
+                const float m_prev = m_pub[((j - 1) % kMSlots) * 128 + t];
+                if (mt > m_prev + kRescale) {
+                    alpha = ex2(m_prev - mt);
+                    need = true;
+                } else {
+                    m = m_prev;
+                }
+            }
+            m_pub[(j % kMSlots) * 128 + t] = m;
+            mbar_arrive(smem_u32(&bars->mref[j % kMSlots]));
+            uint32_t pp[32];
+            float2 ls[4];
+            const float2 m2 = make_float2(-m, -m);
+#pragma unroll
+            for (int q = 0; q < 32; ++q) {
+                const float2 d = add2(make_float2(s[2 * q], s[2 * q + 1]), m2);
+                const float2 e = make_float2(ex2(d.x), ex2(d.y));
+                pp[q] = pair_of<T>(e.x, e.y);
+                const float2 p = ElemTraits<T>::to_f2(*reinterpret_cast<const typename ElemTraits<T>::T2*>(&pp[q]));
+                ls[q & 3] = q < 4 ? p : add2(ls[q & 3], p);
+            }
+            ls[0] = add2(add2(ls[0], ls[1]), add2(ls[2], ls[3]));
+            if (it.seg_tile() < kSets) l_self = 0.f;
+            else if (m != m_l) l_self *= ex2(m_l - m);
+            m_l = m;
+            l_self += ls[0].x + ls[0].y;
+            // P buffer j & 1 is free once PV(j - 2) is done
+            got = j < 2 || mbar_wait(smem_u32(&bars->pv_done[j & 1]), ((j - 2) >> 1) & 1, err, code(kWaitPV));
+            if (!warp_ok(got)) break;
+            if (__any_sync(0xffffffffu, need)) {
+                // the reference moved: rescale O (alpha = 1 elsewhere) once PV(j - 1) is done
+                got = mbar_wait(smem_u32(&bars->pv_done[(j - 1) & 1]), ((j - 1) >> 1) & 1, err, code(kWaitPV));
+                if (!warp_ok(got)) break;
+                tc_fence_after();
+#pragma unroll 1
+                for (int c0 = 0; c0 < 256; c0 += 32) {
+                    uint32_t o[32];
+                    tmem_ld32_sync(trow + kColO + c0, o);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+                    tmem_st32(trow + kColO + c0, o);
+                }
+            }
+            tc_fence_after();
+            tmem_st32(trow + kColP + 32 * (j & 1), pp);
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(smem_u32(&bars->p_full[j & 1]));
+            if (it.t + kSets >= min(te, it.gend)) {
+                volatile float2* lp = l_pub + (j % (2 * kSets)) * 128 + t;
+                lp->x = l_self;
+                lp->y = m;
+            }
+            mbar_arrive(smem_u32(&bars->lpub[j % (2 * kSets)]));
+
+            if (it.seg_last()) {
+                // ---- the segment's partial record
+                got = mbar_wait(smem_u32(&bars->pv_done[j & 1]), (j >> 1) & 1, err, code(kWaitPV));
+                float l_tot = l_self;
+#pragma unroll
+                for (int i = 1; i < kSets; ++i)
+                    if (it.seg_tile() >= i) {
+                        // the set of tile j - i: its sum over the segment ends there
+                        const int js = j - i;
+                        got = got && mbar_wait(smem_u32(&bars->lpub[js % (2 * kSets)]), (js / (2 * kSets)) & 1, err, code(kWaitRef));
+                        const volatile float2* lp = l_pub + (js % (2 * kSets)) * 128 + t;
+                        l_tot += lp->x * ex2(lp->y - m);
+                    }
+                if (!warp_ok(got)) break;
+                tc_fence_after();
+                const int rec = it.g + w, rows = it.d.rows;
+                // the worker's last tile: an idle set writes half of the columns
+                const bool help = j == n - 1;
+                const float f = record_scale(trow + kColO);
+                if (help) {
+                    if (t == 0) {
+                        bars->epi_rec = rec;
+                        bars->epi_rows = rows;
+                    }
+                    bars->epi_f[t] = f;
+                    tc_fence_before();
+                    mbar_arrive(smem_u32(&bars->epi_go));
+                }
+                const long long at = static_cast<long long>(rec) * 128 + t;
+                write_cols(trow + kColO, wk.rec_o + at * 512 + 256 * rank, f, t < rows, help ? 128 : 256);
+                if (t < rows) {
+                    float* ml = reinterpret_cast<float*>(wk.rec_ml + at);
+                    if (rank == 0) *reinterpret_cast<float2*>(ml) = make_float2(m, l_tot);
+                    ml[2 + rank] = 1.f / f;
+                }
+                tc_fence_before();
+                mbar_arrive(smem_u32(&bars->o_free));
+            }
+        }
+        if (n > 0 && sid == n % kSets) {
+            // the set after the last tile's: columns 128 .. 255 of its record
+            const bool got = mbar_wait(smem_u32(&bars->epi_go), 0, err, code(kWaitEpi));
+            if (warp_ok(got)) {
+                tc_fence_after();
+                write_cols(trow + kColO + 128, wk.rec_o + (static_cast<long long>(bars->epi_rec) * 128 + t) * 512 + 256 * rank + 128,
+                           bars->epi_f[t], t < bars->epi_rows, 128);
+            }
+        }
+    }
+
+    // ---------------------------------------------------------------- teardown
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        // the pair finishes together: no CTA leaves while the other may still address it
+        mbar_arrive_remote(mapa(smem_u32(&bars->done), peer));
+        mbar_wait_cluster_full(smem_u32(&bars->done), 0, err, code(kWaitTeardown));
+        if (*err != 0) {
+            // after a failure the peer's partial scores may still be in flight
+            const uint64_t t0 = globaltimer_ns();
+            while (globaltimer_ns() - t0 < 20000ull) {
+            }
+        }
+    }
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tbase, kTmemCols);
+}
+
+// ------------------------------------------------------------------------------------- merge
+
+constexpr int kMergeWarps = 8;
+
+// One output row per `kWarps` warps: each takes every kWarps-th record of the row's groups, keeping
+// the running maximum, sum and weighted latent in fp32; the warps meet in shared memory.
+template <typename T, int kWarps>
+__global__ void __launch_bounds__(32 * kMergeWarps) prefix_merge_kernel(const __grid_constant__ PrefixArgs A, const Work wk) {
+    constexpr int kRows = kMergeWarps / kWarps;   // rows per block
+    __shared__ float sh_o[kWarps > 1 ? kMergeWarps : 1][512];
+    __shared__ float2 sh_ml[kMergeWarps];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    const int sub = warp % kWarps;
+    const int f = blockIdx.x * kRows + warp / kWarps;
+    pdl_wait();
+    const bool live = f < A.B * A.H;
+    float m = -INFINITY, l = 0.f;
+    float o[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] = 0.f;
+    bool bad = false;
+    if (live) {
+        const int b = f / A.H, h = f % A.H;
+        const int T_all = wk.head->tiles, W = wk.head->workers;
+        bad = *wk.status != 0;
+        // the row's groups: its request's, and unless that holds the prefix too, its prefix group's
+        for (int k = 0; k < (wk.fold ? 1 : 2); ++k) {
+            int g, r;
+            if (k == 0) {
+                g = b * ceil_div(A.H, 128) + h / 128;
+                r = h % 128;
+            } else {
+                const int p = prefix_of(A, b);
+                if (p < 0) break;
+                const int at = f - max(A.starts[p], 0) * A.H;
+                g = wk.own + wk.gbase[p] + at / 128;
+                r = at % 128;
+            }
+            const int t0 = wk.group[g].tile0, t1 = wk.group[g + 1].tile0;
+            if (t1 <= t0) continue;
+            bad = bad || wk.bad[g] != 0;
+            const int w0 = w_of(T_all, W, t0), w1 = w_of(T_all, W, t1 - 1);
+            constexpr int kAhead = 4;
+            for (int w = w0 + sub; w <= w1; w += kWarps * kAhead) {
+                uint4 v[kAhead][2];
+                float4 ml[kAhead];
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i)
+                    if (w + i * kWarps <= w1) {
+                        const long long at = static_cast<long long>(g + w + i * kWarps) * 128 + r;
+                        ml[i] = wk.rec_ml[at];
+                        const uint4* src = reinterpret_cast<const uint4*>(wk.rec_o + at * 512);
+                        v[i][0] = src[lane];
+                        v[i][1] = src[32 + lane];
+                    }
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i)
+                    if (w + i * kWarps <= w1) {
+                        const float top = fmaxf(m, ml[i].x);
+                        const float a = ex2(m - top), e0 = ex2(ml[i].x - top);
+                        const float c2[2] = {e0 * ml[i].z, e0 * ml[i].w};
+                        m = top;
+                        l = l * a + e0 * ml[i].y;
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            const uint32_t x[4] = {v[i][q].x, v[i][q].y, v[i][q].z, v[i][q].w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float2 y = floats_of(x[e]);
+                                o[8 * q + 2 * e] = o[8 * q + 2 * e] * a + c2[q] * y.x;
+                                o[8 * q + 2 * e + 1] = o[8 * q + 2 * e + 1] * a + c2[q] * y.y;
+                            }
+                        }
+                    }
+            }
+        }
+    }
+    if constexpr (kWarps > 1) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sh_o[warp][256 * q + 8 * lane + e] = o[8 * q + e];
+        if (lane == 0) sh_ml[warp] = make_float2(m, l);
+        __syncthreads();
+        const int first = warp - sub;
+        float top = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) top = fmaxf(top, sh_ml[first + i].x);
+        float c[kWarps];
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) {
+            c[i] = sh_ml[first + i].x == -INFINITY ? 0.f : ex2(sh_ml[first + i].x - top);
+            l += c[i] * sh_ml[first + i].y;
+        }
+        // each warp finishes its share of the columns
+        T* out = static_cast<T*>(A.out) + static_cast<long long>(f) * 512;
+        if (live)
+            for (int x = sub * 32 + lane; x < 512; x += 32 * kWarps) {
+                float y = 0.f;
+#pragma unroll
+                for (int i = 0; i < kWarps; ++i) y += c[i] * sh_o[first + i][x];
+                out[x] = ElemTraits<T>::from_f(bad ? NAN : (l == 0.f ? 0.f : y / l));
+            }
+    } else if (live) {
+        const float inv = bad ? NAN : (l == 0.f ? 0.f : 1.f / l);
+        uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(A.out) + static_cast<long long>(f) * 512);
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+            out[32 * q + lane] = make_uint4(pair_of<T>(o[8 * q] * inv, o[8 * q + 1] * inv), pair_of<T>(o[8 * q + 2] * inv, o[8 * q + 3] * inv),
+                                            pair_of<T>(o[8 * q + 4] * inv, o[8 * q + 5] * inv), pair_of<T>(o[8 * q + 6] * inv, o[8 * q + 7] * inv));
+    }
+}
+
+// ------------------------------------------------------------------------------------- host
+
+struct Layout {
+    long long groups;     // most groups
+    size_t off_head, off_group, off_base, off_bad, off_sum, off_ml, off_o, total;
+    int W, own, fold;
+};
+
+Layout layout(const PrefixArgs& A, int sms) {
+    Layout L = {};
+    L.fold = A.H % 128 == 0;
+    L.own = A.B * ceil_div(A.H, 128);
+    // rows of a prefix group end inside a tile at most once a group
+    L.groups = L.own + (L.fold ? 0 : static_cast<long long>(A.B) * A.H / 128 + (A.P < A.B ? A.P : A.B));
+    L.W = sms / 2 > 0 ? sms / 2 : 1;
+    auto a256 = [](size_t x) { return (x + 255) / 256 * 256; };
+    size_t off = 256;     // status
+    L.off_head = off; off += 256;
+    L.off_group = off; off = a256(off + sizeof(Group) * static_cast<size_t>(L.groups + 1));
+    L.off_base = off; off = a256(off + sizeof(int) * (static_cast<size_t>(A.P) + 1));
+    L.off_bad = off; off = a256(off + sizeof(int) * static_cast<size_t>(L.groups));
+    L.off_sum = off; off = a256(off + sizeof(float2) * 2 * L.W * 2 * kSets * 128);
+    const size_t recs = static_cast<size_t>(L.groups) + L.W;
+    L.off_ml = off; off = a256(off + recs * 128 * sizeof(float4));
+    L.off_o = off; off = a256(off + recs * 128 * 512 * 2);
+    L.total = off;
+    return L;
+}
+
+template <typename T>
+cudaError_t launch(const PrefixArgs& A, unsigned char* ws, int sms, cudaStream_t s) {
+    const Layout L = layout(A, sms);
+    Work wk;
+    wk.status = reinterpret_cast<int*>(ws);
+    wk.head = reinterpret_cast<Header*>(ws + L.off_head);
+    wk.group = reinterpret_cast<Group*>(ws + L.off_group);
+    wk.gbase = reinterpret_cast<int*>(ws + L.off_base);
+    wk.bad = reinterpret_cast<int*>(ws + L.off_bad);
+    wk.rec_ml = reinterpret_cast<float4*>(ws + L.off_ml);
+    wk.rec_o = reinterpret_cast<uint16_t*>(ws + L.off_o);
+    wk.rowsum = reinterpret_cast<float2*>(ws + L.off_sum);
+    wk.W = L.W;
+    wk.own = L.own;
+    wk.fold = L.fold;
+    // the latent as 8 blocks of 64 columns and the rope key as 8 of 8: one load brings a CTA's four
+    CUtensorMap lat, rope;
+    const uint64_t rows = static_cast<uint64_t>(A.kv_rows), pitch = static_cast<uint64_t>(A.stride) * 2;
+    const uint64_t ld[3] = {64, rows, 8}, ls[2] = {pitch, 128}, rd[3] = {8, rows, 8}, rs[2] = {pitch, 16};
+    const uint32_t lb[3] = {64, kTile, 4}, rb[3] = {8, kTile, 4};
+    if (!encode_tmap_16b(&lat, A.kv, 3, ld, ls, lb, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !encode_tmap_16b(&rope, static_cast<const unsigned char*>(A.kv) + 1024, 3, rd, rs, rb, CU_TENSOR_MAP_SWIZZLE_NONE))
+        return cudaErrorInvalidValue;
+    cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(prefix_attend_kernel<T>), static_cast<int>(kSmemBytes));
+    if (e != cudaSuccess) return e;
+    prefix_plan_kernel<<<1, kPlanThreads, 0, s>>>(A, wk);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * L.W);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmemBytes;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if ((e = cudaLaunchKernelEx(&cfg, prefix_attend_kernel<T>, lat, rope, A, wk)) != cudaSuccess) return e;
+    cfg.dynamicSmemBytes = 0;
+    cfg.blockDim = dim3(32 * kMergeWarps);
+    const int out_rows = A.B * A.H;
+    // few rows have many records each (a row's group spans up to W workers): 8 warps a row
+    if (out_rows <= 4 * sms) {
+        cfg.gridDim = dim3(out_rows);
+        e = cudaLaunchKernelEx(&cfg, prefix_merge_kernel<T, kMergeWarps>, A, wk);
+    } else {
+        cfg.gridDim = dim3(ceil_div(out_rows, kMergeWarps));
+        e = cudaLaunchKernelEx(&cfg, prefix_merge_kernel<T, 1>, A, wk);
+    }
+    count_launches(3);
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+}  // namespace
+
+bool prefix_sm100_supported(const PrefixArgs& A) {
+    auto is16 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    return A.dc == 512 && A.dR == 64 && A.stride % 8 == 0 && A.stride <= (1 << 30) && is16(A.kv) && is16(A.qa) &&
+           is16(A.qr) && is16(A.out) && A.kv_rows < (1ll << 31) - 4 * kTile &&
+           // tiles are counted in 32 bits
+           static_cast<double>(A.B) * A.H / 64.0 * (static_cast<double>(A.max_plen) + A.max_len + 128) < 1e9;
+}
+
+size_t prefix_sm100_workspace(const PrefixArgs& A, int sms) { return layout(A, sms).total; }
+
+cudaError_t launch_prefix_sm100(const PrefixArgs& A, bool bf16, void* workspace, int sms, cudaStream_t s) {
+    unsigned char* ws = static_cast<unsigned char*>(workspace);
+    return bf16 ? launch<__nv_bfloat16>(A, ws, sms, s) : launch<__half>(A, ws, sms, s);
+}
+
+}  // namespace mla
