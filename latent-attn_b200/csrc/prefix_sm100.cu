@@ -29,8 +29,10 @@
 //
 // Warps (128 + 128 kSets threads): warp 0 loads, warp 1 issues the MMAs, warps 2-3 rest; softmax set i
 // takes the tiles j with j % kSets == i, thread = query row. A tile's way through the softmax (read S,
-// exchange, maximum, exponentials, write P) takes about 3 us of latency and little issue time, so the
-// number of sets, each on a tile of its own, sets the pace until the stages of the ring do.
+// exchange, maximum, exponentials, write P) takes about 3 us of latency and little issue time.
+// A parity wait may only start once the barrier's phase before the awaited one is known to be complete
+// (it would pass at once otherwise). So every barrier that a set waits on for its own tiles is used by
+// that set alone: an exchange slot and a P buffer per set.
 #include <cfloat>
 
 #include "mla_internal.cuh"
@@ -54,7 +56,7 @@ constexpr int kXBytes = 128 * 128;                   // 128 rows x 64 fp16 parti
 constexpr int kQRopeBoxBytes = 128 * 16;
 constexpr int kQRopeBytes = 4 * kQRopeBoxBytes;
 constexpr int kMSlots = 4;
-constexpr int kSets = 3;
+constexpr int kSets = 2;   // with the two exchange slots and P buffers: each slot belongs to one set
 constexpr int kThreads = 128 + 128 * kSets;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColO = 0, kColS = 256, kColQ = 320, kColP = 448;
