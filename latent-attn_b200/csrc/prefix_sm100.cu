@@ -10,7 +10,7 @@
 //   3. prefix_merge_kernel merges each output row's records by their maxima and sums.
 // Rounding: P is rounded to the cache's type for its MMA, and the row sums add the rounded values, so
 // that the weights of a row still add up to one; a record's o is stored in fp16 after an exact scaling
-// of each half row by a power of two (2^-11 relative, a quarter of the bytes of fp32's error budget
+// of each 128 columns by a power of two (2^-11 relative, a quarter of the bytes of fp32's error budget
 // being unused); all sums, maxima and accumulators are fp32; the result is rounded once.
 // A group is the M = 128 tile of the MMAs. When 128 divides H it is 128 heads of one request, whose
 // positions are its prefix followed by its own rows. Otherwise the (request, head) rows of a prefix
@@ -20,19 +20,23 @@
 // The pair splits both products evenly and reads every cache byte into shared memory once: CTA r
 // holds columns [256 r, 256 r + 256) of the latent and [32 r, 32 r + 32) of the rope key; it computes
 // the partial scores over them, and the output columns [256 r, + 256). TMEM per CTA: O 256 columns |
-// S 64 | Q latent 128 (two elements a column) | P 2 x 32. (The alternatives: a whole score in each CTA
-// costs 1.53 times the MMAs; splitting the rows instead needs every value column twice in shared
-// memory, and those MMAs with both operands there run at 1319 TFLOP/s at best, 868 with the loads.)
-// The two partial scores are exchanged in fp16 through distributed shared memory (in log2 units after
-// scaling: 2^-11 of a partial; fp32 would double what already takes 0.6 us a tile), and both CTAs add
-// the same two fp16 values, so their softmax is the same bit for bit.
+// two score buffers of 64 | Q latent 128 (two elements a column). (The alternatives: a whole score in
+// each CTA costs 1.53 times the MMAs; splitting the rows instead needs every value column twice in
+// shared memory, and those MMAs with both operands there ran at 1319 TFLOP/s alone, 868 with their
+// loads.) The two partial scores are exchanged in fp16 through distributed shared memory (in log2
+// units after scaling: 2^-11 of a partial), and both CTAs add the same two fp16 values, so their
+// softmax is the same bit for bit.
 //
-// Warps (128 + 128 kSets threads): warp 0 loads, warp 1 issues the MMAs, warps 2-3 rest; softmax set i
+// Warps (128 + 128 kSets threads): warp 0 loads, warp 1 issues the scores' MMAs and warp 2 the value
+// products' (two warps that sleep on their own barriers: one that polls both sees either 0.4 us later),
+// warp 3 rests; softmax set i
 // takes the tiles j with j % kSets == i, thread = query row. A tile's way through the softmax (read S,
-// exchange, maximum, exponentials, write P) takes about 3 us of latency and little issue time.
-// A parity wait may only start once the barrier's phase before the awaited one is known to be complete
-// (it would pass at once otherwise). So every barrier that a set waits on for its own tiles is used by
-// that set alone: an exchange slot and a P buffer per set.
+// exchange, maximum, exponentials, write P) is about 3 us of latency with little issue time, so kSets
+// tiles are under way at once, each in a slot of its own: the peer's partial scores arrive in it, row
+// by row in the layout of an MMA operand, and each thread replaces its row by its row of P, from which
+// the value product reads. The MMA that has read it tells the peer that the slot is free.
+// A parity wait may only start once the phase before the awaited one is known to be complete (it would
+// pass at once otherwise), so a barrier that a set waits on for its own tiles belongs to that set.
 #include <cfloat>
 
 #include "mla_internal.cuh"
@@ -46,20 +50,24 @@ using namespace sm100;
 namespace {
 
 constexpr int kTile = 64;                            // positions per tile
-constexpr int kStages = 5;
+constexpr int kStages = 4;
 constexpr int kChunkBytes = kTile * 128;             // 64 rows x 64 latent columns, 128-byte swizzle
 constexpr int kRopeBoxBytes = kTile * 16;            // 64 rows x 8 rope columns, no swizzle
 constexpr int kRopeBytes = 4 * kRopeBoxBytes;
 constexpr int kStageBytes = kRopeBytes + 4 * kChunkBytes;
-constexpr int kXSlots = 2;                           // exchange slots, tile j in slot j & 1
-constexpr int kXBytes = 128 * 128;                   // 128 rows x 64 fp16 partial scores
+constexpr int kXBytes = 128 * 128;                   // a slot: 128 rows x 64 fp16 partial scores, then P
 constexpr int kQRopeBoxBytes = 128 * 16;
 constexpr int kQRopeBytes = 4 * kQRopeBoxBytes;
+constexpr int kXUnit = 128 * 16;                     // 16-byte unit c of row t is at c * kXUnit + t * 16: a warp's stores
+                                                     // fill whole sectors on their way to the peer
 constexpr int kMSlots = 4;
-constexpr int kSets = 2;   // with the two exchange slots and P buffers: each slot belongs to one set
-constexpr int kThreads = 128 + 128 * kSets;
+constexpr int kSets = 2;
+constexpr int kSlots = 4;                            // exchange and P slots, tile j in slot j % kSlots
+constexpr int kSums = 2 * kSlots;                    // row sums handed between the sets, tile j's in j % kSums
+constexpr int kGroupCost = 2;                        // a group's fixed cost, in tiles, for the split
+constexpr int kThreads = 128 + 256 * kSets;
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kColO = 0, kColS = 256, kColQ = 320, kColP = 448;
+constexpr uint32_t kColO = 0, kColS = 256, kColQ = 384;
 constexpr float kRescale = 8.0f;                     // log2 units
 constexpr float kLowest = -1e37f;                    // reference of rows whose scores are all -inf
 
@@ -74,18 +82,19 @@ struct __align__(16) Group {
     int tile0, ptiles;        // first tile, tiles of the prefix
 };
 struct Header {
-    int groups, tiles;
-    int workers;              // that have a tile: no worker between two others is without
+    int groups;
 };
 struct Work {                 // workspace
     int* status;
     Header* head;
     Group* group;
     int* gbase;               // per prefix group: its first row group (num_groups + 1)
+    int* gcost;               // per group: fixed costs of the groups before it
+    int* wtile;               // per worker: its first tile (W + 1)
     int* bad;                 // per group: it met a row outside the cache
-    float4* rec_ml;           // per record row: m, l, 2^-f of o's columns 0..255 and 256..511
+    float* rec_ml;            // per record row 8 floats: m, l, -, -, and 2^-f of each 128 columns of o
     uint16_t* rec_o;          // o 2^f in fp16
-    float2* rowsum;           // per CTA: [2 kSets][128] row sums and references handed between its sets
+    float2* rowsum;           // per CTA: [kSums][2][128] row sums and references handed between its sets
     int W;                    // workers
     int own;                  // groups of single requests, which come first (B * ceil(H / 128))
     int fold;                 // 1: prefix and own rows in one group (128 divides H)
@@ -94,13 +103,6 @@ struct Work {                 // workspace
 __device__ __forceinline__ int code(int site) { return kStatusTimeout | (site << 8); }
 __device__ __forceinline__ bool warp_ok(bool ok) { return __all_sync(0xffffffffu, ok); }
 __device__ __forceinline__ int clampi(int v, int hi) { return v < 0 ? 0 : (v > hi ? hi : v); }
-
-__device__ __forceinline__ int w_begin(int T, int W, int w) {
-    return static_cast<int>(static_cast<long long>(T) * w / W);
-}
-__device__ __forceinline__ int w_of(int T, int W, int t) {
-    return static_cast<int>(((static_cast<long long>(t) + 1) * W - 1) / T);
-}
 
 // Prefix group of request b, or -1: the last one that starts at or before b, if it holds b.
 __device__ __forceinline__ int prefix_of(const PrefixArgs& A, int b) {
@@ -146,11 +148,11 @@ __device__ int block_scan(int v, int* sh, int* carry) {
 }
 
 __global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(const __grid_constant__ PrefixArgs A, const Work wk) {
-    __shared__ int sh[32], carry;
+    __shared__ int sh[32], carry, cost;
     pdl_launch_dependents();
     const int hb = ceil_div(A.H, 128), tid = threadIdx.x;
     if (tid == 0) {
-        carry = 0;
+        carry = cost = 0;
         *wk.status = 0;
     }
     __syncthreads();
@@ -208,11 +210,29 @@ __global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(const __grid_
             wk.bad[g] = 0;
         }
         d.tile0 = block_scan(tiles, sh, &carry);
-        if (g < G) wk.group[g] = d;
+        const int c = block_scan(tiles > 0 ? kGroupCost : 0, sh, &cost);
+        if (g < G) {
+            wk.group[g] = d;
+            wk.gcost[g] = c;
+        }
     }
     if (tid == 0) {
-        *wk.head = {G, carry, min(wk.W, carry)};
+        wk.head->groups = G;
         wk.group[G].tile0 = carry;   // the end of the last group's tiles
+    }
+    __syncthreads();
+    // Worker w begins at w / W of all tiles and fixed costs. A group's cost lies before its tiles; a
+    // share that begins there begins with the group.
+    for (int w = tid; w <= wk.W; w += kPlanThreads) {
+        const long long u = static_cast<long long>(carry + cost) * w / wk.W;
+        int lo = 0, hi = G;   // last group whose cost and tiles begin at or before u
+        while (lo + 1 < hi) {
+            const int mid = (lo + hi) / 2;
+            if (wk.group[mid].tile0 + wk.gcost[mid] <= u) lo = mid; else hi = mid;
+        }
+        const int t0 = wk.group[lo].tile0, t1 = wk.group[lo + 1].tile0;
+        const long long t = u - wk.gcost[lo] - (t1 > t0 ? kGroupCost : 0);
+        wk.wtile[w] = w == wk.W ? carry : static_cast<int>(t < t0 ? t0 : (t > t1 ? t1 : t));
     }
 }
 
@@ -221,20 +241,19 @@ __global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(const __grid_
 struct __align__(8) Barriers {
     uint64_t kv_full[kStages], kv_empty[kStages];
     uint64_t s_full[kSets];           // per set: the score of its next tile is done
-    uint64_t s_free;
-    uint64_t p_full[2], pv_done[2];   // per P buffer (tile parity)
-    uint64_t x_full[kXSlots];         // the peer's partial scores have arrived
-    uint64_t x_empty[kXSlots];        // credit: the peer has read what this CTA sent into that slot
+    uint64_t s_free[2];               // per score buffer (tile parity): it has been read
+    uint64_t x_full[kSlots];          // the peer's partial scores have arrived in the slot
+    uint64_t p_full[kSlots];          // the slot holds P
+    uint64_t pv_done[kSlots];         // the value product has read it
+    uint64_t x_empty[kSlots];         // and so it has in the peer, whose slot may be written again
     uint64_t mref[kMSlots];           // m_pub slot j % kMSlots holds tile j's reference
-    uint64_t lpub[2 * kSets];         // rowsum slot j % (2 kSets) holds tile j's set's sums (near a segment's end)
-    uint64_t q_ready, o_free, drain, done, epi_go;
-    int epi_rec, epi_rows;
-    float epi_f[128];
+    uint64_t lpub[kSums];           // rowsum slot j % kSums holds tile j's set's sums (near a segment's end)
+    uint64_t q_ready, o_free, drain[2], done;
     uint32_t tmem;
 };
 
-constexpr size_t kSmemBytes = static_cast<size_t>(kStages) * kStageBytes + static_cast<size_t>(kXSlots) * kXBytes +
-                              kQRopeBytes + kMSlots * 128 * sizeof(float) + sizeof(Barriers) + 1024;
+constexpr size_t kSmemBytes = static_cast<size_t>(kStages) * kStageBytes + static_cast<size_t>(kSlots) * kXBytes +
+                              kQRopeBytes + (kMSlots + 4 * kSets) * 128 * sizeof(float) + sizeof(Barriers) + 1024;
 static_assert(kSmemBytes <= 232448, "shared memory budget");
 
 // Walks a worker's tiles; every role walks an identical copy. A segment is the worker's run of tiles
@@ -290,6 +309,12 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// volatile: keeps a run of them together
+__device__ __forceinline__ float ex2_ordered(float x) {
+    float y;
+    asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ uint32_t half2_of(float a, float b) {
     __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&h);
@@ -310,12 +335,12 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
-// 2^f that brings this thread's O row (256 TMEM columns) below 2^15, for the fp16 record; 1 for rows
+// 2^f that brings 128 columns of this thread's O row (TMEM) below 2^15, for the fp16 record; 1 for rows
 // of zeros and for infinities and NaN, which go into the record as they are. Warp-collective.
 __device__ __forceinline__ float record_scale(uint32_t tsrc) {
     float top = 0.f;
 #pragma unroll 1
-    for (int c0 = 0; c0 < 256; c0 += 32) {
+    for (int c0 = 0; c0 < 128; c0 += 32) {
         uint32_t o[32];
         tmem_ld32_sync(tsrc + c0, o);
         float mx[4] = {};
@@ -327,10 +352,10 @@ __device__ __forceinline__ float record_scale(uint32_t tsrc) {
     const int e = static_cast<int>(__float_as_uint(top) >> 23);
     return e > 0 && e < 255 ? __uint_as_float(static_cast<uint32_t>(min(max(268 - e, 1), 253)) << 23) : 1.f;
 }
-// ncols columns of this thread's O row (TMEM) times scale to a record row. Warp-collective.
-__device__ __forceinline__ void write_cols(uint32_t tsrc, uint16_t* orow, float scale, bool row_ok, int ncols) {
+// 128 columns of this thread's O row (TMEM) times scale to a record row. Warp-collective.
+__device__ __forceinline__ void write_cols(uint32_t tsrc, uint16_t* orow, float scale, bool row_ok) {
 #pragma unroll 1
-    for (int c0 = 0; c0 < ncols; c0 += 32) {
+    for (int c0 = 0; c0 < 128; c0 += 32) {
         uint32_t o[32];
         tmem_ld32_sync(tsrc + c0, o);
         if (row_ok) {
@@ -356,12 +381,13 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     unsigned char* stages = smem;
     unsigned char* xbuf = stages + kStages * kStageBytes;
-    unsigned char* qrope = xbuf + kXSlots * kXBytes;
+    unsigned char* qrope = xbuf + kSlots * kXBytes;
     float* m_pub = reinterpret_cast<float*>(qrope + kQRopeBytes);              // [kMSlots][128]
-    Barriers* bars = reinterpret_cast<Barriers*>(m_pub + kMSlots * 128);
+    float* x_max = m_pub + kMSlots * 128;                                      // [kSets][2][half][128]
+    Barriers* bars = reinterpret_cast<Barriers*>(x_max + kSets * 4 * 128);
     // the row sums that one set hands to another at a segment's end: in global memory, where shared
     // memory has no room, and only for the segment's last tiles
-    volatile float2* l_pub = wk.rowsum + static_cast<long long>(blockIdx.x) * 2 * kSets * 128;
+    volatile float2* l_pub = wk.rowsum + static_cast<long long>(blockIdx.x) * kSums * 2 * 128;
     const uint32_t rank = cluster_ctarank(), peer = rank ^ 1u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int w = blockIdx.x >> 1;
@@ -376,26 +402,21 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
             mbar_init(smem_u32(&bars->kv_empty[s]), 1);
         }
         for (int i = 0; i < kSets; ++i) mbar_init(smem_u32(&bars->s_full[i]), 1);
-        mbar_init(smem_u32(&bars->s_free), 128);
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(smem_u32(&bars->p_full[b]), 128);
-            mbar_init(smem_u32(&bars->pv_done[b]), 1);
+        for (int i = 0; i < kSlots; ++i) {
+            mbar_init(smem_u32(&bars->x_full[i]), 1);
+            mbar_init(smem_u32(&bars->p_full[i]), 256);
+            mbar_init(smem_u32(&bars->pv_done[i]), 1);
+            mbar_init(smem_u32(&bars->x_empty[i]), 1);
         }
+        for (int b = 0; b < 2; ++b) mbar_init(smem_u32(&bars->s_free[b]), 256);
         for (int i = 0; i < kMSlots; ++i) mbar_init(smem_u32(&bars->mref[i]), 128);
-        for (int i = 0; i < 2 * kSets; ++i) mbar_init(smem_u32(&bars->lpub[i]), 128);
-        for (int s = 0; s < kXSlots; ++s) {
-            mbar_init(smem_u32(&bars->x_full[s]), 1);
-            mbar_init(smem_u32(&bars->x_empty[s]), 4);   // one arrival per warp of the reading set
-        }
-        mbar_init(smem_u32(&bars->q_ready), 128);
-        mbar_init(smem_u32(&bars->o_free), 128);
-        mbar_init(smem_u32(&bars->drain), 1);
+        for (int i = 0; i < kSums; ++i) mbar_init(smem_u32(&bars->lpub[i]), 256);
+        mbar_init(smem_u32(&bars->q_ready), 256);
+        mbar_init(smem_u32(&bars->o_free), 256);
+        mbar_init(smem_u32(&bars->drain[0]), 1);
+        mbar_init(smem_u32(&bars->drain[1]), 1);
         mbar_init(smem_u32(&bars->done), 1);
-        mbar_init(smem_u32(&bars->epi_go), 128);
         fence_mbar_init();
-        // each exchange slot is armed for its first tile here, and for the next one by the set that
-        // has seen it complete
-        for (int s = 0; s < kXSlots; ++s) mbar_arrive_expect_tx(smem_u32(&bars->x_full[s]), kXBytes);
     }
     if (warp == 1) {
         tmem_alloc(smem_u32(&bars->tmem), kTmemCols);
@@ -406,10 +427,9 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
     tc_fence_after();
     const uint32_t tbase = bars->tmem;
     pdl_wait();   // the plan
-    const Header head = *wk.head;
+    const int groups = wk.head->groups;
     // identical in both CTAs of the pair; a pair without tiles goes straight to the teardown
-    const int tb = w < head.workers ? w_begin(head.tiles, head.workers, w) : 0;
-    const int te = w < head.workers ? w_begin(head.tiles, head.workers, w + 1) : 0;
+    const int tb = wk.wtile[w], te = wk.wtile[w + 1];
     const int n = te - tb;
     const uint32_t stages_u32 = smem_u32(stages), xbuf_u32 = smem_u32(xbuf), qrope_u32 = smem_u32(qrope);
 
@@ -417,7 +437,7 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
         if (n > 0 && warp == 0 && lane == 0) {
             // ------------------------------------------------------------ loads
             Tiles it;
-            it.init(wk, head.groups, tb, te);
+            it.init(wk, groups, tb, te);
             int issued = 0;
             for (int i = 0; it.valid(); ++i, it.next(wk)) {
                 const int st = i % kStages;
@@ -444,96 +464,93 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
             // the last loads land before shared memory is released
             for (int i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
                 mbar_wait(smem_u32(&bars->kv_full[i % kStages]), (i / kStages) & 1, err, code(kWaitLoad), 100000000ull);
-        } else if (n > 0 && warp == 1 && lane == 0) {
-            // ------------------------------------------------------------ MMAs
-            constexpr uint32_t idesc_s = idesc_f16(128, kTile, Fmt<T>::v, false, false);
-            constexpr uint32_t idesc_pv = idesc_f16(128, 256, Fmt<T>::v, false, true);
-            const uint32_t tS = tbase + kColS, tQ = tbase + kColQ, tO = tbase + kColO;
+        } else if (n > 0 && warp == 1) {
+            // ------------------------------------------------------------ scores
+            // The whole warp walks the tiles and waits, one elected lane issues. Score i needs its
+            // stage, its buffer read out, and at a segment's start the group's Q.
+            constexpr uint32_t idesc = idesc_f16(128, kTile, Fmt<T>::v, false, false);
+            const uint32_t tQ = tbase + kColQ;
             const uint64_t dqr = smem_desc_noswz(qrope_u32, kQRopeBoxBytes, 128);
-            auto issue_score = [&](int i) {
-                const uint32_t sa = stages_u32 + (i % kStages) * kStageBytes;
-                const uint64_t dl = smem_desc_sw128(sa + kRopeBytes, 16, 1024);
-                mma_ts(tS, tQ, dl, idesc_s, 0u);
-#pragma unroll
-                for (int k = 1; k < 16; ++k)
-                    mma_ts(tS, tQ + 8 * k, dl + static_cast<uint64_t>(((k >> 2) * kChunkBytes + (k & 3) * 32) >> 4), idesc_s, 1u);
-                const uint64_t dr = smem_desc_noswz(sa, kRopeBoxBytes, 128);
-                mma_ss(tS, dqr, dr, idesc_s, 1u);
-                mma_ss(tS, dqr + static_cast<uint64_t>((2 * kQRopeBoxBytes) >> 4),
-                       dr + static_cast<uint64_t>((2 * kRopeBoxBytes) >> 4), idesc_s, 1u);
-                mma_commit(smem_u32(&bars->s_full[i % kSets]));
-            };
-            auto issue_pv = [&](int i, bool first) {
-                const uint64_t dc = smem_desc_sw128(stages_u32 + (i % kStages) * kStageBytes + kRopeBytes, kChunkBytes, 1024);
-                const uint32_t tP = tbase + kColP + 32 * (i & 1);
-                mma_ts(tO, tP, dc, idesc_pv, first ? 0u : 1u);
-#pragma unroll
-                for (int k = 1; k < kTile / 16; ++k)
-                    mma_ts(tO, tP + 8 * k, dc + static_cast<uint64_t>((2048 * k) >> 4), idesc_pv, 1u);
-                mma_commit(smem_u32(&bars->pv_done[i & 1]));
-                mma_commit(smem_u32(&bars->kv_empty[i % kStages]));
-            };
-            // Scores and value products go in tile order each, whichever is ready first: score(s) needs
-            // S read out, its stage, and at a segment's start the group's Q; PV(v) needs P(v) and at a
-            // segment's start the O of the one before read out.
-            Tiles its, itv;
-            its.init(wk, head.groups, tb, te);
-            itv = its;
-            int next_s = 0, next_v = 0, qseg = 0, vseg = 0;
+            Tiles it;
+            it.init(wk, groups, tb, te);
+            int seg = 0;
             bool ok = true;
-            long long t_last = clock64();
-            const long long budget = wait_budget_cycles(kDefaultWaitNs);
-            for (uint32_t spin = 0; ok && next_v < n; ++spin) {
-                bool progressed = false;
-                if (next_s < n && (next_s == 0 || mbar_test(smem_u32(&bars->s_free), (next_s - 1) & 1)) &&
-                    mbar_test(smem_u32(&bars->kv_full[next_s % kStages]), (next_s / kStages) & 1) &&
-                    (!its.seg_first() || mbar_test(smem_u32(&bars->q_ready), qseg & 1))) {
-                    tc_fence_after();
-                    issue_score(next_s);
-                    if (its.seg_last()) ++qseg;
-                    its.next(wk);
-                    ++next_s;
-                    progressed = true;
+            for (int i = 0; it.valid(); ++i, it.next(wk)) {
+                ok = mbar_wait(smem_u32(&bars->kv_full[i % kStages]), (i / kStages) & 1, err, code(kWaitMma)) &&
+                     (i < 2 || mbar_wait(smem_u32(&bars->s_free[i & 1]), ((i >> 1) - 1) & 1, err, code(kWaitMma))) &&
+                     (!it.seg_first() || mbar_wait(smem_u32(&bars->q_ready), seg & 1, err, code(kWaitMma)));
+                if (!warp_ok(ok)) break;
+                if (it.seg_first()) ++seg;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t sa = stages_u32 + (i % kStages) * kStageBytes;
+                    const uint64_t dl = smem_desc_sw128(sa + kRopeBytes, 16, 1024);
+                    const uint32_t tS = tbase + kColS + 64 * (i & 1);
+                    mma_ts(tS, tQ, dl, idesc, 0u);
+#pragma unroll
+                    for (int k = 1; k < 16; ++k)
+                        mma_ts(tS, tQ + 8 * k, dl + static_cast<uint64_t>(((k >> 2) * kChunkBytes + (k & 3) * 32) >> 4), idesc, 1u);
+                    const uint64_t dr = smem_desc_noswz(sa, kRopeBoxBytes, 128);
+                    mma_ss(tS, dqr, dr, idesc, 1u);
+                    mma_ss(tS, dqr + static_cast<uint64_t>((2 * kQRopeBoxBytes) >> 4),
+                           dr + static_cast<uint64_t>((2 * kRopeBoxBytes) >> 4), idesc, 1u);
+                    mma_commit(smem_u32(&bars->s_full[i % kSets]));
                 }
-                if (next_v < next_s && mbar_test(smem_u32(&bars->p_full[next_v & 1]), (next_v >> 1) & 1) &&
-                    (!itv.seg_first() || vseg == 0 || mbar_test(smem_u32(&bars->o_free), (vseg - 1) & 1))) {
-                    tc_fence_after();
-                    issue_pv(next_v, itv.seg_first());
-                    if (itv.seg_last()) ++vseg;
-                    itv.next(wk);
-                    ++next_v;
-                    progressed = true;
-                }
-                if (progressed) {
-                    t_last = clock64();
-                    continue;
-                }
-                if ((spin & 31u) == 0u) {
-                    const long long dt = clock64() - t_last;
-                    if ((dt > kErrPollCycles && *err != 0) || dt > budget) {
-                        atomicCAS(const_cast<int*>(err), 0, code(kWaitMma));
-                        ok = false;
-                    }
-                }
+                __syncwarp();
             }
-            mma_commit(smem_u32(&bars->drain));   // every MMA is done before the teardown
-            mbar_wait(smem_u32(&bars->drain), 0, err, code(kWaitDrain));
+            // every MMA is done before the teardown
+            if (elect_one()) mma_commit(smem_u32(&bars->drain[0]));
+            __syncwarp();
+            mbar_wait(smem_u32(&bars->drain[0]), 0, err, code(kWaitDrain));
+        } else if (n > 0 && warp == 2) {
+            // ------------------------------------------------------------ value products
+            // Product i needs P(i), and at a segment's start the O of the one before read out.
+            constexpr uint32_t idesc = idesc_f16(128, 256, Fmt<T>::v, false, true);
+            const uint32_t tO = tbase + kColO;
+            Tiles it;
+            it.init(wk, groups, tb, te);
+            int seg = 0;
+            bool ok = true;
+            for (int i = 0; it.valid(); ++i, it.next(wk)) {
+                ok = mbar_wait(smem_u32(&bars->p_full[i % kSlots]), (i / kSlots) & 1, err, code(kWaitMma)) &&
+                     (!it.seg_first() || seg == 0 || mbar_wait(smem_u32(&bars->o_free), (seg - 1) & 1, err, code(kWaitMma)));
+                if (!warp_ok(ok)) break;
+                if (it.seg_first()) ++seg;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t dc = smem_desc_sw128(stages_u32 + (i % kStages) * kStageBytes + kRopeBytes, kChunkBytes, 1024);
+                    const uint64_t dp = smem_desc_noswz(xbuf_u32 + (i % kSlots) * kXBytes, kXUnit, 128);
+                    mma_ss(tO, dp, dc, idesc, it.seg_first() ? 0u : 1u);
+#pragma unroll
+                    for (int k = 1; k < kTile / 16; ++k)
+                        mma_ss(tO, dp + static_cast<uint64_t>((2 * kXUnit * k) >> 4), dc + static_cast<uint64_t>((2048 * k) >> 4), idesc, 1u);
+                    mma_commit(smem_u32(&bars->kv_empty[i % kStages]));
+                    mma_commit(smem_u32(&bars->pv_done[i % kSlots]));
+                    // the peer awaits this for tile i + kSlots; for the last tiles nobody does, and the peer
+                    // may be gone when it arrives
+                    if (i + kSlots < n) mma_commit_to(smem_u32(&bars->x_empty[i % kSlots]), static_cast<uint16_t>(1u << peer));
+                }
+                __syncwarp();
+            }
+            if (elect_one()) mma_commit(smem_u32(&bars->drain[1]));
+            __syncwarp();
+            mbar_wait(smem_u32(&bars->drain[1]), 0, err, code(kWaitDrain));
         }
     } else {
         // ---------------------------------------------------------------- softmax sets
-        const int sid = (warp - 4) >> 2;
-        const int t = (warp & 3) * 32 + lane;             // query row == TMEM lane
+        const int sid = (warp - 4) >> 3, hf = ((warp - 4) >> 2) & 1;
+        const int t = (warp & 3) * 32 + lane;             // query row == TMEM lane; columns 32 hf .. 32 hf + 31 of S
         const uint32_t trow = tbase + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
-        const uint32_t x_local = xbuf_u32 + t * 16;       // 16-byte unit c of row t at c * 2048 + t * 16
-        const uint32_t x_remote = mapa(x_local, peer);
         const float qscale = A.scale * 1.4426950408889634f;
+        // Q of a group: this thread's half of its row's CTA columns into TMEM (two elements a column) and
+        // two of the four rope boxes
         auto load_q = [&](const Group& d) {
             const long long row = d.q_row0 + t;
-            const uint4* lat = reinterpret_cast<const uint4*>(static_cast<const T*>(A.qa) + row * 512 + 256 * rank);
-            const uint4* rope = reinterpret_cast<const uint4*>(static_cast<const T*>(A.qr) + row * 64 + 32 * rank);
+            const uint4* lat = reinterpret_cast<const uint4*>(static_cast<const T*>(A.qa) + row * 512 + 256 * rank + 128 * hf);
+            const uint4* rope = reinterpret_cast<const uint4*>(static_cast<const T*>(A.qr) + row * 64 + 32 * rank + 16 * hf);
             const bool have = t < d.rows;
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < 2; ++c) {
                 uint4 v[8], r;
 #pragma unroll
                 for (int k = 0; k < 8; ++k) v[k] = have ? __ldg(lat + 8 * c + k) : make_uint4(0, 0, 0, 0);
@@ -544,9 +561,9 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
                                             v[4 * q + 1].x, v[4 * q + 1].y, v[4 * q + 1].z, v[4 * q + 1].w,
                                             v[4 * q + 2].x, v[4 * q + 2].y, v[4 * q + 2].z, v[4 * q + 2].w,
                                             v[4 * q + 3].x, v[4 * q + 3].y, v[4 * q + 3].z, v[4 * q + 3].w};
-                    tmem_st16(trow + kColQ + 32 * c + 16 * q, x);
+                    tmem_st16(trow + kColQ + 64 * hf + 32 * c + 16 * q, x);
                 }
-                *reinterpret_cast<uint4*>(qrope + c * kQRopeBoxBytes + t * 16) = r;
+                *reinterpret_cast<uint4*>(qrope + (2 * hf + c) * kQRopeBoxBytes + t * 16) = r;
             }
             fence_proxy_async_smem();
             tmem_st_wait();
@@ -556,42 +573,41 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
         Tiles it;
         bool ok = true;
         if (n > 0) {
-            it.init(wk, head.groups, tb, te);
+            it.init(wk, groups, tb, te);
             if (sid == 0) load_q(it.d);   // the first tile belongs to set 0
             it.skip(wk, sid);
         } else {
             it.t = it.t_end = 0;
         }
-        float l_self = 0.f, m_l = 0.f;    // this set's row sum over its tiles of the segment, and its reference
+        float l_self = 0.f, m_l = 0.f;    // sum over this thread's columns of the set's tiles of the segment, and its reference
         for (int j = sid; ok && it.valid(); j += kSets, it.skip(wk, kSets)) {
-            const int slot = j % kXSlots;
-            const int np = it.np();
+            const int slot = j % kSlots, np = it.np();
+            const uint32_t phase = (j / kSlots) & 1;
+            const uint32_t x_row = xbuf_u32 + slot * kXBytes + 4 * hf * kXUnit + t * 16;
+            const uint32_t x_full = smem_u32(&bars->x_full[slot]);
             // ---- S_r(j) to registers, release S, send the fp16 partial
             bool got = mbar_wait(smem_u32(&bars->s_full[sid]), (j / kSets) & 1, err, code(kWaitS));
             if (!warp_ok(got)) break;
+            if (t == 0 && hf == 0) mbar_arrive_expect_tx(x_full, kXBytes);
             tc_fence_after();
-            uint32_t h[32];
+            uint32_t h[16];
             {
                 uint32_t sr[32];
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    tmem_ld32_sync(trow + kColS + 32 * half, sr);
-#pragma unroll
-                    for (int q = 0; q < 16; ++q)
-                        h[16 * half + q] = half2_of(__uint_as_float(sr[2 * q]) * qscale, __uint_as_float(sr[2 * q + 1]) * qscale);
-                }
+                tmem_ld32_sync(trow + kColS + 64 * (j & 1) + 32 * hf, sr);
                 tc_fence_before();
-                mbar_arrive(smem_u32(&bars->s_free));
+                mbar_arrive(smem_u32(&bars->s_free[j & 1]));
+#pragma unroll
+                for (int q = 0; q < 16; ++q)
+                    h[q] = half2_of(__uint_as_float(sr[2 * q]) * qscale, __uint_as_float(sr[2 * q + 1]) * qscale);
             }
-            // the peer has read its slot's tile j - 2
-            got = j < kXSlots || mbar_wait_cluster(smem_u32(&bars->x_empty[slot]), ((j / kXSlots) - 1) & 1, err, code(kWaitCredit));
+            // the peer's value product of tile j - kSlots has read its slot
+            got = j < kSlots || mbar_wait_cluster(smem_u32(&bars->x_empty[slot]), phase ^ 1, err, code(kWaitCredit));
             if (!warp_ok(got)) break;
             {
-                const uint32_t rbar = mapa(smem_u32(&bars->x_full[slot]), peer);
-                const uint32_t dst = x_remote + slot * kXBytes;
+                const uint32_t dst = mapa(x_row, peer), bar = mapa(x_full, peer);
 #pragma unroll
-                for (int c = 0; c < 8; ++c)
-                    st_async_v4(dst + c * 2048, h[4 * c], h[4 * c + 1], h[4 * c + 2], h[4 * c + 3], rbar);
+                for (int c = 0; c < 4; ++c)
+                    st_async_v4(dst + c * kXUnit, h[4 * c], h[4 * c + 1], h[4 * c + 2], h[4 * c + 3], bar);
             }
             if (it.seg_last() && it.t + 1 < te) {
                 // the score of tile j was the last MMA to read this group's Q
@@ -603,46 +619,49 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
                 // rows past the end: their weights are zero, but zero times what lies there need not be
                 unsigned char* sp = stages + (j % kStages) * kStageBytes + kRopeBytes;
                 const int units = (kTile - np) * 8;
-                for (int v = t; v < 4 * units; v += 128)
+                for (int v = 128 * hf + t; v < 4 * units; v += 256)
                     *reinterpret_cast<uint4*>(sp + (v / units) * kChunkBytes + (np + (v % units) / 8) * 128 + (v % 8) * 16) =
                         make_uint4(0, 0, 0, 0);
                 fence_proxy_async_smem();
             }
-            // ---- the whole score, its reference, P into TMEM buffer j & 1
-            got = mbar_wait_cluster(smem_u32(&bars->x_full[slot]), (j / kXSlots) & 1, err, code(kWaitX));
+            // ---- the whole score, its reference, P into the slot. That the peer's scores are here also says
+            // that this CTA's value product of tile j - kSlots is done (the peer waited for it).
+            got = mbar_wait_cluster(x_full, phase, err, code(kWaitX));
             if (!warp_ok(got)) break;
-            if (t == 0) mbar_arrive_expect_tx(smem_u32(&bars->x_full[slot]), kXBytes);   // for tile j + 2
-            float s[64];
+            // (stage by stage over all columns: the warp issues in order, so column by column it would wait
+            // for every step of every chain)
+            float s[32];
+            uint32_t pv[16];
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                uint4 v;
+            for (int c = 0; c < 4; ++c)
                 asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                             : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                             : "r"(x_local + slot * kXBytes + c * 2048));
-                const uint32_t pv[4] = {v.x, v.y, v.z, v.w};
+                             : "=r"(pv[4 * c]), "=r"(pv[4 * c + 1]), "=r"(pv[4 * c + 2]), "=r"(pv[4 * c + 3])
+                             : "r"(x_row + c * kXUnit));
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const float2 r = add2(floats_of(h[4 * c + q]), floats_of(pv[q]));
-                    s[8 * c + 2 * q] = r.x;
-                    s[8 * c + 2 * q + 1] = r.y;
-                }
+            for (int q = 0; q < 16; ++q) {
+                const float2 r = add2(floats_of(h[q]), floats_of(pv[q]));
+                s[2 * q] = r.x;
+                s[2 * q + 1] = r.y;
             }
-            // credit for the peer, relaxed: it only has to follow the reads above
-            __syncwarp();
-            if (lane == 0) mbar_arrive_remote_relaxed(mapa(smem_u32(&bars->x_empty[slot]), peer));
             if (np < kTile) {
 #pragma unroll
-                for (int k = 0; k < kTile; ++k)
-                    if (k >= np) s[k] = -INFINITY;
+                for (int k = 0; k < 32; ++k)
+                    if (32 * hf + k >= np) s[k] = -INFINITY;
             }
-            float mx[32];
+            float mx[8];
 #pragma unroll
-            for (int k = 0; k < 32; ++k) mx[k] = fmaxf(s[k], s[k + 32]);
+            for (int k = 0; k < 8; ++k) mx[k] = fmaxf(fmaxf(s[k], s[k + 8]), fmaxf(s[k + 16], s[k + 24]));
 #pragma unroll
-            for (int w2 = 16; w2 > 0; w2 >>= 1)
+            for (int w2 = 4; w2 > 0; w2 >>= 1)
 #pragma unroll
                 for (int k = 0; k < w2; ++k) mx[k] = fmaxf(mx[k], mx[k + w2]);
-            const float mt = fmaxf(mx[0], kLowest);
+            // the other half of the row's columns is in the warp that shares this one's TMEM lanes
+            // (slot (j / kSets) & 1 is written again for tile j + 4, after x_full of that tile and hence after
+            // P(j) of every thread here)
+            float* xm = x_max + (sid * 2 + ((j / kSets) & 1)) * 2 * 128;
+            xm[hf * 128 + t] = mx[0];
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + 4 * sid + (warp & 3)) : "memory");
+            const float mt = fmaxf(fmaxf(mx[0], xm[(hf ^ 1) * 128 + t]), kLowest);
             // the reference of the tile before, unless this one exceeds it by more than the threshold
             float m = mt, alpha = 1.f;
             bool need = false;
@@ -657,16 +676,48 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
                     m = m_prev;
                 }
             }
-            m_pub[(j % kMSlots) * 128 + t] = m;
-            mbar_arrive(smem_u32(&bars->mref[j % kMSlots]));
-            uint32_t pp[32];
-            float2 ls[4];
+            if (hf == 0) {
+                m_pub[(j % kMSlots) * 128 + t] = m;
+                mbar_arrive(smem_u32(&bars->mref[j % kMSlots]));
+            }
+            uint32_t pp[16];
             const float2 m2 = make_float2(-m, -m);
 #pragma unroll
-            for (int q = 0; q < 32; ++q) {
+            for (int q = 0; q < 16; ++q) {
                 const float2 d = add2(make_float2(s[2 * q], s[2 * q + 1]), m2);
-                const float2 e = make_float2(ex2(d.x), ex2(d.y));
-                pp[q] = pair_of<T>(e.x, e.y);
+                s[2 * q] = d.x;
+                s[2 * q + 1] = d.y;
+            }
+#pragma unroll
+            for (int q = 0; q < 32; ++q) s[q] = ex2_ordered(s[q]);
+#pragma unroll
+            for (int q = 0; q < 16; ++q) pp[q] = pair_of<T>(s[2 * q], s[2 * q + 1]);
+            if (__any_sync(0xffffffffu, need)) {
+                // the reference moved: rescale O (alpha = 1 elsewhere) once PV(j - 1) is done
+                got = mbar_wait(smem_u32(&bars->pv_done[(j - 1) % kSlots]), ((j - 1) / kSlots) & 1, err, code(kWaitPV));
+                if (!warp_ok(got)) break;
+                tc_fence_after();
+#pragma unroll 1
+                for (int c0 = 0; c0 < 128; c0 += 32) {
+                    uint32_t o[32];
+                    tmem_ld32_sync(trow + kColO + 128 * hf + c0, o);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+                    tmem_st32(trow + kColO + 128 * hf + c0, o);
+                }
+                tmem_st_wait();
+                tc_fence_before();
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(x_row + c * kXUnit),
+                             "r"(pp[4 * c]), "r"(pp[4 * c + 1]), "r"(pp[4 * c + 2]), "r"(pp[4 * c + 3])
+                             : "memory");
+            fence_proxy_async_smem();
+            mbar_arrive(smem_u32(&bars->p_full[slot]));
+            float2 ls[4];
+#pragma unroll
+            for (int q = 0; q < 16; ++q) {
                 const float2 p = ElemTraits<T>::to_f2(*reinterpret_cast<const typename ElemTraits<T>::T2*>(&pp[q]));
                 ls[q & 3] = q < 4 ? p : add2(ls[q & 3], p);
             }
@@ -675,81 +726,39 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
             else if (m != m_l) l_self *= ex2(m_l - m);
             m_l = m;
             l_self += ls[0].x + ls[0].y;
-            // P buffer j & 1 is free once PV(j - 2) is done
-            got = j < 2 || mbar_wait(smem_u32(&bars->pv_done[j & 1]), ((j - 2) >> 1) & 1, err, code(kWaitPV));
-            if (!warp_ok(got)) break;
-            if (__any_sync(0xffffffffu, need)) {
-                // the reference moved: rescale O (alpha = 1 elsewhere) once PV(j - 1) is done
-                got = mbar_wait(smem_u32(&bars->pv_done[(j - 1) & 1]), ((j - 1) >> 1) & 1, err, code(kWaitPV));
-                if (!warp_ok(got)) break;
-                tc_fence_after();
-#pragma unroll 1
-                for (int c0 = 0; c0 < 256; c0 += 32) {
-                    uint32_t o[32];
-                    tmem_ld32_sync(trow + kColO + c0, o);
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-                    tmem_st32(trow + kColO + c0, o);
-                }
-            }
-            tc_fence_after();
-            tmem_st32(trow + kColP + 32 * (j & 1), pp);
-            tmem_st_wait();
-            tc_fence_before();
-            mbar_arrive(smem_u32(&bars->p_full[j & 1]));
             if (it.t + kSets >= min(te, it.gend)) {
-                volatile float2* lp = l_pub + (j % (2 * kSets)) * 128 + t;
+                volatile float2* lp = l_pub + ((j % kSums) * 2 + hf) * 128 + t;
                 lp->x = l_self;
                 lp->y = m;
             }
-            mbar_arrive(smem_u32(&bars->lpub[j % (2 * kSets)]));
+            mbar_arrive(smem_u32(&bars->lpub[j % kSums]));
 
             if (it.seg_last()) {
-                // ---- the segment's partial record
-                got = mbar_wait(smem_u32(&bars->pv_done[j & 1]), (j >> 1) & 1, err, code(kWaitPV));
-                float l_tot = l_self;
+                // ---- the segment's partial record: this thread's 128 columns of the CTA's 256
+                got = mbar_wait(smem_u32(&bars->pv_done[slot]), phase, err, code(kWaitPV));
+                float l_tot = 0.f;
 #pragma unroll
-                for (int i = 1; i < kSets; ++i)
+                for (int i = 0; i < kSets; ++i)
                     if (it.seg_tile() >= i) {
-                        // the set of tile j - i: its sum over the segment ends there
+                        // the set of tile j - i: its sums over the segment end there
                         const int js = j - i;
-                        got = got && mbar_wait(smem_u32(&bars->lpub[js % (2 * kSets)]), (js / (2 * kSets)) & 1, err, code(kWaitRef));
-                        const volatile float2* lp = l_pub + (js % (2 * kSets)) * 128 + t;
-                        l_tot += lp->x * ex2(lp->y - m);
+                        got = got && mbar_wait(smem_u32(&bars->lpub[js % kSums]), (js / kSums) & 1, err, code(kWaitRef));
+                        const volatile float2* lp = l_pub + (js % kSums) * 2 * 128 + t;
+                        l_tot += (lp->x + lp[128].x) * ex2(lp->y - m);
                     }
                 if (!warp_ok(got)) break;
                 tc_fence_after();
-                const int rec = it.g + w, rows = it.d.rows;
-                // the worker's last tile: an idle set writes half of the columns
-                const bool help = j == n - 1;
-                const float f = record_scale(trow + kColO);
-                if (help) {
-                    if (t == 0) {
-                        bars->epi_rec = rec;
-                        bars->epi_rows = rows;
-                    }
-                    bars->epi_f[t] = f;
-                    tc_fence_before();
-                    mbar_arrive(smem_u32(&bars->epi_go));
-                }
-                const long long at = static_cast<long long>(rec) * 128 + t;
-                write_cols(trow + kColO, wk.rec_o + at * 512 + 256 * rank, f, t < rows, help ? 128 : 256);
-                if (t < rows) {
-                    float* ml = reinterpret_cast<float*>(wk.rec_ml + at);
-                    if (rank == 0) *reinterpret_cast<float2*>(ml) = make_float2(m, l_tot);
-                    ml[2 + rank] = 1.f / f;
+                const long long at = static_cast<long long>(it.g + w) * 128 + t;
+                const bool row_ok = t < it.d.rows;
+                const float f = record_scale(trow + kColO + 128 * hf);
+                write_cols(trow + kColO + 128 * hf, wk.rec_o + at * 512 + 256 * rank + 128 * hf, f, row_ok);
+                if (row_ok) {
+                    float* ml = wk.rec_ml + at * 8;
+                    if (rank == 0 && hf == 0) *reinterpret_cast<float2*>(ml) = make_float2(m, l_tot);
+                    ml[4 + 2 * rank + hf] = 1.f / f;
                 }
                 tc_fence_before();
                 mbar_arrive(smem_u32(&bars->o_free));
-            }
-        }
-        if (n > 0 && sid == n % kSets) {
-            // the set after the last tile's: columns 128 .. 255 of its record
-            const bool got = mbar_wait(smem_u32(&bars->epi_go), 0, err, code(kWaitEpi));
-            if (warp_ok(got)) {
-                tc_fence_after();
-                write_cols(trow + kColO + 128, wk.rec_o + (static_cast<long long>(bars->epi_rec) * 128 + t) * 512 + 256 * rank + 128,
-                           bars->epi_f[t], t < bars->epi_rows, 128);
             }
         }
     }
@@ -775,6 +784,7 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
 // ------------------------------------------------------------------------------------- merge
 
 constexpr int kMergeWarps = 8;
+constexpr int kMaxWorkers = 128;
 
 // One output row per `kWarps` warps: each takes every kWarps-th record of the row's groups, keeping
 // the running maximum, sum and weighted latent in fp32; the warps meet in shared memory.
@@ -786,7 +796,10 @@ __global__ void __launch_bounds__(32 * kMergeWarps) prefix_merge_kernel(const __
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     const int sub = warp % kWarps;
     const int f = blockIdx.x * kRows + warp / kWarps;
+    __shared__ int sh_w[kMaxWorkers + 1];
     pdl_wait();
+    for (int w = threadIdx.x; w <= wk.W; w += 32 * kMergeWarps) sh_w[w] = wk.wtile[w];
+    __syncthreads();
     const bool live = f < A.B * A.H;
     float m = -INFINITY, l = 0.f;
     float o[16];
@@ -795,7 +808,6 @@ __global__ void __launch_bounds__(32 * kMergeWarps) prefix_merge_kernel(const __
     bool bad = false;
     if (live) {
         const int b = f / A.H, h = f % A.H;
-        const int T_all = wk.head->tiles, W = wk.head->workers;
         bad = *wk.status != 0;
         // the row's groups: its request's, and unless that holds the prefix too, its prefix group's
         for (int k = 0; k < (wk.fold ? 1 : 2); ++k) {
@@ -813,26 +825,36 @@ __global__ void __launch_bounds__(32 * kMergeWarps) prefix_merge_kernel(const __
             const int t0 = wk.group[g].tile0, t1 = wk.group[g + 1].tile0;
             if (t1 <= t0) continue;
             bad = bad || wk.bad[g] != 0;
-            const int w0 = w_of(T_all, W, t0), w1 = w_of(T_all, W, t1 - 1);
+            int w0 = 0, w1 = wk.W;   // workers of the group's tiles; one between them may have none
+            for (int hi = wk.W; w0 + 1 < hi;) {
+                const int mid = (w0 + hi) / 2;
+                if (sh_w[mid] <= t0) w0 = mid; else hi = mid;
+            }
+            for (int lo = w0; lo + 1 < w1;) {
+                const int mid = (lo + w1) / 2;
+                if (sh_w[mid] < t1) lo = mid; else w1 = mid;
+            }
+            --w1;
             constexpr int kAhead = 4;
             for (int w = w0 + sub; w <= w1; w += kWarps * kAhead) {
                 uint4 v[kAhead][2];
-                float4 ml[kAhead];
+                float2 ml[kAhead], fs[kAhead];
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i)
-                    if (w + i * kWarps <= w1) {
+                    if (w + i * kWarps <= w1 && sh_w[w + i * kWarps] < sh_w[w + i * kWarps + 1]) {
                         const long long at = static_cast<long long>(g + w + i * kWarps) * 128 + r;
-                        ml[i] = wk.rec_ml[at];
+                        ml[i] = *reinterpret_cast<const float2*>(wk.rec_ml + at * 8);
+                        fs[i] = make_float2(wk.rec_ml[at * 8 + 4 + lane / 16], wk.rec_ml[at * 8 + 6 + lane / 16]);
                         const uint4* src = reinterpret_cast<const uint4*>(wk.rec_o + at * 512);
                         v[i][0] = src[lane];
                         v[i][1] = src[32 + lane];
                     }
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i)
-                    if (w + i * kWarps <= w1) {
+                    if (w + i * kWarps <= w1 && sh_w[w + i * kWarps] < sh_w[w + i * kWarps + 1]) {
                         const float top = fmaxf(m, ml[i].x);
                         const float a = ex2(m - top), e0 = ex2(ml[i].x - top);
-                        const float c2[2] = {e0 * ml[i].z, e0 * ml[i].w};
+                        const float c2[2] = {e0 * fs[i].x, e0 * fs[i].y};
                         m = top;
                         l = l * a + e0 * ml[i].y;
 #pragma unroll
@@ -890,7 +912,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) prefix_merge_kernel(const __
 
 struct Layout {
     long long groups;     // most groups
-    size_t off_head, off_group, off_base, off_bad, off_sum, off_ml, off_o, total;
+    size_t off_head, off_group, off_base, off_cost, off_wtile, off_bad, off_sum, off_ml, off_o, total;
     int W, own, fold;
 };
 
@@ -901,15 +923,18 @@ Layout layout(const PrefixArgs& A, int sms) {
     // rows of a prefix group end inside a tile at most once a group
     L.groups = L.own + (L.fold ? 0 : static_cast<long long>(A.B) * A.H / 128 + (A.P < A.B ? A.P : A.B));
     L.W = sms / 2 > 0 ? sms / 2 : 1;
+    if (L.W > kMaxWorkers) L.W = kMaxWorkers;
     auto a256 = [](size_t x) { return (x + 255) / 256 * 256; };
     size_t off = 256;     // status
     L.off_head = off; off += 256;
     L.off_group = off; off = a256(off + sizeof(Group) * static_cast<size_t>(L.groups + 1));
     L.off_base = off; off = a256(off + sizeof(int) * (static_cast<size_t>(A.P) + 1));
+    L.off_cost = off; off = a256(off + sizeof(int) * static_cast<size_t>(L.groups));
+    L.off_wtile = off; off = a256(off + sizeof(int) * (L.W + 1));
     L.off_bad = off; off = a256(off + sizeof(int) * static_cast<size_t>(L.groups));
-    L.off_sum = off; off = a256(off + sizeof(float2) * 2 * L.W * 2 * kSets * 128);
+    L.off_sum = off; off = a256(off + sizeof(float2) * 2 * L.W * kSums * 2 * 128);
     const size_t recs = static_cast<size_t>(L.groups) + L.W;
-    L.off_ml = off; off = a256(off + recs * 128 * sizeof(float4));
+    L.off_ml = off; off = a256(off + recs * 128 * 8 * sizeof(float));
     L.off_o = off; off = a256(off + recs * 128 * 512 * 2);
     L.total = off;
     return L;
@@ -923,8 +948,10 @@ cudaError_t launch(const PrefixArgs& A, unsigned char* ws, int sms, cudaStream_t
     wk.head = reinterpret_cast<Header*>(ws + L.off_head);
     wk.group = reinterpret_cast<Group*>(ws + L.off_group);
     wk.gbase = reinterpret_cast<int*>(ws + L.off_base);
+    wk.gcost = reinterpret_cast<int*>(ws + L.off_cost);
+    wk.wtile = reinterpret_cast<int*>(ws + L.off_wtile);
     wk.bad = reinterpret_cast<int*>(ws + L.off_bad);
-    wk.rec_ml = reinterpret_cast<float4*>(ws + L.off_ml);
+    wk.rec_ml = reinterpret_cast<float*>(ws + L.off_ml);
     wk.rec_o = reinterpret_cast<uint16_t*>(ws + L.off_o);
     wk.rowsum = reinterpret_cast<float2*>(ws + L.off_sum);
     wk.W = L.W;
