@@ -352,6 +352,20 @@ __device__ __forceinline__ float record_scale(uint32_t tsrc) {
     const int e = static_cast<int>(__float_as_uint(top) >> 23);
     return e > 0 && e < 255 ? __uint_as_float(static_cast<uint32_t>(min(max(268 - e, 1), 253)) << 23) : 1.f;
 }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+        "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+// the largest of three (a NaN only if all are)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // 128 columns of this thread's O row (TMEM) times scale to a record row. Warp-collective.
 __device__ __forceinline__ void write_cols(uint32_t tsrc, uint16_t* orow, float scale, bool row_ok) {
 #pragma unroll 1
@@ -597,8 +611,11 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
                 tc_fence_before();
                 mbar_arrive(smem_u32(&bars->s_free[j & 1]));
 #pragma unroll
-                for (int q = 0; q < 16; ++q)
-                    h[q] = half2_of(__uint_as_float(sr[2 * q]) * qscale, __uint_as_float(sr[2 * q + 1]) * qscale);
+                for (int q = 0; q < 16; ++q) {
+                    const float2 v = mul2(make_float2(__uint_as_float(sr[2 * q]), __uint_as_float(sr[2 * q + 1])),
+                                          make_float2(qscale, qscale));
+                    h[q] = half2_of(v.x, v.y);
+                }
             }
             // the peer's value product of tile j - kSlots has read its slot
             got = j < kSlots || mbar_wait_cluster(smem_u32(&bars->x_empty[slot]), phase ^ 1, err, code(kWaitCredit));
@@ -648,13 +665,13 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
                 for (int k = 0; k < 32; ++k)
                     if (32 * hf + k >= np) s[k] = -INFINITY;
             }
-            float mx[8];
+            float mx[11];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) mx[k] = fmaxf(fmaxf(s[k], s[k + 8]), fmaxf(s[k + 16], s[k + 24]));
+            for (int k = 0; k < 10; ++k) mx[k] = max3(s[3 * k], s[3 * k + 1], s[3 * k + 2]);
+            mx[10] = fmaxf(s[30], s[31]);
 #pragma unroll
-            for (int w2 = 4; w2 > 0; w2 >>= 1)
-#pragma unroll
-                for (int k = 0; k < w2; ++k) mx[k] = fmaxf(mx[k], mx[k + w2]);
+            for (int k = 0; k < 3; ++k) mx[k] = max3(mx[3 * k], mx[3 * k + 1], mx[3 * k + 2]);
+            mx[0] = fmaxf(max3(mx[0], mx[1], mx[2]), fmaxf(mx[9], mx[10]));
             // the other half of the row's columns is in the warp that shares this one's TMEM lanes
             // (slot (j / kSets) & 1 is written again for tile j + 4, after x_full of that tile and hence after
             // P(j) of every thread here)
