@@ -74,29 +74,37 @@ constexpr float kLowest = -1e37f;                    // reference of rows whose 
 enum : int { kWaitLoad = 1, kWaitMma = 3, kWaitS = 7, kWaitX = 8, kWaitPV = 9, kWaitTeardown = 10, kWaitDrain = 11,
              kWaitRef = 12, kWaitCredit = 13, kWaitEpi = 14 };
 
-// A group of query rows and what it attends to.
+// A group of query rows with something to attend to.
 struct __align__(16) Group {
     int q_row0, rows;         // flattened (request, head) rows
     int pid, sid;             // prefix group and request whose rows it attends to (-1: none)
     int plen, slen;
     int tile0, ptiles;        // first tile, tiles of the prefix
+    int tile1, pad[3];        // end of its tiles
 };
-struct Header {
-    int groups;
+// What a worker starts with.
+struct __align__(16) Start {
+    int tb, te;               // its tiles
+    int g, pad;               // the first one's group, and that group
+    Group d;
+};
+// Where a row finds its records: group + worker for the workers w0 .. w1 (none: w0 > w1).
+struct __align__(16) Pieces {
+    int g, w0, w1, pad;
 };
 struct Work {                 // workspace
     int* status;
-    Header* head;
-    Group* group;
+    Group* group;             // groups with tiles, in order
+    Start* start;             // per worker
+    Pieces* pieces;           // per group, also those without tiles: single requests' first, then the prefixes'
+    int2* request;            // per request: its prefix's first group among `pieces` (or -1) and first row
     int* gbase;               // per prefix group: its first row group (num_groups + 1)
-    int* gcost;               // per group: fixed costs of the groups before it
-    int* wtile;               // per worker: its first tile (W + 1)
-    int* bad;                 // per group: it met a row outside the cache
+    int* bad;                 // per group with tiles: it met a row outside the cache
     float* rec_ml;            // per record row 8 floats: m, l, -, -, and 2^-f of each 128 columns of o
     uint16_t* rec_o;          // o 2^f in fp16
     float2* rowsum;           // per CTA: [kSums][2][128] row sums and references handed between its sets
     int W;                    // workers
-    int own;                  // groups of single requests, which come first (B * ceil(H / 128))
+    int own;                  // groups of single requests (B * ceil(H / 128))
     int fold;                 // 1: prefix and own rows in one group (128 divides H)
 };
 
@@ -117,87 +125,103 @@ __device__ __forceinline__ int prefix_of(const PrefixArgs& A, int b) {
 // ------------------------------------------------------------------------------------- plan
 
 constexpr int kPlanThreads = 1024;
+constexpr int kPlanCache = 4096;   // groups (and prefix groups) whose sums are kept in shared memory
+constexpr int kMaxWorkers = 128;
 
-// Exclusive sums over the block's threads of v; *carry is advanced by their total.
-__device__ int block_scan(int v, int* sh, int* carry) {
+// Exclusive sums over the block's threads of v (two 32-bit counts in one); *carry is advanced by their total.
+__device__ long long block_scan(long long v, long long* sh, long long* carry) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-    int x = v;
+    long long x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
     if (lane == 31) sh[warp] = x;
     __syncthreads();
-    if (warp == 0) {
-        int s = sh[lane];
+    long long before = 0, total = 0;
+    {
+        long long s = sh[lane];
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, s, o);
+            const long long y = __shfl_up_sync(0xffffffffu, s, o);
             if (lane >= o) s += y;
         }
-        sh[lane] = s;
+        total = __shfl_sync(0xffffffffu, s, 31);
+        before = __shfl_sync(0xffffffffu, s, warp > 0 ? warp - 1 : 0);
     }
-    __syncthreads();
-    const int at = *carry + x - v + (warp ? sh[warp - 1] : 0);
-    const int total = sh[31];
+    const long long at = *carry + x - v + (warp ? before : 0);
     __syncthreads();
     if (threadIdx.x == 0) *carry += total;
     __syncthreads();
     return at;
 }
 
+// One block. Latency is all that counts here: one round of loads for the prefixes, one for the groups,
+// the searches in shared memory (in global memory beyond kPlanCache).
 __global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(const __grid_constant__ PrefixArgs A, const Work wk) {
-    __shared__ int sh[32], carry, cost;
+    __shared__ long long sh[32], carry;
+    __shared__ int sh_base[kPlanCache / 4 + 1];        // gbase
+    __shared__ int sh_unit[kPlanCache + 1];            // per group with tiles: tiles and fixed costs before it
+    __shared__ int sh_cut[kMaxWorkers + 1];            // where each share begins
+    __shared__ int sh_tile[kMaxWorkers + 1];           // per worker with tiles: its first one
+    __shared__ unsigned sh_has[kMaxWorkers / 32];
     pdl_launch_dependents();
     const int hb = ceil_div(A.H, 128), tid = threadIdx.x;
     if (tid == 0) {
-        carry = cost = 0;
+        carry = 0;
         *wk.status = 0;
     }
     __syncthreads();
     int extra = 0;   // row groups of the prefixes
+    const bool base_sh = A.P <= kPlanCache / 4;
     if (!wk.fold) {
         for (int p0 = 0; p0 < A.P; p0 += kPlanThreads) {
             const int p = p0 + tid;
             int n = 0;
             if (p < A.P) {
                 const int s0 = max(A.starts[p], 0), s1 = min(A.starts[p + 1], A.B);
-                n = s1 > s0 ? (static_cast<long long>(s1 - s0) * A.H + 127) / 128 : 0;
+                n = s1 > s0 ? static_cast<int>((static_cast<long long>(s1 - s0) * A.H + 127) / 128) : 0;
             }
-            const int at = block_scan(n, sh, &carry);
-            if (p < A.P) wk.gbase[p] = at;
+            const int at = static_cast<int>(block_scan(n, sh, &carry));
+            if (p < A.P) {
+                if (base_sh) sh_base[p] = at;
+                else wk.gbase[p] = at;
+            }
         }
-        extra = carry;
+        extra = static_cast<int>(carry);
         __syncthreads();
-        if (tid == 0) {
-            wk.gbase[A.P] = extra;
-            carry = 0;
-        }
+        if (tid == 0) carry = 0;
         __syncthreads();
     }
+    const int* gbase = base_sh ? sh_base : wk.gbase;
+    // groups: tiles, then (compacted) the table
     const int G = wk.own + extra;
+    int mine = -1, mine0 = 0, mine1 = 0;   // this thread's last group: its place in the table, its tiles
     for (int g0 = 0; g0 < G; g0 += kPlanThreads) {
         const int g = g0 + tid;
         Group d = {};
         int tiles = 0;
         if (g < wk.own) {
             const int b = g / hb, k = g % hb;
+            const int p = prefix_of(A, b);
             d.q_row0 = b * A.H + 128 * k;
             d.rows = min(128, A.H - 128 * k);
-            d.pid = wk.fold ? prefix_of(A, b) : -1;
+            d.pid = wk.fold ? p : -1;
             d.sid = b;
             d.plen = d.pid >= 0 ? clampi(A.plens[d.pid], A.max_plen) : 0;
             d.slen = clampi(A.lens[b], A.max_len);
+            if (!wk.fold && k == 0)
+                wk.request[b] = p < 0 ? make_int2(-1, 0) : make_int2(wk.own + gbase[p], max(A.starts[p], 0) * A.H);
         } else if (g < G) {
             const int e = g - wk.own;
             int lo = 0, hi = A.P;   // last prefix group that starts at or before e
             while (lo + 1 < hi) {
                 const int mid = (lo + hi) / 2;
-                if (wk.gbase[mid] <= e) lo = mid; else hi = mid;
+                if (gbase[mid] <= e) lo = mid; else hi = mid;
             }
             const int s0 = max(A.starts[lo], 0), s1 = min(A.starts[lo + 1], A.B);
-            const int at = (e - wk.gbase[lo]) * 128;
+            const int at = (e - gbase[lo]) * 128;
             d.q_row0 = s0 * A.H + at;
             d.rows = min(128, (s1 - s0) * A.H - at);
             d.pid = lo;
@@ -207,32 +231,84 @@ __global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(const __grid_
         if (g < G) {
             d.ptiles = ceil_div(d.plen, kTile);
             tiles = d.ptiles + ceil_div(d.slen, kTile);
-            wk.bad[g] = 0;
         }
-        d.tile0 = block_scan(tiles, sh, &carry);
-        const int c = block_scan(tiles > 0 ? kGroupCost : 0, sh, &cost);
-        if (g < G) {
-            wk.group[g] = d;
-            wk.gcost[g] = c;
+        const long long at = block_scan(static_cast<long long>(tiles > 0) << 32 | tiles, sh, &carry);
+        const int c = static_cast<int>(at >> 32);   // groups with tiles before this one
+        d.tile0 = static_cast<int>(at);
+        d.tile1 = d.tile0 + tiles;
+        mine = tiles > 0 ? c : -1;
+        mine0 = d.tile0;
+        mine1 = d.tile1;
+        if (g < G && G > kPlanThreads) wk.pieces[g] = {mine, mine0, mine1, 0};   // until the workers are known
+        if (tiles > 0) {
+            wk.group[c] = d;
+            wk.bad[c] = 0;
+            if (c < kPlanCache) sh_unit[c] = d.tile0 + c * kGroupCost;
         }
     }
-    if (tid == 0) {
-        wk.head->groups = G;
-        wk.group[G].tile0 = carry;   // the end of the last group's tiles
-    }
-    __syncthreads();
+    const int T = static_cast<int>(carry), C = static_cast<int>(carry >> 32);
+    __syncthreads();   // the table is complete (this block's writes are visible to it)
     // Worker w begins at w / W of all tiles and fixed costs. A group's cost lies before its tiles; a
-    // share that begins there begins with the group.
-    for (int w = tid; w <= wk.W; w += kPlanThreads) {
-        const long long u = static_cast<long long>(carry + cost) * w / wk.W;
-        int lo = 0, hi = G;   // last group whose cost and tiles begin at or before u
+    // share that begins there begins with the group. Shares that hold no tile are left out.
+    auto unit = [&](int c) { return c < kPlanCache ? sh_unit[c] : wk.group[c].tile0 + c * kGroupCost; };
+    int first = 0;   // the group that this thread's share begins with
+    if (tid <= wk.W) {
+        const long long u = static_cast<long long>(T + C * kGroupCost) * tid / wk.W;
+        int lo = 0, hi = C;   // last group whose cost and tiles begin at or before u
         while (lo + 1 < hi) {
             const int mid = (lo + hi) / 2;
-            if (wk.group[mid].tile0 + wk.gcost[mid] <= u) lo = mid; else hi = mid;
+            if (unit(mid) <= u) lo = mid; else hi = mid;
         }
-        const int t0 = wk.group[lo].tile0, t1 = wk.group[lo + 1].tile0;
-        const long long t = u - wk.gcost[lo] - (t1 > t0 ? kGroupCost : 0);
-        wk.wtile[w] = w == wk.W ? carry : static_cast<int>(t < t0 ? t0 : (t > t1 ? t1 : t));
+        const int tile0 = C > 0 ? unit(lo) - lo * kGroupCost : 0;
+        const int tile1 = lo + 1 < C ? unit(lo + 1) - (lo + 1) * kGroupCost : T;
+        const long long x = u - static_cast<long long>(lo + 1) * kGroupCost;
+        const int cut = tid == wk.W ? T : static_cast<int>(x < tile0 ? tile0 : (x > tile1 ? tile1 : x));
+        sh_cut[tid] = cut;
+        first = cut == tile1 ? lo + 1 : lo;
+    }
+    __syncthreads();
+    const bool has = tid < wk.W && sh_cut[tid] < sh_cut[tid + 1];
+    if (tid < kMaxWorkers) {
+        const unsigned mask = __ballot_sync(0xffffffffu, has);
+        if ((tid & 31) == 0) sh_has[tid / 32] = mask;
+    }
+    __syncthreads();
+    int workers = 0, at = 0;
+#pragma unroll
+    for (int i = 0; i < kMaxWorkers / 32; ++i) {
+        if (i < tid / 32) at += __popc(sh_has[i]);
+        workers += __popc(sh_has[i]);
+    }
+    if (has) {
+        at += __popc(sh_has[tid / 32] & ((1u << (tid & 31)) - 1));
+        sh_tile[at] = sh_cut[tid];
+        Start st;
+        st.tb = sh_cut[tid];
+        st.te = sh_cut[tid + 1];
+        st.g = first;
+        st.pad = 0;
+        st.d = wk.group[first];
+        wk.start[at] = st;
+    }
+    if (tid >= workers && tid < wk.W) wk.start[tid].tb = wk.start[tid].te = 0;
+    __syncthreads();
+    // the workers of each group
+    for (int g = tid; g < G; g += kPlanThreads) {
+        if (G > kPlanThreads) {
+            const Pieces p = wk.pieces[g];
+            mine = p.g;
+            mine0 = p.w0;
+            mine1 = p.w1;
+        }
+        auto worker = [&](int t) {   // the last one that begins at or before tile t
+            int lo = 0, hi = workers;
+            while (lo + 1 < hi) {
+                const int mid = (lo + hi) / 2;
+                if (sh_tile[mid] <= t) lo = mid; else hi = mid;
+            }
+            return lo;
+        };
+        wk.pieces[g] = {mine, mine >= 0 ? worker(mine0) : 0, mine >= 0 ? worker(mine1 - 1) : -1, 0};
     }
 }
 
@@ -259,26 +335,13 @@ static_assert(kSmemBytes <= 232448, "shared memory budget");
 // Walks a worker's tiles; every role walks an identical copy. A segment is the worker's run of tiles
 // of one group.
 struct Tiles {
-    int t, t_begin, t_end, g, seg0;
+    int t, t_end, g, seg0;
     Group d;
-    int gend;
-    __device__ void load(const Work& wk) {
-        const int4* p = reinterpret_cast<const int4*>(wk.group + g);
-        const int4 a = p[0], b = p[1];
-        d.q_row0 = a.x; d.rows = a.y; d.pid = a.z; d.sid = a.w;
-        d.plen = b.x; d.slen = b.y; d.tile0 = b.z; d.ptiles = b.w;
-        gend = wk.group[g + 1].tile0;
-    }
-    __device__ void init(const Work& wk, int groups, int tb, int te) {
-        t = t_begin = seg0 = tb;
-        t_end = te;
-        int lo = 0, hi = groups;   // last group whose tiles start at or before tb and are not none
-        while (lo + 1 < hi) {
-            const int mid = (lo + hi) / 2;
-            if (wk.group[mid].tile0 <= tb) lo = mid; else hi = mid;
-        }
-        g = lo;
-        load(wk);
+    __device__ void init(const Start& st) {
+        t = seg0 = st.tb;
+        t_end = st.te;
+        g = st.g;
+        d = st.d;
     }
     __device__ bool valid() const { return t < t_end; }
     __device__ bool own() const { return t - d.tile0 >= d.ptiles; }
@@ -286,12 +349,12 @@ struct Tiles {
     __device__ int np() const { return min(kTile, (own() ? d.slen : d.plen) - pos0()); }
     __device__ int seg_tile() const { return t - seg0; }
     __device__ bool seg_first() const { return t == seg0; }
-    __device__ bool seg_last() const { return t + 1 == t_end || t + 1 == gend; }
+    __device__ int seg_end() const { return min(t_end, d.tile1); }
+    __device__ bool seg_last() const { return t + 1 == seg_end(); }
     __device__ void next(const Work& wk) {
         ++t;
-        if (t >= gend && t < t_end) {
-            do { ++g; } while (wk.group[g + 1].tile0 <= t);   // groups without tiles
-            load(wk);
+        if (t == d.tile1 && t < t_end) {
+            d = wk.group[++g];
             seg0 = t;
         }
     }
@@ -441,17 +504,16 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
     tc_fence_after();
     const uint32_t tbase = bars->tmem;
     pdl_wait();   // the plan
-    const int groups = wk.head->groups;
     // identical in both CTAs of the pair; a pair without tiles goes straight to the teardown
-    const int tb = wk.wtile[w], te = wk.wtile[w + 1];
-    const int n = te - tb;
+    const Start start = wk.start[w];
+    const int n = start.te - start.tb;
     const uint32_t stages_u32 = smem_u32(stages), xbuf_u32 = smem_u32(xbuf), qrope_u32 = smem_u32(qrope);
 
     if (warp < 4) {
         if (n > 0 && warp == 0 && lane == 0) {
             // ------------------------------------------------------------ loads
             Tiles it;
-            it.init(wk, groups, tb, te);
+            it.init(start);
             int issued = 0;
             for (int i = 0; it.valid(); ++i, it.next(wk)) {
                 const int st = i % kStages;
@@ -486,7 +548,7 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
             const uint32_t tQ = tbase + kColQ;
             const uint64_t dqr = smem_desc_noswz(qrope_u32, kQRopeBoxBytes, 128);
             Tiles it;
-            it.init(wk, groups, tb, te);
+            it.init(start);
             int seg = 0;
             bool ok = true;
             for (int i = 0; it.valid(); ++i, it.next(wk)) {
@@ -522,7 +584,7 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
             constexpr uint32_t idesc = idesc_f16(128, 256, Fmt<T>::v, false, true);
             const uint32_t tO = tbase + kColO;
             Tiles it;
-            it.init(wk, groups, tb, te);
+            it.init(start);
             int seg = 0;
             bool ok = true;
             for (int i = 0; it.valid(); ++i, it.next(wk)) {
@@ -587,7 +649,7 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
         Tiles it;
         bool ok = true;
         if (n > 0) {
-            it.init(wk, groups, tb, te);
+            it.init(start);
             if (sid == 0) load_q(it.d);   // the first tile belongs to set 0
             it.skip(wk, sid);
         } else {
@@ -626,7 +688,7 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
                 for (int c = 0; c < 4; ++c)
                     st_async_v4(dst + c * kXUnit, h[4 * c], h[4 * c + 1], h[4 * c + 2], h[4 * c + 3], bar);
             }
-            if (it.seg_last() && it.t + 1 < te) {
+            if (it.seg_last() && it.t + 1 < it.t_end) {
                 // the score of tile j was the last MMA to read this group's Q
                 Tiles nx = it;
                 nx.next(wk);
@@ -743,7 +805,7 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
             else if (m != m_l) l_self *= ex2(m_l - m);
             m_l = m;
             l_self += ls[0].x + ls[0].y;
-            if (it.t + kSets >= min(te, it.gend)) {
+            if (it.t + kSets >= it.seg_end()) {
                 volatile float2* lp = l_pub + ((j % kSums) * 2 + hf) * 128 + t;
                 lp->x = l_self;
                 lp->y = m;
@@ -752,8 +814,8 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
 
             if (it.seg_last()) {
                 // ---- the segment's partial record: this thread's 128 columns of the CTA's 256
-                got = mbar_wait(smem_u32(&bars->pv_done[slot]), phase, err, code(kWaitPV));
                 float l_tot = 0.f;
+                got = true;
 #pragma unroll
                 for (int i = 0; i < kSets; ++i)
                     if (it.seg_tile() >= i) {
@@ -763,6 +825,7 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
                         const volatile float2* lp = l_pub + (js % kSums) * 2 * 128 + t;
                         l_tot += (lp->x + lp[128].x) * ex2(lp->y - m);
                     }
+                got = got && mbar_wait(smem_u32(&bars->pv_done[slot]), phase, err, code(kWaitPV));
                 if (!warp_ok(got)) break;
                 tc_fence_after();
                 const long long at = static_cast<long long>(it.g + w) * 128 + t;
@@ -801,7 +864,6 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
 // ------------------------------------------------------------------------------------- merge
 
 constexpr int kMergeWarps = 8;
-constexpr int kMaxWorkers = 128;
 
 // One output row per `kWarps` warps: each takes every kWarps-th record of the row's groups, keeping
 // the running maximum, sum and weighted latent in fp32; the warps meet in shared memory.
@@ -813,10 +875,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) prefix_merge_kernel(const __
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     const int sub = warp % kWarps;
     const int f = blockIdx.x * kRows + warp / kWarps;
-    __shared__ int sh_w[kMaxWorkers + 1];
     pdl_wait();
-    for (int w = threadIdx.x; w <= wk.W; w += 32 * kMergeWarps) sh_w[w] = wk.wtile[w];
-    __syncthreads();
     const bool live = f < A.B * A.H;
     float m = -INFINITY, l = 0.f;
     float o[16];
@@ -825,40 +884,25 @@ __global__ void __launch_bounds__(32 * kMergeWarps) prefix_merge_kernel(const __
     bool bad = false;
     if (live) {
         const int b = f / A.H, h = f % A.H;
-        bad = *wk.status != 0;
         // the row's groups: its request's, and unless that holds the prefix too, its prefix group's
-        for (int k = 0; k < (wk.fold ? 1 : 2); ++k) {
-            int g, r;
-            if (k == 0) {
-                g = b * ceil_div(A.H, 128) + h / 128;
-                r = h % 128;
-            } else {
-                const int p = prefix_of(A, b);
-                if (p < 0) break;
-                const int at = f - max(A.starts[p], 0) * A.H;
-                g = wk.own + wk.gbase[p] + at / 128;
-                r = at % 128;
-            }
-            const int t0 = wk.group[g].tile0, t1 = wk.group[g + 1].tile0;
-            if (t1 <= t0) continue;
+        const int2 rq = wk.fold ? make_int2(-1, 0) : wk.request[b];
+        Pieces piece[2];
+        piece[0] = wk.pieces[b * ceil_div(A.H, 128) + h / 128];
+        bad = *wk.status != 0;
+        piece[1].g = -1;
+        if (rq.x >= 0) piece[1] = wk.pieces[rq.x + (f - rq.y) / 128];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if (piece[k].g < 0) continue;
+            const int g = piece[k].g, w1 = piece[k].w1, r = k == 0 ? h % 128 : (f - rq.y) % 128;
             bad = bad || wk.bad[g] != 0;
-            int w0 = 0, w1 = wk.W;   // workers of the group's tiles; one between them may have none
-            for (int hi = wk.W; w0 + 1 < hi;) {
-                const int mid = (w0 + hi) / 2;
-                if (sh_w[mid] <= t0) w0 = mid; else hi = mid;
-            }
-            for (int lo = w0; lo + 1 < w1;) {
-                const int mid = (lo + w1) / 2;
-                if (sh_w[mid] < t1) lo = mid; else w1 = mid;
-            }
-            --w1;
             constexpr int kAhead = 4;
-            for (int w = w0 + sub; w <= w1; w += kWarps * kAhead) {
+            for (int w = piece[k].w0 + sub; w <= w1; w += kWarps * kAhead) {
                 uint4 v[kAhead][2];
                 float2 ml[kAhead], fs[kAhead];
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i)
-                    if (w + i * kWarps <= w1 && sh_w[w + i * kWarps] < sh_w[w + i * kWarps + 1]) {
+                    if (w + i * kWarps <= w1) {
                         const long long at = static_cast<long long>(g + w + i * kWarps) * 128 + r;
                         ml[i] = *reinterpret_cast<const float2*>(wk.rec_ml + at * 8);
                         fs[i] = make_float2(wk.rec_ml[at * 8 + 4 + lane / 16], wk.rec_ml[at * 8 + 6 + lane / 16]);
@@ -868,7 +912,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) prefix_merge_kernel(const __
                     }
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i)
-                    if (w + i * kWarps <= w1 && sh_w[w + i * kWarps] < sh_w[w + i * kWarps + 1]) {
+                    if (w + i * kWarps <= w1) {
                         const float top = fmaxf(m, ml[i].x);
                         const float a = ex2(m - top), e0 = ex2(ml[i].x - top);
                         const float c2[2] = {e0 * fs[i].x, e0 * fs[i].y};
@@ -929,7 +973,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) prefix_merge_kernel(const __
 
 struct Layout {
     long long groups;     // most groups
-    size_t off_head, off_group, off_base, off_cost, off_wtile, off_bad, off_sum, off_ml, off_o, total;
+    size_t off_group, off_start, off_pieces, off_request, off_base, off_bad, off_sum, off_ml, off_o, total;
     int W, own, fold;
 };
 
@@ -941,18 +985,22 @@ Layout layout(const PrefixArgs& A, int sms) {
     L.groups = L.own + (L.fold ? 0 : static_cast<long long>(A.B) * A.H / 128 + (A.P < A.B ? A.P : A.B));
     L.W = sms / 2 > 0 ? sms / 2 : 1;
     if (L.W > kMaxWorkers) L.W = kMaxWorkers;
-    auto a256 = [](size_t x) { return (x + 255) / 256 * 256; };
+    const size_t groups = static_cast<size_t>(L.groups), recs = groups + L.W;
     size_t off = 256;     // status
-    L.off_head = off; off += 256;
-    L.off_group = off; off = a256(off + sizeof(Group) * static_cast<size_t>(L.groups + 1));
-    L.off_base = off; off = a256(off + sizeof(int) * (static_cast<size_t>(A.P) + 1));
-    L.off_cost = off; off = a256(off + sizeof(int) * static_cast<size_t>(L.groups));
-    L.off_wtile = off; off = a256(off + sizeof(int) * (L.W + 1));
-    L.off_bad = off; off = a256(off + sizeof(int) * static_cast<size_t>(L.groups));
-    L.off_sum = off; off = a256(off + sizeof(float2) * 2 * L.W * kSums * 2 * 128);
-    const size_t recs = static_cast<size_t>(L.groups) + L.W;
-    L.off_ml = off; off = a256(off + recs * 128 * 8 * sizeof(float));
-    L.off_o = off; off = a256(off + recs * 128 * 512 * 2);
+    auto take = [&](size_t bytes) {
+        const size_t at = off;
+        off = (off + bytes + 255) / 256 * 256;
+        return at;
+    };
+    L.off_group = take(sizeof(Group) * groups);
+    L.off_start = take(sizeof(Start) * L.W);
+    L.off_pieces = take(sizeof(Pieces) * groups);
+    L.off_request = take(sizeof(int2) * A.B);
+    L.off_base = take(sizeof(int) * A.P);
+    L.off_bad = take(sizeof(int) * groups);
+    L.off_sum = take(sizeof(float2) * 2 * L.W * kSums * 2 * 128);
+    L.off_ml = take(recs * 128 * 8 * sizeof(float));
+    L.off_o = take(recs * 128 * 512 * 2);
     L.total = off;
     return L;
 }
@@ -962,11 +1010,11 @@ cudaError_t launch(const PrefixArgs& A, unsigned char* ws, int sms, cudaStream_t
     const Layout L = layout(A, sms);
     Work wk;
     wk.status = reinterpret_cast<int*>(ws);
-    wk.head = reinterpret_cast<Header*>(ws + L.off_head);
     wk.group = reinterpret_cast<Group*>(ws + L.off_group);
+    wk.start = reinterpret_cast<Start*>(ws + L.off_start);
+    wk.pieces = reinterpret_cast<Pieces*>(ws + L.off_pieces);
+    wk.request = reinterpret_cast<int2*>(ws + L.off_request);
     wk.gbase = reinterpret_cast<int*>(ws + L.off_base);
-    wk.gcost = reinterpret_cast<int*>(ws + L.off_cost);
-    wk.wtile = reinterpret_cast<int*>(ws + L.off_wtile);
     wk.bad = reinterpret_cast<int*>(ws + L.off_bad);
     wk.rec_ml = reinterpret_cast<float*>(ws + L.off_ml);
     wk.rec_o = reinterpret_cast<uint16_t*>(ws + L.off_o);
