@@ -61,11 +61,11 @@ constexpr int kQRopeBytes = 4 * kQRopeBoxBytes;
 constexpr int kXUnit = 128 * 16;                     // 16-byte unit c of row t is at c * kXUnit + t * 16: a warp's stores
                                                      // fill whole sectors on their way to the peer
 constexpr int kMSlots = 4;
-constexpr int kSets = 2;
-constexpr int kSlots = 4;                            // exchange and P slots, tile j in slot j % kSlots
+constexpr int kSets = 3;
+constexpr int kSlots = 3;                            // exchange and P slots, tile j in slot j % kSlots
 constexpr int kSums = 2 * kSlots;                    // row sums handed between the sets, tile j's in j % kSums
 constexpr int kGroupCost = 2;                        // a group's fixed cost, in tiles, for the split
-constexpr int kThreads = 128 + 256 * kSets;
+constexpr int kThreads = 128 + 128 * kSets;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColO = 0, kColS = 256, kColQ = 384;
 constexpr float kRescale = 8.0f;                     // log2 units
@@ -102,7 +102,7 @@ struct Work {                 // workspace
     int* bad;                 // per group with tiles: it met a row outside the cache
     float* rec_ml;            // per record row 8 floats: m, l, -, -, and 2^-f of each 128 columns of o
     uint16_t* rec_o;          // o 2^f in fp16
-    float2* rowsum;           // per CTA: [kSums][2][128] row sums and references handed between its sets
+    float2* rowsum;           // per CTA: [kSums][128] row sums and references handed between its sets
     int W;                    // workers
     int own;                  // groups of single requests (B * ceil(H / 128))
     int fold;                 // 1: prefix and own rows in one group (128 divides H)
@@ -329,7 +329,7 @@ struct __align__(8) Barriers {
 };
 
 constexpr size_t kSmemBytes = static_cast<size_t>(kStages) * kStageBytes + static_cast<size_t>(kSlots) * kXBytes +
-                              kQRopeBytes + (kMSlots + 4 * kSets) * 128 * sizeof(float) + sizeof(Barriers) + 1024;
+                              kQRopeBytes + kMSlots * 128 * sizeof(float) + sizeof(Barriers) + 1024;
 static_assert(kSmemBytes <= 232448, "shared memory budget");
 
 // Walks a worker's tiles; every role walks an identical copy. A segment is the worker's run of tiles
@@ -460,11 +460,10 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
     unsigned char* xbuf = stages + kStages * kStageBytes;
     unsigned char* qrope = xbuf + kSlots * kXBytes;
     float* m_pub = reinterpret_cast<float*>(qrope + kQRopeBytes);              // [kMSlots][128]
-    float* x_max = m_pub + kMSlots * 128;                                      // [kSets][2][half][128]
-    Barriers* bars = reinterpret_cast<Barriers*>(x_max + kSets * 4 * 128);
+    Barriers* bars = reinterpret_cast<Barriers*>(m_pub + kMSlots * 128);
     // the row sums that one set hands to another at a segment's end: in global memory, where shared
     // memory has no room, and only for the segment's last tiles
-    volatile float2* l_pub = wk.rowsum + static_cast<long long>(blockIdx.x) * kSums * 2 * 128;
+    volatile float2* l_pub = wk.rowsum + static_cast<long long>(blockIdx.x) * kSums * 128;
     const uint32_t rank = cluster_ctarank(), peer = rank ^ 1u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int w = blockIdx.x >> 1;
@@ -481,15 +480,15 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
         for (int i = 0; i < kSets; ++i) mbar_init(smem_u32(&bars->s_full[i]), 1);
         for (int i = 0; i < kSlots; ++i) {
             mbar_init(smem_u32(&bars->x_full[i]), 1);
-            mbar_init(smem_u32(&bars->p_full[i]), 256);
+            mbar_init(smem_u32(&bars->p_full[i]), 128);
             mbar_init(smem_u32(&bars->pv_done[i]), 1);
             mbar_init(smem_u32(&bars->x_empty[i]), 1);
         }
-        for (int b = 0; b < 2; ++b) mbar_init(smem_u32(&bars->s_free[b]), 256);
+        for (int b = 0; b < 2; ++b) mbar_init(smem_u32(&bars->s_free[b]), 128);
         for (int i = 0; i < kMSlots; ++i) mbar_init(smem_u32(&bars->mref[i]), 128);
-        for (int i = 0; i < kSums; ++i) mbar_init(smem_u32(&bars->lpub[i]), 256);
-        mbar_init(smem_u32(&bars->q_ready), 256);
-        mbar_init(smem_u32(&bars->o_free), 256);
+        for (int i = 0; i < kSums; ++i) mbar_init(smem_u32(&bars->lpub[i]), 128);
+        mbar_init(smem_u32(&bars->q_ready), 128);
+        mbar_init(smem_u32(&bars->o_free), 128);
         mbar_init(smem_u32(&bars->drain[0]), 1);
         mbar_init(smem_u32(&bars->drain[1]), 1);
         mbar_init(smem_u32(&bars->done), 1);
@@ -614,19 +613,19 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
         }
     } else {
         // ---------------------------------------------------------------- softmax sets
-        const int sid = (warp - 4) >> 3, hf = ((warp - 4) >> 2) & 1;
-        const int t = (warp & 3) * 32 + lane;             // query row == TMEM lane; columns 32 hf .. 32 hf + 31 of S
+        const int sid = (warp - 4) >> 2;
+        const int t = (warp & 3) * 32 + lane;             // query row == TMEM lane
         const uint32_t trow = tbase + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
         const float qscale = A.scale * 1.4426950408889634f;
         // Q of a group: this thread's half of its row's CTA columns into TMEM (two elements a column) and
         // two of the four rope boxes
         auto load_q = [&](const Group& d) {
             const long long row = d.q_row0 + t;
-            const uint4* lat = reinterpret_cast<const uint4*>(static_cast<const T*>(A.qa) + row * 512 + 256 * rank + 128 * hf);
-            const uint4* rope = reinterpret_cast<const uint4*>(static_cast<const T*>(A.qr) + row * 64 + 32 * rank + 16 * hf);
+            const uint4* lat = reinterpret_cast<const uint4*>(static_cast<const T*>(A.qa) + row * 512 + 256 * rank);
+            const uint4* rope = reinterpret_cast<const uint4*>(static_cast<const T*>(A.qr) + row * 64 + 32 * rank);
             const bool have = t < d.rows;
 #pragma unroll 1
-            for (int c = 0; c < 2; ++c) {
+            for (int c = 0; c < 4; ++c) {
                 uint4 v[8], r;
 #pragma unroll
                 for (int k = 0; k < 8; ++k) v[k] = have ? __ldg(lat + 8 * c + k) : make_uint4(0, 0, 0, 0);
@@ -637,9 +636,9 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
                                             v[4 * q + 1].x, v[4 * q + 1].y, v[4 * q + 1].z, v[4 * q + 1].w,
                                             v[4 * q + 2].x, v[4 * q + 2].y, v[4 * q + 2].z, v[4 * q + 2].w,
                                             v[4 * q + 3].x, v[4 * q + 3].y, v[4 * q + 3].z, v[4 * q + 3].w};
-                    tmem_st16(trow + kColQ + 64 * hf + 32 * c + 16 * q, x);
+                    tmem_st16(trow + kColQ + 32 * c + 16 * q, x);
                 }
-                *reinterpret_cast<uint4*>(qrope + (2 * hf + c) * kQRopeBoxBytes + t * 16) = r;
+                *reinterpret_cast<uint4*>(qrope + c * kQRopeBoxBytes + t * 16) = r;
             }
             fence_proxy_async_smem();
             tmem_st_wait();
@@ -659,24 +658,27 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
         for (int j = sid; ok && it.valid(); j += kSets, it.skip(wk, kSets)) {
             const int slot = j % kSlots, np = it.np();
             const uint32_t phase = (j / kSlots) & 1;
-            const uint32_t x_row = xbuf_u32 + slot * kXBytes + 4 * hf * kXUnit + t * 16;
+            const uint32_t x_row = xbuf_u32 + slot * kXBytes + t * 16;
             const uint32_t x_full = smem_u32(&bars->x_full[slot]);
             // ---- S_r(j) to registers, release S, send the fp16 partial
             bool got = mbar_wait(smem_u32(&bars->s_full[sid]), (j / kSets) & 1, err, code(kWaitS));
             if (!warp_ok(got)) break;
-            if (t == 0 && hf == 0) mbar_arrive_expect_tx(x_full, kXBytes);
+            if (t == 0) mbar_arrive_expect_tx(x_full, kXBytes);
             tc_fence_after();
-            uint32_t h[16];
-            {
+            uint32_t h[32];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
                 uint32_t sr[32];
-                tmem_ld32_sync(trow + kColS + 64 * (j & 1) + 32 * hf, sr);
-                tc_fence_before();
-                mbar_arrive(smem_u32(&bars->s_free[j & 1]));
+                tmem_ld32_sync(trow + kColS + 64 * (j & 1) + 32 * c, sr);
+                if (c == 2 - 1) {
+                    tc_fence_before();
+                    mbar_arrive(smem_u32(&bars->s_free[j & 1]));
+                }
 #pragma unroll
                 for (int q = 0; q < 16; ++q) {
                     const float2 v = mul2(make_float2(__uint_as_float(sr[2 * q]), __uint_as_float(sr[2 * q + 1])),
                                           make_float2(qscale, qscale));
-                    h[q] = half2_of(v.x, v.y);
+                    h[16 * c + q] = half2_of(v.x, v.y);
                 }
             }
             // the peer's value product of tile j - kSlots has read its slot
@@ -685,7 +687,7 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
             {
                 const uint32_t dst = mapa(x_row, peer), bar = mapa(x_full, peer);
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                for (int c = 0; c < 8; ++c)
                     st_async_v4(dst + c * kXUnit, h[4 * c], h[4 * c + 1], h[4 * c + 2], h[4 * c + 3], bar);
             }
             if (it.seg_last() && it.t + 1 < it.t_end) {
@@ -698,7 +700,7 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
                 // rows past the end: their weights are zero, but zero times what lies there need not be
                 unsigned char* sp = stages + (j % kStages) * kStageBytes + kRopeBytes;
                 const int units = (kTile - np) * 8;
-                for (int v = 128 * hf + t; v < 4 * units; v += 256)
+                for (int v = t; v < 4 * units; v += 128)
                     *reinterpret_cast<uint4*>(sp + (v / units) * kChunkBytes + (np + (v % units) / 8) * 128 + (v % 8) * 16) =
                         make_uint4(0, 0, 0, 0);
                 fence_proxy_async_smem();
@@ -709,38 +711,31 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
             if (!warp_ok(got)) break;
             // (stage by stage over all columns: the warp issues in order, so column by column it would wait
             // for every step of every chain)
-            float s[32];
-            uint32_t pv[16];
+            float s[64];
+            uint32_t pv[32];
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 8; ++c)
                 asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
                              : "=r"(pv[4 * c]), "=r"(pv[4 * c + 1]), "=r"(pv[4 * c + 2]), "=r"(pv[4 * c + 3])
                              : "r"(x_row + c * kXUnit));
 #pragma unroll
-            for (int q = 0; q < 16; ++q) {
+            for (int q = 0; q < 32; ++q) {
                 const float2 r = add2(floats_of(h[q]), floats_of(pv[q]));
                 s[2 * q] = r.x;
                 s[2 * q + 1] = r.y;
             }
             if (np < kTile) {
 #pragma unroll
-                for (int k = 0; k < 32; ++k)
-                    if (32 * hf + k >= np) s[k] = -INFINITY;
+                for (int k = 0; k < 64; ++k)
+                    if (k >= np) s[k] = -INFINITY;
             }
-            float mx[11];
+            float mt = max3(s[0], s[1], kLowest);
+            {
+                float mx[4] = {mt, s[2], s[3], s[4]};
 #pragma unroll
-            for (int k = 0; k < 10; ++k) mx[k] = max3(s[3 * k], s[3 * k + 1], s[3 * k + 2]);
-            mx[10] = fmaxf(s[30], s[31]);
-#pragma unroll
-            for (int k = 0; k < 3; ++k) mx[k] = max3(mx[3 * k], mx[3 * k + 1], mx[3 * k + 2]);
-            mx[0] = fmaxf(max3(mx[0], mx[1], mx[2]), fmaxf(mx[9], mx[10]));
-            // the other half of the row's columns is in the warp that shares this one's TMEM lanes
-            // (slot (j / kSets) & 1 is written again for tile j + 4, after x_full of that tile and hence after
-            // P(j) of every thread here)
-            float* xm = x_max + (sid * 2 + ((j / kSets) & 1)) * 2 * 128;
-            xm[hf * 128 + t] = mx[0];
-            asm volatile("bar.sync %0, 64;" ::"r"(1 + 4 * sid + (warp & 3)) : "memory");
-            const float mt = fmaxf(fmaxf(mx[0], xm[(hf ^ 1) * 128 + t]), kLowest);
+                for (int k = 5; k + 1 < 64; k += 2) mx[(k / 2) & 3] = max3(mx[(k / 2) & 3], s[k], s[k + 1]);
+                mt = fmaxf(max3(mx[0], mx[1], mx[2]), fmaxf(mx[3], s[64 - 1]));
+            }
             // the reference of the tile before, unless this one exceeds it by more than the threshold
             float m = mt, alpha = 1.f;
             bool need = false;
@@ -755,40 +750,38 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
                     m = m_prev;
                 }
             }
-            if (hf == 0) {
-                m_pub[(j % kMSlots) * 128 + t] = m;
-                mbar_arrive(smem_u32(&bars->mref[j % kMSlots]));
-            }
-            uint32_t pp[16];
+            m_pub[(j % kMSlots) * 128 + t] = m;
+            mbar_arrive(smem_u32(&bars->mref[j % kMSlots]));
+            uint32_t pp[32];
             const float2 m2 = make_float2(-m, -m);
 #pragma unroll
-            for (int q = 0; q < 16; ++q) {
+            for (int q = 0; q < 32; ++q) {
                 const float2 d = add2(make_float2(s[2 * q], s[2 * q + 1]), m2);
                 s[2 * q] = d.x;
                 s[2 * q + 1] = d.y;
             }
 #pragma unroll
-            for (int q = 0; q < 32; ++q) s[q] = ex2_ordered(s[q]);
+            for (int q = 0; q < 64; ++q) s[q] = ex2_ordered(s[q]);
 #pragma unroll
-            for (int q = 0; q < 16; ++q) pp[q] = pair_of<T>(s[2 * q], s[2 * q + 1]);
+            for (int q = 0; q < 32; ++q) pp[q] = pair_of<T>(s[2 * q], s[2 * q + 1]);
             if (__any_sync(0xffffffffu, need)) {
                 // the reference moved: rescale O (alpha = 1 elsewhere) once PV(j - 1) is done
                 got = mbar_wait(smem_u32(&bars->pv_done[(j - 1) % kSlots]), ((j - 1) / kSlots) & 1, err, code(kWaitPV));
                 if (!warp_ok(got)) break;
                 tc_fence_after();
 #pragma unroll 1
-                for (int c0 = 0; c0 < 128; c0 += 32) {
+                for (int c0 = 0; c0 < 256; c0 += 32) {
                     uint32_t o[32];
-                    tmem_ld32_sync(trow + kColO + 128 * hf + c0, o);
+                    tmem_ld32_sync(trow + kColO + c0, o);
 #pragma unroll
                     for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-                    tmem_st32(trow + kColO + 128 * hf + c0, o);
+                    tmem_st32(trow + kColO + c0, o);
                 }
                 tmem_st_wait();
                 tc_fence_before();
             }
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 8; ++c)
                 asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(x_row + c * kXUnit),
                              "r"(pp[4 * c]), "r"(pp[4 * c + 1]), "r"(pp[4 * c + 2]), "r"(pp[4 * c + 3])
                              : "memory");
@@ -796,7 +789,7 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
             mbar_arrive(smem_u32(&bars->p_full[slot]));
             float2 ls[4];
 #pragma unroll
-            for (int q = 0; q < 16; ++q) {
+            for (int q = 0; q < 32; ++q) {
                 const float2 p = ElemTraits<T>::to_f2(*reinterpret_cast<const typename ElemTraits<T>::T2*>(&pp[q]));
                 ls[q & 3] = q < 4 ? p : add2(ls[q & 3], p);
             }
@@ -806,14 +799,14 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
             m_l = m;
             l_self += ls[0].x + ls[0].y;
             if (it.t + kSets >= it.seg_end()) {
-                volatile float2* lp = l_pub + ((j % kSums) * 2 + hf) * 128 + t;
+                volatile float2* lp = l_pub + (j % kSums) * 128 + t;
                 lp->x = l_self;
                 lp->y = m;
             }
             mbar_arrive(smem_u32(&bars->lpub[j % kSums]));
 
             if (it.seg_last()) {
-                // ---- the segment's partial record: this thread's 128 columns of the CTA's 256
+                // ---- the segment's partial record: this thread's row of the CTA's 256 columns
                 float l_tot = 0.f;
                 got = true;
 #pragma unroll
@@ -822,20 +815,21 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
                         // the set of tile j - i: its sums over the segment end there
                         const int js = j - i;
                         got = got && mbar_wait(smem_u32(&bars->lpub[js % kSums]), (js / kSums) & 1, err, code(kWaitRef));
-                        const volatile float2* lp = l_pub + (js % kSums) * 2 * 128 + t;
-                        l_tot += (lp->x + lp[128].x) * ex2(lp->y - m);
+                        const volatile float2* lp = l_pub + (js % kSums) * 128 + t;
+                        l_tot += lp->x * ex2(lp->y - m);
                     }
                 got = got && mbar_wait(smem_u32(&bars->pv_done[slot]), phase, err, code(kWaitPV));
                 if (!warp_ok(got)) break;
                 tc_fence_after();
                 const long long at = static_cast<long long>(it.g + w) * 128 + t;
                 const bool row_ok = t < it.d.rows;
-                const float f = record_scale(trow + kColO + 128 * hf);
-                write_cols(trow + kColO + 128 * hf, wk.rec_o + at * 512 + 256 * rank + 128 * hf, f, row_ok);
-                if (row_ok) {
-                    float* ml = wk.rec_ml + at * 8;
-                    if (rank == 0 && hf == 0) *reinterpret_cast<float2*>(ml) = make_float2(m, l_tot);
-                    ml[4 + 2 * rank + hf] = 1.f / f;
+                float* ml = wk.rec_ml + at * 8;
+                if (row_ok && rank == 0) *reinterpret_cast<float2*>(ml) = make_float2(m, l_tot);
+#pragma unroll 1
+                for (int c = 0; c < 2; ++c) {
+                    const float f = record_scale(trow + kColO + 128 * c);
+                    write_cols(trow + kColO + 128 * c, wk.rec_o + at * 512 + 256 * rank + 128 * c, f, row_ok);
+                    if (row_ok) ml[4 + 2 * rank + c] = 1.f / f;
                 }
                 tc_fence_before();
                 mbar_arrive(smem_u32(&bars->o_free));
@@ -998,7 +992,7 @@ Layout layout(const PrefixArgs& A, int sms) {
     L.off_request = take(sizeof(int2) * A.B);
     L.off_base = take(sizeof(int) * A.P);
     L.off_bad = take(sizeof(int) * groups);
-    L.off_sum = take(sizeof(float2) * 2 * L.W * kSums * 2 * 128);
+    L.off_sum = take(sizeof(float2) * 2 * L.W * kSums * 128);
     L.off_ml = take(recs * 128 * 8 * sizeof(float));
     L.off_o = take(recs * 128 * 512 * 2);
     L.total = off;
