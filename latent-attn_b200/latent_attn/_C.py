@@ -686,38 +686,61 @@ def mla_cache_append(kv_cache: torch.Tensor, c_t: torch.Tensor, k_rope: torch.Te
 # serving operators: append with rotation, shared-prefix decode (no reference counterpart)
 # ---------------------------------------------------------------------------
 
-def _check_ints(t: Optional[torch.Tensor], name: str, shape, device, dtype=torch.int32) -> None:
-    if t is None:
-        return
-    if t.dtype != dtype or t.device != device or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-        raise RuntimeError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
+# These run once a decode step, where the checks are a good part of a small call: each is one
+# comparison of what must hold, and says what is wrong only when it does not.
+
+_I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
 
 
-def _check_table(t: Optional[torch.Tensor], name: str, rows: int, device) -> None:
-    if t is not None and (t.dtype != torch.int32 or t.device != device or t.dim() != 2 or t.size(0) != rows
-                          or not t.is_contiguous()):
-        raise RuntimeError(f"{name} must be a contiguous int32 tensor of shape ({rows}, pages) on {device}")
+def _wrong(t: torch.Tensor, name: str, dtype, index: int, shape, contiguous: bool) -> None:
+    want = "x".join("*" if n < 0 else str(n) for n in shape)
+    got = "x".join(str(n) for n in t.shape)
+    raise RuntimeError(f"{name} must be a{' contiguous' if contiguous else ''} {dtype} tensor of shape ({want}) on "
+                       f"cuda:{index}, got {t.dtype} ({got}), strides {tuple(t.stride())}, on {t.device}")
 
 
-def _check_rows(t: torch.Tensor, name: str, shape, like: torch.Tensor) -> None:
-    """A 16-bit tensor of the cache's type with unit inner stride."""
-    if t.dtype != like.dtype or t.device != like.device:
-        raise RuntimeError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
-    if tuple(t.shape) != tuple(shape):
-        raise RuntimeError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
-    if t.numel() and t.size(-1) > 1 and t.stride(-1) != 1:
-        raise RuntimeError(f"{name} must have unit inner stride")
+def _rows(t: torch.Tensor, name: str, dtype, index: int, shape):
+    """Strides of a tensor of that type, device and shape; the innermost one must be 1."""
+    st = t.stride()
+    if t.dtype is not dtype or t.get_device() != index or t.shape != shape:
+        _wrong(t, name, dtype, index, shape, False)
+    if st[-1] != 1 and shape[-1] > 1 and t.numel():
+        raise RuntimeError(f"{name} must have unit inner stride, got strides {tuple(st)}")
+    return st
 
 
-def _unexpanded(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    """`t`, copied if a dimension of it is broadcast: a stride of 0 means the default in the C structs."""
-    return t.contiguous() if t is not None and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)) else t
+def _dense(t: torch.Tensor, name: str, dtype, index: int, shape) -> int:
+    """Address of a contiguous tensor of that type, device and shape."""
+    if t.dtype is not dtype or t.get_device() != index or t.shape != shape or not t.is_contiguous():
+        _wrong(t, name, dtype, index, shape, True)
+    return t.data_ptr()
 
 
-def _check_cache(kv_cache: torch.Tensor, width: int) -> None:
-    if kv_cache.dtype not in _DT or not kv_cache.is_cuda or kv_cache.dim() != 2 or kv_cache.size(1) != width \
-            or kv_cache.stride(1) != 1:
+def _table(t: torch.Tensor, name: str, index: int, rows: int):
+    """(address, pages per row) of a page table."""
+    if t.dtype is not _I32 or t.get_device() != index or t.dim() != 2 or t.size(0) != rows or not t.is_contiguous():
+        _wrong(t, name, _I32, index, (rows, -1), True)
+    return t.data_ptr(), t.size(1)
+
+
+def _cache(kv_cache: torch.Tensor, width: int):
+    """(type, device index, row stride) of the cache."""
+    dt, index = kv_cache.dtype, kv_cache.get_device()
+    if dt not in _DT or index < 0 or kv_cache.dim() != 2 or kv_cache.size(1) != width or kv_cache.stride(1) != 1:
         raise RuntimeError(f"kv_cache must be a CUDA fp16/bf16 (rows, {width}) tensor with unit inner stride")
+    return dt, index, kv_cache.stride(0)
+
+
+def _current_stream(index: int) -> int:
+    return _RAW_STREAM(index) if _RAW_STREAM is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def _spread(t: torch.Tensor, st):
+    """(tensor, strides) without broadcast dimensions: a stride of 0 means the default in the C structs."""
+    if 0 in st and any(s == 0 and n > 1 for s, n in zip(st, t.shape)):
+        t = t.contiguous()
+        st = t.stride()
+    return t, st
 
 
 def mla_cache_append_rope(kv_cache: torch.Tensor, c: torch.Tensor, k_rope: torch.Tensor, cu_tokens: torch.Tensor,
@@ -742,52 +765,46 @@ def mla_cache_append_rope(kv_cache: torch.Tensor, c: torch.Tensor, k_rope: torch
     ``seq_lens`` is only read; ``new_lens`` (B,) receives the lengths after the call. ``status`` (CUDA
     int32): bit 0, a token past ``max_seq_len`` was dropped; bit 1, a row lay outside the cache."""
     cfg = _cfg(d_model, kv_lora_rank, qk_nope_head_dim, qk_rope_head_dim, num_heads, v_head_dim)
-    dc, dR, H = int(kv_lora_rank), int(qk_rope_head_dim), int(num_heads)
-    _check_cache(kv_cache, dc + dR)
-    dev = kv_cache.device
+    dc, dR, H = kv_lora_rank, qk_rope_head_dim, num_heads
+    dt, dev, kv_stride = _cache(kv_cache, dc + dR)
     T, B = c.size(0), seq_lens.numel()
-    _check_rows(c, "c", (T, dc), kv_cache)
-    _check_rows(k_rope, "k_rope", (T, dR), kv_cache)
-    _check_ints(cu_tokens, "cu_tokens", (B + 1,), dev)
-    _check_ints(seq_lens, "seq_lens", (B,), dev)
-    _check_ints(new_lens, "new_lens", (B,), dev)
-    _check_ints(kv_offsets, "kv_offsets", (B,), dev, torch.int64)
-    _check_table(page_table, "page_table", B, dev)
-    if status is not None and (status.dtype != torch.int32 or status.device != dev):
+    c, c_st = _spread(c, _rows(c, "c", dt, dev, (T, dc)))
+    k_rope, k_st = _spread(k_rope, _rows(k_rope, "k_rope", dt, dev, (T, dR)))
+    cu_p = _dense(cu_tokens, "cu_tokens", _I32, dev, (B + 1,))
+    lens_p = _dense(seq_lens, "seq_lens", _I32, dev, (B,))
+    new_p = None if new_lens is None else _dense(new_lens, "new_lens", _I32, dev, (B,))
+    off_p = None if kv_offsets is None else _dense(kv_offsets, "kv_offsets", _I64, dev, (B,))
+    table_p, pages = (None, 0) if page_table is None else _table(page_table, "page_table", dev, B)
+    if status is not None and (status.dtype is not _I32 or status.get_device() != dev):
         raise RuntimeError("status must be a CUDA int32 tensor")
-    _check_tables(rope_cos, rope_sin)
-    if rope_cos is not None:
+    cos_p = sin_p = None
+    if rope_cos is not None or rope_sin is not None:
+        _check_tables(rope_cos, rope_sin)
         for t, n in ((rope_cos, "rope_cos"), (rope_sin, "rope_sin")):
-            if t.dim() != 2 or t.size(1) != dR // 2 or t.size(0) < max_seq_len or t.device != dev:
-                raise RuntimeError(f"{n} must be (>= {max_seq_len}, {dR // 2}) on {dev}")
-    if norm_weight is not None:
-        _check_rows(norm_weight, "norm_weight", (dc,), kv_cache)
-    if q_rope is None and q_out is not None:
-        raise RuntimeError("q_out needs q_rope")
-    if q_out is not None and _unexpanded(q_out) is not q_out:
-        raise RuntimeError("q_out's rows overlap")
-    c, k_rope, q_rope = _unexpanded(c), _unexpanded(k_rope), _unexpanded(q_rope)
+            if t.dim() != 2 or t.size(1) != dR // 2 or t.size(0) < max_seq_len or t.get_device() != dev:
+                raise RuntimeError(f"{n} must be (>= {max_seq_len}, {dR // 2}) on cuda:{dev}")
+        cos_p, sin_p = rope_cos.data_ptr(), rope_sin.data_ptr()
+    w_p = None if norm_weight is None else _dense(norm_weight, "norm_weight", dt, dev, (dc,))
+    q_p = qo_p = None
+    q_st = qo_st = (0, 0, 1)
     if q_rope is not None:
-        _check_rows(q_rope, "q_rope", (T, H, dR), kv_cache)
+        q_rope, q_st = _spread(q_rope, _rows(q_rope, "q_rope", dt, dev, (T, H, dR)))
         if q_out is None:
-            q_out = torch.empty(T, H, dR, dtype=q_rope.dtype, device=dev)
-        _check_rows(q_out, "q_out", (T, H, dR), kv_cache)
-    a = _lib.MlaAppendRopeArgs()
-    a.dtype = _DT[kv_cache.dtype]
-    a.batch, a.tokens = B, T
-    a.kv_cache, a.kv_row_stride, a.kv_total_rows = kv_cache.data_ptr(), kv_cache.stride(0), kv_cache.size(0)
-    a.c, a.c_stride = c.data_ptr(), c.stride(0)
-    a.k_rope, a.k_stride = k_rope.data_ptr(), k_rope.stride(0)
-    a.cu_tokens, a.seq_lens, a.max_seq_len = cu_tokens.data_ptr(), seq_lens.data_ptr(), int(max_seq_len)
-    a.kv_offsets, a.page_table, a.page_rows = _ptr(kv_offsets), _ptr(page_table), int(page_rows)
-    a.max_pages = int(page_table.size(1)) if page_table is not None else 0
-    a.norm_weight, a.norm_eps = _ptr(norm_weight), float(norm_eps)
-    a.rope_cos, a.rope_sin, a.rope_theta = _ptr(rope_cos), _ptr(rope_sin), float(rope_theta)
-    if q_rope is not None and T:
-        a.q_rope, a.q_token_stride, a.q_head_stride = q_rope.data_ptr(), q_rope.stride(0), q_rope.stride(1)
-        a.q_out, a.q_out_token_stride, a.q_out_head_stride = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
-    a.new_lens, a.status = _ptr(new_lens), _ptr(status)
-    _lib.check(_lib.load().mla_cache_append_rope(C.byref(cfg), C.byref(a), C.c_void_p(_stream(dev))))
+            q_out = torch.empty(T, H, dR, dtype=dt, device=kv_cache.device)
+        qo_st = _rows(q_out, "q_out", dt, dev, (T, H, dR))
+        if _spread(q_out, qo_st)[0] is not q_out:
+            raise RuntimeError("q_out's rows overlap")
+        if T:
+            q_p, qo_p = q_rope.data_ptr(), q_out.data_ptr()
+    elif q_out is not None:
+        raise RuntimeError("q_out needs q_rope")
+    a = _lib.MlaAppendRopeArgs(_DT[dt], B, T, kv_cache.data_ptr(), kv_stride, kv_cache.size(0), c.data_ptr(), c_st[0],
+                               k_rope.data_ptr(), k_st[0], cu_p, lens_p, max_seq_len, off_p, table_p, page_rows, pages,
+                               w_p, norm_eps, cos_p, sin_p, rope_theta, q_p, q_st[0], q_st[1], qo_p, qo_st[0], qo_st[1],
+                               new_p, None if status is None else status.data_ptr())
+    st = _lib.load().mla_cache_append_rope(cfg, a, _current_stream(dev))
+    if st:
+        _lib.check(st)
     return q_out
 
 
@@ -810,49 +827,38 @@ def mla_prefix_decode(kv_cache: torch.Tensor, q_absorbed: torch.Tensor, q_rope: 
     index tensors are on the device; ``max_prefix_len`` and ``max_seq_len`` bound the lengths (longer
     ones are cut). ``workspace``: uint8, kept by callers that must not allocate."""
     cfg = _cfg(d_model, kv_lora_rank, qk_nope_head_dim, qk_rope_head_dim, num_heads, v_head_dim)
-    dc, dR, H = int(kv_lora_rank), int(qk_rope_head_dim), int(num_heads)
-    _check_cache(kv_cache, dc + dR)
-    dev = kv_cache.device
+    dc, dR, H = kv_lora_rank, qk_rope_head_dim, num_heads
+    dt, dev, kv_stride = _cache(kv_cache, dc + dR)
     if q_absorbed.dim() != 3:
         raise RuntimeError("q_absorbed must be 3D (batch, num_heads, kv_lora_rank)")
     B, P = q_absorbed.size(0), prefix_lens.numel()
-    _check_rows(q_absorbed, "q_absorbed", (B, H, dc), kv_cache)
-    _check_rows(q_rope, "q_rope", (B, H, dR), kv_cache)
-    if not q_absorbed.is_contiguous() or not q_rope.is_contiguous():
-        raise RuntimeError("q_absorbed and q_rope must be contiguous")
-    _check_ints(group_starts, "group_starts", (P + 1,), dev)
-    _check_ints(prefix_lens, "prefix_lens", (P,), dev)
-    _check_ints(seq_lens, "seq_lens", (B,), dev)
-    _check_ints(prefix_offsets, "prefix_offsets", (P,), dev, torch.int64)
-    _check_ints(kv_offsets, "kv_offsets", (B,), dev, torch.int64)
-    _check_table(prefix_table, "prefix_table", P, dev)
-    _check_table(page_table, "page_table", B, dev)
+    qa_p = _dense(q_absorbed, "q_absorbed", dt, dev, (B, H, dc))
+    qr_p = _dense(q_rope, "q_rope", dt, dev, (B, H, dR))
+    starts_p = _dense(group_starts, "group_starts", _I32, dev, (P + 1,))
+    plens_p = _dense(prefix_lens, "prefix_lens", _I32, dev, (P,))
+    lens_p = _dense(seq_lens, "seq_lens", _I32, dev, (B,))
+    poff_p = None if prefix_offsets is None else _dense(prefix_offsets, "prefix_offsets", _I64, dev, (P,))
+    off_p = None if kv_offsets is None else _dense(kv_offsets, "kv_offsets", _I64, dev, (B,))
+    ptable_p, ppages = (None, 0) if prefix_table is None else _table(prefix_table, "prefix_table", dev, P)
+    table_p, pages = (None, 0) if page_table is None else _table(page_table, "page_table", dev, B)
     if out is None:
-        out = torch.empty(B, H, dc, dtype=kv_cache.dtype, device=dev)
+        out = torch.empty_like(q_absorbed)
+        out_p = out.data_ptr()
     else:
-        _check_rows(out, "out", (B, H, dc), kv_cache)
-        if not out.is_contiguous():
-            raise RuntimeError("out must be contiguous")
-    a = _lib.MlaPrefixArgs()
-    a.dtype = _DT[kv_cache.dtype]
-    a.batch, a.num_groups = B, P
-    a.kv_cache, a.kv_row_stride, a.kv_total_rows = kv_cache.data_ptr(), kv_cache.stride(0), kv_cache.size(0)
-    a.q_absorbed, a.q_rope, a.group_starts = q_absorbed.data_ptr(), q_rope.data_ptr(), group_starts.data_ptr()
-    a.prefix_lens, a.max_prefix_len = prefix_lens.data_ptr(), int(max_prefix_len)
-    a.seq_lens, a.max_seq_len = seq_lens.data_ptr(), int(max_seq_len)
-    a.prefix_offsets, a.kv_offsets = _ptr(prefix_offsets), _ptr(kv_offsets)
-    if prefix_table is not None:
-        a.prefix_table, a.max_prefix_pages = prefix_table.data_ptr(), int(prefix_table.size(1))
-    if page_table is not None:
-        a.page_table, a.max_pages = page_table.data_ptr(), int(page_table.size(1))
-    a.page_rows, a.softmax_scale, a.output, a.kernel = int(page_rows), float(softmax_scale), out.data_ptr(), int(kernel)
+        out_p = _dense(out, "out", dt, dev, (B, H, dc))
+    a = _lib.MlaPrefixArgs(_DT[dt], B, P, kv_cache.data_ptr(), kv_stride, kv_cache.size(0), qa_p, qr_p, starts_p, plens_p,
+                           max_prefix_len, lens_p, max_seq_len, poff_p, off_p, ptable_p, ppages, table_p, pages, page_rows,
+                           softmax_scale, out_p, kernel)
     lib = _lib.load()
-    n = C.c_size_t(0)
-    _lib.check(lib.mla_prefix_decode_workspace_size(C.byref(cfg), C.byref(a), C.byref(n)))
-    if workspace is None or workspace.numel() * workspace.element_size() < n.value or workspace.data_ptr() % 256:
-        workspace = torch.empty(max(int(n.value), 1), dtype=torch.uint8, device=dev)
-    _lib.check(lib.mla_prefix_decode(C.byref(cfg), C.byref(a), C.c_void_p(workspace.data_ptr()), n,
-                                     C.c_void_p(_stream(dev))))
+    n = C.c_size_t()
+    st = lib.mla_prefix_decode_workspace_size(cfg, a, n)
+    if not st:
+        need = n.value
+        if workspace is None or workspace.nbytes < need or workspace.data_ptr() % 256:
+            workspace = torch.empty(need, dtype=torch.uint8, device=kv_cache.device)
+        st = lib.mla_prefix_decode(cfg, a, workspace.data_ptr(), need, _current_stream(dev))
+    if st:
+        _lib.check(st)
     return out
 
 
@@ -865,35 +871,35 @@ def linear_lora(x: torch.Tensor, W: torch.Tensor, lora_a: torch.Tensor, lora_b: 
     256, ``adapter_ids`` (M,) int32 in any order, ``scales`` (adapters,) fp32. All fp16 or bf16 of one
     type, which the result (M, N) has too. K is a multiple of 8. ``workspace``: uint8, kept by callers
     that must not allocate."""
-    for t, n, d in ((x, "x", 2), (W, "W", 2), (lora_a, "lora_a", 3), (lora_b, "lora_b", 3)):
-        if t.dtype not in _DT or not t.is_cuda or t.dim() != d:
-            raise RuntimeError(f"{n} must be a {d}D float16 or bfloat16 CUDA tensor")
+    dt, dev = x.dtype, x.get_device()
+    if dt not in _DT or dev < 0 or x.dim() != 2 or W.dim() != 2 or lora_a.dim() != 3:
+        raise RuntimeError("x and W must be 2D, lora_a and lora_b 3D float16 or bfloat16 CUDA tensors")
     (M, K), N, (adapters, rank, _) = x.shape, W.size(0), lora_a.shape
-    _check_rows(W, "W", (N, K), x)
-    _check_rows(lora_a, "lora_a", (adapters, rank, K), x)
-    _check_rows(lora_b, "lora_b", (adapters, N, rank), x)
-    if not W.is_contiguous() or not lora_a.is_contiguous() or not lora_b.is_contiguous():
-        raise RuntimeError("W, lora_a and lora_b must be contiguous")
-    _check_rows(x, "x", (M, K), x)
-    _check_ints(adapter_ids, "adapter_ids", (M,), x.device)
-    _check_ints(scales, "scales", (adapters,), x.device, torch.float32)
+    x, x_st = _spread(x, _rows(x, "x", dt, dev, (M, K)))
+    W_p = _dense(W, "W", dt, dev, (N, K))
+    a_p = _dense(lora_a, "lora_a", dt, dev, (adapters, rank, K))
+    b_p = _dense(lora_b, "lora_b", dt, dev, (adapters, N, rank))
+    ids_p = _dense(adapter_ids, "adapter_ids", _I32, dev, (M,))
+    scales_p = None if scales is None else _dense(scales, "scales", _F32, dev, (adapters,))
     if out is None:
-        out = torch.empty(M, N, dtype=x.dtype, device=x.device)
+        out = torch.empty(M, N, dtype=dt, device=x.device)
+        out_p = out.data_ptr()
     else:
-        _check_rows(out, "out", (M, N), x)
-        if not out.is_contiguous():
-            raise RuntimeError("out must be contiguous")
+        out_p = _dense(out, "out", dt, dev, (M, N))
     if M == 0:
         return out
-    x = _unexpanded(x)
-    a = _lib.MlaLoraArgs(_DT[x.dtype], M, N, K, x.data_ptr(), x.stride(0) if M > 1 else K, W.data_ptr(), adapters, rank,
-                         lora_a.data_ptr(), lora_b.data_ptr(), adapter_ids.data_ptr(), _ptr(scales), out.data_ptr())
+    a = _lib.MlaLoraArgs(_DT[dt], M, N, K, x.data_ptr(), x_st[0] if M > 1 else K, W_p, adapters, rank, a_p, b_p, ids_p,
+                         scales_p, out_p)
     lib = _lib.load()
-    n = C.c_size_t(0)
-    _lib.check(lib.mla_linear_lora_workspace_size(C.byref(a), C.byref(n)))
-    if workspace is None or workspace.numel() * workspace.element_size() < n.value or workspace.data_ptr() % 256:
-        workspace = torch.empty(int(n.value), dtype=torch.uint8, device=x.device)
-    _lib.check(lib.mla_linear_lora(C.byref(a), C.c_void_p(workspace.data_ptr()), n, C.c_void_p(_stream(x.device))))
+    n = C.c_size_t()
+    st = lib.mla_linear_lora_workspace_size(a, n)
+    if not st:
+        need = n.value
+        if workspace is None or workspace.nbytes < need or workspace.data_ptr() % 256:
+            workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+        st = lib.mla_linear_lora(a, workspace.data_ptr(), need, _current_stream(dev))
+    if st:
+        _lib.check(st)
     return out
 
 
