@@ -3,20 +3,21 @@
 // X (M, K), W (N, K), A (adapters, r, K), B (adapters, N, r), Y (M, N), all fp16 or bf16.
 //
 // Two kernels, the second launched beside the first (programmatic dependent launch):
-//   1. lora_shrink_kernel: U = s_a A_a x[m] for each block of up to 256 tokens and each adapter that
-//      occurs in it, one row per token and zeros for the other tokens, so that U is a matrix with the
-//      active adapters' ranks as extra columns: the delta is U . [B_a1 | B_a2 | ..]^T, a product over
-//      (active adapters x rank) more K columns of the same GEMM.
-//   2. lora_gemm_kernel: Y^T tiles [128 weight rows x up to 256 tokens] on tcgen05, K columns first
-//      (which need nothing of kernel 1), then the rank columns. Rank columns are taken 16 at a time
-//      (one MMA K-step), so an adapter of rank 16 costs one step, and only the adapters that a block
-//      of tokens really uses are read.
-// Small batches are bound by W's bytes (each read once for all tokens), prompts by the tensor pipe.
+//   1. lora_shrink_kernel: U = s_a A_a x[m], for each block of up to 256 tokens and each adapter that
+//      occurs in it. A batch of one block is also put in adapter order (the rows of X are copied).
+//   2. lora_gemm_kernel: Y^T tiles [256 weight rows x up to 256 tokens] on tcgen05, a pair of CTAs each
+//      (cta_group::2: 128 weight rows and half of the tokens' rows in each CTA's shared memory, so that
+//      a token's row is loaded once for 256 weight rows). First the K columns, then the ranks as extra
+//      K columns: for each active adapter a product of B_a's 256 rows with U's rows of the adapter's
+//      tokens, 16 ranks an MMA, added into those tokens' columns only. Only the adapters that a block
+//      really uses are read, and an MMA covers whole groups of 32 columns.
+// Small batches are bound by W's bytes (each read once for all tokens), prompts by the tensor pipe and
+// by what L2 delivers to the SMs (without multicast a pair needs 62 KB for 0.5 us of MMAs).
 //
-// Work split: whole tiles go round robin over one CTA per SM; the tiles that do not fill a last
-// round are cut along K into equal shares for all CTAs, so no SM idles. A CTA that shares a tile
-// stores its fp32 partial and counts itself; the one that completes the count adds all partials in
-// their order along K, so results do not depend on who came last. No CTA waits for another.
+// Work split: whole tiles go round robin over the pairs; the tiles that do not fill a last round are
+// cut along K into equal shares for all pairs, so no SM idles. A CTA that shares a tile stores its
+// fp32 partial and counts itself; the one that completes the count adds all partials in their order
+// along K, so results do not depend on who came last. No CTA waits for another pair's.
 //
 // A zero of U times an infinite or NaN value of another request's adapter would be NaN, so an output
 // that is not finite is computed again from its own operands alone (own_element): a broken adapter
@@ -34,26 +35,34 @@ using namespace sm100;
 
 namespace {
 
-constexpr int kRows = 128;            // weight rows per tile (MMA M)
+constexpr int kRows = 128;            // weight rows per CTA (256 per pair and tile)
 constexpr int kMaxTok = 256;          // tokens per tile (MMA N)
-constexpr int kChunk = 64;            // K elements per stage
+constexpr int kChunk = 64;            // K elements per 128-byte row
+constexpr int kGroup = 2;             // chunks per stage
 constexpr int kStep = 16;             // K elements per MMA
+constexpr int kColStep = 32;          // an MMA of a CTA pair covers a multiple of 32 columns, from one on
+constexpr int kSteps = 4 * kGroup;    // rank steps per stage
 constexpr int kGemmThreads = 192;     // warp 0 loads, warp 1 issues, warps 2-5 read out
-constexpr int kSmemCap = 200 * 1024;
+constexpr int kSmemCap = 192 * 1024;  // leaves room for a block of the shrink kernel on the SM
+constexpr int kMaxStages = 6;
 constexpr int kMinChunks = 4;         // shortest share of a cut tile
-constexpr int kShrinkWarps = 16;
-constexpr int kShrinkTok = 32;        // tokens per shrink block
+constexpr int kShrinkWarps = 8;
+constexpr int kShrinkTok = 32;        // tokens per shrink cluster
+constexpr int kCopyClusters = 8;      // clusters that copy X into adapter order
+constexpr int kTable = 1024;          // adapters that the shrink kernel counts in a table
 enum : int { kWaitLoad = 1, kWaitMma = 3, kWaitAcc = 4, kWaitOut = 5 };
 
 struct Plan {
     int M, N, K, r;
-    int tb, nb;                       // tokens per block (a multiple of 16), blocks
+    int tb, nb;                       // tokens per block (a multiple of 32), blocks
+    int sorted;                       // one block, its columns in adapter order
     int adapters, slots, rsteps;      // most adapters of a block, MMA steps per adapter
-    int kc, tiles;                    // K chunks, tiles (weight rows / 128 x blocks)
-    int grid, full;                   // CTAs, whole tiles (a multiple of grid)
-    int tail_ctas;                    // CTAs that share the other tiles
+    int kc, tiles;                    // K chunks, tiles (weight rows / 256 x blocks)
+    int pairs, full;                  // CTA pairs, whole tiles (a multiple of pairs)
+    int tail_pairs;                   // pairs that share the other tiles
     int stages, stage_bytes;
-    size_t off_status, off_count, off_meta, off_u, off_part, total;
+    int ksplit;                       // CTAs of a shrink cluster
+    size_t off_status, off_count, off_meta, off_perm, off_x, off_u, off_part, total;
 };
 
 int up(int a, int b) { return (a + b - 1) / b * b; }
@@ -62,35 +71,46 @@ Plan make_plan(int M, int N, int K, int adapters, int rank, int sms) {
     Plan p = {};
     p.M = M; p.N = N; p.K = K; p.r = rank; p.adapters = adapters;
     p.nb = ceil_div(M, kMaxTok);
-    p.tb = up(ceil_div(M, p.nb), kStep);
+    p.tb = up(ceil_div(M, p.nb), kColStep);
     p.nb = ceil_div(M, p.tb);
+    // with up to 32 tokens an MMA covers them all anyway
+    p.sorted = p.nb == 1 && p.tb > kColStep;
     p.slots = adapters < p.tb ? adapters : p.tb;
     p.rsteps = ceil_div(rank, kStep);
     p.kc = ceil_div(K, kChunk);
-    p.tiles = ceil_div(N, kRows) * p.nb;
-    p.grid = sms;
-    p.full = p.tiles / p.grid * p.grid;
+    p.tiles = ceil_div(N, 2 * kRows) * p.nb;
+    p.pairs = sms / 2;
+    p.full = p.tiles / p.pairs * p.pairs;
     const int rest = p.tiles - p.full;
-    const long long chunks = static_cast<long long>(rest) * p.kc;
-    long long ctas = chunks / kMinChunks;
-    if (ctas > p.grid) ctas = p.grid;
-    if (ctas < rest) ctas = rest;
-    p.tail_ctas = static_cast<int>(ctas);
-    if (p.full == 0) p.grid = p.tail_ctas;
-    p.stage_bytes = (kRows + p.tb) * 128;
+    long long shares = static_cast<long long>(rest) * p.kc / kMinChunks;
+    if (shares > p.pairs) shares = p.pairs;
+    if (shares < rest) shares = rest;
+    p.tail_pairs = static_cast<int>(shares);
+    if (p.full == 0) p.pairs = p.tail_pairs;
+    p.stage_bytes = kGroup * (kRows + p.tb / 2) * 128;
     p.stages = kSmemCap / p.stage_bytes;
-    if (p.stages > 10) p.stages = 10;
-    auto a256 = [](size_t x) { return (x + 255) / 256 * 256; };
+    if (p.stages > kMaxStages) p.stages = kMaxStages;
+    p.ksplit = 1;
+    while (p.ksplit < 8 && K >= 32 * kShrinkWarps * 2 * p.ksplit) p.ksplit *= 2;
     size_t off = 0;
-    p.off_status = off; off += 256;
-    p.off_count = off; off = a256(off + sizeof(int) * static_cast<size_t>(p.grid));
-    p.off_meta = off; off = a256(off + sizeof(int) * static_cast<size_t>(p.nb) * (p.slots + 1));
-    p.off_u = off; off = a256(off + static_cast<size_t>(p.nb) * p.slots * p.rsteps * p.tb * kStep * 2);
-    p.off_part = off;
-    if (rest > 0 && p.tail_ctas > rest) off += static_cast<size_t>(p.tail_ctas) * 2 * kRows * p.tb * sizeof(float);
-    p.total = a256(off);
+    auto take = [&](size_t bytes) {
+        const size_t at = off;
+        off = (off + bytes + 255) / 256 * 256;
+        return at;
+    };
+    p.off_status = take(256);
+    p.off_count = take(sizeof(int) * 2 * static_cast<size_t>(p.pairs));
+    p.off_meta = take(sizeof(int2) * static_cast<size_t>(p.nb) * (p.slots + 1));
+    p.off_perm = take(sizeof(int) * kMaxTok);
+    p.off_x = take(p.sorted ? static_cast<size_t>(p.tb) * K * 2 : 0);
+    p.off_u = take(static_cast<size_t>(p.nb) * p.slots * p.rsteps * p.tb * kStep * 2);
+    p.off_part = take(rest > 0 && p.tail_pairs > rest ? static_cast<size_t>(p.tail_pairs) * 4 * kRows * p.tb * sizeof(float) : 0);
+    p.total = off;
     return p;
 }
+
+// An adapter of a token block: its id, the first of its tokens' columns and how many an MMA covers.
+__device__ __forceinline__ int2 pack_slot(int id, int lo, int n) { return make_int2(id, lo << 16 | n); }
 
 template <typename T> struct Fmt;
 template <> struct Fmt<__half> { static constexpr uint32_t v = 0; };
@@ -117,98 +137,170 @@ __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], uint32_t 
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Block (unit, rank step, token block). A unit is one adapter of the token block with up to 32 of
-// its tokens. 16 warps cut K; each holds the 16 ranks x 32 tokens in registers as warp-level MMA
-// tiles and reads A's and x's rows straight from global memory, 16 bytes a lane: the sum over K may
-// take its columns in any order, so lane t of a quad takes columns 8 t .. 8 t + 7 of each 32, for both
-// operands alike. Tokens are gathered by their rows' addresses. The partial sums meet in shared
-// memory in warp order. (16 ranks x 32 tokens are too small for tcgen05's 128-row tile, and the whole
-// kernel is a few microseconds of latency beside the GEMM's start.)
-template <typename T>
+// Cluster (unit, kQ rank steps, token block) of ksplit CTAs that cut K. A unit is one adapter of the
+// token block with up to 32 of its tokens. Each of a CTA's warps takes every (8 ksplit)-th 32 columns
+// of K and holds the 16 kQ ranks x 32 tokens in registers as warp-level MMA tiles, reading A's and x's rows
+// straight from global memory, 16 bytes a lane: the sum over K may take its columns in any order, so
+// lane t of a quad takes columns 8 t .. 8 t + 7 of each 32, for both operands alike. Tokens are
+// gathered by their rows' addresses. Partial sums meet in shared memory, in warp order and then in
+// CTA order. (16 ranks x 32 tokens are too small for tcgen05's 128-row tile; the kernel is a few
+// microseconds of latency beside the GEMM's first loads of W.)
+// The clusters after the units copy X's rows into adapter order.
+template <typename T, int kQ>
 __global__ void __launch_bounds__(32 * kShrinkWarps) lora_shrink_kernel(const LoraArgs A, const Plan P, unsigned char* ws) {
     __shared__ __align__(16) int ids[kMaxTok];
-    __shared__ int unit_id, unit_sub, unit_slot;
-    __shared__ int warp_slots[8], warp_units[8];
+    __shared__ int col_of[kMaxTok], tok_of[kMaxTok];      // a token's column, and back
+    __shared__ int base[kMaxTok];                         // per leader (an adapter's first token): first column
+    __shared__ int unit_id, unit_sub, unit_slot, unit_lo, unit_n;
+    __shared__ int warp_sum[kShrinkWarps];
     __shared__ int list[kShrinkTok];
-    __shared__ float red[kShrinkWarps][kStep][kShrinkTok + 1];
+    // per adapter while the tokens are counted (tokens so far, first, last), then the warps' partial sums
+    __shared__ union {
+        struct {
+            short n[kTable], first[kTable], last[kTable];
+        } tab;
+        float red[kShrinkWarps][kStep][kShrinkTok + 1];
+    } sh;
+    __shared__ float part[kQ][kStep][kShrinkTok];         // this CTA's sums
     pdl_launch_dependents();
     const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
-    const int unit = blockIdx.x, q = blockIdx.y, blk = blockIdx.z;
+    const int unit = blockIdx.x / P.ksplit, kpart = blockIdx.x % P.ksplit, blk = blockIdx.z;
+    const int q0 = blockIdx.y * kQ;
+    const int units = P.slots + P.tb / kShrinkTok;
     const int m0 = blk * P.tb, mt = min(P.tb, P.M - m0);
-    if (tid < kMaxTok) {
+    {
         const int id = tid < mt ? A.ids[m0 + tid] : -1;
         ids[tid] = id >= 0 && id < P.adapters ? id : -1;
+        tok_of[tid] = -1;
     }
     if (tid < kShrinkTok) list[tid] = -1;
     if (tid == 0) unit_id = -1;
     if (blockIdx.x + blockIdx.y + blockIdx.z == 0) {
         int* count = reinterpret_cast<int*>(ws + P.off_count);
-        for (int i = tid; i < P.grid; i += blockDim.x) count[i] = 0;
+        for (int i = tid; i < 2 * P.pairs; i += blockDim.x) count[i] = 0;
         if (tid == 0) *reinterpret_cast<int*>(ws + P.off_status) = 0;
     }
     __syncthreads();
-    // the block's adapters in order of their first token; a token's rank among its adapter's
-    int id = -1, count = 0, rank_in = 0, first = kMaxTok;
-    if (tid < kMaxTok && (id = ids[tid]) >= 0) {
-        for (int j = 0; j < mt; ++j)
-            if (ids[j] == id) {
-                if (count == 0) first = j;
-                rank_in += j < tid;
-                ++count;
+    // this token's rank among its adapter's (or among those without one), the adapter's first and last token
+    const int id = ids[tid];
+    int count = 0, rank_in = 0, first = kMaxTok, last = 0;
+    if (P.adapters <= kTable) {
+        // one warp after the other enters its tokens, 32 at a time matched among each other
+        for (int i = tid; i < P.adapters; i += blockDim.x) sh.tab.n[i] = 0;
+        __syncthreads();
+        const unsigned same = __match_any_sync(0xffffffffu, id), less = (1u << lane) - 1;
+        for (int w = 0; w < kShrinkWarps; ++w) {
+            if (w == warp) {
+                if (id >= 0) rank_in = sh.tab.n[id] + __popc(same & less);
+                __syncwarp();
+                if (id >= 0 && lane == 31 - __clz(same)) {
+                    if (rank_in + 1 == __popc(same)) sh.tab.first[id] = static_cast<short>(warp * 32 + __ffs(same) - 1);
+                    sh.tab.n[id] = static_cast<short>(rank_in + 1);
+                    sh.tab.last[id] = static_cast<short>(tid);
+                }
             }
+            __syncthreads();
+        }
+        if (id >= 0) {
+            count = sh.tab.n[id];
+            first = sh.tab.first[id];
+            last = sh.tab.last[id];
+        }
+    } else {
+        for (int j0 = 0; j0 < mt; j0 += 4) {
+            const int4 v = *reinterpret_cast<const int4*>(ids + j0);
+            const int w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (w[k] == id && id >= 0) {
+                    if (count == 0) first = j0 + k;
+                    last = j0 + k;
+                    rank_in += j0 + k < tid;
+                    ++count;
+                }
+        }
+    }
+    {
+        // tokens without an adapter before this one
+        const unsigned none = __ballot_sync(0xffffffffu, id < 0);
+        if (lane == 0) warp_sum[warp] = __popc(none);
+        __syncthreads();
+        if (id < 0) {
+            rank_in = __popc(none & ((1u << lane) - 1));
+            for (int w = 0; w < warp; ++w) rank_in += warp_sum[w];
+        }
+        __syncthreads();
     }
     const bool leader = id >= 0 && first == tid;
     const int groups = leader ? (count + kShrinkTok - 1) / kShrinkTok : 0;
-    int s_incl = leader, u_incl = groups;
+    // sums over the leaders before: adapters, units, tokens (each below 1024)
+    const int v = leader ? 1 | groups << 10 | count << 20 : 0;
+    int x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int a = __shfl_up_sync(0xffffffffu, s_incl, o), b = __shfl_up_sync(0xffffffffu, u_incl, o);
-        if (lane >= o) {
-            s_incl += a;
-            u_incl += b;
-        }
+        const int a = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += a;
     }
-    if (warp < 8 && lane == 31) {
-        warp_slots[warp] = s_incl;
-        warp_units[warp] = u_incl;
-    }
+    if (lane == 31) warp_sum[warp] = x;
     __syncthreads();
-    if (warp < 8) {
-        int s0 = 0, u0 = 0;
-        for (int w = 0; w < warp; ++w) {
-            s0 += warp_slots[w];
-            u0 += warp_units[w];
-        }
-        const int slot = s0 + s_incl - 1, u1 = u0 + u_incl;
-        if (leader && unit >= u1 - groups && unit < u1) {
+    int total = 0, before = x - v;
+    for (int w = 0; w < kShrinkWarps; ++w) {
+        if (w < warp) before += warp_sum[w];
+        total += warp_sum[w];
+    }
+    const int slot = before & 1023, u0 = before >> 10 & 1023, b0 = before >> 20;
+    int2* meta = reinterpret_cast<int2*>(ws + P.off_meta) + static_cast<size_t>(blk) * (P.slots + 1);
+    const bool writer = blockIdx.x == 0 && q0 == 0;
+    if (leader) {
+        base[tid] = b0;
+        // the columns an MMA covers: the adapter's tokens (all between its first and its last where the
+        // block is not sorted), from a multiple of 32 (where an accumulator may begin) to one
+        const int c0 = P.sorted ? b0 : first, c1 = P.sorted ? b0 + count : last + 1;
+        const int lo = c0 / kColStep * kColStep, n = (c1 - lo + kColStep - 1) / kColStep * kColStep;
+        if (unit >= u0 && unit < u0 + groups) {
             unit_id = id;
             unit_slot = slot;
-            unit_sub = unit - (u1 - groups);
+            unit_sub = unit - u0;
+            unit_lo = lo;
+            unit_n = n;
         }
-        if (unit == 0 && q == 0) {
-            int* meta = reinterpret_cast<int*>(ws + P.off_meta) + static_cast<size_t>(blk) * (P.slots + 1);
-            if (leader) meta[1 + slot] = id;
-            if (tid == kMaxTok - 1) meta[0] = slot + 1;
-        }
+        if (writer) meta[1 + slot] = pack_slot(id, lo, n);
     }
+    if (writer && tid == 0) meta[0] = make_int2(total & 1023, 0);
     __syncthreads();
+    if (tid < mt) {
+        const int c = !P.sorted ? tid : id >= 0 ? base[first] + rank_in : (total >> 20) + rank_in;
+        col_of[tid] = c;
+        tok_of[c] = tid;
+        if (writer && P.sorted) reinterpret_cast<int*>(ws + P.off_perm)[c] = tid;
+    }
     const int a = unit_id, sub = unit_sub;
-    if (a < 0) return;
-    if (tid < kMaxTok && id == a && rank_in / kShrinkTok == sub) list[rank_in % kShrinkTok] = tid;
+    if (tid < mt && a >= 0 && id == a && rank_in / kShrinkTok == sub) list[rank_in % kShrinkTok] = tid;
     __syncthreads();
-    T* u = reinterpret_cast<T*>(ws + P.off_u) +
-           (static_cast<size_t>(blk) * P.slots * P.rsteps + unit_slot * P.rsteps + q) * P.tb * kStep;
-    if (sub == 0)   // the other tokens' rows of this adapter's columns
-        for (int i = tid; i < P.tb * 2; i += blockDim.x)
-            if (ids[i / 2] != a) reinterpret_cast<uint4*>(u)[i] = make_uint4(0, 0, 0, 0);
+    if (unit >= units) {
+        // copy: the clusters' CTAs take the columns in turn (one rank step's worth of blocks is enough)
+        if (q0 == 0) {
+            const int nvec = P.K / 8;
+            T* xp = reinterpret_cast<T*>(ws + P.off_x);
+            for (int c = (unit - units) * P.ksplit + kpart; c < mt; c += kCopyClusters * P.ksplit) {
+                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(A.x) + static_cast<long long>(tok_of[c]) * A.x_stride);
+                uint4* dst = reinterpret_cast<uint4*>(xp + static_cast<size_t>(c) * P.K);
+                for (int i = tid; i < nvec; i += blockDim.x) dst[i] = __ldg(src + i);
+            }
+        }
+        return;   // the whole cluster
+    }
+    if (a < 0) return;   // the whole cluster: no such unit
     const int g = lane / 4, t = lane % 4;
-    const T* arow[2];
+    const T* arow[kQ][2];
     const T* xrow[4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int k = q * kStep + g + 8 * i;
-        arow[i] = k < P.r ? static_cast<const T*>(A.a) + (static_cast<long long>(a) * P.r + k) * P.K : nullptr;
-    }
+    for (int e = 0; e < kQ; ++e)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int k = (q0 + e) * kStep + g + 8 * i;
+            arow[e][i] = k < P.r ? static_cast<const T*>(A.a) + (static_cast<long long>(a) * P.r + k) * P.K : nullptr;
+        }
     int nt = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -216,16 +308,19 @@ __global__ void __launch_bounds__(32 * kShrinkWarps) lora_shrink_kernel(const Lo
         xrow[i] = m >= 0 ? static_cast<const T*>(A.x) + (m0 + m) * A.x_stride : nullptr;
         if (list[8 * i] >= 0) nt = i + 1;
     }
-    float acc[4][4] = {};
-    constexpr int kUnroll = 4;
-    for (int k0 = 32 * warp; k0 < P.K; k0 += 32 * kShrinkWarps * kUnroll) {
-        uint4 va[kUnroll][2], vx[kUnroll][4];
+    float acc[kQ][4][4] = {};
+    constexpr int kUnroll = kQ == 1 ? 4 : 2;
+    const int stride = 32 * kShrinkWarps * P.ksplit;
+    for (int k0 = 32 * (kpart * kShrinkWarps + warp); k0 < P.K; k0 += stride * kUnroll) {
+        uint4 va[kUnroll][kQ][2], vx[kUnroll][4];
 #pragma unroll
         for (int j = 0; j < kUnroll; ++j) {
-            const int k = k0 + j * 32 * kShrinkWarps + 8 * t;
+            const int k = k0 + j * stride + 8 * t;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                va[j][i] = arow[i] && k < P.K ? __ldg(reinterpret_cast<const uint4*>(arow[i] + k)) : make_uint4(0, 0, 0, 0);
+            for (int e = 0; e < kQ; ++e)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    va[j][e][i] = arow[e][i] && k < P.K ? __ldg(reinterpret_cast<const uint4*>(arow[e][i] + k)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 vx[j][i] = xrow[i] && k < P.K ? __ldg(reinterpret_cast<const uint4*>(xrow[i] + k)) : make_uint4(0, 0, 0, 0);
@@ -234,26 +329,61 @@ __global__ void __launch_bounds__(32 * kShrinkWarps) lora_shrink_kernel(const Lo
         for (int j = 0; j < kUnroll; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (i < nt) {
-                    mma16816<T>(acc[i], va[j][0].x, va[j][1].x, va[j][0].y, va[j][1].y, vx[j][i].x, vx[j][i].y);
-                    mma16816<T>(acc[i], va[j][0].z, va[j][1].z, va[j][0].w, va[j][1].w, vx[j][i].z, vx[j][i].w);
-                }
+                if (i < nt)
+#pragma unroll
+                    for (int e = 0; e < kQ; ++e) {
+                        const uint4 r0 = va[j][e][0], r1 = va[j][e][1], v = vx[j][i];
+                        mma16816<T>(acc[e][i], r0.x, r1.x, r0.y, r1.y, v.x, v.y);
+                        mma16816<T>(acc[e][i], r0.z, r1.z, r0.w, r1.w, v.z, v.w);
+                    }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        red[warp][g][8 * i + 2 * t] = acc[i][0];
-        red[warp][g][8 * i + 2 * t + 1] = acc[i][1];
-        red[warp][g + 8][8 * i + 2 * t] = acc[i][2];
-        red[warp][g + 8][8 * i + 2 * t + 1] = acc[i][3];
-    }
-    __syncthreads();
-    const int k = tid % kStep, m = list[tid / kStep];   // 512 threads: 16 ranks x 32 tokens
-    if (m >= 0) {
-        float v = 0.f;
+    for (int e = 0; e < kQ; ++e) {
+        __syncthreads();   // (the table, or the step before, has been read)
 #pragma unroll
-        for (int w = 0; w < kShrinkWarps; ++w) v += red[w][k][tid / kStep];
-        u[m * kStep + k] = ElemTraits<T>::from_f(A.scales ? v * A.scales[a] : v);
+        for (int i = 0; i < 4; ++i) {
+            sh.red[warp][g][8 * i + 2 * t] = acc[e][i][0];
+            sh.red[warp][g][8 * i + 2 * t + 1] = acc[e][i][1];
+            sh.red[warp][g + 8][8 * i + 2 * t] = acc[e][i][2];
+            sh.red[warp][g + 8][8 * i + 2 * t + 1] = acc[e][i][3];
+        }
+        __syncthreads();
+        for (int i = tid; i < kStep * kShrinkTok; i += blockDim.x) {
+            float s = 0.f;
+#pragma unroll
+            for (int w = 0; w < kShrinkWarps; ++w) s += sh.red[w][i / kShrinkTok][i % kShrinkTok];
+            part[e][i / kShrinkTok][i % kShrinkTok] = s;
+        }
     }
+    if (P.ksplit > 1) cluster_sync();
+    else __syncthreads();
+    // the adapter's U rows: its tokens' values, zeros in the other columns that the MMA covers; the
+    // cluster's CTAs take the tokens in turn
+    const float scale = A.scales ? A.scales[a] : 1.f;
+#pragma unroll
+    for (int e = 0; e < kQ; ++e) {
+        if (q0 + e >= P.rsteps) break;
+        T* u = reinterpret_cast<T*>(ws + P.off_u) +
+               (static_cast<size_t>(blk) * P.slots * P.rsteps + unit_slot * P.rsteps + q0 + e) * P.tb * kStep;
+        for (int i = tid + kpart * blockDim.x; i < kStep * kShrinkTok; i += blockDim.x * P.ksplit) {
+            const int k = i % kStep, j = i / kStep, m = list[j];
+            if (m < 0) continue;
+            const uint32_t at = smem_u32(&part[e][k][j]);
+            float s = 0.f;
+            for (int c = 0; c < P.ksplit; ++c) {
+                float y;
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y) : "r"(mapa(at, c)));
+                s += y;
+            }
+            u[col_of[m] * kStep + k] = ElemTraits<T>::from_f(s * scale);
+        }
+        if (sub == 0 && kpart == P.ksplit - 1)
+            for (int i = tid; i < unit_n * 2; i += blockDim.x) {
+                const int c = unit_lo + i / 2, m = tok_of[c];
+                if (m < 0 || ids[m] != a) reinterpret_cast<uint4*>(u)[unit_lo * 2 + i] = make_uint4(0, 0, 0, 0);
+            }
+    }
+    if (P.ksplit > 1) cluster_sync();   // no CTA leaves while its sums may be read
 }
 
 // ------------------------------------------------------------------------------------- GEMM
@@ -262,29 +392,29 @@ struct Maps {
     CUtensorMap w, x, b, u;
 };
 
-// One piece of a CTA's work: chunks [c0, c1) of a tile's K columns.
+// One piece of a pair's work: chunks [c0, c1) of a tile's K columns.
 struct Item {
     int tile, c0, c1;
     int j;           // index among the cut tiles, or -1
 };
-// Walks the CTA's pieces; every role walks an identical copy.
+// Walks the pair's pieces; every role walks an identical copy.
 struct Walk {
     int next_full;
     long long c, c_end;
     __device__ explicit Walk(const Plan& P) {
-        const int w = blockIdx.x;
+        const int w = blockIdx.x / 2;
         next_full = w;
         c = c_end = 0;
-        if (w < P.tail_ctas) {
+        if (w < P.tail_pairs) {
             const long long total = static_cast<long long>(P.tiles - P.full) * P.kc;
-            c = total * w / P.tail_ctas;
-            c_end = total * (w + 1) / P.tail_ctas;
+            c = total * w / P.tail_pairs;
+            c_end = total * (w + 1) / P.tail_pairs;
         }
     }
     __device__ bool next(const Plan& P, Item* it) {
         if (next_full < P.full) {
             *it = {next_full, 0, P.kc, -1};
-            next_full += P.grid;
+            next_full += P.pairs;
             return true;
         }
         if (c >= c_end) return false;
@@ -299,45 +429,63 @@ struct Walk {
 };
 
 struct __align__(8) Bars {
-    uint64_t full[10], empty[10], acc_full[2], acc_empty[2];
+    uint64_t full[kMaxStages];        // leader: both CTAs' loads of the stage have landed
+    uint64_t empty[kMaxStages];       // both: the MMAs have read it
+    uint64_t acc_full[2];             // both: the accumulator is complete
+    uint64_t acc_empty[2];            // leader: both CTAs have read it out
     uint32_t tmem;
     int last;
+    int perm[kMaxTok];                // output row of each column (sorted)
+    int2 slots[2][kMaxTok];           // the block's adapters, for the loading and the issuing warp
 };
 
 __device__ __forceinline__ int code(int site) { return kStatusTimeout | (site << 8); }
 
-// Output element (token m of the block, weight row n) from the token's own operands: the rare path of
-// outputs that came out infinite or NaN.
+// The adapters of token block blk into sl (one warp); returns how many.
+__device__ __forceinline__ int load_slots(const Plan& P, const unsigned char* ws, int blk, int2* sl, int lane) {
+    const int2* meta = reinterpret_cast<const int2*>(ws + P.off_meta) + static_cast<size_t>(blk) * (P.slots + 1);
+    const int n = meta[0].x;
+    __syncwarp();
+    for (int i = lane; i < n; i += 32) sl[i] = meta[1 + i];
+    __syncwarp();
+    return n;
+}
+
+// Output element (column c of the block, token m, weight row n) from the token's own operands: the rare
+// path of outputs that came out infinite or NaN.
 template <typename T>
-__device__ __noinline__ float own_element(const LoraArgs& A, const Plan& P, const unsigned char* ws, int blk, int m, int n) {
-    const T* x = static_cast<const T*>(A.x) + static_cast<long long>(blk * P.tb + m) * A.x_stride;
+__device__ __noinline__ float own_element(const LoraArgs& A, const Plan& P, const unsigned char* ws, int blk, int c, int m, int n) {
+    const T* x = static_cast<const T*>(A.x) + static_cast<long long>(m) * A.x_stride;
     const T* w = static_cast<const T*>(A.w) + static_cast<long long>(n) * P.K;
     float v = 0.f;
     for (int k = 0; k < P.K; ++k) v = fmaf(ElemTraits<T>::to_f(x[k]), ElemTraits<T>::to_f(w[k]), v);
-    const int id = A.ids[blk * P.tb + m];
+    const int id = A.ids[m];
     if (id < 0 || id >= P.adapters) return v;
-    const int* meta = reinterpret_cast<const int*>(ws + P.off_meta) + static_cast<size_t>(blk) * (P.slots + 1);
+    const int2* meta = reinterpret_cast<const int2*>(ws + P.off_meta) + static_cast<size_t>(blk) * (P.slots + 1);
     int slot = 0;
-    while (slot < meta[0] && meta[1 + slot] != id) ++slot;
+    while (slot < meta[0].x && meta[1 + slot].x != id) ++slot;
     const T* u = reinterpret_cast<const T*>(ws + P.off_u);
     const T* b = static_cast<const T*>(A.b) + (static_cast<long long>(id) * P.N + n) * P.r;
     for (int k = 0; k < P.r; ++k) {
         const size_t step = static_cast<size_t>(blk) * P.slots * P.rsteps + slot * P.rsteps + k / kStep;
-        v = fmaf(ElemTraits<T>::to_f(u[(step * P.tb + m) * kStep + k % kStep]), ElemTraits<T>::to_f(b[k]), v);
+        v = fmaf(ElemTraits<T>::to_f(u[(step * P.tb + c) * kStep + k % kStep]), ElemTraits<T>::to_f(b[k]), v);
     }
     return v;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
 lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan P,
                  const __grid_constant__ LoraArgs A, unsigned char* ws) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     Bars* bars = reinterpret_cast<Bars*>(smem + P.stages * P.stage_bytes);
     const uint32_t ring = smem_u32(smem);
+    const uint32_t rank = cluster_ctarank();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int* err = reinterpret_cast<int*>(ws + P.off_status);
+    // a stage: W chunks (then the adapters' B rows) | X chunks (then U rows)
+    const uint32_t x_off = kGroup * kRows * 128, x_chunk = P.tb / 2 * 128, u_step = P.tb / 2 * 32;
     if (threadIdx.x == 0) {
         for (int s = 0; s < P.stages; ++s) {
             mbar_init(smem_u32(&bars->full[s]), 1);
@@ -345,205 +493,304 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(smem_u32(&bars->acc_full[b]), 1);
-            mbar_init(smem_u32(&bars->acc_empty[b]), 128);
+            mbar_init(smem_u32(&bars->acc_empty[b]), 8);   // one arrival per reading warp of the pair
         }
         fence_mbar_init();
         tma_prefetch_desc(&maps.w);
         tma_prefetch_desc(&maps.x);
     }
     if (warp == 1) {
-        tmem_alloc(smem_u32(&bars->tmem), 512);
-        tmem_relinquish();
+        tmem_alloc_pair(smem_u32(&bars->tmem), 512);
+        tmem_relinquish_pair();
     }
     tc_fence_before();
-    __syncthreads();
+    cluster_sync();
     tc_fence_after();
     const uint32_t tbase = bars->tmem;
-    const int* meta = reinterpret_cast<const int*>(ws + P.off_meta);
 
     if (warp == 0) {
-        // ---- loads
-        if (lane == 0) {
-            Walk walk(P);
-            Item it;
-            int i = 0;
-            bool ok = true, waited = false;
-            auto stage = [&](uint32_t* dst, uint32_t* fb) -> bool {
+        // ---- loads: this CTA's weight rows and half of the tokens' rows
+        Walk walk(P);
+        Item it;
+        int i = 0, blk_slots = -1, nslots = 0;
+        bool ok = true, waited = !P.sorted;   // X in adapter order comes from the shrink kernel
+        bool meta_ready = false;
+        int held = 0;                         // stages whose W is on its way while X is waited for
+        while (ok && walk.next(P, &it)) {
+            const int n0 = it.tile / P.nb * 2 * kRows + static_cast<int>(rank) * kRows, blk = it.tile % P.nb;
+            const int half = (min(P.tb, P.M - blk * P.tb) + kColStep - 1) / kColStep * (kColStep / 2);   // columns of this CTA's half
+            const int x0 = (P.sorted ? 0 : blk * P.tb) + static_cast<int>(rank) * half;
+            for (int c = it.c0; c < it.c1; c += kGroup, ++i) {
                 const int s = i % P.stages;
-                if (i >= P.stages && !mbar_wait(smem_u32(&bars->empty[s]), ((i / P.stages) - 1) & 1, err, code(kWaitLoad)))
-                    return false;
-                *fb = smem_u32(&bars->full[s]);
-                *dst = ring + s * P.stage_bytes;
-                ++i;
-                return true;
-            };
-            while (ok && walk.next(P, &it)) {
-                const int n0 = it.tile / P.nb * kRows, blk = it.tile % P.nb;
-                uint32_t dst, fb;
-                for (int c = it.c0; c < it.c1; ++c) {
-                    if (!(ok = stage(&dst, &fb))) break;
-                    mbar_arrive_expect_tx(fb, static_cast<uint32_t>(P.stage_bytes));
-                    tma_load_2d(dst, &maps.w, fb, kChunk * c, n0);
-                    tma_load_2d(dst + kRows * 128, &maps.x, fb, kChunk * c, blk * P.tb);
+                ok = i < P.stages || mbar_wait_cluster(smem_u32(&bars->empty[s]), ((i / P.stages) - 1) & 1, err, code(kWaitLoad));
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
+                    break;
                 }
-                if (!ok || it.c1 < P.kc) continue;
+                const int n = min(kGroup, it.c1 - c);
+                const uint32_t fb = mapa(smem_u32(&bars->full[s]), 0), dst = ring + s * P.stage_bytes;
+                if (elect_one()) {
+                    if (rank == 0)
+                        mbar_arrive_expect_tx(smem_u32(&bars->full[s]), 2u * n * (kRows * 128 + x_chunk));
+                    for (int k = 0; k < n; ++k)
+                        tma_load_2d_pair(dst + k * kRows * 128, &maps.w, fb, kChunk * (c + k), n0);
+                    if (waited)
+                        for (int k = 0; k < n; ++k)
+                            tma_load_2d_pair(dst + x_off + k * x_chunk, &maps.x, fb, kChunk * (c + k), x0);
+                }
+                __syncwarp();
                 if (!waited) {
-                    pdl_wait();   // U and the adapters' list come from the shrink kernel
-                    waited = true;
-                }
-                const int* m = meta + static_cast<size_t>(blk) * (P.slots + 1);
-                const int steps = m[0] * P.rsteps;
-                for (int s0 = 0; s0 < steps; s0 += 4) {
-                    if (!(ok = stage(&dst, &fb))) break;
-                    const int n = min(4, steps - s0);
-                    mbar_arrive_expect_tx(fb, static_cast<uint32_t>(n * (kRows + P.tb) * 32));
-                    for (int k = 0; k < n; ++k) {
-                        const int slot = (s0 + k) / P.rsteps, q = (s0 + k) % P.rsteps;
-                        tma_load_3d(dst + k * kRows * 32, &maps.b, fb, q * kStep, n0, m[1 + slot]);
-                        tma_load_2d(dst + kRows * 128 + k * P.tb * 32, &maps.u, fb, 0,
-                                    (blk * P.slots * P.rsteps + s0 + k) * P.tb);
+                    // W of the first stages streams in while the shrink kernel puts X in order
+                    ++held;
+                    if (held == P.stages || c + kGroup >= it.c1) {
+                        pdl_wait();
+                        waited = meta_ready = true;
+                        if (elect_one())
+                            for (int h = 0; h < held; ++h) {
+                                const int hc = c - (held - 1 - h) * kGroup, hs = i - (held - 1 - h);
+                                const uint32_t hb = mapa(smem_u32(&bars->full[hs % P.stages]), 0);
+                                for (int k = 0; k < min(kGroup, it.c1 - hc); ++k)
+                                    tma_load_2d_pair(ring + (hs % P.stages) * P.stage_bytes + x_off + k * x_chunk, &maps.x, hb,
+                                                     kChunk * (hc + k), x0);
+                            }
+                        __syncwarp();
                     }
                 }
             }
-            if (!waited) pdl_wait();
-            // no load may still be in flight when shared memory is released
-            for (int k = i > P.stages ? i - P.stages : 0; k < i; ++k)
-                mbar_wait(smem_u32(&bars->full[k % P.stages]), (k / P.stages) & 1, err, code(kWaitLoad), 100000000ull);
+            if (!ok || it.c1 < P.kc) continue;
+            if (!meta_ready) {
+                pdl_wait();   // U and the adapters' list come from the shrink kernel
+                meta_ready = true;
+            }
+            if (blk != blk_slots) nslots = load_slots(P, ws, blk, bars->slots[0], lane);
+            blk_slots = blk;
+            const int steps = nslots * P.rsteps;
+            for (int s0 = 0; s0 < steps; s0 += kSteps, ++i) {
+                const int s = i % P.stages;
+                ok = i < P.stages || mbar_wait_cluster(smem_u32(&bars->empty[s]), ((i / P.stages) - 1) & 1, err, code(kWaitLoad));
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
+                    break;
+                }
+                const int n = min(kSteps, steps - s0);
+                if (elect_one()) {
+                    const uint32_t fb = mapa(smem_u32(&bars->full[s]), 0), dst = ring + s * P.stage_bytes;
+                    if (rank == 0) mbar_arrive_expect_tx(smem_u32(&bars->full[s]), 2u * n * (kRows * 32 + u_step));
+                    for (int k = 0; k < n; ++k) {
+                        const int slot = (s0 + k) / P.rsteps, q = (s0 + k) % P.rsteps;
+                        const int2 sl = bars->slots[0][slot];
+                        tma_load_3d_pair(dst + k * kRows * 32, &maps.b, fb, q * kStep, n0, sl.x);
+                        // (a box of half a block's rows from the half's first column on; only the covered ones are used)
+                        tma_load_2d_pair(dst + x_off + k * u_step, &maps.u, fb, 0,
+                                         (blk * P.slots * P.rsteps + s0 + k) * P.tb + (sl.y >> 16) +
+                                             static_cast<int>(rank) * (sl.y & 0xffff) / 2);
+                    }
+                }
+                __syncwarp();
+            }
         }
+        if (!meta_ready) pdl_wait();
     } else if (warp == 1) {
-        // ---- MMAs
-        if (lane == 0) {
+        // ---- MMAs of the pair
+        if (rank == 0) {
             Walk walk(P);
             Item it;
-            int i = 0, n = 0;
-            bool ok = true, waited = false;
+            int i = 0, n = 0, blk_slots = -1, nslots = 0;
+            bool ok = true, meta_ready = false;
             for (; ok && walk.next(P, &it); ++n) {
                 const int blk = it.tile % P.nb;
-                const int toks = min(P.tb, P.M - blk * P.tb);
-                const uint32_t idesc = idesc_f16(kRows, (toks + 15) / 16 * 16, Fmt<T>::v, false, false);
+                const int cols = (min(P.tb, P.M - blk * P.tb) + kColStep - 1) / kColStep * kColStep;
+                const uint32_t idesc = idesc_f16(256, cols, Fmt<T>::v, false, false);
                 const uint32_t d = tbase + 256 * (n & 1);
-                if (n >= 2 && !(ok = mbar_wait(smem_u32(&bars->acc_empty[n & 1]), ((n >> 1) - 1) & 1, err, code(kWaitAcc)))) break;
+                ok = n < 2 || mbar_wait_cluster(smem_u32(&bars->acc_empty[n & 1]), ((n >> 1) - 1) & 1, err, code(kWaitAcc));
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
+                    break;
+                }
                 tc_fence_after();
-                uint32_t acc = 0;
-                for (int c = it.c0; c < it.c1; ++c, ++i) {
+                for (int c = it.c0; c < it.c1; c += kGroup, ++i) {
                     const int s = i % P.stages;
-                    if (!(ok = mbar_wait(smem_u32(&bars->full[s]), (i / P.stages) & 1, err, code(kWaitMma)))) break;
-                    tc_fence_after();
-                    const uint32_t a = ring + s * P.stage_bytes;
-                    const uint64_t ad = smem_desc_sw128(a, 16, 1024), bd = smem_desc_sw128(a + kRows * 128, 16, 1024);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        mma_ss(d, ad + static_cast<uint64_t>(2 * k), bd + static_cast<uint64_t>(2 * k), idesc, acc);
-                        acc = 1;
+                    ok = mbar_wait_cluster(smem_u32(&bars->full[s]), (i / P.stages) & 1, err, code(kWaitMma));
+                    if (!__all_sync(0xffffffffu, ok)) {
+                        ok = false;
+                        break;
                     }
-                    mma_commit(smem_u32(&bars->empty[s]));
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t a = ring + s * P.stage_bytes;
+                        for (int k = 0; k < min(kGroup, it.c1 - c); ++k) {
+                            const uint64_t ad = smem_desc_sw128(a + k * kRows * 128, 16, 1024);
+                            const uint64_t bd = smem_desc_sw128(a + x_off + k * x_chunk, 16, 1024);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                mma_ss_pair(d, ad + static_cast<uint64_t>(2 * e), bd + static_cast<uint64_t>(2 * e), idesc,
+                                            c + k > it.c0 || e > 0 ? 1u : 0u);
+                        }
+                        mma_commit_pair_both(smem_u32(&bars->empty[s]));
+                    }
+                    __syncwarp();
                 }
                 if (ok && it.c1 == P.kc) {
-                    if (!waited) {
+                    if (!meta_ready) {
                         pdl_wait();
-                        waited = true;
+                        meta_ready = true;
                     }
-                    const int steps = meta[static_cast<size_t>(blk) * (P.slots + 1)] * P.rsteps;
-                    for (int s0 = 0; s0 < steps; s0 += 4, ++i) {
+                    if (blk != blk_slots) nslots = load_slots(P, ws, blk, bars->slots[1], lane);
+                    blk_slots = blk;
+                    const int steps = nslots * P.rsteps;
+                    for (int s0 = 0; s0 < steps; s0 += kSteps, ++i) {
                         const int s = i % P.stages;
-                        if (!(ok = mbar_wait(smem_u32(&bars->full[s]), (i / P.stages) & 1, err, code(kWaitMma)))) break;
+                        ok = mbar_wait_cluster(smem_u32(&bars->full[s]), (i / P.stages) & 1, err, code(kWaitMma));
+                        if (!__all_sync(0xffffffffu, ok)) {
+                            ok = false;
+                            break;
+                        }
                         tc_fence_after();
-                        const uint32_t a = ring + s * P.stage_bytes;
-                        for (int k = 0; k < min(4, steps - s0); ++k)
-                            mma_ss(d, smem_desc_sw32(a + k * kRows * 32), smem_desc_sw32(a + kRows * 128 + k * P.tb * 32),
-                                   idesc, 1u);
-                        mma_commit(smem_u32(&bars->empty[s]));
+                        if (elect_one()) {
+                            const uint32_t a = ring + s * P.stage_bytes;
+                            for (int k = 0; k < min(kSteps, steps - s0); ++k) {
+                                const int sl = bars->slots[1][(s0 + k) / P.rsteps].y;
+                                mma_ss_pair(d + (sl >> 16), smem_desc_sw32(a + k * kRows * 32), smem_desc_sw32(a + x_off + k * u_step),
+                                            idesc_f16(256, sl & 0xffff, Fmt<T>::v, false, false), 1u);
+                            }
+                            mma_commit_pair_both(smem_u32(&bars->empty[s]));
+                        }
+                        __syncwarp();
                     }
                 }
-                mma_commit(smem_u32(&bars->acc_full[n & 1]));
+                if (elect_one()) mma_commit_pair_both(smem_u32(&bars->acc_full[n & 1]));
+                __syncwarp();
             }
         }
     } else {
         // ---- read-out: thread = weight row = TMEM lane
         const int row = (warp & 3) * 32 + lane;
         const uint32_t trow = tbase + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
+        const uint32_t acc_empty0 = mapa(smem_u32(&bars->acc_empty[0]), 0), acc_empty1 = mapa(smem_u32(&bars->acc_empty[1]), 0);
         Walk walk(P);
         Item it;
         bool ok = true;
-        pdl_wait();   // the partials' counters are cleared by the shrink kernel
+        pdl_wait();   // the counters are cleared and the columns' order is written by the shrink kernel
+        if (P.sorted)
+            for (int c = threadIdx.x - 64; c < P.M; c += 128) bars->perm[c] = reinterpret_cast<const int*>(ws + P.off_perm)[c];
+        asm volatile("bar.sync 1, 128;" ::: "memory");
         for (int n = 0; walk.next(P, &it); ++n) {
             const int blk = it.tile % P.nb, m0 = blk * P.tb, toks = min(P.tb, P.M - m0);
-            const int col = it.tile / P.nb * kRows + row;
+            const int col = it.tile / P.nb * 2 * kRows + static_cast<int>(rank) * kRows + row;
             const uint32_t d = trow + 256 * (n & 1);
-            const bool got = mbar_wait(smem_u32(&bars->acc_full[n & 1]), (n >> 1) & 1, err, code(kWaitOut));
+            const bool got = mbar_wait_cluster(smem_u32(&bars->acc_full[n & 1]), (n >> 1) & 1, err, code(kWaitOut));
             ok = __all_sync(0xffffffffu, got) && ok;
             tc_fence_after();
-            T* out = static_cast<T*>(A.y) + static_cast<long long>(m0) * P.N + col;
-            auto store = [&](int m, float v) {
-                if (!isfinite(v) && ok && meta[static_cast<size_t>(blk) * (P.slots + 1)] > 0)
-                    v = own_element<T>(A, P, ws, blk, m, col);
-                out[static_cast<long long>(m) * P.N] = ElemTraits<T>::from_f(v);
+            const bool any = reinterpret_cast<const int2*>(ws + P.off_meta)[static_cast<size_t>(blk) * (P.slots + 1)].x > 0;
+            auto store = [&](int c, float v) {
+                const int m = P.sorted ? bars->perm[c] : m0 + c;
+                if (!isfinite(v) && ok && any) v = own_element<T>(A, P, ws, blk, c, m, col);
+                static_cast<T*>(A.y)[static_cast<long long>(m) * P.N + col] = ElemTraits<T>::from_f(v);
             };
-            // the CTAs that share the tile
-            int w0 = blockIdx.x, w1 = blockIdx.x;
+            auto release = [&] {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (rank == 0) mbar_arrive(smem_u32(&bars->acc_empty[n & 1]));
+                    else mbar_arrive_remote(n & 1 ? acc_empty1 : acc_empty0);
+                }
+            };
+            // the pairs that share the tile
+            int w0 = blockIdx.x / 2, w1 = w0;
             const long long total = static_cast<long long>(P.tiles - P.full) * P.kc;
             if (it.j >= 0) {
-                w0 = static_cast<int>(((static_cast<long long>(it.j) * P.kc + 1) * P.tail_ctas - 1) / total);
-                w1 = static_cast<int>(((static_cast<long long>(it.j) + 1) * P.kc * P.tail_ctas - 1) / total);
+                w0 = static_cast<int>(((static_cast<long long>(it.j) * P.kc + 1) * P.tail_pairs - 1) / total);
+                w1 = static_cast<int>(((static_cast<long long>(it.j) + 1) * P.kc * P.tail_pairs - 1) / total);
             }
             if (w0 == w1) {
-                for (int m = 0; m < toks; m += 16) {
+                for (int c = 0; c < toks; c += 16) {
                     uint32_t v[16];
-                    tmem_ld16_sync(d + m, v);
+                    tmem_ld16_sync(d + c, v);
                     if (col < P.N)
 #pragma unroll
                         for (int k = 0; k < 16; ++k)
-                            if (m + k < toks) store(m + k, ok ? __uint_as_float(v[k]) : NAN);
+                            if (c + k < toks) store(c + k, ok ? __uint_as_float(v[k]) : NAN);
                 }
-                tc_fence_before();
-                mbar_arrive(smem_u32(&bars->acc_empty[n & 1]));
+                release();
                 continue;
             }
-            float* parts = reinterpret_cast<float*>(ws + P.off_part);
-            auto part = [&](int w) -> float* {
-                // a CTA touches at most two cut tiles: the first into its slot 0, the second into slot 1
-                const int first = static_cast<int>(total * w / P.tail_ctas / P.kc);
-                return parts + (static_cast<size_t>(w) * 2 + (first == it.j ? 0 : 1)) * kRows * P.tb;
+            // partials as float4 of 4 columns: column group g of row r at g * kRows + r
+            float4* parts = reinterpret_cast<float4*>(ws + P.off_part);
+            auto part = [&](int w) -> float4* {
+                // a pair touches at most two cut tiles: the first into its place 0, the second into place 1
+                const int first = static_cast<int>(total * w / P.tail_pairs / P.kc);
+                return parts + ((static_cast<size_t>(w) * 2 + (first == it.j ? 0 : 1)) * 2 + rank) * kRows * P.tb / 4 + row;
             };
-            float* mine = part(blockIdx.x);
-            for (int m = 0; m < toks; m += 16) {
+            const int me = blockIdx.x / 2;
+            float4* mine = part(me);
+            for (int c = 0; c < toks; c += 16) {
                 uint32_t v[16];
-                tmem_ld16_sync(d + m, v);
+                tmem_ld16_sync(d + c, v);
 #pragma unroll
-                for (int k = 0; k < 16; ++k)
-                    mine[(m + k) * kRows + row] = ok ? __uint_as_float(v[k]) : NAN;
+                for (int k = 0; k < 4; ++k)
+                    mine[(c / 4 + k) * kRows] = make_float4(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1]),
+                                                            __uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3]));
             }
-            tc_fence_before();
-            mbar_arrive(smem_u32(&bars->acc_empty[n & 1]));
             __threadfence();
             asm volatile("bar.sync 1, 128;" ::: "memory");
             if (threadIdx.x == 64) {
-                int* count = reinterpret_cast<int*>(ws + P.off_count) + it.j;
+                int* count = reinterpret_cast<int*>(ws + P.off_count) + 2 * it.j + rank;
                 bars->last = atomicAdd(count, 1) == w1 - w0;
             }
             asm volatile("bar.sync 1, 128;" ::: "memory");
-            if (!bars->last) continue;
+            if (!bars->last) {
+                release();
+                continue;
+            }
             __threadfence();
-            for (int m = 0; m < toks; m += 8) {
-                float v[8] = {};
-                for (int w = w0; w <= w1; ++w) {
-                    const float* src = part(w) + m * kRows + row;
+            // add the partials in order, this CTA's own from the accumulator; the others' of 16 columns are
+            // requested together, three pairs at a time, one round trip each
+            for (int c = 0; c < toks; c += 16) {
+                uint32_t own[16];
+                tmem_ld16_sync(d + c, own);
+                float v[16] = {};
+                for (int wa = w0; wa <= w1; wa += 3) {
+                    float4 y[3][4];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) v[k] += __ldcg(src + k * kRows);   // tb is a multiple of 16
+                    for (int i = 0; i < 3; ++i)
+                        if (wa + i <= w1 && wa + i != me) {
+                            const float4* src = part(wa + i) + c / 4 * kRows;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) y[i][k] = __ldcg(src + k * kRows);
+                        }
+#pragma unroll
+                    for (int i = 0; i < 3; ++i)
+                        if (wa + i <= w1) {
+                            const bool self = wa + i == me;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                v[4 * k] += self ? __uint_as_float(own[4 * k]) : y[i][k].x;
+                                v[4 * k + 1] += self ? __uint_as_float(own[4 * k + 1]) : y[i][k].y;
+                                v[4 * k + 2] += self ? __uint_as_float(own[4 * k + 2]) : y[i][k].z;
+                                v[4 * k + 3] += self ? __uint_as_float(own[4 * k + 3]) : y[i][k].w;
+                            }
+                        }
                 }
                 if (col < P.N)
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        if (m + k < toks) store(m + k, v[k]);
+                    for (int k = 0; k < 16; ++k)
+                        if (c + k < toks) store(c + k, ok ? v[k] : NAN);
             }
+            release();
+        }
+    }
+    // ---- teardown
+    __syncthreads();
+    if (threadIdx.x == 0 && *err != 0) {
+        // after a failure, loads or arrivals may still be in flight towards either CTA
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 20000ull) {
         }
     }
     tc_fence_before();
-    __syncthreads();
-    if (warp == 1) {
-        tc_fence_after();
-        tmem_dealloc(tbase, 512);
-    }
+    cluster_sync();   // no CTA leaves (or frees tensor memory) while the pair may still address it
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc_pair(tbase, 512);
 }
 
 template <typename T>
@@ -552,33 +799,42 @@ cudaError_t launch(const LoraArgs& A, unsigned char* ws, int sms, cudaStream_t s
     Maps maps;
     const uint64_t K = static_cast<uint64_t>(A.K), N = static_cast<uint64_t>(A.N), r = static_cast<uint64_t>(A.rank);
     const uint64_t wd[2] = {K, N}, ws1[1] = {K * 2};
-    const uint64_t xd[2] = {K, static_cast<uint64_t>(A.M)}, xs[1] = {static_cast<uint64_t>(A.x_stride) * 2};
+    const uint64_t xd[2] = {K, static_cast<uint64_t>(A.M)}, xs[1] = {(P.sorted ? K : static_cast<uint64_t>(A.x_stride)) * 2};
     const uint64_t bd[3] = {r, N, static_cast<uint64_t>(A.adapters)}, bs[2] = {r * 2, r * N * 2};
     const uint64_t ud[2] = {kStep, static_cast<uint64_t>(P.nb) * P.slots * P.rsteps * P.tb}, us[1] = {kStep * 2};
-    const uint32_t tb = static_cast<uint32_t>(P.tb);
-    const uint32_t wb[2] = {kChunk, kRows}, xb[2] = {kChunk, tb}, bb[3] = {kStep, kRows, 1}, ub[2] = {kStep, tb};
+    const uint32_t half = static_cast<uint32_t>(P.tb) / 2;
+    const uint32_t wb[2] = {kChunk, kRows}, xb[2] = {kChunk, half}, bb[3] = {kStep, kRows, 1}, ub[2] = {kStep, half};
     if (!encode_tmap_16b(&maps.w, A.w, 2, wd, ws1, wb, CU_TENSOR_MAP_SWIZZLE_128B) ||
-        !encode_tmap_16b(&maps.x, A.x, 2, xd, xs, xb, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !encode_tmap_16b(&maps.x, P.sorted ? ws + P.off_x : A.x, 2, xd, xs, xb, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !encode_tmap_16b(&maps.b, A.b, 3, bd, bs, bb, CU_TENSOR_MAP_SWIZZLE_32B) ||
         !encode_tmap_16b(&maps.u, ws + P.off_u, 2, ud, us, ub, CU_TENSOR_MAP_SWIZZLE_32B))
         return cudaErrorInvalidValue;
-    const int units = P.slots + P.tb / kShrinkTok;
-    lora_shrink_kernel<T><<<dim3(units, P.rsteps, P.nb), 32 * kShrinkWarps, 0, s>>>(A, P, ws);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
     const int smem = P.stages * P.stage_bytes + static_cast<int>(sizeof(Bars)) + 1024;
-    e = ensure_dynamic_smem(reinterpret_cast<const void*>(lora_gemm_kernel<T>), kSmemCap + static_cast<int>(sizeof(Bars)) + 1024);
+    cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(lora_gemm_kernel<T>),
+                                        kSmemCap + static_cast<int>(sizeof(Bars)) + 1024);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(P.grid);
-    cfg.blockDim = dim3(kGemmThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
     cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    const int clusters = P.slots + P.tb / kShrinkTok + (P.sorted ? kCopyClusters : 0);
+    // two rank steps a cluster where there are two: x's rows are read once for both
+    const int steps = P.rsteps > 1 ? 2 : 1;
+    cfg.gridDim = dim3(clusters * P.ksplit, ceil_div(P.rsteps, steps), P.nb);
+    cfg.blockDim = dim3(32 * kShrinkWarps);
+    cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = P.ksplit;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    e = steps == 2 ? cudaLaunchKernelEx(&cfg, lora_shrink_kernel<T, 2>, A, P, ws)
+                   : cudaLaunchKernelEx(&cfg, lora_shrink_kernel<T, 1>, A, P, ws);
+    if (e != cudaSuccess) return e;
+    cfg.gridDim = dim3(2 * P.pairs);
+    cfg.blockDim = dim3(kGemmThreads);
+    cfg.dynamicSmemBytes = smem;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
     e = cudaLaunchKernelEx(&cfg, lora_gemm_kernel<T>, maps, P, A, ws);
     count_launches(2);
     return e != cudaSuccess ? e : cudaGetLastError();
