@@ -30,6 +30,8 @@
 #include "sm100_ptx.cuh"
 #include "tma_host.cuh"
 
+#include <cstddef>
+
 namespace mla {
 using namespace sm100;
 
@@ -46,6 +48,8 @@ constexpr int kGemmThreads = 192;     // warp 0 loads, warp 1 issues, warps 2-5 
 constexpr int kSmemCap = 192 * 1024;  // leaves room for a block of the shrink kernel on the SM
 constexpr int kMaxStages = 6;
 constexpr int kMinChunks = 4;         // shortest share of a cut tile
+constexpr int kJoinCols = 64;         // columns of a cut tile that are counted and added at a time
+constexpr int kJoins = kMaxTok / kJoinCols;
 constexpr int kShrinkWarps = 8;
 constexpr int kShrinkTok = 32;        // tokens per shrink cluster
 constexpr int kCopyClusters = 8;      // clusters that copy X into adapter order
@@ -99,7 +103,7 @@ Plan make_plan(int M, int N, int K, int adapters, int rank, int sms) {
         return at;
     };
     p.off_status = take(256);
-    p.off_count = take(sizeof(int) * 2 * static_cast<size_t>(p.pairs));
+    p.off_count = take(sizeof(int) * 2 * kJoins * static_cast<size_t>(p.pairs));
     p.off_meta = take(sizeof(int2) * static_cast<size_t>(p.nb) * (p.slots + 1));
     p.off_perm = take(sizeof(int) * kMaxTok);
     p.off_x = take(p.sorted ? static_cast<size_t>(p.tb) * K * 2 : 0);
@@ -177,7 +181,7 @@ __global__ void __launch_bounds__(32 * kShrinkWarps) lora_shrink_kernel(const Lo
     if (tid == 0) unit_id = -1;
     if (blockIdx.x + blockIdx.y + blockIdx.z == 0) {
         int* count = reinterpret_cast<int*>(ws + P.off_count);
-        for (int i = tid; i < 2 * P.pairs; i += blockDim.x) count[i] = 0;
+        for (int i = tid; i < 2 * kJoins * P.pairs; i += blockDim.x) count[i] = 0;
         if (tid == 0) *reinterpret_cast<int*>(ws + P.off_status) = 0;
     }
     __syncthreads();
@@ -428,16 +432,18 @@ struct Walk {
     }
 };
 
-struct __align__(8) Bars {
+struct __align__(16) Bars {
     uint64_t full[kMaxStages];        // leader: both CTAs' loads of the stage have landed
     uint64_t empty[kMaxStages];       // both: the MMAs have read it
     uint64_t acc_full[2];             // both: the accumulator is complete
     uint64_t acc_empty[2];            // leader: both CTAs have read it out
     uint32_t tmem;
     int last;
-    int perm[kMaxTok];                // output row of each column (sorted)
+    __align__(16) int perm[kMaxTok];  // output row of each column (sorted)
     int2 slots[2][kMaxTok];           // the block's adapters, for the loading and the issuing warp
 };
+
+static_assert(offsetof(Bars, perm) % 16 == 0, "read as int4");
 
 __device__ __forceinline__ int code(int site) { return kStatusTimeout | (site << 8); }
 
@@ -682,10 +688,35 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
             ok = __all_sync(0xffffffffu, got) && ok;
             tc_fence_after();
             const bool any = reinterpret_cast<const int2*>(ws + P.off_meta)[static_cast<size_t>(blk) * (P.slots + 1)].x > 0;
-            auto store = [&](int c, float v) {
-                const int m = P.sorted ? bars->perm[c] : m0 + c;
-                if (!isfinite(v) && ok && any) v = own_element<T>(A, P, ws, blk, c, m, col);
-                static_cast<T*>(A.y)[static_cast<long long>(m) * P.N + col] = ElemTraits<T>::from_f(v);
+            // 16 columns from c on of this thread's weight row
+            auto store16 = [&](int c, const float* v) {
+                if (col >= P.N) return;
+                int m[16];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int4 w = P.sorted ? *reinterpret_cast<const int4*>(bars->perm + c + 4 * k)
+                                            : make_int4(m0 + c + 4 * k, m0 + c + 4 * k + 1, m0 + c + 4 * k + 2, m0 + c + 4 * k + 3);
+                    m[4 * k] = w.x;
+                    m[4 * k + 1] = w.y;
+                    m[4 * k + 2] = w.z;
+                    m[4 * k + 3] = w.w;
+                }
+                bool finite = true;
+#pragma unroll
+                for (int k = 0; k < 16; ++k) finite = finite && isfinite(v[k]);
+                T* y = static_cast<T*>(A.y) + col;
+                if (c + 16 <= toks && ok && (finite || !any)) {
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) y[static_cast<long long>(m[k]) * P.N] = ElemTraits<T>::from_f(v[k]);
+                    return;
+                }
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                    if (c + k < toks) {
+                        float e = ok ? v[k] : NAN;
+                        if (!isfinite(e) && ok && any) e = own_element<T>(A, P, ws, blk, c + k, m[k], col);
+                        y[static_cast<long long>(m[k]) * P.N] = ElemTraits<T>::from_f(e);
+                    }
             };
             auto release = [&] {
                 tc_fence_before();
@@ -704,12 +735,12 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
             }
             if (w0 == w1) {
                 for (int c = 0; c < toks; c += 16) {
-                    uint32_t v[16];
-                    tmem_ld16_sync(d + c, v);
-                    if (col < P.N)
+                    uint32_t u[16];
+                    tmem_ld16_sync(d + c, u);
+                    float v[16];
 #pragma unroll
-                        for (int k = 0; k < 16; ++k)
-                            if (c + k < toks) store(c + k, ok ? __uint_as_float(v[k]) : NAN);
+                    for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(u[k]);
+                    store16(c, v);
                 }
                 release();
                 continue;
@@ -721,60 +752,61 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
                 const int first = static_cast<int>(total * w / P.tail_pairs / P.kc);
                 return parts + ((static_cast<size_t>(w) * 2 + (first == it.j ? 0 : 1)) * 2 + rank) * kRows * P.tb / 4 + row;
             };
-            const int me = blockIdx.x / 2;
+            const int me = blockIdx.x / 2, joins = (toks + kJoinCols - 1) / kJoinCols;
             float4* mine = part(me);
-            for (int c = 0; c < toks; c += 16) {
-                uint32_t v[16];
-                tmem_ld16_sync(d + c, v);
+            // the pairs of a tile begin at different columns, so that those which end together share the additions
+            int at = (me - w0) * joins / (w1 - w0 + 1);
+            for (int b = 0; b < joins; ++b, at = at + 1 < joins ? at + 1 : 0) {
+                const int cb = at * kJoinCols, ce = min(toks, cb + kJoinCols);
+                for (int c = cb; c < ce; c += 16) {
+                    uint32_t v[16];
+                    tmem_ld16_sync(d + c, v);
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    mine[(c / 4 + k) * kRows] = make_float4(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1]),
-                                                            __uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3]));
-            }
-            __threadfence();
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            if (threadIdx.x == 64) {
-                int* count = reinterpret_cast<int*>(ws + P.off_count) + 2 * it.j + rank;
-                bars->last = atomicAdd(count, 1) == w1 - w0;
-            }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            if (!bars->last) {
-                release();
-                continue;
-            }
-            __threadfence();
-            // add the partials in order, this CTA's own from the accumulator; the others' of 16 columns are
-            // requested together, three pairs at a time, one round trip each
-            for (int c = 0; c < toks; c += 16) {
-                uint32_t own[16];
-                tmem_ld16_sync(d + c, own);
-                float v[16] = {};
-                for (int wa = w0; wa <= w1; wa += 3) {
-                    float4 y[3][4];
-#pragma unroll
-                    for (int i = 0; i < 3; ++i)
-                        if (wa + i <= w1 && wa + i != me) {
-                            const float4* src = part(wa + i) + c / 4 * kRows;
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) y[i][k] = __ldcg(src + k * kRows);
-                        }
-#pragma unroll
-                    for (int i = 0; i < 3; ++i)
-                        if (wa + i <= w1) {
-                            const bool self = wa + i == me;
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                v[4 * k] += self ? __uint_as_float(own[4 * k]) : y[i][k].x;
-                                v[4 * k + 1] += self ? __uint_as_float(own[4 * k + 1]) : y[i][k].y;
-                                v[4 * k + 2] += self ? __uint_as_float(own[4 * k + 2]) : y[i][k].z;
-                                v[4 * k + 3] += self ? __uint_as_float(own[4 * k + 3]) : y[i][k].w;
-                            }
-                        }
+                    for (int k = 0; k < 4; ++k)
+                        mine[(c / 4 + k) * kRows] = make_float4(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1]),
+                                                                __uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3]));
                 }
-                if (col < P.N)
+                __threadfence();
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                if (threadIdx.x == 64) {
+                    int* count = reinterpret_cast<int*>(ws + P.off_count) + (2 * it.j + rank) * kJoins + at;
+                    bars->last = atomicAdd(count, 1) == w1 - w0;
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                if (!bars->last) continue;
+                __threadfence();
+                // add the partials in order, this CTA's own from the accumulator; the others' of 32 columns
+                // are requested together, two pairs at a time, one round trip each
+                for (int c = cb; c < ce; c += 32) {
+                    uint32_t own[32];
+                    tmem_ld32_sync(d + c, own);
+                    float v[32] = {};
+                    for (int wa = w0; wa <= w1; wa += 2) {
+                        float4 y[2][8];
 #pragma unroll
-                    for (int k = 0; k < 16; ++k)
-                        if (c + k < toks) store(c + k, ok ? v[k] : NAN);
+                        for (int i = 0; i < 2; ++i)
+                            if (wa + i <= w1 && wa + i != me) {
+                                const float4* src = part(wa + i) + c / 4 * kRows;
+#pragma unroll
+                                for (int k = 0; k < 8; ++k)
+                                    if (k < 4 || c + 16 < ce) y[i][k] = __ldcg(src + k * kRows);
+                            }
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            if (wa + i <= w1) {
+                                const bool self = wa + i == me;
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) {
+                                    v[4 * k] += self ? __uint_as_float(own[4 * k]) : y[i][k].x;
+                                    v[4 * k + 1] += self ? __uint_as_float(own[4 * k + 1]) : y[i][k].y;
+                                    v[4 * k + 2] += self ? __uint_as_float(own[4 * k + 2]) : y[i][k].z;
+                                    v[4 * k + 3] += self ? __uint_as_float(own[4 * k + 3]) : y[i][k].w;
+                                }
+                            }
+                    }
+                    store16(c, v);
+                    if (c + 16 < ce) store16(c + 16, v + 16);
+                }
             }
             release();
         }
