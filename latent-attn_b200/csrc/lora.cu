@@ -43,7 +43,6 @@ constexpr int kChunk = 64;            // K elements per 128-byte row
 constexpr int kGroup = 2;             // chunks per stage
 constexpr int kStep = 16;             // K elements per MMA
 constexpr int kColStep = 32;          // an MMA of a CTA pair covers a multiple of 32 columns, from one on
-constexpr int kSteps = 4 * kGroup;    // rank steps per stage
 constexpr int kGemmThreads = 192;     // warp 0 loads, warp 1 issues, warps 2-5 read out
 constexpr int kSmemCap = 192 * 1024;  // leaves room for a block of the shrink kernel on the SM
 constexpr int kMaxStages = 6;
@@ -52,7 +51,6 @@ constexpr int kJoinCols = 64;         // columns of a cut tile that are counted 
 constexpr int kJoins = kMaxTok / kJoinCols;
 constexpr int kShrinkWarps = 8;
 constexpr int kShrinkTok = 32;        // tokens per shrink cluster
-constexpr int kCopyClusters = 8;      // clusters that copy X into adapter order
 constexpr int kTable = 1024;          // adapters that the shrink kernel counts in a table
 enum : int { kWaitLoad = 1, kWaitMma = 3, kWaitAcc = 4, kWaitOut = 5 };
 
@@ -61,11 +59,12 @@ struct Plan {
     int tb, nb;                       // tokens per block (a multiple of 32), blocks
     int sorted;                       // one block, its columns in adapter order
     int adapters, slots, rsteps;      // most adapters of a block, MMA steps per adapter
+    int kw, rchunks;                  // ranks per row of B's and U's tiles (16, 32 or 64), tiles per adapter
     int kc, tiles;                    // K chunks, tiles (weight rows / 256 x blocks)
     int pairs, full;                  // CTA pairs, whole tiles (a multiple of pairs)
     int tail_pairs;                   // pairs that share the other tiles
     int stages, stage_bytes;
-    int ksplit;                       // CTAs of a shrink cluster
+    int ksplit, clusters, per_blk;    // CTAs of a shrink cluster, clusters in all and per token block
     size_t off_status, off_count, off_meta, off_perm, off_x, off_u, off_part, total;
 };
 
@@ -81,6 +80,8 @@ Plan make_plan(int M, int N, int K, int adapters, int rank, int sms) {
     p.sorted = p.nb == 1 && p.tb > kColStep;
     p.slots = adapters < p.tb ? adapters : p.tb;
     p.rsteps = ceil_div(rank, kStep);
+    p.kw = rank > 32 ? 64 : rank > 16 ? 32 : 16;
+    p.rchunks = ceil_div(rank, p.kw);
     p.kc = ceil_div(K, kChunk);
     p.tiles = ceil_div(N, 2 * kRows) * p.nb;
     p.pairs = sms / 2;
@@ -96,6 +97,13 @@ Plan make_plan(int M, int N, int K, int adapters, int rank, int sms) {
     if (p.stages > kMaxStages) p.stages = kMaxStages;
     p.ksplit = 1;
     while (p.ksplit < 8 && K >= 32 * kShrinkWarps * 2 * p.ksplit) p.ksplit *= 2;
+    // as many shrink clusters as have work, at most two CTAs per SM: they share a token block's units or
+    // walk the blocks
+    const int most = (p.slots < M ? p.slots : M) + (M < p.tb ? M : p.tb) / kShrinkTok;   // units of a block
+    const int qs = ceil_div(p.rsteps, p.rsteps > 1 ? 2 : 1);
+    const int fit = 2 * sms / p.ksplit;
+    p.per_blk = fit / p.nb < 1 ? 1 : fit / p.nb < most * qs ? fit / p.nb : most * qs;
+    p.clusters = p.per_blk * (fit / p.per_blk < p.nb ? fit / p.per_blk : p.nb);
     size_t off = 0;
     auto take = [&](size_t bytes) {
         const size_t at = off;
@@ -107,7 +115,7 @@ Plan make_plan(int M, int N, int K, int adapters, int rank, int sms) {
     p.off_meta = take(sizeof(int2) * static_cast<size_t>(p.nb) * (p.slots + 1));
     p.off_perm = take(sizeof(int) * kMaxTok);
     p.off_x = take(p.sorted ? static_cast<size_t>(p.tb) * K * 2 : 0);
-    p.off_u = take(static_cast<size_t>(p.nb) * p.slots * p.rsteps * p.tb * kStep * 2);
+    p.off_u = take(static_cast<size_t>(p.nb) * p.slots * p.rchunks * p.tb * p.kw * 2);
     p.off_part = take(rest > 0 && p.tail_pairs > rest ? static_cast<size_t>(p.tail_pairs) * 4 * kRows * p.tb * sizeof(float) : 0);
     p.total = off;
     return p;
@@ -141,253 +149,263 @@ __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], uint32_t 
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Cluster (unit, kQ rank steps, token block) of ksplit CTAs that cut K. A unit is one adapter of the
-// token block with up to 32 of its tokens. Each of a CTA's warps takes every (8 ksplit)-th 32 columns
-// of K and holds the 16 kQ ranks x 32 tokens in registers as warp-level MMA tiles, reading A's and x's rows
-// straight from global memory, 16 bytes a lane: the sum over K may take its columns in any order, so
-// lane t of a quad takes columns 8 t .. 8 t + 7 of each 32, for both operands alike. Tokens are
-// gathered by their rows' addresses. Partial sums meet in shared memory, in warp order and then in
-// CTA order. (16 ranks x 32 tokens are too small for tcgen05's 128-row tile; the kernel is a few
-// microseconds of latency beside the GEMM's first loads of W.)
-// The clusters after the units copy X's rows into adapter order.
-template <typename T, int kQ>
-__global__ void __launch_bounds__(32 * kShrinkWarps) lora_shrink_kernel(const LoraArgs A, const Plan P, unsigned char* ws) {
-    __shared__ __align__(16) int ids[kMaxTok];
-    __shared__ int col_of[kMaxTok], tok_of[kMaxTok];      // a token's column, and back
-    __shared__ int base[kMaxTok];                         // per leader (an adapter's first token): first column
-    __shared__ int unit_id, unit_sub, unit_slot, unit_lo, unit_n;
-    __shared__ int warp_sum[kShrinkWarps];
-    __shared__ int list[kShrinkTok];
-    // per adapter while the tokens are counted (tokens so far, first, last), then the warps' partial sums
-    __shared__ union {
-        struct {
-            short n[kTable], first[kTable], last[kTable];
-        } tab;
-        float red[kShrinkWarps][kStep][kShrinkTok + 1];
-    } sh;
-    __shared__ float part[kQ][kStep][kShrinkTok];         // this CTA's sums
-    pdl_launch_dependents();
+// The tokens of a block by adapter.
+struct Order {
+    int ids[kMaxTok];                       // adapter, or -1
+    short col_of[kMaxTok], tok_of[kMaxTok]; // a token's column, and back (-1)
+    // of an adapter, at its first token: first column in adapter order, slot, first unit, columns an MMA covers
+    short base[kMaxTok], slot[kMaxTok], unit0[kMaxTok];
+    short2 cover[kMaxTok];
+    short unit_lead[kMaxTok + kMaxTok / kShrinkTok];   // a unit's adapter, as its first token
+    int warp_sum[kShrinkWarps];
+    int slots, units;
+};
+// Per adapter while the tokens are counted: tokens so far, first, last.
+struct Table {
+    short n[kTable], first[kTable], last[kTable];
+};
+struct Own {
+    int id, first, rank_in;               // this thread's token: adapter, the adapter's first token, place among its tokens
+};
+
+// Sorts block blk's tokens by adapter (stable), one thread a token. Adapters follow the order of their
+// first tokens; tokens without one come last.
+__device__ __forceinline__ Own order_tokens(Order& o, Table& tab, const LoraArgs& A, const Plan& P, int blk) {
     const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
-    const int unit = blockIdx.x / P.ksplit, kpart = blockIdx.x % P.ksplit, blk = blockIdx.z;
-    const int q0 = blockIdx.y * kQ;
-    const int units = P.slots + P.tb / kShrinkTok;
     const int m0 = blk * P.tb, mt = min(P.tb, P.M - m0);
-    {
-        const int id = tid < mt ? A.ids[m0 + tid] : -1;
-        ids[tid] = id >= 0 && id < P.adapters ? id : -1;
-        tok_of[tid] = -1;
-    }
-    if (tid < kShrinkTok) list[tid] = -1;
-    if (tid == 0) unit_id = -1;
-    if (blockIdx.x + blockIdx.y + blockIdx.z == 0) {
-        int* count = reinterpret_cast<int*>(ws + P.off_count);
-        for (int i = tid; i < 2 * kJoins * P.pairs; i += blockDim.x) count[i] = 0;
-        if (tid == 0) *reinterpret_cast<int*>(ws + P.off_status) = 0;
-    }
-    __syncthreads();
-    // this token's rank among its adapter's (or among those without one), the adapter's first and last token
-    const int id = ids[tid];
+    __syncthreads();   // (the block before has been read)
+    const int raw = tid < mt ? A.ids[m0 + tid] : -1, id = raw >= 0 && raw < P.adapters ? raw : -1;
+    o.ids[tid] = id;
+    o.tok_of[tid] = -1;
     int count = 0, rank_in = 0, first = kMaxTok, last = 0;
     if (P.adapters <= kTable) {
         // one warp after the other enters its tokens, 32 at a time matched among each other
-        for (int i = tid; i < P.adapters; i += blockDim.x) sh.tab.n[i] = 0;
+        for (int i = tid; i < P.adapters; i += blockDim.x) tab.n[i] = 0;
         __syncthreads();
         const unsigned same = __match_any_sync(0xffffffffu, id), less = (1u << lane) - 1;
-        for (int w = 0; w < kShrinkWarps; ++w) {
+        for (int w = 0; w < kShrinkWarps && w * 32 < mt; ++w) {
             if (w == warp) {
-                if (id >= 0) rank_in = sh.tab.n[id] + __popc(same & less);
+                if (id >= 0) rank_in = tab.n[id] + __popc(same & less);
                 __syncwarp();
                 if (id >= 0 && lane == 31 - __clz(same)) {
-                    if (rank_in + 1 == __popc(same)) sh.tab.first[id] = static_cast<short>(warp * 32 + __ffs(same) - 1);
-                    sh.tab.n[id] = static_cast<short>(rank_in + 1);
-                    sh.tab.last[id] = static_cast<short>(tid);
+                    if (rank_in + 1 == __popc(same)) tab.first[id] = static_cast<short>(warp * 32 + __ffs(same) - 1);
+                    tab.n[id] = static_cast<short>(rank_in + 1);
+                    tab.last[id] = static_cast<short>(tid);
                 }
             }
             __syncthreads();
         }
         if (id >= 0) {
-            count = sh.tab.n[id];
-            first = sh.tab.first[id];
-            last = sh.tab.last[id];
+            count = tab.n[id];
+            first = tab.first[id];
+            last = tab.last[id];
         }
     } else {
-        for (int j0 = 0; j0 < mt; j0 += 4) {
-            const int4 v = *reinterpret_cast<const int4*>(ids + j0);
-            const int w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (w[k] == id && id >= 0) {
-                    if (count == 0) first = j0 + k;
-                    last = j0 + k;
-                    rank_in += j0 + k < tid;
-                    ++count;
-                }
-        }
-    }
-    {
-        // tokens without an adapter before this one
-        const unsigned none = __ballot_sync(0xffffffffu, id < 0);
-        if (lane == 0) warp_sum[warp] = __popc(none);
         __syncthreads();
-        if (id < 0) {
-            rank_in = __popc(none & ((1u << lane) - 1));
-            for (int w = 0; w < warp; ++w) rank_in += warp_sum[w];
-        }
-        __syncthreads();
+        for (int j = 0; j < mt; ++j)
+            if (o.ids[j] == id && id >= 0) {
+                if (count == 0) first = j;
+                last = j;
+                rank_in += j < tid;
+                ++count;
+            }
     }
+    const unsigned none = __ballot_sync(0xffffffffu, id < 0);
+    if (lane == 0) o.warp_sum[warp] = __popc(none);
+    __syncthreads();
+    if (id < 0) {
+        rank_in = __popc(none & ((1u << lane) - 1));
+        for (int w = 0; w < warp; ++w) rank_in += o.warp_sum[w];
+    }
+    __syncthreads();
     const bool leader = id >= 0 && first == tid;
     const int groups = leader ? (count + kShrinkTok - 1) / kShrinkTok : 0;
     // sums over the leaders before: adapters, units, tokens (each below 1024)
     const int v = leader ? 1 | groups << 10 | count << 20 : 0;
     int x = v;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int a = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += a;
+    for (int d = 1; d < 32; d <<= 1) {
+        const int a = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += a;
     }
-    if (lane == 31) warp_sum[warp] = x;
+    if (lane == 31) o.warp_sum[warp] = x;
     __syncthreads();
     int total = 0, before = x - v;
     for (int w = 0; w < kShrinkWarps; ++w) {
-        if (w < warp) before += warp_sum[w];
-        total += warp_sum[w];
+        if (w < warp) before += o.warp_sum[w];
+        total += o.warp_sum[w];
     }
-    const int slot = before & 1023, u0 = before >> 10 & 1023, b0 = before >> 20;
-    int2* meta = reinterpret_cast<int2*>(ws + P.off_meta) + static_cast<size_t>(blk) * (P.slots + 1);
-    const bool writer = blockIdx.x == 0 && q0 == 0;
     if (leader) {
-        base[tid] = b0;
+        const int u0 = before >> 10 & 1023, b0 = before >> 20;
+        o.base[tid] = static_cast<short>(b0);
+        o.slot[tid] = static_cast<short>(before & 1023);
+        o.unit0[tid] = static_cast<short>(u0);
+        for (int i = 0; i < groups; ++i) o.unit_lead[u0 + i] = static_cast<short>(tid);
         // the columns an MMA covers: the adapter's tokens (all between its first and its last where the
         // block is not sorted), from a multiple of 32 (where an accumulator may begin) to one
         const int c0 = P.sorted ? b0 : first, c1 = P.sorted ? b0 + count : last + 1;
-        const int lo = c0 / kColStep * kColStep, n = (c1 - lo + kColStep - 1) / kColStep * kColStep;
-        if (unit >= u0 && unit < u0 + groups) {
-            unit_id = id;
-            unit_slot = slot;
-            unit_sub = unit - u0;
-            unit_lo = lo;
-            unit_n = n;
-        }
-        if (writer) meta[1 + slot] = pack_slot(id, lo, n);
+        const int lo = c0 / kColStep * kColStep;
+        o.cover[tid] = make_short2(static_cast<short>(lo), static_cast<short>((c1 - lo + kColStep - 1) / kColStep * kColStep));
     }
-    if (writer && tid == 0) meta[0] = make_int2(total & 1023, 0);
+    if (tid == 0) {
+        o.slots = total & 1023;
+        o.units = total >> 10 & 1023;
+    }
     __syncthreads();
     if (tid < mt) {
-        const int c = !P.sorted ? tid : id >= 0 ? base[first] + rank_in : (total >> 20) + rank_in;
-        col_of[tid] = c;
-        tok_of[c] = tid;
-        if (writer && P.sorted) reinterpret_cast<int*>(ws + P.off_perm)[c] = tid;
+        const int c = !P.sorted ? tid : id >= 0 ? o.base[first] + rank_in : (total >> 20) + rank_in;
+        o.col_of[tid] = static_cast<short>(c);
+        o.tok_of[c] = static_cast<short>(tid);
     }
-    const int a = unit_id, sub = unit_sub;
-    if (tid < mt && a >= 0 && id == a && rank_in / kShrinkTok == sub) list[rank_in % kShrinkTok] = tid;
     __syncthreads();
-    if (unit >= units) {
-        // copy: the clusters' CTAs take the columns in turn (one rank step's worth of blocks is enough)
-        if (q0 == 0) {
+    return {id, first, rank_in};
+}
+
+// Clusters of ksplit CTAs, which cut K, walk items of one unit and kQ rank steps: a unit is one adapter
+// of a token block with up to 32 of its tokens. Each of a CTA's warps takes every (8 ksplit)-th 32
+// columns of K and holds the 16 kQ ranks x 32 tokens in registers as warp-level MMA tiles, reading A's
+// and x's rows straight from global memory, 16 bytes a lane: the sum over K may take its columns in any
+// order, so lane t of a quad takes columns 8 t .. 8 t + 7 of each 32, for both operands alike. Tokens
+// are gathered by their rows' addresses. Partial sums meet in shared memory, in warp order and then in
+// CTA order. (16 ranks x 32 tokens are too small for tcgen05's 128-row tile; the kernel runs beside the
+// GEMM's K columns, one CTA an SM.)
+template <typename T, int kQ>
+__global__ void __launch_bounds__(32 * kShrinkWarps, 2) lora_shrink_kernel(const LoraArgs A, const Plan P, unsigned char* ws) {
+    __shared__ Order o;
+    __shared__ int list[kShrinkTok];
+    __shared__ union {
+        Table tab;
+        float red[kShrinkWarps][kStep][kShrinkTok + 1];   // the warps' partial sums
+    } sh;
+    __shared__ float part[kQ][kStep][kShrinkTok];         // this CTA's sums
+    pdl_launch_dependents();
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+    const int cluster = blockIdx.x / P.ksplit, kpart = blockIdx.x % P.ksplit;
+    if (blockIdx.x == 0) {
+        int* count = reinterpret_cast<int*>(ws + P.off_count);
+        for (int i = tid; i < 2 * kJoins * P.pairs; i += blockDim.x) count[i] = 0;
+        if (tid == 0) *reinterpret_cast<int*>(ws + P.off_status) = 0;
+    }
+    const int qsteps = (P.rsteps + kQ - 1) / kQ;
+    for (int blk = cluster / P.per_blk; blk < P.nb; blk += P.clusters / P.per_blk) {
+        const int m0 = blk * P.tb;
+        const Own own = order_tokens(o, sh.tab, A, P, blk);
+        if (cluster % P.per_blk == 0 && kpart == 0) {
+            int2* meta = reinterpret_cast<int2*>(ws + P.off_meta) + static_cast<size_t>(blk) * (P.slots + 1);
+            if (own.id >= 0 && own.first == tid) meta[1 + o.slot[tid]] = pack_slot(own.id, o.cover[tid].x, o.cover[tid].y);
+            if (tid == 0) meta[0] = make_int2(o.slots, 0);
+        }
+        if (P.sorted) {
+            // X's rows in adapter order, and the order; the CTAs take the columns in turn
             const int nvec = P.K / 8;
-            T* xp = reinterpret_cast<T*>(ws + P.off_x);
-            for (int c = (unit - units) * P.ksplit + kpart; c < mt; c += kCopyClusters * P.ksplit) {
-                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(A.x) + static_cast<long long>(tok_of[c]) * A.x_stride);
-                uint4* dst = reinterpret_cast<uint4*>(xp + static_cast<size_t>(c) * P.K);
+            if (blockIdx.x == 0 && tid < P.M) reinterpret_cast<int*>(ws + P.off_perm)[tid] = o.tok_of[tid];
+            for (int c = blockIdx.x; c < P.M; c += gridDim.x) {
+                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(A.x) + static_cast<long long>(o.tok_of[c]) * A.x_stride);
+                uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(ws + P.off_x) + static_cast<size_t>(c) * P.K);
+#pragma unroll 4
                 for (int i = tid; i < nvec; i += blockDim.x) dst[i] = __ldg(src + i);
             }
         }
-        return;   // the whole cluster
-    }
-    if (a < 0) return;   // the whole cluster: no such unit
-    const int g = lane / 4, t = lane % 4;
-    const T* arow[kQ][2];
-    const T* xrow[4];
+        for (int item = cluster % P.per_blk; item < o.units * qsteps; item += P.per_blk) {
+            const int lead = o.unit_lead[item / qsteps], sub = item / qsteps - o.unit0[lead], q0 = item % qsteps * kQ;
+            const int a = o.ids[lead], unit_slot = o.slot[lead], unit_lo = o.cover[lead].x, unit_n = o.cover[lead].y;
+            if (tid < kShrinkTok) list[tid] = -1;
+            __syncthreads();
+            if (own.id == a && own.rank_in / kShrinkTok == sub) list[own.rank_in % kShrinkTok] = tid;
+            __syncthreads();
+            const int g = lane / 4, t = lane % 4;
+            const T* arow = static_cast<const T*>(A.a) + (static_cast<long long>(a) * P.r + q0 * kStep + g) * P.K;
+            const int left = P.r - q0 * kStep - g;   // ranks from this lane's first on
+            const T* xrow[4];
+            int nt = 0;
 #pragma unroll
-    for (int e = 0; e < kQ; ++e)
+            for (int i = 0; i < 4; ++i) {
+                const int m = list[8 * i + g];
+                xrow[i] = m >= 0 ? static_cast<const T*>(A.x) + (m0 + m) * A.x_stride : nullptr;
+                if (list[8 * i] >= 0) nt = i + 1;
+            }
+            float acc[kQ][4][4] = {};
+            constexpr int kUnroll = kQ == 1 ? 4 : 2;
+            const int stride = 32 * kShrinkWarps * P.ksplit;
+            for (int k0 = 32 * (kpart * kShrinkWarps + warp); k0 < P.K; k0 += stride * kUnroll) {
+                uint4 va[kUnroll][kQ][2], vx[kUnroll][4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int k = (q0 + e) * kStep + g + 8 * i;
-            arow[e][i] = k < P.r ? static_cast<const T*>(A.a) + (static_cast<long long>(a) * P.r + k) * P.K : nullptr;
-        }
-    int nt = 0;
+                for (int j = 0; j < kUnroll; ++j) {
+                    const int k = k0 + j * stride + 8 * t;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int m = list[8 * i + g];
-        xrow[i] = m >= 0 ? static_cast<const T*>(A.x) + (m0 + m) * A.x_stride : nullptr;
-        if (list[8 * i] >= 0) nt = i + 1;
-    }
-    float acc[kQ][4][4] = {};
-    constexpr int kUnroll = kQ == 1 ? 4 : 2;
-    const int stride = 32 * kShrinkWarps * P.ksplit;
-    for (int k0 = 32 * (kpart * kShrinkWarps + warp); k0 < P.K; k0 += stride * kUnroll) {
-        uint4 va[kUnroll][kQ][2], vx[kUnroll][4];
+                    for (int e = 0; e < kQ; ++e)
 #pragma unroll
-        for (int j = 0; j < kUnroll; ++j) {
-            const int k = k0 + j * stride + 8 * t;
+                        for (int i = 0; i < 2; ++i)
+                            va[j][e][i] = e * kStep + 8 * i < left && k < P.K
+                                              ? __ldg(reinterpret_cast<const uint4*>(arow + (e * kStep + 8 * i) * static_cast<long long>(P.K) + k))
+                                              : make_uint4(0, 0, 0, 0);
 #pragma unroll
-            for (int e = 0; e < kQ; ++e)
+                    for (int i = 0; i < 4; ++i)
+                        vx[j][i] = xrow[i] && k < P.K ? __ldg(reinterpret_cast<const uint4*>(xrow[i] + k)) : make_uint4(0, 0, 0, 0);
+                }
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    va[j][e][i] = arow[e][i] && k < P.K ? __ldg(reinterpret_cast<const uint4*>(arow[e][i] + k)) : make_uint4(0, 0, 0, 0);
+                for (int j = 0; j < kUnroll; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                vx[j][i] = xrow[i] && k < P.K ? __ldg(reinterpret_cast<const uint4*>(xrow[i] + k)) : make_uint4(0, 0, 0, 0);
-        }
+                    for (int i = 0; i < 4; ++i)
+                        if (i < nt)
 #pragma unroll
-        for (int j = 0; j < kUnroll; ++j)
+                            for (int e = 0; e < kQ; ++e) {
+                                const uint4 r0 = va[j][e][0], r1 = va[j][e][1], v = vx[j][i];
+                                mma16816<T>(acc[e][i], r0.x, r1.x, r0.y, r1.y, v.x, v.y);
+                                mma16816<T>(acc[e][i], r0.z, r1.z, r0.w, r1.w, v.z, v.w);
+                            }
+            }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (i < nt)
+            for (int e = 0; e < kQ; ++e) {
+                __syncthreads();   // (the step before has been read)
 #pragma unroll
-                    for (int e = 0; e < kQ; ++e) {
-                        const uint4 r0 = va[j][e][0], r1 = va[j][e][1], v = vx[j][i];
-                        mma16816<T>(acc[e][i], r0.x, r1.x, r0.y, r1.y, v.x, v.y);
-                        mma16816<T>(acc[e][i], r0.z, r1.z, r0.w, r1.w, v.z, v.w);
+                for (int i = 0; i < 4; ++i) {
+                    sh.red[warp][g][8 * i + 2 * t] = acc[e][i][0];
+                    sh.red[warp][g][8 * i + 2 * t + 1] = acc[e][i][1];
+                    sh.red[warp][g + 8][8 * i + 2 * t] = acc[e][i][2];
+                    sh.red[warp][g + 8][8 * i + 2 * t + 1] = acc[e][i][3];
+                }
+                __syncthreads();
+                for (int i = tid; i < kStep * kShrinkTok; i += blockDim.x) {
+                    float s = 0.f;
+#pragma unroll
+                    for (int w = 0; w < kShrinkWarps; ++w) s += sh.red[w][i / kShrinkTok][i % kShrinkTok];
+                    part[e][i / kShrinkTok][i % kShrinkTok] = s;
+                }
+            }
+            if (P.ksplit > 1) cluster_sync();
+            else __syncthreads();
+            // the adapter's U rows: its tokens' values, zeros in the other columns that the MMA covers; the
+            // cluster's CTAs take the tokens in turn
+            const float scale = A.scales ? A.scales[a] : 1.f;
+#pragma unroll
+            for (int e = 0; e < kQ; ++e) {
+                if (q0 + e >= P.rsteps) break;
+                const int spc = P.kw / kStep, q = q0 + e;
+                T* u = reinterpret_cast<T*>(ws + P.off_u) + q % spc * kStep +
+                       ((static_cast<size_t>(blk) * P.slots + unit_slot) * P.rchunks + q / spc) * P.tb * P.kw;
+                for (int i = tid + kpart * blockDim.x; i < kStep * kShrinkTok; i += blockDim.x * P.ksplit) {
+                    const int k = i % kStep, j = i / kStep, m = list[j];
+                    if (m < 0) continue;
+                    const uint32_t at = smem_u32(&part[e][k][j]);
+                    float s = 0.f;
+                    for (int c = 0; c < P.ksplit; ++c) {
+                        float y;
+                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y) : "r"(mapa(at, c)));
+                        s += y;
                     }
-    }
-#pragma unroll
-    for (int e = 0; e < kQ; ++e) {
-        __syncthreads();   // (the table, or the step before, has been read)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            sh.red[warp][g][8 * i + 2 * t] = acc[e][i][0];
-            sh.red[warp][g][8 * i + 2 * t + 1] = acc[e][i][1];
-            sh.red[warp][g + 8][8 * i + 2 * t] = acc[e][i][2];
-            sh.red[warp][g + 8][8 * i + 2 * t + 1] = acc[e][i][3];
-        }
-        __syncthreads();
-        for (int i = tid; i < kStep * kShrinkTok; i += blockDim.x) {
-            float s = 0.f;
-#pragma unroll
-            for (int w = 0; w < kShrinkWarps; ++w) s += sh.red[w][i / kShrinkTok][i % kShrinkTok];
-            part[e][i / kShrinkTok][i % kShrinkTok] = s;
-        }
-    }
-    if (P.ksplit > 1) cluster_sync();
-    else __syncthreads();
-    // the adapter's U rows: its tokens' values, zeros in the other columns that the MMA covers; the
-    // cluster's CTAs take the tokens in turn
-    const float scale = A.scales ? A.scales[a] : 1.f;
-#pragma unroll
-    for (int e = 0; e < kQ; ++e) {
-        if (q0 + e >= P.rsteps) break;
-        T* u = reinterpret_cast<T*>(ws + P.off_u) +
-               (static_cast<size_t>(blk) * P.slots * P.rsteps + unit_slot * P.rsteps + q0 + e) * P.tb * kStep;
-        for (int i = tid + kpart * blockDim.x; i < kStep * kShrinkTok; i += blockDim.x * P.ksplit) {
-            const int k = i % kStep, j = i / kStep, m = list[j];
-            if (m < 0) continue;
-            const uint32_t at = smem_u32(&part[e][k][j]);
-            float s = 0.f;
-            for (int c = 0; c < P.ksplit; ++c) {
-                float y;
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y) : "r"(mapa(at, c)));
-                s += y;
+                    u[o.col_of[m] * P.kw + k] = ElemTraits<T>::from_f(s * scale);
+                }
+                if (sub == 0 && kpart == P.ksplit - 1)
+                    for (int i = tid; i < unit_n * 2; i += blockDim.x) {
+                        const int c = unit_lo + i / 2, m = o.tok_of[c];
+                        if (m < 0 || o.ids[m] != a) *reinterpret_cast<uint4*>(u + c * P.kw + i % 2 * 8) = make_uint4(0, 0, 0, 0);
+                    }
             }
-            u[col_of[m] * kStep + k] = ElemTraits<T>::from_f(s * scale);
+            if (P.ksplit > 1) cluster_sync();   // no CTA leaves or goes on while its sums may be read
+            else __syncthreads();
         }
-        if (sub == 0 && kpart == P.ksplit - 1)
-            for (int i = tid; i < unit_n * 2; i += blockDim.x) {
-                const int c = unit_lo + i / 2, m = tok_of[c];
-                if (m < 0 || ids[m] != a) reinterpret_cast<uint4*>(u)[unit_lo * 2 + i] = make_uint4(0, 0, 0, 0);
-            }
     }
-    if (P.ksplit > 1) cluster_sync();   // no CTA leaves while its sums may be read
 }
 
 // ------------------------------------------------------------------------------------- GEMM
@@ -447,6 +465,11 @@ static_assert(offsetof(Bars, perm) % 16 == 0, "read as int4");
 
 __device__ __forceinline__ int code(int site) { return kStatusTimeout | (site << 8); }
 
+// K-major tile whose rows hold kw ranks, swizzled to its row length
+__device__ __forceinline__ uint64_t rank_desc(uint32_t addr, int kw) {
+    return kw == 64 ? smem_desc_sw128(addr, 16, 1024) : kw == 32 ? smem_desc_sw64(addr) : smem_desc_sw32(addr);
+}
+
 // The adapters of token block blk into sl (one warp); returns how many.
 __device__ __forceinline__ int load_slots(const Plan& P, const unsigned char* ws, int blk, int2* sl, int lane) {
     const int2* meta = reinterpret_cast<const int2*>(ws + P.off_meta) + static_cast<size_t>(blk) * (P.slots + 1);
@@ -473,8 +496,8 @@ __device__ __noinline__ float own_element(const LoraArgs& A, const Plan& P, cons
     const T* u = reinterpret_cast<const T*>(ws + P.off_u);
     const T* b = static_cast<const T*>(A.b) + (static_cast<long long>(id) * P.N + n) * P.r;
     for (int k = 0; k < P.r; ++k) {
-        const size_t step = static_cast<size_t>(blk) * P.slots * P.rsteps + slot * P.rsteps + k / kStep;
-        v = fmaf(ElemTraits<T>::to_f(u[(step * P.tb + c) * kStep + k % kStep]), ElemTraits<T>::to_f(b[k]), v);
+        const size_t chunk = (static_cast<size_t>(blk) * P.slots + slot) * P.rchunks + k / P.kw;
+        v = fmaf(ElemTraits<T>::to_f(u[(chunk * P.tb + c) * P.kw + k % P.kw]), ElemTraits<T>::to_f(b[k]), v);
     }
     return v;
 }
@@ -491,7 +514,9 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int* err = reinterpret_cast<int*>(ws + P.off_status);
     // a stage: W chunks (then the adapters' B rows) | X chunks (then U rows)
-    const uint32_t x_off = kGroup * kRows * 128, x_chunk = P.tb / 2 * 128, u_step = P.tb / 2 * 32;
+    const uint32_t x_off = kGroup * kRows * 128, x_chunk = P.tb / 2 * 128;
+    const uint32_t b_chunk = kRows * P.kw * 2, u_chunk = P.tb / 2 * P.kw * 2;
+    const int per_stage = kGroup * kChunk / P.kw;   // of B's and U's tiles
     if (threadIdx.x == 0) {
         for (int s = 0; s < P.stages; ++s) {
             mbar_init(smem_u32(&bars->full[s]), 1);
@@ -516,6 +541,8 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
 
     if (warp == 0) {
         // ---- loads: this CTA's weight rows and half of the tokens' rows
+        // (this and the issuing warp start before the shrink kernel has cleared the status word: their waits
+        // end on completion or on their own limit and do not look at it)
         Walk walk(P);
         Item it;
         int i = 0, blk_slots = -1, nslots = 0;
@@ -528,7 +555,7 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
             const int x0 = (P.sorted ? 0 : blk * P.tb) + static_cast<int>(rank) * half;
             for (int c = it.c0; c < it.c1; c += kGroup, ++i) {
                 const int s = i % P.stages;
-                ok = i < P.stages || mbar_wait_cluster(smem_u32(&bars->empty[s]), ((i / P.stages) - 1) & 1, err, code(kWaitLoad));
+                ok = i < P.stages || mbar_wait_cluster_full(smem_u32(&bars->empty[s]), ((i / P.stages) - 1) & 1, err, code(kWaitLoad));
                 if (!__all_sync(0xffffffffu, ok)) {
                     ok = false;
                     break;
@@ -570,26 +597,29 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
             }
             if (blk != blk_slots) nslots = load_slots(P, ws, blk, bars->slots[0], lane);
             blk_slots = blk;
-            const int steps = nslots * P.rsteps;
-            for (int s0 = 0; s0 < steps; s0 += kSteps, ++i) {
+            const int chunks = nslots * P.rchunks;
+            for (int s0 = 0; s0 < chunks; s0 += per_stage, ++i) {
                 const int s = i % P.stages;
-                ok = i < P.stages || mbar_wait_cluster(smem_u32(&bars->empty[s]), ((i / P.stages) - 1) & 1, err, code(kWaitLoad));
+                ok = i < P.stages || mbar_wait_cluster_full(smem_u32(&bars->empty[s]), ((i / P.stages) - 1) & 1, err, code(kWaitLoad));
                 if (!__all_sync(0xffffffffu, ok)) {
                     ok = false;
                     break;
                 }
-                const int n = min(kSteps, steps - s0);
+                const int n = min(per_stage, chunks - s0);
                 if (elect_one()) {
                     const uint32_t fb = mapa(smem_u32(&bars->full[s]), 0), dst = ring + s * P.stage_bytes;
-                    if (rank == 0) mbar_arrive_expect_tx(smem_u32(&bars->full[s]), 2u * n * (kRows * 32 + u_step));
+                    if (rank == 0) {
+                        uint32_t bytes = 2u * n * b_chunk;
+                        for (int k = 0; k < n; ++k) bytes += (bars->slots[0][(s0 + k) / P.rchunks].y & 0xffff) * P.kw * 2;
+                        mbar_arrive_expect_tx(smem_u32(&bars->full[s]), bytes);
+                    }
                     for (int k = 0; k < n; ++k) {
-                        const int slot = (s0 + k) / P.rsteps, q = (s0 + k) % P.rsteps;
-                        const int2 sl = bars->slots[0][slot];
-                        tma_load_3d_pair(dst + k * kRows * 32, &maps.b, fb, q * kStep, n0, sl.x);
-                        // (a box of half a block's rows from the half's first column on; only the covered ones are used)
-                        tma_load_2d_pair(dst + x_off + k * u_step, &maps.u, fb, 0,
-                                         (blk * P.slots * P.rsteps + s0 + k) * P.tb + (sl.y >> 16) +
-                                             static_cast<int>(rank) * (sl.y & 0xffff) / 2);
+                        const int2 sl = bars->slots[0][(s0 + k) / P.rchunks];
+                        tma_load_3d_pair(dst + k * b_chunk, &maps.b, fb, (s0 + k) % P.rchunks * P.kw, n0, sl.x);
+                        const int half_n = (sl.y & 0xffff) / 2;
+                        const int u0 = (blk * P.slots * P.rchunks + s0 + k) * P.tb + (sl.y >> 16) + static_cast<int>(rank) * half_n;
+                        for (int c = 0; c < half_n; c += kColStep / 2)
+                            tma_load_2d_pair(dst + x_off + k * u_chunk + c * P.kw * 2, &maps.u, fb, 0, u0 + c);
                     }
                 }
                 __syncwarp();
@@ -608,7 +638,7 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
                 const int cols = (min(P.tb, P.M - blk * P.tb) + kColStep - 1) / kColStep * kColStep;
                 const uint32_t idesc = idesc_f16(256, cols, Fmt<T>::v, false, false);
                 const uint32_t d = tbase + 256 * (n & 1);
-                ok = n < 2 || mbar_wait_cluster(smem_u32(&bars->acc_empty[n & 1]), ((n >> 1) - 1) & 1, err, code(kWaitAcc));
+                ok = n < 2 || mbar_wait_cluster_full(smem_u32(&bars->acc_empty[n & 1]), ((n >> 1) - 1) & 1, err, code(kWaitAcc));
                 if (!__all_sync(0xffffffffu, ok)) {
                     ok = false;
                     break;
@@ -616,7 +646,7 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
                 tc_fence_after();
                 for (int c = it.c0; c < it.c1; c += kGroup, ++i) {
                     const int s = i % P.stages;
-                    ok = mbar_wait_cluster(smem_u32(&bars->full[s]), (i / P.stages) & 1, err, code(kWaitMma));
+                    ok = mbar_wait_cluster_full(smem_u32(&bars->full[s]), (i / P.stages) & 1, err, code(kWaitMma));
                     if (!__all_sync(0xffffffffu, ok)) {
                         ok = false;
                         break;
@@ -643,10 +673,10 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
                     }
                     if (blk != blk_slots) nslots = load_slots(P, ws, blk, bars->slots[1], lane);
                     blk_slots = blk;
-                    const int steps = nslots * P.rsteps;
-                    for (int s0 = 0; s0 < steps; s0 += kSteps, ++i) {
+                    const int chunks = nslots * P.rchunks;
+                    for (int s0 = 0; s0 < chunks; s0 += per_stage, ++i) {
                         const int s = i % P.stages;
-                        ok = mbar_wait_cluster(smem_u32(&bars->full[s]), (i / P.stages) & 1, err, code(kWaitMma));
+                        ok = mbar_wait_cluster_full(smem_u32(&bars->full[s]), (i / P.stages) & 1, err, code(kWaitMma));
                         if (!__all_sync(0xffffffffu, ok)) {
                             ok = false;
                             break;
@@ -654,10 +684,13 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
                         tc_fence_after();
                         if (elect_one()) {
                             const uint32_t a = ring + s * P.stage_bytes;
-                            for (int k = 0; k < min(kSteps, steps - s0); ++k) {
-                                const int sl = bars->slots[1][(s0 + k) / P.rsteps].y;
-                                mma_ss_pair(d + (sl >> 16), smem_desc_sw32(a + k * kRows * 32), smem_desc_sw32(a + x_off + k * u_step),
-                                            idesc_f16(256, sl & 0xffff, Fmt<T>::v, false, false), 1u);
+                            for (int k = 0; k < min(per_stage, chunks - s0); ++k) {
+                                const int sl = bars->slots[1][(s0 + k) / P.rchunks].y;
+                                const int steps = min(P.kw / kStep, P.rsteps - (s0 + k) % P.rchunks * (P.kw / kStep));
+                                const uint64_t ad = rank_desc(a + k * b_chunk, P.kw), bd = rank_desc(a + x_off + k * u_chunk, P.kw);
+                                const uint32_t id = idesc_f16(256, sl & 0xffff, Fmt<T>::v, false, false);
+                                for (int e = 0; e < steps; ++e)
+                                    mma_ss_pair(d + (sl >> 16), ad + static_cast<uint64_t>(2 * e), bd + static_cast<uint64_t>(2 * e), id, 1u);
                             }
                             mma_commit_pair_both(smem_u32(&bars->empty[s]));
                         }
@@ -833,40 +866,42 @@ cudaError_t launch(const LoraArgs& A, unsigned char* ws, int sms, cudaStream_t s
     const uint64_t wd[2] = {K, N}, ws1[1] = {K * 2};
     const uint64_t xd[2] = {K, static_cast<uint64_t>(A.M)}, xs[1] = {(P.sorted ? K : static_cast<uint64_t>(A.x_stride)) * 2};
     const uint64_t bd[3] = {r, N, static_cast<uint64_t>(A.adapters)}, bs[2] = {r * 2, r * N * 2};
-    const uint64_t ud[2] = {kStep, static_cast<uint64_t>(P.nb) * P.slots * P.rsteps * P.tb}, us[1] = {kStep * 2};
+    const uint64_t kw = static_cast<uint64_t>(P.kw);
+    const uint64_t ud[2] = {kw, static_cast<uint64_t>(P.nb) * P.slots * P.rchunks * P.tb}, us[1] = {kw * 2};
     const uint32_t half = static_cast<uint32_t>(P.tb) / 2;
-    const uint32_t wb[2] = {kChunk, kRows}, xb[2] = {kChunk, half}, bb[3] = {kStep, kRows, 1}, ub[2] = {kStep, half};
+    const uint32_t wb[2] = {kChunk, kRows}, xb[2] = {kChunk, half}, bb[3] = {static_cast<uint32_t>(P.kw), kRows, 1},
+                   ub[2] = {static_cast<uint32_t>(P.kw), kColStep / 2};
+    const CUtensorMapSwizzle rswz = P.kw == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : P.kw == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                                                         : CU_TENSOR_MAP_SWIZZLE_32B;
     if (!encode_tmap_16b(&maps.w, A.w, 2, wd, ws1, wb, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !encode_tmap_16b(&maps.x, P.sorted ? ws + P.off_x : A.x, 2, xd, xs, xb, CU_TENSOR_MAP_SWIZZLE_128B) ||
-        !encode_tmap_16b(&maps.b, A.b, 3, bd, bs, bb, CU_TENSOR_MAP_SWIZZLE_32B) ||
-        !encode_tmap_16b(&maps.u, ws + P.off_u, 2, ud, us, ub, CU_TENSOR_MAP_SWIZZLE_32B))
+        !encode_tmap_16b(&maps.b, A.b, 3, bd, bs, bb, rswz) ||
+        !encode_tmap_16b(&maps.u, ws + P.off_u, 2, ud, us, ub, rswz))
         return cudaErrorInvalidValue;
     const int smem = P.stages * P.stage_bytes + static_cast<int>(sizeof(Bars)) + 1024;
     cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(lora_gemm_kernel<T>),
                                         kSmemCap + static_cast<int>(sizeof(Bars)) + 1024);
     if (e != cudaSuccess) return e;
+    // two rank steps at a time where there are two: x's rows are read once for both
+    const auto shrink = P.rsteps > 1 ? lora_shrink_kernel<T, 2> : lora_shrink_kernel<T, 1>;
     cudaLaunchAttribute attr[1];
-    cudaLaunchConfig_t cfg = {};
-    const int clusters = P.slots + P.tb / kShrinkTok + (P.sorted ? kCopyClusters : 0);
-    // two rank steps a cluster where there are two: x's rows are read once for both
-    const int steps = P.rsteps > 1 ? 2 : 1;
-    cfg.gridDim = dim3(clusters * P.ksplit, ceil_div(P.rsteps, steps), P.nb);
-    cfg.blockDim = dim3(32 * kShrinkWarps);
-    cfg.stream = s;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = P.ksplit;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
-    e = steps == 2 ? cudaLaunchKernelEx(&cfg, lora_shrink_kernel<T, 2>, A, P, ws)
-                   : cudaLaunchKernelEx(&cfg, lora_shrink_kernel<T, 1>, A, P, ws);
-    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(P.clusters * P.ksplit);
+    cfg.blockDim = dim3(32 * kShrinkWarps);
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if ((e = cudaLaunchKernelEx(&cfg, shrink, A, P, ws)) != cudaSuccess) return e;
+    // the GEMM is let in as soon as all CTAs of the shrink kernel run
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3(2 * P.pairs);
     cfg.blockDim = dim3(kGemmThreads);
     cfg.dynamicSmemBytes = smem;
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
     e = cudaLaunchKernelEx(&cfg, lora_gemm_kernel<T>, maps, P, A, ws);
     count_launches(2);
     return e != cudaSuccess ? e : cudaGetLastError();

@@ -229,6 +229,12 @@ __host__ __device__ constexpr uint64_t smem_desc_sw32(uint32_t addr) {
            (1ull << 46) | (6ull << 61);
 }
 
+// The same with rows of two steps (64 bytes, 64-byte swizzle): 8-row groups 512 bytes apart.
+__host__ __device__ constexpr uint64_t smem_desc_sw64(uint32_t addr) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (1ull << 16) | (static_cast<uint64_t>(512 >> 4) << 32) |
+           (1ull << 46) | (4ull << 61);
+}
+
 // No-swizzle K-major operand: core matrices of 8 rows x 16 bytes; lbo = byte distance between
 // the two core matrices of a K = 16 step, sbo = byte distance between 8-row groups.
 __host__ __device__ constexpr uint64_t smem_desc_noswz(uint32_t addr, uint32_t lbo, uint32_t sbo) {
