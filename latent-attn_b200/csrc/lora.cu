@@ -47,6 +47,8 @@ constexpr int kGemmThreads = 192;     // warp 0 loads, warp 1 issues, warps 2-5 
 constexpr int kSmemCap = 192 * 1024;  // leaves room for a block of the shrink kernel on the SM
 constexpr int kMaxStages = 6;
 constexpr int kMinChunks = 4;         // shortest share of a cut tile
+constexpr int kSliceTok = 128;        // blocks of at least so many tokens are cut by columns
+constexpr int kMinSlice = 64;         // narrowest slice
 constexpr int kJoinCols = 64;         // columns of a cut tile that are counted and added at a time
 constexpr int kJoins = kMaxTok / kJoinCols;
 constexpr int kShrinkWarps = 8;
@@ -62,6 +64,7 @@ struct Plan {
     int kw, rchunks;                  // ranks per row of B's and U's tiles (16, 32 or 64), tiles per adapter
     int kc, tiles;                    // K chunks, tiles (weight rows / 256 x blocks)
     int pairs, full;                  // CTA pairs, whole tiles (a multiple of pairs)
+    int slices, slice;                // column slices that the other tiles are cut into, 0: along K; their width
     int tail_pairs;                   // pairs that share the other tiles
     int stages, stage_bytes;
     int ksplit, clusters, per_blk;    // CTAs of a shrink cluster, clusters in all and per token block
@@ -87,10 +90,18 @@ Plan make_plan(int M, int N, int K, int adapters, int rank, int sms) {
     p.pairs = sms / 2;
     p.full = p.tiles / p.pairs * p.pairs;
     const int rest = p.tiles - p.full;
-    long long shares = static_cast<long long>(rest) * p.kc / kMinChunks;
-    if (shares > p.pairs) shares = p.pairs;
-    if (shares < rest) shares = rest;
-    p.tail_pairs = static_cast<int>(shares);
+    if (p.tb >= kSliceTok) {
+        p.slices = rest == 0 ? 1 : p.pairs / rest < p.tb / kMinSlice ? p.pairs / rest : p.tb / kMinSlice;
+        p.slice = up(ceil_div(p.tb, p.slices), kColStep);
+        p.slices = ceil_div(p.tb, p.slice);
+        p.tail_pairs = rest * p.slices;
+    } else {
+        long long shares = static_cast<long long>(rest) * p.kc / kMinChunks;
+        if (shares > p.pairs) shares = p.pairs;
+        if (shares < rest) shares = rest;
+        p.slice = p.tb;
+        p.tail_pairs = static_cast<int>(shares);
+    }
     if (p.full == 0) p.pairs = p.tail_pairs;
     p.stage_bytes = kGroup * (kRows + p.tb / 2) * 128;
     p.stages = kSmemCap / p.stage_bytes;
@@ -116,13 +127,19 @@ Plan make_plan(int M, int N, int K, int adapters, int rank, int sms) {
     p.off_perm = take(sizeof(int) * kMaxTok);
     p.off_x = take(p.sorted ? static_cast<size_t>(p.tb) * K * 2 : 0);
     p.off_u = take(static_cast<size_t>(p.nb) * p.slots * p.rchunks * p.tb * p.kw * 2);
-    p.off_part = take(rest > 0 && p.tail_pairs > rest ? static_cast<size_t>(p.tail_pairs) * 4 * kRows * p.tb * sizeof(float) : 0);
+    p.off_part = take(p.slices == 0 && p.tail_pairs > rest ? static_cast<size_t>(p.tail_pairs) * 4 * kRows * p.tb * sizeof(float) : 0);
     p.total = off;
     return p;
 }
 
-// An adapter of a token block: its id, the first of its tokens' columns and how many an MMA covers.
-__device__ __forceinline__ int2 pack_slot(int id, int lo, int n) { return make_int2(id, lo << 16 | n); }
+// An adapter of a token block: its id, its place in the block's list, the first of its tokens' columns
+// and how many an MMA covers (both multiples of 32).
+__device__ __forceinline__ int2 pack_slot(int id, int slot, int lo, int n) {
+    return make_int2(id, slot << 16 | lo / kColStep << 8 | n / kColStep);
+}
+__device__ __forceinline__ int slot_of(int2 s) { return s.y >> 16; }
+__device__ __forceinline__ int slot_lo(int2 s) { return (s.y >> 8 & 255) * kColStep; }
+__device__ __forceinline__ int slot_n(int2 s) { return (s.y & 255) * kColStep; }
 
 template <typename T> struct Fmt;
 template <> struct Fmt<__half> { static constexpr uint32_t v = 0; };
@@ -292,7 +309,7 @@ __global__ void __launch_bounds__(32 * kShrinkWarps, 2) lora_shrink_kernel(const
         const Own own = order_tokens(o, sh.tab, A, P, blk);
         if (cluster % P.per_blk == 0 && kpart == 0) {
             int2* meta = reinterpret_cast<int2*>(ws + P.off_meta) + static_cast<size_t>(blk) * (P.slots + 1);
-            if (own.id >= 0 && own.first == tid) meta[1 + o.slot[tid]] = pack_slot(own.id, o.cover[tid].x, o.cover[tid].y);
+            if (own.id >= 0 && own.first == tid) meta[1 + o.slot[tid]] = pack_slot(own.id, o.slot[tid], o.cover[tid].x, o.cover[tid].y);
             if (tid == 0) meta[0] = make_int2(o.slots, 0);
         }
         if (P.sorted) {
@@ -411,40 +428,53 @@ __global__ void __launch_bounds__(32 * kShrinkWarps, 2) lora_shrink_kernel(const
 // ------------------------------------------------------------------------------------- GEMM
 
 struct Maps {
-    CUtensorMap w, x, b, u;
+    CUtensorMap w, x, xs, b, u;
 };
 
-// One piece of a pair's work: chunks [c0, c1) of a tile's K columns.
+// One piece of a pair's work: chunks [c0, c1) of K and columns [lo, lo + cols) of a tile.
 struct Item {
     int tile, c0, c1;
-    int j;           // index among the cut tiles, or -1
+    int lo, cols;
+    int j;           // index among the tiles cut along K, or -1
 };
 // Walks the pair's pieces; every role walks an identical copy.
 struct Walk {
-    int next_full;
+    int next_full, slice;
     long long c, c_end;
     __device__ explicit Walk(const Plan& P) {
         const int w = blockIdx.x / 2;
         next_full = w;
         c = c_end = 0;
-        if (w < P.tail_pairs) {
+        slice = P.slices > 0 && w < P.tail_pairs ? w : -1;
+        if (P.slices == 0 && w < P.tail_pairs) {
             const long long total = static_cast<long long>(P.tiles - P.full) * P.kc;
             c = total * w / P.tail_pairs;
             c_end = total * (w + 1) / P.tail_pairs;
         }
     }
+    // columns of a tile's block: its tokens, up to a multiple of 32
+    static __device__ int block_cols(const Plan& P, int tile) {
+        return (min(P.tb, P.M - tile % P.nb * P.tb) + kColStep - 1) / kColStep * kColStep;
+    }
     __device__ bool next(const Plan& P, Item* it) {
         if (next_full < P.full) {
-            *it = {next_full, 0, P.kc, -1};
+            *it = {next_full, 0, P.kc, 0, block_cols(P, next_full), -1};
             next_full += P.pairs;
             return true;
+        }
+        if (slice >= 0) {
+            const int tile = P.full + slice / P.slices, lo = slice % P.slices * P.slice;
+            const int cols = min(P.slice, block_cols(P, tile) - lo);
+            slice = -1;
+            *it = {tile, 0, P.kc, lo, cols, -1};
+            return cols > 0;
         }
         if (c >= c_end) return false;
         const int j = static_cast<int>(c / P.kc);
         const int c0 = static_cast<int>(c % P.kc);
         const int n = static_cast<int>(c_end - c);
         const int c1 = min(P.kc, c0 + n);
-        *it = {P.full + j, c0, c1, j};
+        *it = {P.full + j, c0, c1, 0, block_cols(P, P.full + j), j};
         c += c1 - c0;
         return true;
     }
@@ -470,14 +500,22 @@ __device__ __forceinline__ uint64_t rank_desc(uint32_t addr, int kw) {
     return kw == 64 ? smem_desc_sw128(addr, 16, 1024) : kw == 32 ? smem_desc_sw64(addr) : smem_desc_sw32(addr);
 }
 
-// The adapters of token block blk into sl (one warp); returns how many.
-__device__ __forceinline__ int load_slots(const Plan& P, const unsigned char* ws, int blk, int2* sl, int lane) {
+// The adapters of token block blk that have columns of [lo, lo + cols) into sl (one warp), their columns
+// from lo on; returns how many.
+__device__ __forceinline__ int load_slots(const Plan& P, const unsigned char* ws, int blk, int lo, int cols, int2* sl, int lane) {
     const int2* meta = reinterpret_cast<const int2*>(ws + P.off_meta) + static_cast<size_t>(blk) * (P.slots + 1);
     const int n = meta[0].x;
+    int kept = 0;
     __syncwarp();
-    for (int i = lane; i < n; i += 32) sl[i] = meta[1 + i];
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        const int2 s = i0 + lane < n ? meta[1 + i0 + lane] : make_int2(0, 0);
+        const int a = max(slot_lo(s), lo), b = min(slot_lo(s) + slot_n(s), lo + cols);
+        const unsigned in = __ballot_sync(0xffffffffu, i0 + lane < n && a < b);
+        if (in >> lane & 1) sl[kept + __popc(in & ((1u << lane) - 1))] = pack_slot(s.x, slot_of(s), a - lo, b - a);
+        kept += __popc(in);
+    }
     __syncwarp();
-    return n;
+    return kept;
 }
 
 // Output element (column c of the block, token m, weight row n) from the token's own operands: the rare
@@ -545,14 +583,17 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
         // end on completion or on their own limit and do not look at it)
         Walk walk(P);
         Item it;
-        int i = 0, blk_slots = -1, nslots = 0;
+        int i = 0, blk_slots = -1, lo_slots = -1, nslots = 0;
         bool ok = true, waited = !P.sorted;   // X in adapter order comes from the shrink kernel
         bool meta_ready = false;
         int held = 0;                         // stages whose W is on its way while X is waited for
         while (ok && walk.next(P, &it)) {
             const int n0 = it.tile / P.nb * 2 * kRows + static_cast<int>(rank) * kRows, blk = it.tile % P.nb;
-            const int half = (min(P.tb, P.M - blk * P.tb) + kColStep - 1) / kColStep * (kColStep / 2);   // columns of this CTA's half
-            const int x0 = (P.sorted ? 0 : blk * P.tb) + static_cast<int>(rank) * half;
+            const int x0 = (P.sorted ? 0 : blk * P.tb) + it.lo + static_cast<int>(rank) * it.cols / 2;   // this CTA's half
+            // (boxes of half a block's or half a slice's rows; only the columns of the piece are used)
+            const bool cut = P.slices > 0 && it.tile >= P.full;
+            const CUtensorMap* xmap = cut ? &maps.xs : &maps.x;
+            const uint32_t x_bytes = cut ? P.slice / 2 * 128 : x_chunk;
             for (int c = it.c0; c < it.c1; c += kGroup, ++i) {
                 const int s = i % P.stages;
                 ok = i < P.stages || mbar_wait_cluster_full(smem_u32(&bars->empty[s]), ((i / P.stages) - 1) & 1, err, code(kWaitLoad));
@@ -564,12 +605,12 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
                 const uint32_t fb = mapa(smem_u32(&bars->full[s]), 0), dst = ring + s * P.stage_bytes;
                 if (elect_one()) {
                     if (rank == 0)
-                        mbar_arrive_expect_tx(smem_u32(&bars->full[s]), 2u * n * (kRows * 128 + x_chunk));
+                        mbar_arrive_expect_tx(smem_u32(&bars->full[s]), 2u * n * (kRows * 128 + x_bytes));
                     for (int k = 0; k < n; ++k)
                         tma_load_2d_pair(dst + k * kRows * 128, &maps.w, fb, kChunk * (c + k), n0);
                     if (waited)
                         for (int k = 0; k < n; ++k)
-                            tma_load_2d_pair(dst + x_off + k * x_chunk, &maps.x, fb, kChunk * (c + k), x0);
+                            tma_load_2d_pair(dst + x_off + k * x_chunk, xmap, fb, kChunk * (c + k), x0);
                 }
                 __syncwarp();
                 if (!waited) {
@@ -583,7 +624,7 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
                                 const int hc = c - (held - 1 - h) * kGroup, hs = i - (held - 1 - h);
                                 const uint32_t hb = mapa(smem_u32(&bars->full[hs % P.stages]), 0);
                                 for (int k = 0; k < min(kGroup, it.c1 - hc); ++k)
-                                    tma_load_2d_pair(ring + (hs % P.stages) * P.stage_bytes + x_off + k * x_chunk, &maps.x, hb,
+                                    tma_load_2d_pair(ring + (hs % P.stages) * P.stage_bytes + x_off + k * x_chunk, xmap, hb,
                                                      kChunk * (hc + k), x0);
                             }
                         __syncwarp();
@@ -595,8 +636,9 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
                 pdl_wait();   // U and the adapters' list come from the shrink kernel
                 meta_ready = true;
             }
-            if (blk != blk_slots) nslots = load_slots(P, ws, blk, bars->slots[0], lane);
+            if (blk != blk_slots || it.lo != lo_slots) nslots = load_slots(P, ws, blk, it.lo, it.cols, bars->slots[0], lane);
             blk_slots = blk;
+            lo_slots = it.lo;
             const int chunks = nslots * P.rchunks;
             for (int s0 = 0; s0 < chunks; s0 += per_stage, ++i) {
                 const int s = i % P.stages;
@@ -610,14 +652,15 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
                     const uint32_t fb = mapa(smem_u32(&bars->full[s]), 0), dst = ring + s * P.stage_bytes;
                     if (rank == 0) {
                         uint32_t bytes = 2u * n * b_chunk;
-                        for (int k = 0; k < n; ++k) bytes += (bars->slots[0][(s0 + k) / P.rchunks].y & 0xffff) * P.kw * 2;
+                        for (int k = 0; k < n; ++k) bytes += slot_n(bars->slots[0][(s0 + k) / P.rchunks]) * P.kw * 2;
                         mbar_arrive_expect_tx(smem_u32(&bars->full[s]), bytes);
                     }
                     for (int k = 0; k < n; ++k) {
                         const int2 sl = bars->slots[0][(s0 + k) / P.rchunks];
-                        tma_load_3d_pair(dst + k * b_chunk, &maps.b, fb, (s0 + k) % P.rchunks * P.kw, n0, sl.x);
-                        const int half_n = (sl.y & 0xffff) / 2;
-                        const int u0 = (blk * P.slots * P.rchunks + s0 + k) * P.tb + (sl.y >> 16) + static_cast<int>(rank) * half_n;
+                        const int q = (s0 + k) % P.rchunks, half_n = slot_n(sl) / 2;
+                        tma_load_3d_pair(dst + k * b_chunk, &maps.b, fb, q * P.kw, n0, sl.x);
+                        const int u0 = ((blk * P.slots + slot_of(sl)) * P.rchunks + q) * P.tb + it.lo + slot_lo(sl) +
+                                       static_cast<int>(rank) * half_n;
                         for (int c = 0; c < half_n; c += kColStep / 2)
                             tma_load_2d_pair(dst + x_off + k * u_chunk + c * P.kw * 2, &maps.u, fb, 0, u0 + c);
                     }
@@ -631,12 +674,11 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
         if (rank == 0) {
             Walk walk(P);
             Item it;
-            int i = 0, n = 0, blk_slots = -1, nslots = 0;
+            int i = 0, n = 0, blk_slots = -1, lo_slots = -1, nslots = 0;
             bool ok = true, meta_ready = false;
             for (; ok && walk.next(P, &it); ++n) {
                 const int blk = it.tile % P.nb;
-                const int cols = (min(P.tb, P.M - blk * P.tb) + kColStep - 1) / kColStep * kColStep;
-                const uint32_t idesc = idesc_f16(256, cols, Fmt<T>::v, false, false);
+                const uint32_t idesc = idesc_f16(256, it.cols, Fmt<T>::v, false, false);
                 const uint32_t d = tbase + 256 * (n & 1);
                 ok = n < 2 || mbar_wait_cluster_full(smem_u32(&bars->acc_empty[n & 1]), ((n >> 1) - 1) & 1, err, code(kWaitAcc));
                 if (!__all_sync(0xffffffffu, ok)) {
@@ -671,8 +713,9 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
                         pdl_wait();
                         meta_ready = true;
                     }
-                    if (blk != blk_slots) nslots = load_slots(P, ws, blk, bars->slots[1], lane);
+                    if (blk != blk_slots || it.lo != lo_slots) nslots = load_slots(P, ws, blk, it.lo, it.cols, bars->slots[1], lane);
                     blk_slots = blk;
+                    lo_slots = it.lo;
                     const int chunks = nslots * P.rchunks;
                     for (int s0 = 0; s0 < chunks; s0 += per_stage, ++i) {
                         const int s = i % P.stages;
@@ -685,12 +728,12 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
                         if (elect_one()) {
                             const uint32_t a = ring + s * P.stage_bytes;
                             for (int k = 0; k < min(per_stage, chunks - s0); ++k) {
-                                const int sl = bars->slots[1][(s0 + k) / P.rchunks].y;
+                                const int2 sl = bars->slots[1][(s0 + k) / P.rchunks];
                                 const int steps = min(P.kw / kStep, P.rsteps - (s0 + k) % P.rchunks * (P.kw / kStep));
                                 const uint64_t ad = rank_desc(a + k * b_chunk, P.kw), bd = rank_desc(a + x_off + k * u_chunk, P.kw);
-                                const uint32_t id = idesc_f16(256, sl & 0xffff, Fmt<T>::v, false, false);
+                                const uint32_t id = idesc_f16(256, slot_n(sl), Fmt<T>::v, false, false);
                                 for (int e = 0; e < steps; ++e)
-                                    mma_ss_pair(d + (sl >> 16), ad + static_cast<uint64_t>(2 * e), bd + static_cast<uint64_t>(2 * e), id, 1u);
+                                    mma_ss_pair(d + slot_lo(sl), ad + static_cast<uint64_t>(2 * e), bd + static_cast<uint64_t>(2 * e), id, 1u);
                             }
                             mma_commit_pair_both(smem_u32(&bars->empty[s]));
                         }
@@ -767,13 +810,13 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
                 w1 = static_cast<int>(((static_cast<long long>(it.j) + 1) * P.kc * P.tail_pairs - 1) / total);
             }
             if (w0 == w1) {
-                for (int c = 0; c < toks; c += 16) {
+                for (int c = 0; c < min(it.cols, toks - it.lo); c += 16) {
                     uint32_t u[16];
                     tmem_ld16_sync(d + c, u);
                     float v[16];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(u[k]);
-                    store16(c, v);
+                    store16(it.lo + c, v);
                 }
                 release();
                 continue;
@@ -869,12 +912,14 @@ cudaError_t launch(const LoraArgs& A, unsigned char* ws, int sms, cudaStream_t s
     const uint64_t kw = static_cast<uint64_t>(P.kw);
     const uint64_t ud[2] = {kw, static_cast<uint64_t>(P.nb) * P.slots * P.rchunks * P.tb}, us[1] = {kw * 2};
     const uint32_t half = static_cast<uint32_t>(P.tb) / 2;
+    const uint32_t sb[2] = {kChunk, static_cast<uint32_t>(P.slice) / 2};
     const uint32_t wb[2] = {kChunk, kRows}, xb[2] = {kChunk, half}, bb[3] = {static_cast<uint32_t>(P.kw), kRows, 1},
                    ub[2] = {static_cast<uint32_t>(P.kw), kColStep / 2};
     const CUtensorMapSwizzle rswz = P.kw == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : P.kw == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
                                                                                          : CU_TENSOR_MAP_SWIZZLE_32B;
     if (!encode_tmap_16b(&maps.w, A.w, 2, wd, ws1, wb, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !encode_tmap_16b(&maps.x, P.sorted ? ws + P.off_x : A.x, 2, xd, xs, xb, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !encode_tmap_16b(&maps.xs, P.sorted ? ws + P.off_x : A.x, 2, xd, xs, sb, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !encode_tmap_16b(&maps.b, A.b, 3, bd, bs, bb, rswz) ||
         !encode_tmap_16b(&maps.u, ws + P.off_u, 2, ud, us, ub, rswz))
         return cudaErrorInvalidValue;
