@@ -73,6 +73,9 @@ struct Plan {
 
 int up(int a, int b) { return (a + b - 1) / b * b; }
 
+// Rank steps of a shrink item: x's rows are read once for all of them.
+int shrink_steps(int rsteps) { return rsteps > 2 ? 4 : rsteps > 1 ? 2 : 1; }
+
 Plan make_plan(int M, int N, int K, int adapters, int rank, int sms) {
     Plan p = {};
     p.M = M; p.N = N; p.K = K; p.r = rank; p.adapters = adapters;
@@ -111,7 +114,7 @@ Plan make_plan(int M, int N, int K, int adapters, int rank, int sms) {
     // as many shrink clusters as have work, at most two CTAs per SM: they share a token block's units or
     // walk the blocks
     const int most = (p.slots < M ? p.slots : M) + (M < p.tb ? M : p.tb) / kShrinkTok;   // units of a block
-    const int qs = ceil_div(p.rsteps, p.rsteps > 1 ? 2 : 1);
+    const int qs = ceil_div(p.rsteps, shrink_steps(p.rsteps));
     const int fit = 2 * sms / p.ksplit;
     p.per_blk = fit / p.nb < 1 ? 1 : fit / p.nb < most * qs ? fit / p.nb : most * qs;
     p.clusters = p.per_blk * (fit / p.per_blk < p.nb ? fit / p.per_blk : p.nb);
@@ -342,7 +345,7 @@ __global__ void __launch_bounds__(32 * kShrinkWarps, 2) lora_shrink_kernel(const
                 if (list[8 * i] >= 0) nt = i + 1;
             }
             float acc[kQ][4][4] = {};
-            constexpr int kUnroll = kQ == 1 ? 4 : 2;
+            constexpr int kUnroll = 4 / kQ;
             const int stride = 32 * kShrinkWarps * P.ksplit;
             for (int k0 = 32 * (kpart * kShrinkWarps + warp); k0 < P.K; k0 += stride * kUnroll) {
                 uint4 va[kUnroll][kQ][2], vx[kUnroll][4];
@@ -927,8 +930,8 @@ cudaError_t launch(const LoraArgs& A, unsigned char* ws, int sms, cudaStream_t s
     cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(lora_gemm_kernel<T>),
                                         kSmemCap + static_cast<int>(sizeof(Bars)) + 1024);
     if (e != cudaSuccess) return e;
-    // two rank steps at a time where there are two: x's rows are read once for both
-    const auto shrink = P.rsteps > 1 ? lora_shrink_kernel<T, 2> : lora_shrink_kernel<T, 1>;
+    const int steps = shrink_steps(P.rsteps);
+    const auto shrink = steps == 4 ? lora_shrink_kernel<T, 4> : steps == 2 ? lora_shrink_kernel<T, 2> : lora_shrink_kernel<T, 1>;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = P.ksplit;
