@@ -48,9 +48,10 @@ constexpr int kSmemCap = 192 * 1024;  // leaves room for a block of the shrink k
 constexpr int kMaxStages = 6;
 constexpr int kMinChunks = 4;         // shortest share of a cut tile
 constexpr int kSliceTok = 128;        // blocks of at least so many tokens are cut by columns
+constexpr int kSortTok = 128;         // a single block of more tokens is put in adapter order
 constexpr int kMinSlice = 64;         // narrowest slice
-constexpr int kJoinCols = 64;         // columns of a cut tile that are counted and added at a time
-constexpr int kJoins = kMaxTok / kJoinCols;
+constexpr int kJoinCols = 32;         // columns of a tile cut along K that are counted and added at a time
+constexpr int kJoins = kSliceTok / kJoinCols;
 constexpr int kShrinkWarps = 8;
 constexpr int kShrinkTok = 32;        // tokens per shrink cluster
 constexpr int kTable = 1024;          // adapters that the shrink kernel counts in a table
@@ -82,8 +83,8 @@ Plan make_plan(int M, int N, int K, int adapters, int rank, int sms) {
     p.nb = ceil_div(M, kMaxTok);
     p.tb = up(ceil_div(M, p.nb), kColStep);
     p.nb = ceil_div(M, p.tb);
-    // with up to 32 tokens an MMA covers them all anyway
-    p.sorted = p.nb == 1 && p.tb > kColStep;
+    // with up to 128 tokens an MMA over all columns costs less than the copy of X
+    p.sorted = p.nb == 1 && p.tb > kSortTok;
     p.slots = adapters < p.tb ? adapters : p.tb;
     p.rsteps = ceil_div(rank, kStep);
     p.kw = rank > 32 ? 64 : rank > 16 ? 32 : 16;
@@ -833,59 +834,65 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
             };
             const int me = blockIdx.x / 2, joins = (toks + kJoinCols - 1) / kJoinCols;
             float4* mine = part(me);
-            // the pairs of a tile begin at different columns, so that those which end together share the additions
-            int at = (me - w0) * joins / (w1 - w0 + 1);
-            for (int b = 0; b < joins; ++b, at = at + 1 < joins ? at + 1 : 0) {
-                const int cb = at * kJoinCols, ce = min(toks, cb + kJoinCols);
-                for (int c = cb; c < ce; c += 16) {
-                    uint32_t v[16];
-                    tmem_ld16_sync(d + c, v);
+            for (int c = 0; c < toks; c += 16) {
+                uint32_t v[16];
+                tmem_ld16_sync(d + c, v);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        mine[(c / 4 + k) * kRows] = make_float4(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1]),
-                                                                __uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3]));
-                }
-                __threadfence();
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                if (threadIdx.x == 64) {
-                    int* count = reinterpret_cast<int*>(ws + P.off_count) + (2 * it.j + rank) * kJoins + at;
-                    bars->last = atomicAdd(count, 1) == w1 - w0;
-                }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                if (!bars->last) continue;
-                __threadfence();
-                // add the partials in order, this CTA's own from the accumulator; the others' of 32 columns
-                // are requested together, two pairs at a time, one round trip each
-                for (int c = cb; c < ce; c += 32) {
-                    uint32_t own[32];
-                    tmem_ld32_sync(d + c, own);
-                    float v[32] = {};
-                    for (int wa = w0; wa <= w1; wa += 2) {
-                        float4 y[2][8];
+                for (int k = 0; k < 4; ++k)
+                    mine[(c / 4 + k) * kRows] = make_float4(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1]),
+                                                            __uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3]));
+            }
+            __threadfence();
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (threadIdx.x == 64) {
+                // the columns for which this CTA is the last of the tile's; the pairs begin at different
+                // ones, so that those which end together share the additions
+                int* count = reinterpret_cast<int*>(ws + P.off_count) + (2 * it.j + rank) * kJoins;
+                int seen[kJoins], last = 0;
+                const int at = (me - w0) * joins / (w1 - w0 + 1);
 #pragma unroll
-                        for (int i = 0; i < 2; ++i)
-                            if (wa + i <= w1 && wa + i != me) {
-                                const float4* src = part(wa + i) + c / 4 * kRows;
+                for (int b = 0; b < kJoins; ++b)
+                    if (b < joins) seen[b] = atomicAdd(count + (at + b) % joins, 1);
 #pragma unroll
-                                for (int k = 0; k < 8; ++k)
-                                    if (k < 4 || c + 16 < ce) y[i][k] = __ldcg(src + k * kRows);
+                for (int b = 0; b < kJoins; ++b)
+                    if (b < joins && seen[b] == w1 - w0) last |= 1 << (at + b) % joins;
+                bars->last = last;
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            const int last = bars->last;
+            if (last) __threadfence();
+            // add the partials in order, this CTA's own from the accumulator; the others' are requested two
+            // pairs at a time, one round trip each
+            for (int c = 0; c < toks; c += kJoinCols) {
+                if (!(last >> c / kJoinCols & 1)) continue;
+                uint32_t own[32];
+                tmem_ld32_sync(d + c, own);
+                float v[32] = {};
+                for (int wa = w0; wa <= w1; wa += 2) {
+                    float4 y[2][8];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        if (wa + i <= w1 && wa + i != me) {
+                            const float4* src = part(wa + i) + c / 4 * kRows;
+#pragma unroll
+                            for (int k = 0; k < 8; ++k)
+                                if (k < 4 || c + 16 < toks) y[i][k] = __ldcg(src + k * kRows);
+                        }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        if (wa + i <= w1) {
+                            const bool self = wa + i == me;
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                v[4 * k] += self ? __uint_as_float(own[4 * k]) : y[i][k].x;
+                                v[4 * k + 1] += self ? __uint_as_float(own[4 * k + 1]) : y[i][k].y;
+                                v[4 * k + 2] += self ? __uint_as_float(own[4 * k + 2]) : y[i][k].z;
+                                v[4 * k + 3] += self ? __uint_as_float(own[4 * k + 3]) : y[i][k].w;
                             }
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-                            if (wa + i <= w1) {
-                                const bool self = wa + i == me;
-#pragma unroll
-                                for (int k = 0; k < 8; ++k) {
-                                    v[4 * k] += self ? __uint_as_float(own[4 * k]) : y[i][k].x;
-                                    v[4 * k + 1] += self ? __uint_as_float(own[4 * k + 1]) : y[i][k].y;
-                                    v[4 * k + 2] += self ? __uint_as_float(own[4 * k + 2]) : y[i][k].z;
-                                    v[4 * k + 3] += self ? __uint_as_float(own[4 * k + 3]) : y[i][k].w;
-                                }
-                            }
-                    }
-                    store16(c, v);
-                    if (c + 16 < ce) store16(c + 16, v + 16);
+                        }
                 }
+                store16(c, v);
+                if (c + 16 < toks) store16(c + 16, v + 16);
             }
             release();
         }
