@@ -10,8 +10,7 @@
 //   3. prefix_merge_kernel merges each output row's records by their maxima and sums.
 // Rounding: P is rounded to the cache's type for its MMA, and the row sums add the rounded values, so
 // that the weights of a row still add up to one; a record's o is stored in fp16 after an exact scaling
-// of each 128 columns by a power of two (2^-11 relative, a quarter of the bytes of fp32's error budget
-// being unused); all sums, maxima and accumulators are fp32; the result is rounded once.
+// of each 64 columns by a power of two (2^-11 relative to their largest, at half of fp32's bytes); all sums, maxima and accumulators are fp32; the result is rounded once.
 // A group is the M = 128 tile of the MMAs. When 128 divides H it is 128 heads of one request, whose
 // positions are its prefix followed by its own rows. Otherwise the (request, head) rows of a prefix
 // group are packed across requests, so that one pass over the prefix serves 128 / H requests, and
@@ -64,10 +63,12 @@ constexpr int kMSlots = 4;
 constexpr int kSets = 3;
 constexpr int kSlots = 3;                            // exchange and P slots, tile j in slot j % kSlots
 constexpr int kSums = 2 * kSlots;                    // row sums handed between the sets, tile j's in j % kSums
-constexpr int kGroupCost = 2;                        // a group's fixed cost, in tiles, for the split
+constexpr int kGroupCost = 4;                        // a group's fixed cost, in tiles, for the split (a batch of
+                                                     // questions about a document of 131072: 2: 185 us, 4: 155, 6: 162)
 constexpr int kThreads = 128 + 128 * kSets;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColO = 0, kColS = 256, kColQ = 384;
+constexpr int kMl = 12;
 constexpr float kRescale = 8.0f;                     // log2 units
 constexpr float kLowest = -1e37f;                    // reference of rows whose scores are all -inf
 
@@ -100,7 +101,7 @@ struct Work {                 // workspace
     int2* request;            // per request: its prefix's first group among `pieces` (or -1) and first row
     int* gbase;               // per prefix group: its first row group (num_groups + 1)
     int* bad;                 // per group with tiles: it met a row outside the cache
-    float* rec_ml;            // per record row 8 floats: m, l, -, -, and 2^-f of each 128 columns of o
+    float* rec_ml;            // per record row kMl floats: m, l, -, -, and 2^-f of each 64 columns of o
     uint16_t* rec_o;          // o 2^f in fp16
     float2* rowsum;           // per CTA: [kSums][128] row sums and references handed between its sets
     int W;                    // workers
@@ -324,7 +325,8 @@ struct __align__(8) Barriers {
     uint64_t x_empty[kSlots];         // and so it has in the peer, whose slot may be written again
     uint64_t mref[kMSlots];           // m_pub slot j % kMSlots holds tile j's reference
     uint64_t lpub[kSums];           // rowsum slot j % kSums holds tile j's set's sums (near a segment's end)
-    uint64_t q_ready, o_free, drain[2], done;
+    uint64_t q_first, q_ready;        // the first group's Q is in place; a later one's
+    uint64_t o_free, drain[2], done;
     uint32_t tmem;
 };
 
@@ -398,23 +400,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
-// 2^f that brings 128 columns of this thread's O row (TMEM) below 2^15, for the fp16 record; 1 for rows
-// of zeros and for infinities and NaN, which go into the record as they are. Warp-collective.
-__device__ __forceinline__ float record_scale(uint32_t tsrc) {
-    float top = 0.f;
-#pragma unroll 1
-    for (int c0 = 0; c0 < 128; c0 += 32) {
-        uint32_t o[32];
-        tmem_ld32_sync(tsrc + c0, o);
-        float mx[4] = {};
-#pragma unroll
-        for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], fabsf(__uint_as_float(o[i])));
-        top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
-    }
-    // exponent field of 2^(14 - floor(log2 top)), kept where both 2^f and 2^-f are normal
-    const int e = static_cast<int>(__float_as_uint(top) >> 23);
-    return e > 0 && e < 255 ? __uint_as_float(static_cast<uint32_t>(min(max(268 - e, 1), 253)) << 23) : 1.f;
-}
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
     float2 d;
     asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
@@ -429,25 +414,32 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
-// 128 columns of this thread's O row (TMEM) times scale to a record row. Warp-collective.
-__device__ __forceinline__ void write_cols(uint32_t tsrc, uint16_t* orow, float scale, bool row_ok) {
-#pragma unroll 1
-    for (int c0 = 0; c0 < 128; c0 += 32) {
-        uint32_t o[32];
-        tmem_ld32_sync(tsrc + c0, o);
-        if (row_ok) {
+// 64 columns of this thread's O row (TMEM) to a record row, times the 2^f that brings them below 2^15
+// (1 for zeros, and for infinities and NaN, which go into the record as they are); returns 2^-f.
+// Warp-collective.
+__device__ __forceinline__ float write_cols(uint32_t tsrc, uint16_t* orow, bool row_ok) {
+    uint32_t o[64];
+    tmem_ld64_sync(tsrc, o);
+    float mx[4] = {};
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                uint32_t v[8];
+    for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], fabsf(__uint_as_float(o[i])));
+    // exponent field of 2^(14 - floor(log2 top)), kept where both 2^f and 2^-f are normal
+    const int e = static_cast<int>(__float_as_uint(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]))) >> 23);
+    const int f = e > 0 && e < 255 ? min(max(268 - e, 1), 253) : 127;
+    const float scale = __uint_as_float(static_cast<uint32_t>(f) << 23);
+    if (row_ok) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    v[i] = half2_of(__uint_as_float(o[16 * q + 2 * i]) * scale, __uint_as_float(o[16 * q + 2 * i + 1]) * scale);
-                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(orow + c0 + 16 * q),
-                             "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-                             : "memory");
-            }
+        for (int q = 0; q < 4; ++q) {
+            uint32_t v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                v[i] = half2_of(__uint_as_float(o[16 * q + 2 * i]) * scale, __uint_as_float(o[16 * q + 2 * i + 1]) * scale);
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(orow + 16 * q),
+                         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                         : "memory");
         }
     }
+    return __uint_as_float(static_cast<uint32_t>(254 - f) << 23);
 }
 
 template <typename T>
@@ -487,6 +479,7 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
         for (int b = 0; b < 2; ++b) mbar_init(smem_u32(&bars->s_free[b]), 128);
         for (int i = 0; i < kMSlots; ++i) mbar_init(smem_u32(&bars->mref[i]), 128);
         for (int i = 0; i < kSums; ++i) mbar_init(smem_u32(&bars->lpub[i]), 128);
+        mbar_init(smem_u32(&bars->q_first), 128 * kSets);
         mbar_init(smem_u32(&bars->q_ready), 128);
         mbar_init(smem_u32(&bars->o_free), 128);
         mbar_init(smem_u32(&bars->drain[0]), 1);
@@ -553,7 +546,8 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
             for (int i = 0; it.valid(); ++i, it.next(wk)) {
                 ok = mbar_wait(smem_u32(&bars->kv_full[i % kStages]), (i / kStages) & 1, err, code(kWaitMma)) &&
                      (i < 2 || mbar_wait(smem_u32(&bars->s_free[i & 1]), ((i >> 1) - 1) & 1, err, code(kWaitMma))) &&
-                     (!it.seg_first() || mbar_wait(smem_u32(&bars->q_ready), seg & 1, err, code(kWaitMma)));
+                     (!it.seg_first() || (seg == 0 ? mbar_wait(smem_u32(&bars->q_first), 0, err, code(kWaitMma))
+                                                   : mbar_wait(smem_u32(&bars->q_ready), (seg - 1) & 1, err, code(kWaitMma))));
                 if (!warp_ok(ok)) break;
                 if (it.seg_first()) ++seg;
                 tc_fence_after();
@@ -619,13 +613,13 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
         const float qscale = A.scale * 1.4426950408889634f;
         // Q of a group: this thread's half of its row's CTA columns into TMEM (two elements a column) and
         // two of the four rope boxes
-        auto load_q = [&](const Group& d) {
+        auto load_q = [&](const Group& d, int c0, int step, uint64_t* ready) {
             const long long row = d.q_row0 + t;
             const uint4* lat = reinterpret_cast<const uint4*>(static_cast<const T*>(A.qa) + row * 512 + 256 * rank);
             const uint4* rope = reinterpret_cast<const uint4*>(static_cast<const T*>(A.qr) + row * 64 + 32 * rank);
             const bool have = t < d.rows;
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
+            for (int c = c0; c < 4; c += step) {
                 uint4 v[8], r;
 #pragma unroll
                 for (int k = 0; k < 8; ++k) v[k] = have ? __ldg(lat + 8 * c + k) : make_uint4(0, 0, 0, 0);
@@ -643,13 +637,13 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
             fence_proxy_async_smem();
             tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(smem_u32(&bars->q_ready));
+            mbar_arrive(smem_u32(ready));
         };
         Tiles it;
         bool ok = true;
         if (n > 0) {
             it.init(start);
-            if (sid == 0) load_q(it.d);   // the first tile belongs to set 0
+            load_q(it.d, sid, kSets, &bars->q_first);   // the first group's Q: the sets share it
             it.skip(wk, sid);
         } else {
             it.t = it.t_end = 0;
@@ -694,7 +688,7 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
                 // the score of tile j was the last MMA to read this group's Q
                 Tiles nx = it;
                 nx.next(wk);
-                load_q(nx.d);
+                load_q(nx.d, 0, 1, &bars->q_ready);
             }
             if (np < kTile) {
                 // rows past the end: their weights are zero, but zero times what lies there need not be
@@ -823,14 +817,13 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
                 tc_fence_after();
                 const long long at = static_cast<long long>(it.g + w) * 128 + t;
                 const bool row_ok = t < it.d.rows;
-                float* ml = wk.rec_ml + at * 8;
+                float* ml = wk.rec_ml + at * kMl;
                 if (row_ok && rank == 0) *reinterpret_cast<float2*>(ml) = make_float2(m, l_tot);
-#pragma unroll 1
-                for (int c = 0; c < 2; ++c) {
-                    const float f = record_scale(trow + kColO + 128 * c);
-                    write_cols(trow + kColO + 128 * c, wk.rec_o + at * 512 + 256 * rank + 128 * c, f, row_ok);
-                    if (row_ok) ml[4 + 2 * rank + c] = 1.f / f;
-                }
+                float f[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    f[c] = write_cols(trow + kColO + 64 * c, wk.rec_o + at * 512 + 256 * rank + 64 * c, row_ok);
+                if (row_ok) *reinterpret_cast<float4*>(ml + 4 + 4 * rank) = make_float4(f[0], f[1], f[2], f[3]);
                 tc_fence_before();
                 mbar_arrive(smem_u32(&bars->o_free));
             }
@@ -898,8 +891,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps) prefix_merge_kernel(const __
                 for (int i = 0; i < kAhead; ++i)
                     if (w + i * kWarps <= w1) {
                         const long long at = static_cast<long long>(g + w + i * kWarps) * 128 + r;
-                        ml[i] = *reinterpret_cast<const float2*>(wk.rec_ml + at * 8);
-                        fs[i] = make_float2(wk.rec_ml[at * 8 + 4 + lane / 16], wk.rec_ml[at * 8 + 6 + lane / 16]);
+                        ml[i] = *reinterpret_cast<const float2*>(wk.rec_ml + at * kMl);
+                        fs[i] = make_float2(wk.rec_ml[at * kMl + 4 + lane / 8], wk.rec_ml[at * kMl + 8 + lane / 8]);
                         const uint4* src = reinterpret_cast<const uint4*>(wk.rec_o + at * 512);
                         v[i][0] = src[lane];
                         v[i][1] = src[32 + lane];
@@ -993,7 +986,7 @@ Layout layout(const PrefixArgs& A, int sms) {
     L.off_base = take(sizeof(int) * A.P);
     L.off_bad = take(sizeof(int) * groups);
     L.off_sum = take(sizeof(float2) * 2 * L.W * kSums * 128);
-    L.off_ml = take(recs * 128 * 8 * sizeof(float));
+    L.off_ml = take(recs * 128 * kMl * sizeof(float));
     L.off_o = take(recs * 128 * 512 * 2);
     L.total = off;
     return L;
