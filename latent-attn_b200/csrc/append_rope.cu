@@ -179,7 +179,7 @@ __device__ __forceinline__ void append_task_vec(const AppendRope& A, int t, int 
     const int h1 = min(A.H, part * kHeadsPerTask);
     const T* q = static_cast<const T*>(A.q) + t * A.q_ts;
     T* qo = static_cast<T*>(A.qo) + t * A.qo_ts;
-    constexpr int kSteps = 4;
+    constexpr int kSteps = 2;
     int h = (part - 1) * kHeadsPerTask + hl;
     bool first = true;
     float c[8], s[8];
@@ -258,8 +258,10 @@ __device__ void append_task_any(const AppendRope& A, int t, int part, int lane) 
             rotate(static_cast<const T*>(A.q) + t * A.q_ts + h * A.q_hs, static_cast<T*>(A.qo) + t * A.qo_ts + h * A.qo_hs, i);
 }
 
+// (four blocks an SM: prompts want warps in flight more than long ones; two blocks with four steps of
+// heads at a time took 36.8 us for 12 prompts of up to 4099 tokens and 16 heads, four with two 32.4)
 template <typename T, bool kVec>
-__global__ void __launch_bounds__(kAppendThreads) append_rope_kernel(const __grid_constant__ AppendRope A, int parts) {
+__global__ void __launch_bounds__(kAppendThreads, 4) append_rope_kernel(const __grid_constant__ AppendRope A, int parts) {
     const long long warp = (static_cast<long long>(blockIdx.x) * kAppendThreads + threadIdx.x) / 32;
     const int lane = threadIdx.x & 31;
     if (A.new_lens) {
