@@ -114,18 +114,19 @@ __device__ __forceinline__ bool warp_ok(bool ok) { return __all_sync(0xffffffffu
 __device__ __forceinline__ int clampi(int v, int hi) { return v < 0 ? 0 : (v > hi ? hi : v); }
 
 // Prefix group of request b, or -1: the last one that starts at or before b, if it holds b.
-__device__ __forceinline__ int prefix_of(const PrefixArgs& A, int b) {
-    int lo = 0, hi = A.P;
+__device__ __forceinline__ int prefix_of(const int* starts, int P, int b) {
+    int lo = 0, hi = P;
     while (lo + 1 < hi) {
         const int mid = (lo + hi) / 2;
-        if (A.starts[mid] <= b) lo = mid; else hi = mid;
+        if (starts[mid] <= b) lo = mid; else hi = mid;
     }
-    return A.starts[lo] <= b && b < A.starts[lo + 1] ? lo : -1;
+    return starts[lo] <= b && b < starts[lo + 1] ? lo : -1;
 }
 
 // ------------------------------------------------------------------------------------- plan
 
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 1024;  // most; 256 where they cover the groups (fewer warps meet at the barriers)
+constexpr int kPlanGroups = 256;    // groups with tiles that are kept in shared memory
 constexpr int kPlanCache = 4096;   // groups (and prefix groups) whose sums are kept in shared memory
 constexpr int kMaxWorkers = 128;
 
@@ -142,7 +143,7 @@ __device__ long long block_scan(long long v, long long* sh, long long* carry) {
     __syncthreads();
     long long before = 0, total = 0;
     {
-        long long s = sh[lane];
+        long long s = lane < blockDim.x / 32 ? sh[lane] : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const long long y = __shfl_up_sync(0xffffffffu, s, o);
@@ -158,30 +159,40 @@ __device__ long long block_scan(long long v, long long* sh, long long* carry) {
     return at;
 }
 
-// One block. Latency is all that counts here: one round of loads for the prefixes, one for the groups,
-// the searches in shared memory (in global memory beyond kPlanCache).
+// One block. Latency is all that counts here: one round of loads for everything, the searches in shared
+// memory (in global memory beyond kPlanCache).
 __global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(const __grid_constant__ PrefixArgs A, const Work wk) {
     __shared__ long long sh[32], carry;
+    __shared__ int sh_starts[kPlanCache / 4 + 1], sh_plens[kPlanCache / 4];
     __shared__ int sh_base[kPlanCache / 4 + 1];        // gbase
     __shared__ int sh_unit[kPlanCache + 1];            // per group with tiles: tiles and fixed costs before it
+    __shared__ Group sh_group[kPlanGroups];
     __shared__ int sh_cut[kMaxWorkers + 1];            // where each share begins
     __shared__ int sh_tile[kMaxWorkers + 1];           // per worker with tiles: its first one
     __shared__ unsigned sh_has[kMaxWorkers / 32];
     pdl_launch_dependents();
-    const int hb = ceil_div(A.H, 128), tid = threadIdx.x;
+    const int hb = ceil_div(A.H, 128), tid = threadIdx.x, threads = blockDim.x;
+    const int len0 = tid < wk.own ? A.lens[tid / hb] : 0;   // this thread's first own group
+    const bool base_sh = A.P <= kPlanCache / 4;
+    if (base_sh)
+        for (int p = tid; p <= A.P; p += threads) {
+            sh_starts[p] = A.starts[p];
+            if (p < A.P) sh_plens[p] = A.plens[p];
+        }
+    const int* starts = base_sh ? sh_starts : A.starts;
+    const int* plens = base_sh ? sh_plens : A.plens;
     if (tid == 0) {
         carry = 0;
         *wk.status = 0;
     }
     __syncthreads();
     int extra = 0;   // row groups of the prefixes
-    const bool base_sh = A.P <= kPlanCache / 4;
     if (!wk.fold) {
-        for (int p0 = 0; p0 < A.P; p0 += kPlanThreads) {
+        for (int p0 = 0; p0 < A.P; p0 += threads) {
             const int p = p0 + tid;
             int n = 0;
             if (p < A.P) {
-                const int s0 = max(A.starts[p], 0), s1 = min(A.starts[p + 1], A.B);
+                const int s0 = max(starts[p], 0), s1 = min(starts[p + 1], A.B);
                 n = s1 > s0 ? static_cast<int>((static_cast<long long>(s1 - s0) * A.H + 127) / 128) : 0;
             }
             const int at = static_cast<int>(block_scan(n, sh, &carry));
@@ -199,21 +210,21 @@ __global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(const __grid_
     // groups: tiles, then (compacted) the table
     const int G = wk.own + extra;
     int mine = -1, mine0 = 0, mine1 = 0;   // this thread's last group: its place in the table, its tiles
-    for (int g0 = 0; g0 < G; g0 += kPlanThreads) {
+    for (int g0 = 0; g0 < G; g0 += threads) {
         const int g = g0 + tid;
         Group d = {};
         int tiles = 0;
         if (g < wk.own) {
             const int b = g / hb, k = g % hb;
-            const int p = prefix_of(A, b);
+            const int p = prefix_of(starts, A.P, b);
             d.q_row0 = b * A.H + 128 * k;
             d.rows = min(128, A.H - 128 * k);
             d.pid = wk.fold ? p : -1;
             d.sid = b;
-            d.plen = d.pid >= 0 ? clampi(A.plens[d.pid], A.max_plen) : 0;
-            d.slen = clampi(A.lens[b], A.max_len);
+            d.plen = d.pid >= 0 ? clampi(plens[d.pid], A.max_plen) : 0;
+            d.slen = clampi(g0 == 0 ? len0 : A.lens[b], A.max_len);
             if (!wk.fold && k == 0)
-                wk.request[b] = p < 0 ? make_int2(-1, 0) : make_int2(wk.own + gbase[p], max(A.starts[p], 0) * A.H);
+                wk.request[b] = p < 0 ? make_int2(-1, 0) : make_int2(wk.own + gbase[p], max(starts[p], 0) * A.H);
         } else if (g < G) {
             const int e = g - wk.own;
             int lo = 0, hi = A.P;   // last prefix group that starts at or before e
@@ -221,13 +232,13 @@ __global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(const __grid_
                 const int mid = (lo + hi) / 2;
                 if (gbase[mid] <= e) lo = mid; else hi = mid;
             }
-            const int s0 = max(A.starts[lo], 0), s1 = min(A.starts[lo + 1], A.B);
+            const int s0 = max(starts[lo], 0), s1 = min(starts[lo + 1], A.B);
             const int at = (e - gbase[lo]) * 128;
             d.q_row0 = s0 * A.H + at;
             d.rows = min(128, (s1 - s0) * A.H - at);
             d.pid = lo;
             d.sid = -1;
-            d.plen = clampi(A.plens[lo], A.max_plen);
+            d.plen = clampi(plens[lo], A.max_plen);
         }
         if (g < G) {
             d.ptiles = ceil_div(d.plen, kTile);
@@ -240,9 +251,10 @@ __global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(const __grid_
         mine = tiles > 0 ? c : -1;
         mine0 = d.tile0;
         mine1 = d.tile1;
-        if (g < G && G > kPlanThreads) wk.pieces[g] = {mine, mine0, mine1, 0};   // until the workers are known
+        if (g < G && G > threads) wk.pieces[g] = {mine, mine0, mine1, 0};   // until the workers are known
         if (tiles > 0) {
             wk.group[c] = d;
+            if (c < kPlanGroups) sh_group[c] = d;
             wk.bad[c] = 0;
             if (c < kPlanCache) sh_unit[c] = d.tile0 + c * kGroupCost;
         }
@@ -288,14 +300,14 @@ __global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(const __grid_
         st.te = sh_cut[tid + 1];
         st.g = first;
         st.pad = 0;
-        st.d = wk.group[first];
+        st.d = first < kPlanGroups ? sh_group[first] : wk.group[first];
         wk.start[at] = st;
     }
     if (tid >= workers && tid < wk.W) wk.start[tid].tb = wk.start[tid].te = 0;
     __syncthreads();
     // the workers of each group
-    for (int g = tid; g < G; g += kPlanThreads) {
-        if (G > kPlanThreads) {
+    for (int g = tid; g < G; g += threads) {
+        if (G > threads) {
             const Pieces p = wk.pieces[g];
             mine = p.g;
             mine0 = p.w0;
@@ -1019,7 +1031,7 @@ cudaError_t launch(const PrefixArgs& A, unsigned char* ws, int sms, cudaStream_t
         return cudaErrorInvalidValue;
     cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(prefix_attend_kernel<T>), static_cast<int>(kSmemBytes));
     if (e != cudaSuccess) return e;
-    prefix_plan_kernel<<<1, kPlanThreads, 0, s>>>(A, wk);
+    prefix_plan_kernel<<<1, L.groups <= 256 ? 256 : kPlanThreads, 0, s>>>(A, wk);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
