@@ -48,6 +48,10 @@ constexpr int kSmemCap = 192 * 1024;  // leaves room for a block of the shrink k
 constexpr int kMaxStages = 6;
 constexpr int kMinChunks = 4;         // shortest share of a cut tile
 constexpr int kSliceTok = 128;        // blocks of at least so many tokens are cut by columns
+constexpr int kFewTokens = 2;         // up to so many tokens take the CUDA-core kernel (8192 x 5120, rank 16: one token
+                                      // 16.8 us and 31 on the MMAs, two 22.6 and 29, four 38 and 29)
+constexpr int kGemvWarps = 8, kGemvBlocks = 4;
+constexpr int kGemvSteps = 2;         // 512-byte steps of a weight row in flight
 constexpr int kSortTok = 128;         // a single block of more tokens is put in adapter order
 constexpr int kMinSlice = 64;         // narrowest slice
 constexpr int kJoinCols = 32;         // columns of a tile cut along K that are counted and added at a time
@@ -911,9 +915,110 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
     if (warp == 1) tmem_dealloc_pair(tbase, 512);
 }
 
+// ------------------------------------------------------------------------------------- a few tokens
+
+template <typename T>
+__device__ __forceinline__ void to_float8(const uint4& v, float (&f)[8]) {
+    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 p = ElemTraits<T>::to_f2(*reinterpret_cast<const typename ElemTraits<T>::T2*>(&x[i]));
+        f[2 * i] = p.x;
+        f[2 * i + 1] = p.y;
+    }
+}
+// 16 bytes that are used once (X, which every row of W meets, keeps its place in L1)
+__device__ __forceinline__ uint4 load_once(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// Up to kFewTokens tokens: a warp takes two weight rows at a time, 16 bytes of each a lane and step, and
+// adds the tokens' adapters (U from the shrink kernel) before its lanes' sums meet. All that counts is
+// the stream of W: 32 warps an SM keep 64 KB of it in flight (16 warps with four steps each: 20.3 us for
+// one token onto 8192 rows of 5120, 32 with two: 16.8; onto 65536 rows of 7168 139 us, 6.8 TB/s).
+template <typename T, int kM>
+__global__ void __launch_bounds__(32 * kGemvWarps, kGemvBlocks) lora_gemv_kernel(const LoraArgs A, const Plan P, const unsigned char* ws) {
+    const int lane = threadIdx.x & 31, warps = gridDim.x * kGemvWarps;
+    const T* x = static_cast<const T*>(A.x);
+    const T* u[kM];        // the token's row of U, or none
+    long long b_row[kM];   // its adapter's first row of B
+    bool ready = false;
+    for (int pair = blockIdx.x * kGemvWarps + threadIdx.x / 32; pair * 2 < P.N; pair += warps) {
+        const int n0 = 2 * pair, n1 = min(n0 + 1, P.N - 1);
+        const T* w0 = static_cast<const T*>(A.w) + static_cast<long long>(n0) * P.K;
+        const T* w1 = static_cast<const T*>(A.w) + static_cast<long long>(n1) * P.K;
+        float acc[2][kM] = {};
+        auto add = [&](const uint4& v0, const uint4& v1, const uint4& xs, int m) {
+            float f0[8], f1[8], y[8];
+            to_float8<T>(v0, f0);
+            to_float8<T>(v1, f1);
+            to_float8<T>(xs, y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                acc[0][m] = fmaf(f0[i], y[i], acc[0][m]);
+                acc[1][m] = fmaf(f1[i], y[i], acc[1][m]);
+            }
+        };
+        for (int k0 = 8 * lane; k0 < P.K; k0 += 256 * kGemvSteps) {
+            uint4 v[2][kGemvSteps];
+#pragma unroll
+            for (int j = 0; j < kGemvSteps; ++j)
+                if (k0 + 256 * j < P.K) {
+                    v[0][j] = load_once(w0 + k0 + 256 * j);
+                    v[1][j] = load_once(w1 + k0 + 256 * j);
+                }
+#pragma unroll
+            for (int j = 0; j < kGemvSteps; ++j)
+                if (k0 + 256 * j < P.K)
+#pragma unroll
+                    for (int m = 0; m < kM; ++m)
+                        if (m < P.M)
+                            add(v[0][j], v[1][j], __ldg(reinterpret_cast<const uint4*>(x + m * A.x_stride + k0 + 256 * j)), m);
+        }
+        if (!ready) {
+            ready = true;
+            pdl_wait();
+            const int2* meta = reinterpret_cast<const int2*>(ws + P.off_meta);
+#pragma unroll
+            for (int m = 0; m < kM; ++m) {
+                u[m] = nullptr;
+                b_row[m] = 0;
+                const int id = m < P.M ? A.ids[m] : -1;
+                if (id < 0 || id >= P.adapters) continue;
+                int slot = 0;
+                while (slot < meta[0].x && meta[1 + slot].x != id) ++slot;
+                u[m] = reinterpret_cast<const T*>(ws + P.off_u) + (static_cast<size_t>(slot) * P.rchunks * P.tb + m) * P.kw;
+                b_row[m] = static_cast<long long>(id) * P.N;
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < kM; ++m)
+            if (u[m])
+                for (int k = 8 * lane; k < P.r; k += 256) {
+                    const T* b = static_cast<const T*>(A.b);
+                    add(load_once(b + (b_row[m] + n0) * P.r + k), load_once(b + (b_row[m] + n1) * P.r + k),
+                        __ldcg(reinterpret_cast<const uint4*>(u[m] + static_cast<size_t>(k / P.kw) * P.tb * P.kw + k % P.kw)), m);
+                }
+#pragma unroll
+        for (int m = 0; m < kM; ++m)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float y = acc[i][m];
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+                if (lane == 2 * m + i && m < P.M && n0 + i < P.N)
+                    static_cast<T*>(A.y)[static_cast<long long>(m) * P.N + n0 + i] = ElemTraits<T>::from_f(y);
+            }
+    }
+    if (!ready) pdl_wait();
+}
+
 template <typename T>
 cudaError_t launch(const LoraArgs& A, unsigned char* ws, int sms, cudaStream_t s) {
     const Plan P = make_plan(A.M, A.N, A.K, A.adapters, A.rank, sms);
+    const bool few = A.M <= kFewTokens;
     Maps maps;
     const uint64_t K = static_cast<uint64_t>(A.K), N = static_cast<uint64_t>(A.N), r = static_cast<uint64_t>(A.rank);
     const uint64_t wd[2] = {K, N}, ws1[1] = {K * 2};
@@ -927,11 +1032,11 @@ cudaError_t launch(const LoraArgs& A, unsigned char* ws, int sms, cudaStream_t s
                    ub[2] = {static_cast<uint32_t>(P.kw), kColStep / 2};
     const CUtensorMapSwizzle rswz = P.kw == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : P.kw == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
                                                                                          : CU_TENSOR_MAP_SWIZZLE_32B;
-    if (!encode_tmap_16b(&maps.w, A.w, 2, wd, ws1, wb, CU_TENSOR_MAP_SWIZZLE_128B) ||
+    if (!few && (!encode_tmap_16b(&maps.w, A.w, 2, wd, ws1, wb, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !encode_tmap_16b(&maps.x, P.sorted ? ws + P.off_x : A.x, 2, xd, xs, xb, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !encode_tmap_16b(&maps.xs, P.sorted ? ws + P.off_x : A.x, 2, xd, xs, sb, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !encode_tmap_16b(&maps.b, A.b, 3, bd, bs, bb, rswz) ||
-        !encode_tmap_16b(&maps.u, ws + P.off_u, 2, ud, us, ub, rswz))
+        !encode_tmap_16b(&maps.u, ws + P.off_u, 2, ud, us, ub, rswz)))
         return cudaErrorInvalidValue;
     const int smem = P.stages * P.stage_bytes + static_cast<int>(sizeof(Bars)) + 1024;
     cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(lora_gemm_kernel<T>),
@@ -954,6 +1059,15 @@ cudaError_t launch(const LoraArgs& A, unsigned char* ws, int sms, cudaStream_t s
     // the GEMM is let in as soon as all CTAs of the shrink kernel run
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    if (few) {
+        const int blocks = ceil_div(ceil_div(P.N, 2), kGemvWarps);
+        cfg.gridDim = dim3(blocks < kGemvBlocks * sms ? blocks : kGemvBlocks * sms);
+        cfg.blockDim = dim3(32 * kGemvWarps);
+        e = A.M == 1 ? cudaLaunchKernelEx(&cfg, lora_gemv_kernel<T, 1>, A, P, static_cast<const unsigned char*>(ws))
+                     : cudaLaunchKernelEx(&cfg, lora_gemv_kernel<T, kFewTokens>, A, P, static_cast<const unsigned char*>(ws));
+        count_launches(2);
+        return e != cudaSuccess ? e : cudaGetLastError();
+    }
     cfg.gridDim = dim3(2 * P.pairs);
     cfg.blockDim = dim3(kGemmThreads);
     cfg.dynamicSmemBytes = smem;
