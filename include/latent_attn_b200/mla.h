@@ -455,7 +455,8 @@ MLA_API mla_status_t mla_prefix_decode(const mla_config_t* cfg, const mla_prefix
  * an id outside [0, num_adapters) means no adapter. Any mix of adapters in any order; only those
  * that occur are read. Replaces, like mla_linear, the torch matmuls of LatentAttentionLayer.forward
  * (latent_attn/__init__.py:126, :128, :145), for requests with adapters; no reference counterpart.
- * tcgen05 kernel; the same call gives the same bits every time. Products and sums in fp32,
+ * tcgen05 kernel (CUDA cores for one or two tokens); the same call gives the same bits every time. The
+ * workspace holds A_a X[m] per 256 tokens and adapter that may occur there. Products and sums in fp32,
  * A_a X[m] and Y rounded once to the operands' type. */
 typedef struct mla_lora_args {
   mla_dtype_t dtype;            /* of X, W, A, B, Y: F16 or BF16 */

@@ -2,22 +2,29 @@
 //     Y[m] = W x[m] + s_a B_a (A_a x[m]),   a = ids[m]   (no second term where a is no adapter)
 // X (M, K), W (N, K), A (adapters, r, K), B (adapters, N, r), Y (M, N), all fp16 or bf16.
 //
-// Two kernels, the second launched beside the first (programmatic dependent launch):
+// Two kernels, the second let in while the first still runs (programmatic dependent launch):
 //   1. lora_shrink_kernel: U = s_a A_a x[m], for each block of up to 256 tokens and each adapter that
-//      occurs in it. A batch of one block is also put in adapter order (the rows of X are copied).
+//      occurs in it. A single block of more than 128 tokens is also put in adapter order (the rows of X
+//      are copied): its MMAs then cover few columns that are not the adapter's.
 //   2. lora_gemm_kernel: Y^T tiles [256 weight rows x up to 256 tokens] on tcgen05, a pair of CTAs each
 //      (cta_group::2: 128 weight rows and half of the tokens' rows in each CTA's shared memory, so that
 //      a token's row is loaded once for 256 weight rows). First the K columns, then the ranks as extra
 //      K columns: for each active adapter a product of B_a's 256 rows with U's rows of the adapter's
-//      tokens, 16 ranks an MMA, added into those tokens' columns only. Only the adapters that a block
-//      really uses are read, and an MMA covers whole groups of 32 columns.
+//      tokens, added into those tokens' columns only. Only the adapters that a block really uses are
+//      read, and an MMA covers whole groups of 32 columns.
+//      Or lora_gemv_kernel on the CUDA cores, for one or two tokens.
 // Small batches are bound by W's bytes (each read once for all tokens), prompts by the tensor pipe and
-// by what L2 delivers to the SMs (without multicast a pair needs 62 KB for 0.5 us of MMAs).
+// by what L2 delivers to the SMs (without multicast a pair needs 62 KB for 0.5 us of MMAs). Without
+// adapters the GEMM takes 212 us for 256 tokens onto 65536 rows of 7168 (1.14 PFLOP/s) and 266 us for
+// 2051 tokens onto 5120 rows of 16384; with 32 adapters of rank 64 and 4 of rank 32 it is 275 and 303 us,
+// of which 23 and 49 us are the shrink kernel's.
 //
-// Work split: whole tiles go round robin over the pairs; the tiles that do not fill a last round are
-// cut along K into equal shares for all pairs, so no SM idles. A CTA that shares a tile stores its
-// fp32 partial and counts itself; the one that completes the count adds all partials in their order
-// along K, so results do not depend on who came last. No CTA waits for another pair's.
+// Work split: whole tiles go round robin over the pairs, and the tiles that do not fill a last round are
+// cut. Blocks of 128 tokens and more are cut by columns (slices of 64 and more, no sums to join: 256
+// tokens onto 65536 rows 281 us, cut along K 298). Smaller ones, which W's bytes bound, are cut along K
+// into equal shares for all pairs. A CTA that shares such a tile stores its fp32 partial and counts
+// itself, per 32 columns; the one that completes a count adds all partials in their order along K, so
+// results do not depend on who came last. No CTA waits for another pair's.
 //
 // A zero of U times an infinite or NaN value of another request's adapter would be NaN, so an output
 // that is not finite is computed again from its own operands alone (own_element): a broken adapter
@@ -292,8 +299,9 @@ __device__ __forceinline__ Own order_tokens(Order& o, Table& tab, const LoraArgs
 // and x's rows straight from global memory, 16 bytes a lane: the sum over K may take its columns in any
 // order, so lane t of a quad takes columns 8 t .. 8 t + 7 of each 32, for both operands alike. Tokens
 // are gathered by their rows' addresses. Partial sums meet in shared memory, in warp order and then in
-// CTA order. (16 ranks x 32 tokens are too small for tcgen05's 128-row tile; the kernel runs beside the
-// GEMM's K columns, one CTA an SM.)
+// CTA order. (16 ranks x 32 tokens are too small for tcgen05's 128-row tile. Letting the GEMM run beside
+// it, with registers left for both, was slower: its few loads in flight wait behind the GEMM's, 108 us
+// instead of 23 for 256 tokens with 32 adapters of rank 64 over K = 7168.)
 template <typename T, int kQ>
 __global__ void __launch_bounds__(32 * kShrinkWarps, 2) lora_shrink_kernel(const LoraArgs A, const Plan P, unsigned char* ws) {
     __shared__ Order o;
