@@ -17,6 +17,16 @@ mla_status_t check_dtype(mla_dtype_t d) {
     return MLA_OK;
 }
 
+// A launch may throw on the host (no memory, a lock): nothing of that crosses a C entry.
+template <typename F>
+cudaError_t launch(F f) {
+    try {
+        return f();
+    } catch (...) {
+        return cudaErrorMemoryAllocation;
+    }
+}
+
 }  // namespace
 
 extern "C" {
@@ -84,7 +94,7 @@ mla_status_t mla_cache_append_rope(const mla_config_t* cfg, const mla_append_rop
         const double theta = a->rope_theta > 0.f ? static_cast<double>(a->rope_theta) : 10000.0;
         for (int i = 0; i < dR / 2; ++i) A.freq[i] = static_cast<float>(std::pow(theta, -2.0 * i / static_cast<double>(dR)));
     }
-    const cudaError_t e = mla::launch_append_rope(A, a->dtype == MLA_DTYPE_BF16, reinterpret_cast<cudaStream_t>(stream));
+    const cudaError_t e = launch([&] { return mla::launch_append_rope(A, a->dtype == MLA_DTYPE_BF16, reinterpret_cast<cudaStream_t>(stream)); });
     return e == cudaSuccess ? MLA_OK : api_cuda_fail(e, "append kernel launch");
 }
 
@@ -183,9 +193,9 @@ mla_status_t mla_prefix_decode(const mla_config_t* cfg, const mla_prefix_args_t*
         if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
             return api_fail(MLA_ERR_WORKSPACE, "workspace is null or not 256-byte aligned");
         if (workspace_bytes < need) return api_fail(MLA_ERR_WORKSPACE, "workspace too small: %zu < %zu bytes", workspace_bytes, need);
-        e = mla::launch_prefix_sm100(A, bf16, workspace, sms, s);
+        e = launch([&] { return mla::launch_prefix_sm100(A, bf16, workspace, sms, s); });
     } else {
-        e = mla::launch_prefix_simt(A, bf16, s);
+        e = launch([&] { return mla::launch_prefix_simt(A, bf16, s); });
     }
     return e == cudaSuccess ? MLA_OK : api_cuda_fail(e, "prefix decode kernel launch");
 }
@@ -202,6 +212,9 @@ static mla_status_t make_lora(const mla_lora_args_t* a, mla::LoraArgs* A, int* s
     if (a->rank <= 0 || a->rank % 8 != 0 || a->rank > 256)
         return api_fail(MLA_ERR_UNSUPPORTED, "rank must be a multiple of 8 and <= 256 (got %d)", a->rank);
     if (a->M > (1 << 23) || a->N > (1 << 28)) return api_fail(MLA_ERR_UNSUPPORTED, "M must be <= 2^23 and N <= 2^28");
+    // rows of the intermediate A_a X[m] (per 256 tokens, adapter and 64 ranks), counted in 32 bits
+    if ((a->M + 255ll) * (a->num_adapters < 256 ? a->num_adapters : 256) * ((a->rank + 63) / 64) > 0x7fffffffll)
+        return api_fail(MLA_ERR_UNSUPPORTED, "too many tokens for %d adapters of rank %d (M=%d)", a->num_adapters, a->rank, a->M);
     if (!a->X || !a->W || !a->lora_a || !a->lora_b || !a->adapter_ids || !a->Y)
         return api_fail(MLA_ERR_INVALID_ARGUMENT, "null pointer");
     if (a->x_stride != 0 && a->x_stride < a->K) return api_fail(MLA_ERR_INVALID_ARGUMENT, "x_stride %lld < K", (long long)a->x_stride);
@@ -235,7 +248,9 @@ mla_status_t mla_linear_lora(const mla_lora_args_t* a, void* workspace, size_t w
     if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
         return api_fail(MLA_ERR_WORKSPACE, "workspace is null or not 256-byte aligned");
     if (workspace_bytes < need) return api_fail(MLA_ERR_WORKSPACE, "workspace too small: %zu < %zu bytes", workspace_bytes, need);
-    const cudaError_t e = mla::launch_lora(A, a->dtype == MLA_DTYPE_BF16, workspace, sms, reinterpret_cast<cudaStream_t>(stream));
+    const cudaError_t e = launch([&] {
+        return mla::launch_lora(A, a->dtype == MLA_DTYPE_BF16, workspace, sms, reinterpret_cast<cudaStream_t>(stream));
+    });
     return e == cudaSuccess ? MLA_OK : api_cuda_fail(e, "projection with adapters: kernel launch");
 }
 

@@ -57,6 +57,16 @@ def test_entries_refuse_null_and_bad_arguments():
     _refused(lambda: lib.mla_linear_lora(C.byref(_lib.MlaLoraArgs()), None, 0, None))
 
 
+@pytest.mark.parametrize("m,adapters,rank", [(1 << 23, 256, 8), (1 << 23, 128, 128), (1 << 24, 1, 8), (1, 1, 264),
+                                             (1, 1, 12), (1, 0, 8), (0, 1, 8)])
+def test_projection_refuses_sizes_before_it_looks_at_memory(m, adapters, rank):
+    lib = _lib.load()
+    a = _lib.MlaLoraArgs(1, m, 64, 64, 16, 0, 16, adapters, rank, 16, 16, 16, None, 16)
+    size = C.c_size_t()
+    with pytest.raises(_lib.MlaError, match="tokens|rank|M must|num_adapters|positive"):
+        _lib.check(lib.mla_linear_lora_workspace_size(C.byref(a), C.byref(size)))
+
+
 def test_shared_prefix_batch_lays_out_positions():
     cfg = MLAConfig(512, 512, 128, 64, 16, 128)
     b = SharedPrefixBatch(cfg, "cpu", [2, 1], [100, 0], [3, 0, 7], 10, prefix_offsets=[0, 0], own_offsets=[200, 220, 240])
