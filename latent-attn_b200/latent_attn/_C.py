@@ -690,6 +690,8 @@ def mla_cache_append(kv_cache: torch.Tensor, c_t: torch.Tensor, k_rope: torch.Te
 # comparison of what must hold, and says what is wrong only when it does not.
 
 _I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
+_pack_append, _pack_prefix, _pack_lora = (_lib.packer(t) for t in (_lib.MlaAppendRopeArgs, _lib.MlaPrefixArgs,
+                                                                  _lib.MlaLoraArgs))
 
 
 def _wrong(t: torch.Tensor, name: str, dtype, index: int, shape, contiguous: bool) -> None:
@@ -772,20 +774,20 @@ def mla_cache_append_rope(kv_cache: torch.Tensor, c: torch.Tensor, k_rope: torch
     k_rope, k_st = _spread(k_rope, _rows(k_rope, "k_rope", dt, dev, (T, dR)))
     cu_p = _dense(cu_tokens, "cu_tokens", _I32, dev, (B + 1,))
     lens_p = _dense(seq_lens, "seq_lens", _I32, dev, (B,))
-    new_p = None if new_lens is None else _dense(new_lens, "new_lens", _I32, dev, (B,))
-    off_p = None if kv_offsets is None else _dense(kv_offsets, "kv_offsets", _I64, dev, (B,))
-    table_p, pages = (None, 0) if page_table is None else _table(page_table, "page_table", dev, B)
+    new_p = 0 if new_lens is None else _dense(new_lens, "new_lens", _I32, dev, (B,))
+    off_p = 0 if kv_offsets is None else _dense(kv_offsets, "kv_offsets", _I64, dev, (B,))
+    table_p, pages = (0, 0) if page_table is None else _table(page_table, "page_table", dev, B)
     if status is not None and (status.dtype is not _I32 or status.get_device() != dev):
         raise RuntimeError("status must be a CUDA int32 tensor")
-    cos_p = sin_p = None
+    cos_p = sin_p = 0
     if rope_cos is not None or rope_sin is not None:
         _check_tables(rope_cos, rope_sin)
         for t, n in ((rope_cos, "rope_cos"), (rope_sin, "rope_sin")):
             if t.dim() != 2 or t.size(1) != dR // 2 or t.size(0) < max_seq_len or t.get_device() != dev:
                 raise RuntimeError(f"{n} must be (>= {max_seq_len}, {dR // 2}) on cuda:{dev}")
         cos_p, sin_p = rope_cos.data_ptr(), rope_sin.data_ptr()
-    w_p = None if norm_weight is None else _dense(norm_weight, "norm_weight", dt, dev, (dc,))
-    q_p = qo_p = None
+    w_p = 0 if norm_weight is None else _dense(norm_weight, "norm_weight", dt, dev, (dc,))
+    q_p = qo_p = 0
     q_st = qo_st = (0, 0, 1)
     if q_rope is not None:
         q_rope, q_st = _spread(q_rope, _rows(q_rope, "q_rope", dt, dev, (T, H, dR)))
@@ -798,11 +800,11 @@ def mla_cache_append_rope(kv_cache: torch.Tensor, c: torch.Tensor, k_rope: torch
             q_p, qo_p = q_rope.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise RuntimeError("q_out needs q_rope")
-    a = _lib.MlaAppendRopeArgs(_DT[dt], B, T, kv_cache.data_ptr(), kv_stride, kv_cache.size(0), c.data_ptr(), c_st[0],
-                               k_rope.data_ptr(), k_st[0], cu_p, lens_p, max_seq_len, off_p, table_p, page_rows, pages,
-                               w_p, norm_eps, cos_p, sin_p, rope_theta, q_p, q_st[0], q_st[1], qo_p, qo_st[0], qo_st[1],
-                               new_p, None if status is None else status.data_ptr())
-    st = _lib.load().mla_cache_append_rope(cfg, a, _current_stream(dev))
+    a = _pack_append(_DT[dt], B, T, kv_cache.data_ptr(), kv_stride, kv_cache.size(0), c.data_ptr(), c_st[0],
+                     k_rope.data_ptr(), k_st[0], cu_p, lens_p, max_seq_len, off_p, table_p, page_rows, pages, w_p,
+                     norm_eps, cos_p, sin_p, rope_theta, q_p, q_st[0], q_st[1], qo_p, qo_st[0], qo_st[1], new_p,
+                     0 if status is None else status.data_ptr())
+    st = _lib.load_packed().mla_cache_append_rope(C.addressof(cfg), a, _current_stream(dev))
     if st:
         _lib.check(st)
     return q_out
@@ -837,26 +839,26 @@ def mla_prefix_decode(kv_cache: torch.Tensor, q_absorbed: torch.Tensor, q_rope: 
     starts_p = _dense(group_starts, "group_starts", _I32, dev, (P + 1,))
     plens_p = _dense(prefix_lens, "prefix_lens", _I32, dev, (P,))
     lens_p = _dense(seq_lens, "seq_lens", _I32, dev, (B,))
-    poff_p = None if prefix_offsets is None else _dense(prefix_offsets, "prefix_offsets", _I64, dev, (P,))
-    off_p = None if kv_offsets is None else _dense(kv_offsets, "kv_offsets", _I64, dev, (B,))
-    ptable_p, ppages = (None, 0) if prefix_table is None else _table(prefix_table, "prefix_table", dev, P)
-    table_p, pages = (None, 0) if page_table is None else _table(page_table, "page_table", dev, B)
+    poff_p = 0 if prefix_offsets is None else _dense(prefix_offsets, "prefix_offsets", _I64, dev, (P,))
+    off_p = 0 if kv_offsets is None else _dense(kv_offsets, "kv_offsets", _I64, dev, (B,))
+    ptable_p, ppages = (0, 0) if prefix_table is None else _table(prefix_table, "prefix_table", dev, P)
+    table_p, pages = (0, 0) if page_table is None else _table(page_table, "page_table", dev, B)
     if out is None:
         out = torch.empty_like(q_absorbed)
         out_p = out.data_ptr()
     else:
         out_p = _dense(out, "out", dt, dev, (B, H, dc))
-    a = _lib.MlaPrefixArgs(_DT[dt], B, P, kv_cache.data_ptr(), kv_stride, kv_cache.size(0), qa_p, qr_p, starts_p, plens_p,
-                           max_prefix_len, lens_p, max_seq_len, poff_p, off_p, ptable_p, ppages, table_p, pages, page_rows,
-                           softmax_scale, out_p, kernel)
-    lib = _lib.load()
+    a = _pack_prefix(_DT[dt], B, P, kv_cache.data_ptr(), kv_stride, kv_cache.size(0), qa_p, qr_p, starts_p, plens_p,
+                     max_prefix_len, lens_p, max_seq_len, poff_p, off_p, ptable_p, ppages, table_p, pages, page_rows,
+                     softmax_scale, out_p, kernel)
+    lib, cfg_p = _lib.load_packed(), C.addressof(cfg)
     n = C.c_size_t()
-    st = lib.mla_prefix_decode_workspace_size(cfg, a, n)
+    st = lib.mla_prefix_decode_workspace_size(cfg_p, a, n)
     if not st:
         need = n.value
         if workspace is None or workspace.nbytes < need or workspace.data_ptr() % 256:
             workspace = torch.empty(need, dtype=torch.uint8, device=kv_cache.device)
-        st = lib.mla_prefix_decode(cfg, a, workspace.data_ptr(), need, _current_stream(dev))
+        st = lib.mla_prefix_decode(cfg_p, a, workspace.data_ptr(), need, _current_stream(dev))
     if st:
         _lib.check(st)
     return out
@@ -880,7 +882,7 @@ def linear_lora(x: torch.Tensor, W: torch.Tensor, lora_a: torch.Tensor, lora_b: 
     a_p = _dense(lora_a, "lora_a", dt, dev, (adapters, rank, K))
     b_p = _dense(lora_b, "lora_b", dt, dev, (adapters, N, rank))
     ids_p = _dense(adapter_ids, "adapter_ids", _I32, dev, (M,))
-    scales_p = None if scales is None else _dense(scales, "scales", _F32, dev, (adapters,))
+    scales_p = 0 if scales is None else _dense(scales, "scales", _F32, dev, (adapters,))
     if out is None:
         out = torch.empty(M, N, dtype=dt, device=x.device)
         out_p = out.data_ptr()
@@ -888,9 +890,9 @@ def linear_lora(x: torch.Tensor, W: torch.Tensor, lora_a: torch.Tensor, lora_b: 
         out_p = _dense(out, "out", dt, dev, (M, N))
     if M == 0:
         return out
-    a = _lib.MlaLoraArgs(_DT[dt], M, N, K, x.data_ptr(), x_st[0] if M > 1 else K, W_p, adapters, rank, a_p, b_p, ids_p,
-                         scales_p, out_p)
-    lib = _lib.load()
+    a = _pack_lora(_DT[dt], M, N, K, x.data_ptr(), x_st[0] if M > 1 else K, W_p, adapters, rank, a_p, b_p, ids_p,
+                   scales_p, out_p)
+    lib = _lib.load_packed()
     n = C.c_size_t()
     st = lib.mla_linear_lora_workspace_size(a, n)
     if not st:
