@@ -104,6 +104,7 @@ struct Work {                 // workspace
     int2* request;            // per request: its prefix's first group among `pieces` (or -1) and first row
     int* gbase;               // per prefix group: its first row group (num_groups + 1)
     int* bad;                 // per group with tiles: it met a row outside the cache
+    int* done;                // per worker: its CTAs whose records are written
     float* rec_ml;            // per record row kMl floats: m, l, -, -, and 2^-f of each 64 columns of o
     uint16_t* rec_o;          // o 2^f in fp16
     float2* rowsum;           // per CTA: [kSums][128] row sums and references handed between its sets
@@ -188,6 +189,7 @@ __global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(const __grid_
         carry = 0;
         *wk.status = 0;
     }
+    if (tid < wk.W) wk.done[tid] = 0;
     __syncthreads();
     int extra = 0;   // row groups of the prefixes
     if (!wk.fold) {
@@ -477,7 +479,6 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
     volatile int* err = wk.status;
 
     if (threadIdx.x == 0) {
-        pdl_launch_dependents();
         tma_prefetch_desc(&tmap);
         tma_prefetch_desc(&tmap_rope);
         for (int s = 0; s < kStages; ++s) {
@@ -511,6 +512,8 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
     tc_fence_after();
     const uint32_t tbase = bars->tmem;
     pdl_wait();   // the plan
+    // the merge may start: the plan is complete for it too, and every CTA whose records it awaits runs
+    pdl_launch_dependents();
     // identical in both CTAs of the pair; a pair without tiles goes straight to the teardown
     const Start start = wk.start[w];
     const int n = start.te - start.tb;
@@ -848,6 +851,8 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
     // ---------------------------------------------------------------- teardown
     __syncthreads();
     if (threadIdx.x == 0) {
+        __threadfence();
+        atomicAdd(&wk.done[w], 1);   // this CTA's records are written (or, after a failure, the status is)
         // the pair finishes together: no CTA leaves while the other may still address it
         mbar_arrive_remote(mapa(smem_u32(&bars->done), peer));
         mbar_wait_cluster_full(smem_u32(&bars->done), 0, err, code(kWaitTeardown));
@@ -867,8 +872,26 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
 
 constexpr int kMergeWarps = 8;
 
+// Waits until the workers w0 .. w1 have written their records; false when one of them does not (warp-wide).
+// They all run: the kernel is let in by the last of them to start.
+__device__ __forceinline__ bool await_workers(const int* done, int w0, int w1, int lane) {
+    const uint64_t t0 = globaltimer_ns();
+    for (int w = w0 + lane; __any_sync(0xffffffffu, w <= w1); w += 32) {
+        for (;;) {
+            int n = 2;
+            if (w <= w1) asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(n) : "l"(done + w) : "memory");
+            if (__all_sync(0xffffffffu, n >= 2)) break;
+            if (__any_sync(0xffffffffu, globaltimer_ns() - t0 > kDefaultWaitNs)) return false;
+            __nanosleep(64);
+        }
+    }
+    __syncwarp();
+    return true;
+}
+
 // One output row per `kWarps` warps: each takes every kWarps-th record of the row's groups, keeping
-// the running maximum, sum and weighted latent in fp32; the warps meet in shared memory.
+// the running maximum, sum and weighted latent in fp32; the warps meet in shared memory. A row starts
+// as soon as the workers of its own records are done, beside those that still work.
 template <typename T, int kWarps>
 __global__ void __launch_bounds__(32 * kMergeWarps) prefix_merge_kernel(const __grid_constant__ PrefixArgs A, const Work wk) {
     constexpr int kRows = kMergeWarps / kWarps;   // rows per block
@@ -877,7 +900,6 @@ __global__ void __launch_bounds__(32 * kMergeWarps) prefix_merge_kernel(const __
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     const int sub = warp % kWarps;
     const int f = blockIdx.x * kRows + warp / kWarps;
-    pdl_wait();
     const bool live = f < A.B * A.H;
     float m = -INFINITY, l = 0.f;
     float o[16];
@@ -890,14 +912,14 @@ __global__ void __launch_bounds__(32 * kMergeWarps) prefix_merge_kernel(const __
         const int2 rq = wk.fold ? make_int2(-1, 0) : wk.request[b];
         Pieces piece[2];
         piece[0] = wk.pieces[b * ceil_div(A.H, 128) + h / 128];
-        bad = *wk.status != 0;
         piece[1].g = -1;
         if (rq.x >= 0) piece[1] = wk.pieces[rq.x + (f - rq.y) / 128];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             if (piece[k].g < 0) continue;
             const int g = piece[k].g, w1 = piece[k].w1, r = k == 0 ? h % 128 : (f - rq.y) % 128;
-            bad = bad || wk.bad[g] != 0;
+            bad = !await_workers(wk.done, piece[k].w0, w1, lane) || bad;
+            bad = bad || *static_cast<volatile int*>(wk.status) != 0 || __ldcg(wk.bad + g) != 0;
             constexpr int kAhead = 4;
             for (int w = piece[k].w0 + sub; w <= w1; w += kWarps * kAhead) {
                 uint4 v[kAhead][2];
@@ -906,11 +928,11 @@ __global__ void __launch_bounds__(32 * kMergeWarps) prefix_merge_kernel(const __
                 for (int i = 0; i < kAhead; ++i)
                     if (w + i * kWarps <= w1) {
                         const long long at = static_cast<long long>(g + w + i * kWarps) * 128 + r;
-                        ml[i] = *reinterpret_cast<const float2*>(wk.rec_ml + at * kMl);
-                        fs[i] = make_float2(wk.rec_ml[at * kMl + 4 + lane / 8], wk.rec_ml[at * kMl + 8 + lane / 8]);
+                        ml[i] = __ldcg(reinterpret_cast<const float2*>(wk.rec_ml + at * kMl));
+                        fs[i] = make_float2(__ldcg(wk.rec_ml + at * kMl + 4 + lane / 8), __ldcg(wk.rec_ml + at * kMl + 8 + lane / 8));
                         const uint4* src = reinterpret_cast<const uint4*>(wk.rec_o + at * 512);
-                        v[i][0] = src[lane];
-                        v[i][1] = src[32 + lane];
+                        v[i][0] = __ldcg(src + lane);
+                        v[i][1] = __ldcg(src + 32 + lane);
                     }
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i)
@@ -969,13 +991,14 @@ __global__ void __launch_bounds__(32 * kMergeWarps) prefix_merge_kernel(const __
             out[32 * q + lane] = make_uint4(pair_of<T>(o[8 * q] * inv, o[8 * q + 1] * inv), pair_of<T>(o[8 * q + 2] * inv, o[8 * q + 3] * inv),
                                             pair_of<T>(o[8 * q + 4] * inv, o[8 * q + 5] * inv), pair_of<T>(o[8 * q + 6] * inv, o[8 * q + 7] * inv));
     }
+    pdl_wait();   // this kernel ends after the one before it
 }
 
 // ------------------------------------------------------------------------------------- host
 
 struct Layout {
     long long groups;     // most groups
-    size_t off_group, off_start, off_pieces, off_request, off_base, off_bad, off_sum, off_ml, off_o, total;
+    size_t off_group, off_start, off_pieces, off_request, off_base, off_bad, off_done, off_sum, off_ml, off_o, total;
     int W, own, fold;
 };
 
@@ -1000,6 +1023,7 @@ Layout layout(const PrefixArgs& A, int sms) {
     L.off_request = take(sizeof(int2) * A.B);
     L.off_base = take(sizeof(int) * A.P);
     L.off_bad = take(sizeof(int) * groups);
+    L.off_done = take(sizeof(int) * L.W);
     L.off_sum = take(sizeof(float2) * 2 * L.W * kSums * 128);
     L.off_ml = take(recs * 128 * kMl * sizeof(float));
     L.off_o = take(recs * 128 * 512 * 2);
@@ -1018,6 +1042,7 @@ cudaError_t launch(const PrefixArgs& A, unsigned char* ws, int sms, cudaStream_t
     wk.request = reinterpret_cast<int2*>(ws + L.off_request);
     wk.gbase = reinterpret_cast<int*>(ws + L.off_base);
     wk.bad = reinterpret_cast<int*>(ws + L.off_bad);
+    wk.done = reinterpret_cast<int*>(ws + L.off_done);
     wk.rec_ml = reinterpret_cast<float*>(ws + L.off_ml);
     wk.rec_o = reinterpret_cast<uint16_t*>(ws + L.off_o);
     wk.rowsum = reinterpret_cast<float2*>(ws + L.off_sum);
