@@ -873,36 +873,44 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
             asm volatile("bar.sync 1, 128;" ::: "memory");
             const int last = bars->last;
             if (last) __threadfence();
-            // add the partials in order, this CTA's own from the accumulator; the others' are requested two
+            // add the partials in order, this CTA's own from the accumulator; the others' are requested three
             // pairs at a time, one round trip each
             for (int c = 0; c < toks; c += kJoinCols) {
                 if (!(last >> c / kJoinCols & 1)) continue;
                 uint32_t own[32];
                 tmem_ld32_sync(d + c, own);
                 float v[32] = {};
-                for (int wa = w0; wa <= w1; wa += 2) {
-                    float4 y[2][8];
+                bool mine_in = false;
+                auto add_own = [&] {
+                    mine_in = true;
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        if (wa + i <= w1 && wa + i != me) {
-                            const float4* src = part(wa + i) + c / 4 * kRows;
+                    for (int k = 0; k < 32; ++k) v[k] += __uint_as_float(own[k]);
+                };
+                for (int o = 0; o < w1 - w0; o += 3) {
+                    float4 y[3][8];
+#pragma unroll
+                    for (int i = 0; i < 3; ++i)
+                        if (o + i < w1 - w0) {
+                            const int wa = w0 + o + i + (w0 + o + i >= me);
+                            const float4* src = part(wa) + c / 4 * kRows;
 #pragma unroll
                             for (int k = 0; k < 8; ++k)
                                 if (k < 4 || c + 16 < toks) y[i][k] = __ldcg(src + k * kRows);
                         }
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        if (wa + i <= w1) {
-                            const bool self = wa + i == me;
+                    for (int i = 0; i < 3; ++i)
+                        if (o + i < w1 - w0) {
+                            if (!mine_in && w0 + o + i >= me) add_own();
 #pragma unroll
                             for (int k = 0; k < 8; ++k) {
-                                v[4 * k] += self ? __uint_as_float(own[4 * k]) : y[i][k].x;
-                                v[4 * k + 1] += self ? __uint_as_float(own[4 * k + 1]) : y[i][k].y;
-                                v[4 * k + 2] += self ? __uint_as_float(own[4 * k + 2]) : y[i][k].z;
-                                v[4 * k + 3] += self ? __uint_as_float(own[4 * k + 3]) : y[i][k].w;
+                                v[4 * k] += y[i][k].x;
+                                v[4 * k + 1] += y[i][k].y;
+                                v[4 * k + 2] += y[i][k].z;
+                                v[4 * k + 3] += y[i][k].w;
                             }
                         }
                 }
+                if (!mine_in) add_own();
                 store16(c, v);
                 if (c + 16 < toks) store16(c + 16, v + 16);
             }
