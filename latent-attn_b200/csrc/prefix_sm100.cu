@@ -36,7 +36,7 @@
 // slot is free.
 // Bound by that chain and the MMAs: a tile takes 1.13 us (0.78 at the measured tensor rate), a batch 20 us
 // beside its tiles (plan 4, first loads 4, last softmax and record 5, merge 5). 64 requests of 128 heads
-// over a prefix of 8192: 158 us, 940 TFLOP/s; 32 of 16 heads over one of 131072: 154 us, 950 TFLOP/s.
+// over a prefix of 8192: 157 us, 960 TFLOP/s; 32 of 16 heads over one of 131072: 154 us, 950 TFLOP/s.
 // A parity wait may only start once the phase before the awaited one is known to be complete (it would
 // pass at once otherwise), so a barrier that a set waits on for its own tiles belongs to that set.
 #include <cfloat>
@@ -431,6 +431,19 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
+// 32 bytes a lane, in one request where the address allows it: lanes on different rows cost one tag each
+// and request.
+__device__ __forceinline__ void load32(const uint4* p, bool aligned, uint4& a, uint4& b) {
+    if (aligned) {
+        asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+                     : "l"(p));
+    } else {
+        a = __ldg(p);
+        b = __ldg(p + 1);
+    }
+}
+
 // 64 columns of this thread's O row (TMEM) to a record row, times the 2^f that brings them below 2^15
 // (1 for zeros, and for infinities and NaN, which go into the record as they are); returns 2^-f.
 // Warp-collective.
@@ -635,22 +648,33 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
             const long long row = d.q_row0 + t;
             const uint4* lat = reinterpret_cast<const uint4*>(static_cast<const T*>(A.qa) + row * 512 + 256 * rank);
             const uint4* rope = reinterpret_cast<const uint4*>(static_cast<const T*>(A.qr) + row * 64 + 32 * rank);
-            const bool have = t < d.rows;
+            const bool have = t < d.rows, q32 = reinterpret_cast<uintptr_t>(A.qa) % 32 == 0;
 #pragma unroll 1
-            for (int c = c0; c < 4; c += step) {
-                uint4 v[8], r;
+            for (int c = c0; c < 4; c += 2 * step) {   // two blocks of 64 columns a round trip
+                uint4 v[2][8], r[2];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] = have ? __ldg(lat + 8 * c + k) : make_uint4(0, 0, 0, 0);
-                r = have ? __ldg(rope + c) : make_uint4(0, 0, 0, 0);
+                for (int e = 0; e < 2; ++e) {
+                    const bool on = have && c + e * step < 4;
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const uint32_t x[16] = {v[4 * q].x, v[4 * q].y, v[4 * q].z, v[4 * q].w,
-                                            v[4 * q + 1].x, v[4 * q + 1].y, v[4 * q + 1].z, v[4 * q + 1].w,
-                                            v[4 * q + 2].x, v[4 * q + 2].y, v[4 * q + 2].z, v[4 * q + 2].w,
-                                            v[4 * q + 3].x, v[4 * q + 3].y, v[4 * q + 3].z, v[4 * q + 3].w};
-                    tmem_st16(trow + kColQ + 32 * c + 16 * q, x);
+                    for (int k = 0; k < 4; ++k) {
+                        v[e][2 * k] = v[e][2 * k + 1] = make_uint4(0, 0, 0, 0);
+                        if (on) load32(lat + 8 * (c + e * step) + 2 * k, q32, v[e][2 * k], v[e][2 * k + 1]);
+                    }
+                    r[e] = on ? __ldg(rope + c + e * step) : make_uint4(0, 0, 0, 0);
                 }
-                *reinterpret_cast<uint4*>(qrope + c * kQRopeBoxBytes + t * 16) = r;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    if (c + e * step >= 4) break;
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const uint32_t x[16] = {v[e][4 * q].x, v[e][4 * q].y, v[e][4 * q].z, v[e][4 * q].w,
+                                                v[e][4 * q + 1].x, v[e][4 * q + 1].y, v[e][4 * q + 1].z, v[e][4 * q + 1].w,
+                                                v[e][4 * q + 2].x, v[e][4 * q + 2].y, v[e][4 * q + 2].z, v[e][4 * q + 2].w,
+                                                v[e][4 * q + 3].x, v[e][4 * q + 3].y, v[e][4 * q + 3].z, v[e][4 * q + 3].w};
+                        tmem_st16(trow + kColQ + 32 * (c + e * step) + 16 * q, x);
+                    }
+                    *reinterpret_cast<uint4*>(qrope + (c + e * step) * kQRopeBoxBytes + t * 16) = r[e];
+                }
             }
             fence_proxy_async_smem();
             tmem_st_wait();
@@ -672,8 +696,18 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
             const uint32_t phase = (j / kSlots) & 1;
             const uint32_t x_row = xbuf_u32 + slot * kXBytes + t * 16;
             const uint32_t x_full = smem_u32(&bars->x_full[slot]);
+            bool got = true;
+            if (it.seg_first() && j > 0) {
+                // A new group: its Q replaces the one that the score of tile j - 1 was the last to read. (This set
+                // waits for its score anyway; the one of tile j - 1 would be held up. That barrier is another
+                // set's, but its phase before is complete: this set's tile j - kSets came after it.)
+                got = mbar_wait(smem_u32(&bars->s_full[(j - 1) % kSets]), ((j - 1) / kSets) & 1, err, code(kWaitS));
+                if (!warp_ok(got)) break;
+                tc_fence_after();
+                load_q(it.d, 0, 1, &bars->q_ready);
+            }
             // ---- S_r(j) to registers, release S, send the fp16 partial
-            bool got = mbar_wait(smem_u32(&bars->s_full[sid]), (j / kSets) & 1, err, code(kWaitS));
+            got = mbar_wait(smem_u32(&bars->s_full[sid]), (j / kSets) & 1, err, code(kWaitS));
             if (!warp_ok(got)) break;
             if (t == 0) mbar_arrive_expect_tx(x_full, kXBytes);
             tc_fence_after();
@@ -701,12 +735,6 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
 #pragma unroll
                 for (int c = 0; c < 8; ++c)
                     st_async_v4(dst + c * kXUnit, h[4 * c], h[4 * c + 1], h[4 * c + 2], h[4 * c + 3], bar);
-            }
-            if (it.seg_last() && it.t + 1 < it.t_end) {
-                // the score of tile j was the last MMA to read this group's Q
-                Tiles nx = it;
-                nx.next(wk);
-                load_q(nx.d, 0, 1, &bars->q_ready);
             }
             if (np < kTile) {
                 // rows past the end: their weights are zero, but zero times what lies there need not be
