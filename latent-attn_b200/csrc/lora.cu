@@ -20,7 +20,7 @@
 // of which 23 and 49 us are the shrink kernel's.
 //
 // Work split: whole tiles go round robin over the pairs, and the tiles that do not fill a last round are
-// cut. Blocks of 128 tokens and more are cut by columns (slices of 64 and more, no sums to join: 256
+// cut. Blocks of 128 tokens and more are cut by columns (no sums to join: 256
 // tokens onto 65536 rows 281 us, cut along K 298). Smaller ones, which W's bytes bound, are cut along K
 // into equal shares for all pairs. A CTA that shares such a tile stores its fp32 partial and counts
 // itself, per 32 columns; the one that completes a count adds all partials in their order along K, so
@@ -60,7 +60,7 @@ constexpr int kFewTokens = 2;         // up to so many tokens take the CUDA-core
 constexpr int kGemvWarps = 8, kGemvBlocks = 4;
 constexpr int kGemvSteps = 2;         // 512-byte steps of a weight row in flight
 constexpr int kSortTok = 128;         // a single block of more tokens is put in adapter order
-constexpr int kMinSlice = 64;         // narrowest slice
+constexpr int kMinSlice = 32;         // narrowest slice (648 tokens onto 804 rows of 15848: 64: 74 us, 32: 67)
 constexpr int kJoinCols = 32;         // columns of a tile cut along K that are counted and added at a time
 constexpr int kJoins = kSliceTok / kJoinCols;
 constexpr int kShrinkWarps = 8;
@@ -78,6 +78,7 @@ struct Plan {
     int pairs, full;                  // CTA pairs, whole tiles (a multiple of pairs)
     int slices, slice;                // column slices that the other tiles are cut into, 0: along K; their width
     int tail_pairs;                   // pairs that share the other tiles
+    int width;                        // most columns of a piece
     int stages, stage_bytes;
     int ksplit, clusters, per_blk;    // CTAs of a shrink cluster, clusters in all and per token block
     size_t off_status, off_count, off_meta, off_perm, off_x, off_u, off_part, total;
@@ -118,7 +119,8 @@ Plan make_plan(int M, int N, int K, int adapters, int rank, int sms) {
         p.tail_pairs = static_cast<int>(shares);
     }
     if (p.full == 0) p.pairs = p.tail_pairs;
-    p.stage_bytes = kGroup * (kRows + p.tb / 2) * 128;
+    p.width = p.full == 0 && p.slices > 0 ? p.slice : p.tb;
+    p.stage_bytes = kGroup * (kRows + p.width / 2) * 128;
     p.stages = kSmemCap / p.stage_bytes;
     if (p.stages > kMaxStages) p.stages = kMaxStages;
     p.ksplit = 1;
@@ -568,8 +570,8 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int* err = reinterpret_cast<int*>(ws + P.off_status);
     // a stage: W chunks (then the adapters' B rows) | X chunks (then U rows)
-    const uint32_t x_off = kGroup * kRows * 128, x_chunk = P.tb / 2 * 128;
-    const uint32_t b_chunk = kRows * P.kw * 2, u_chunk = P.tb / 2 * P.kw * 2;
+    const uint32_t x_off = kGroup * kRows * 128, x_chunk = P.width / 2 * 128;
+    const uint32_t b_chunk = kRows * P.kw * 2, u_chunk = P.width / 2 * P.kw * 2;
     const int per_stage = kGroup * kChunk / P.kw;   // of B's and U's tiles
     if (threadIdx.x == 0) {
         for (int s = 0; s < P.stages; ++s) {
