@@ -7,7 +7,8 @@
 //      are laid end to end and cut evenly over the workers, and a worker writes one partial record
 //      (m, l, o) per group that it touches, at index group + worker (unique: walking the tiles in
 //      order, every step to the next (group, worker) piece advances one of the two).
-//   3. prefix_merge_kernel merges each output row's records by their maxima and sums.
+//   3. prefix_merge_kernel merges each output row's records by their maxima and sums, once the row's own
+//      workers have written them (they all run when it starts, so that its bounded wait ends).
 // Rounding: P is rounded to the cache's type for its MMA, and the row sums add the rounded values, so
 // that the weights of a row still add up to one; a record's o is stored in fp16 after an exact scaling
 // of each 64 columns by a power of two (2^-11 relative to their largest, at half of fp32's bytes); all sums, maxima and accumulators are fp32; the result is rounded once.
@@ -34,8 +35,9 @@
 // scores arrive in it, row by row in the layout of an MMA operand, and each thread replaces its row by
 // its row of P, from which the value product reads. The MMA that has read it tells the peer that the
 // slot is free.
-// Bound by that chain and the MMAs: a tile takes 1.13 us (0.78 at the measured tensor rate), a batch 20 us
-// beside its tiles (plan 4, first loads 4, last softmax and record 5, merge 5). 64 requests of 128 heads
+// Bound by that chain and the MMAs: a tile takes 1.13 us (0.78 at the measured tensor rate), a batch 16 us
+// beside its tiles (plan 4, first loads 3, last softmax and record 4, merge 3, launches), a group of its
+// own about 3. 64 requests of 128 heads
 // over a prefix of 8192: 157 us, 960 TFLOP/s; 32 of 16 heads over one of 131072: 154 us, 950 TFLOP/s.
 // A parity wait may only start once the phase before the awaited one is known to be complete (it would
 // pass at once otherwise), so a barrier that a set waits on for its own tiles belongs to that set.
