@@ -428,7 +428,8 @@ typedef struct mla_prefix_args {
   int64_t kv_total_rows;        /* > 0 */
   const void* q_absorbed;       /* (B, H, d_c) */
   const void* q_rope;           /* (B, H, d_R), rotated to the token's position */
-  const int* group_starts;      /* device (num_groups + 1,): requests outside every group have no prefix */
+  const int* group_starts;      /* device (num_groups + 1,), non-decreasing (else every output is NaN): requests
+                                 * outside every group have no prefix */
   const int* prefix_lens;       /* device (num_groups,) */
   int max_prefix_len;           /* upper bound, >= 0 */
   const int* seq_lens;          /* device (B,) */

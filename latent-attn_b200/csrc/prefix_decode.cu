@@ -27,6 +27,9 @@ __global__ void __launch_bounds__(32 * kSimtWarps) prefix_simt_kernel(const __gr
     const T* qa = static_cast<const T*>(A.qa) + static_cast<long long>(blockIdx.x) * A.dc;
     const T* qr = static_cast<const T*>(A.qr) + static_cast<long long>(blockIdx.x) * A.dR;
     const T* kv = static_cast<const T*>(A.kv);
+    int falls = 0;          // group_starts decreases: every output is NaN
+    for (int p = threadIdx.x; p < A.P; p += 32 * kSimtWarps) falls |= A.starts[p] > A.starts[p + 1];
+    const bool sorted = !__syncthreads_or(falls);
     int lo = 0, hi = A.P;   // last group whose start is at or before b
     while (lo + 1 < hi) {
         const int mid = (lo + hi) / 2;
@@ -34,7 +37,7 @@ __global__ void __launch_bounds__(32 * kSimtWarps) prefix_simt_kernel(const __gr
     }
     const bool grouped = A.starts[lo] <= b && b < A.starts[lo + 1];
     const int np = grouped ? min(max(A.plens[lo], 0), A.max_plen) : 0;
-    const int n = np + min(max(A.lens[b], 0), A.max_len);
+    const int n = sorted ? np + min(max(A.lens[b], 0), A.max_len) : 0;
     const int ne = A.dc / 32, nr = (A.dR + 31) / 32;
     float q[kMaxLane], k[kMaxLane], o[kMaxLane], r[kMaxRope];
 #pragma unroll
@@ -99,7 +102,7 @@ __global__ void __launch_bounds__(32 * kSimtWarps) prefix_simt_kernel(const __gr
     }
     __syncthreads();
     float top = -INFINITY, total = 0.f;
-    int any_bad = 0;
+    int any_bad = !sorted;
 #pragma unroll
     for (int w = 0; w < kSimtWarps; ++w) {
         top = fmaxf(top, sh_m[w]);

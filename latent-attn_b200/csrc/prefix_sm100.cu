@@ -100,6 +100,7 @@ struct __align__(16) Pieces {
 };
 struct Work {                 // workspace
     int* status;
+    int* unsorted;            // group_starts decreases somewhere: no group is built, every output is NaN
     Group* group;             // groups with tiles, in order
     Start* start;             // per worker
     Pieces* pieces;           // per group, also those without tiles: single requests' first, then the prefixes'
@@ -180,11 +181,16 @@ __global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(const __grid_
     const int hb = ceil_div(A.H, 128), tid = threadIdx.x, threads = blockDim.x;
     const int len0 = tid < wk.own ? A.lens[tid / hb] : 0;   // this thread's first own group
     const bool base_sh = A.P <= kPlanCache / 4;
-    if (base_sh)
-        for (int p = tid; p <= A.P; p += threads) {
-            sh_starts[p] = A.starts[p];
-            if (p < A.P) sh_plens[p] = A.plens[p];
+    int falls = 0;
+    for (int p = tid; p < A.P; p += threads) {
+        const int s0 = A.starts[p], s1 = A.starts[p + 1];
+        falls |= s0 > s1;
+        if (base_sh) {
+            sh_starts[p] = s0;
+            if (p + 1 == A.P) sh_starts[A.P] = s1;
+            sh_plens[p] = A.plens[p];
         }
+    }
     const int* starts = base_sh ? sh_starts : A.starts;
     const int* plens = base_sh ? sh_plens : A.plens;
     if (tid == 0) {
@@ -192,9 +198,11 @@ __global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(const __grid_
         *wk.status = 0;
     }
     if (tid < wk.W) wk.done[tid] = 0;
-    __syncthreads();
+    // the tables hold the groups of disjoint ranges of requests; ranges that fall back could be any number
+    const bool sorted = !__syncthreads_or(falls);
+    if (tid == 0) *wk.unsorted = !sorted;
     int extra = 0;   // row groups of the prefixes
-    if (!wk.fold) {
+    if (!wk.fold && sorted) {
         for (int p0 = 0; p0 < A.P; p0 += threads) {
             const int p = p0 + tid;
             int n = 0;
@@ -215,7 +223,7 @@ __global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(const __grid_
     }
     const int* gbase = base_sh ? sh_base : wk.gbase;
     // groups: tiles, then (compacted) the table
-    const int G = wk.own + extra;
+    const int G = sorted ? wk.own + extra : 0;
     int mine = -1, mine0 = 0, mine1 = 0;   // this thread's last group: its place in the table, its tiles
     for (int g0 = 0; g0 < G; g0 += threads) {
         const int g = g0 + tid;
@@ -935,8 +943,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps) prefix_merge_kernel(const __
     float o[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[i] = 0.f;
-    bool bad = false;
-    if (live) {
+    bool bad = __ldcg(wk.unsorted) != 0;
+    if (live && !bad) {
         const int b = f / A.H, h = f % A.H;
         // the row's groups: its request's, and unless that holds the prefix too, its prefix group's
         const int2 rq = wk.fold ? make_int2(-1, 0) : wk.request[b];
@@ -1041,7 +1049,7 @@ Layout layout(const PrefixArgs& A, int sms) {
     L.W = sms / 2 > 0 ? sms / 2 : 1;
     if (L.W > kMaxWorkers) L.W = kMaxWorkers;
     const size_t groups = static_cast<size_t>(L.groups), recs = groups + L.W;
-    size_t off = 256;     // status
+    size_t off = 256;     // status, unsorted
     auto take = [&](size_t bytes) {
         const size_t at = off;
         off = (off + bytes + 255) / 256 * 256;
@@ -1066,6 +1074,7 @@ cudaError_t launch(const PrefixArgs& A, unsigned char* ws, int sms, cudaStream_t
     const Layout L = layout(A, sms);
     Work wk;
     wk.status = reinterpret_cast<int*>(ws);
+    wk.unsorted = wk.status + 1;
     wk.group = reinterpret_cast<Group*>(ws + L.off_group);
     wk.start = reinterpret_cast<Start*>(ws + L.off_start);
     wk.pieces = reinterpret_cast<Pieces*>(ws + L.off_pieces);

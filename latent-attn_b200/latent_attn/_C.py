@@ -823,6 +823,7 @@ def mla_prefix_decode(kv_cache: torch.Tensor, q_absorbed: torch.Tensor, q_rope: 
     Request b of group g (``group_starts[g] <= b < group_starts[g + 1]``) attends to the
     ``prefix_lens[g]`` rows of its group's prefix and its own ``seq_lens[b]`` rows of ``kv_cache``,
     whose keys are rotated already (``mla_cache_append_rope``); a request without rows gives zeros.
+    ``group_starts`` is non-decreasing (where it is not, every output is NaN).
     ``q_absorbed`` (B, H, d_c) and ``q_rope`` (B, H, d_R, rotated) have the cache's type. Contiguous
     layout: ``prefix_offsets`` (groups,) and ``kv_offsets`` (B,) int64 first rows. Paged: ``page_rows``
     (a multiple of 64) with ``prefix_table`` (groups, pages) and ``page_table`` (B, pages) int32. All

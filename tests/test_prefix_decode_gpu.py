@@ -16,7 +16,7 @@ import math
 import pytest
 import torch
 
-from latent_attn import MLAConfig
+from latent_attn import MLAConfig, _lib
 from latent_attn.functional import mla_prefix_decode
 
 pytestmark = pytest.mark.gpu
@@ -291,3 +291,36 @@ def test_refusals():
         mla_prefix_decode(c.kv.to(DEV), c.qa.to(DEV).transpose(0, 1).contiguous().transpose(0, 1), c.qr.to(DEV), cfg, **c.args())
     with pytest.raises(RuntimeError, match="kv_cache"):
         mla_prefix_decode(c.kv.to(DEV)[:, :570], c.qa.to(DEV), c.qr.to(DEV), cfg, **c.args())
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("heads", [16, 128])
+@pytest.mark.parametrize("starts", [[0, 64] * 32, [0, 5, 3, 64], [64, 0], [0, 1 << 30, -(1 << 30), 64],
+                                    [0, 64] * 700])
+def test_decreasing_group_starts(kernel, heads, starts, monkeypatch):
+    """Ranges of requests that overlap: NaN everywhere, and nothing outside the workspace or the output. Each
+    pair of [0, 64] alone has as many row groups as the workspace has for all requests."""
+    P = len(starts) - 1
+    g = torch.Generator().manual_seed(heads)
+    kv = torch.randn(1024, 576, generator=g).to(torch.bfloat16).to(DEV)
+    qa = torch.randn(64, heads, 512, generator=g).to(torch.bfloat16).to(DEV)
+    qr = torch.randn(64, heads, 64, generator=g).to(torch.bfloat16).to(DEV)
+    kw = dict(prefix_lens=torch.full((P,), 130, dtype=torch.int32, device=DEV), max_prefix_len=130,
+              seq_lens=torch.arange(64, dtype=torch.int32, device=DEV), max_seq_len=64,
+              prefix_offsets=torch.zeros(P, dtype=torch.int64, device=DEV),
+              kv_offsets=torch.arange(64, device=DEV) * 8, kernel=kernel)
+    cfg = MLAConfig(0, 512, 128, 64, heads, 128)
+    packed, need = _lib.load_packed(), []
+    real = packed.mla_prefix_decode
+    monkeypatch.setattr(packed, "mla_prefix_decode", lambda *a: need.append(a[3]) or real(*a))
+    ws = torch.full((192 << 20,), 0xA5, dtype=torch.uint8, device=DEV)
+    wide = torch.full((3, 64, heads, 512), 7.0, dtype=torch.bfloat16, device=DEV)
+    mla_prefix_decode(kv, qa, qr, cfg, group_starts=torch.tensor(starts, dtype=torch.int32, device=DEV),
+                      out=wide[1], workspace=ws, **kw)
+    assert torch.isnan(wide[1]).all() and (wide[0] == 7).all() and (wide[2] == 7).all()
+    assert need[0] < ws.numel() and (ws[need[0]:] == 0xA5).all()
+    # the same workspace serves a proper call after it
+    want = mla_prefix_decode(kv, qa, qr, cfg, group_starts=torch.tensor(sorted(starts), dtype=torch.int32, device=DEV), **kw)
+    got = mla_prefix_decode(kv, qa, qr, cfg, group_starts=torch.tensor(sorted(starts), dtype=torch.int32, device=DEV),
+                            workspace=ws, **kw)
+    assert torch.isfinite(got).all() and torch.equal(got, want)
