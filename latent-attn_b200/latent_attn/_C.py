@@ -124,7 +124,18 @@ def _decode_args(dtype, batch, shared, kv_cache, max_seq_len, q_rope, W_UV, rope
     return a
 
 
+def _check_workspace(workspace: Optional[torch.Tensor], index: int, pinned: bool = False) -> None:
+    """The kernels write to a caller's workspace by its address and size alone (``pinned``: it may also lie
+    in pinned host memory)."""
+    if workspace is None:
+        return
+    if not workspace.is_contiguous() or (workspace.get_device() != index and not (pinned and workspace.is_pinned())):
+        raise RuntimeError(f"workspace must be a contiguous tensor on cuda:{index}, got one with strides "
+                           f"{tuple(workspace.stride())} on {workspace.device}")
+
+
 def _workspace(cfg, args, device, workspace: Optional[torch.Tensor]) -> torch.Tensor:
+    _check_workspace(workspace, device.index, pinned=True)
     lib = _lib.load()
     n = C.c_size_t(0)
     _lib.check(lib.mla_decode_workspace_size(C.byref(cfg), C.byref(args), C.byref(n)))
@@ -276,6 +287,7 @@ def _run_decode(cfg, dtype, batch, shared, kv_cache, max_seq_len, q_rope, W_UV, 
                         **kw)
     lib = _lib.load()
     stream = C.c_void_p(_stream(kv_cache.device))
+    _check_workspace(workspace, kv_cache.get_device(), pinned=True)
     if workspace is not None and workspace.data_ptr() % 256 == 0:
         # a caller's workspace is tried as it is: the call itself checks its size, and only a
         # too-small one costs the size query and an allocation
@@ -828,7 +840,7 @@ def mla_prefix_decode(kv_cache: torch.Tensor, q_absorbed: torch.Tensor, q_rope: 
     layout: ``prefix_offsets`` (groups,) and ``kv_offsets`` (B,) int64 first rows. Paged: ``page_rows``
     (a multiple of 64) with ``prefix_table`` (groups, pages) and ``page_table`` (B, pages) int32. All
     index tensors are on the device; ``max_prefix_len`` and ``max_seq_len`` bound the lengths (longer
-    ones are cut). ``workspace``: uint8, kept by callers that must not allocate."""
+    ones are cut). ``workspace``: uint8 on the cache's device, kept by callers that must not allocate."""
     cfg = _cfg(d_model, kv_lora_rank, qk_nope_head_dim, qk_rope_head_dim, num_heads, v_head_dim)
     dc, dR, H = kv_lora_rank, qk_rope_head_dim, num_heads
     dt, dev, kv_stride = _cache(kv_cache, dc + dR)
@@ -852,6 +864,7 @@ def mla_prefix_decode(kv_cache: torch.Tensor, q_absorbed: torch.Tensor, q_rope: 
     a = _pack_prefix(_DT[dt], B, P, kv_cache.data_ptr(), kv_stride, kv_cache.size(0), qa_p, qr_p, starts_p, plens_p,
                      max_prefix_len, lens_p, max_seq_len, poff_p, off_p, ptable_p, ppages, table_p, pages, page_rows,
                      softmax_scale, out_p, kernel)
+    _check_workspace(workspace, dev)
     lib, cfg_p = _lib.load_packed(), C.addressof(cfg)
     n = C.c_size_t()
     st = lib.mla_prefix_decode_workspace_size(cfg_p, a, n)
@@ -872,8 +885,8 @@ def linear_lora(x: torch.Tensor, W: torch.Tensor, lora_a: torch.Tensor, lora_b: 
     lora_b[a] @ (lora_a[a] @ x[m])`` with ``a = adapter_ids[m]`` (an id outside the loaded adapters:
     none). ``lora_a`` (adapters, rank, K), ``lora_b`` (adapters, N, rank), rank a multiple of 8 up to
     256, ``adapter_ids`` (M,) int32 in any order, ``scales`` (adapters,) fp32. All fp16 or bf16 of one
-    type, which the result (M, N) has too. K is a multiple of 8. ``workspace``: uint8, kept by callers
-    that must not allocate."""
+    type, which the result (M, N) has too. K is a multiple of 8. ``workspace``: uint8 on x's device, kept
+    by callers that must not allocate."""
     dt, dev = x.dtype, x.get_device()
     if dt not in _DT or dev < 0 or x.dim() != 2 or W.dim() != 2 or lora_a.dim() != 3:
         raise RuntimeError("x and W must be 2D, lora_a and lora_b 3D float16 or bfloat16 CUDA tensors")
@@ -889,6 +902,7 @@ def linear_lora(x: torch.Tensor, W: torch.Tensor, lora_a: torch.Tensor, lora_b: 
         out_p = out.data_ptr()
     else:
         out_p = _dense(out, "out", dt, dev, (M, N))
+    _check_workspace(workspace, dev)
     if M == 0:
         return out
     a = _pack_lora(_DT[dt], M, N, K, x.data_ptr(), x_st[0] if M > 1 else K, W_p, adapters, rank, a_p, b_p, ids_p,

@@ -167,3 +167,13 @@ def test_refusals():
     refuses("multiples of 8", x[:, :60].contiguous(), W[:, :60].contiguous(), A[..., :60].contiguous(), B, ids)
     refuses("num_adapters", x, W, A[:0], B[:0], ids)
     refuses("aligned", torch.empty(4 * 64 + 1, dtype=torch.bfloat16, device=DEV)[1:].view(4, 64), W, A, B, ids)
+
+
+def test_workspaces_that_the_kernels_cannot_write_are_refused():
+    x, W, A, B, ids, scales = make(40, 64, 64, 16, 2, torch.bfloat16)
+    for ws in (torch.empty(64 << 20, dtype=torch.uint8), torch.empty(64 << 20, dtype=torch.uint8).pin_memory(),
+               torch.empty(1, dtype=torch.uint8, device=DEV).expand(64 << 20)):
+        with pytest.raises(RuntimeError, match="workspace must be"):
+            linear_lora(x, W, A, B, ids, scales=scales, workspace=ws)
+    check(linear_lora(x, W, A, B, ids, scales=scales, workspace=torch.empty(1, dtype=torch.uint8, device=DEV)),
+          exact(x, W, A, B, ids, scales))                        # too small: one is allocated

@@ -557,3 +557,17 @@ def test_pinned_host_queries_and_output(B):
     torch.cuda.synchronize()
     assert got is out_h
     assert torch.equal(out_h, want.cpu())
+
+
+def test_workspaces_that_the_kernels_cannot_write_are_refused():
+    dev = torch.device("cuda:0")
+    cfg = MLAConfig.deepseek_v2()
+    inp = synthetic.baseline_inputs(num_heads=128, seq_lens=[256], seed=11)
+    cos, sin = synthetic.build_rope_tables(256, 64, device=dev)
+    args = (inp.kv_cache.to(dev), inp.q_rope.float().to(dev), inp.W_UV.to(dev), cos, sin, cfg)
+    kw = dict(q_nope=inp.q_nope.float().to(dev), W_UK=inp.W_UK.to(dev), max_seq_len=256)
+    for ws in (torch.empty(1 << 26, dtype=torch.uint8), torch.empty(1, dtype=torch.uint8, device=dev).expand(1 << 26)):
+        with pytest.raises(RuntimeError, match="workspace must be"):
+            mla_decode(*args, workspace=ws, **kw)
+    want = mla_decode(*args, **kw)
+    assert torch.equal(mla_decode(*args, workspace=torch.empty(1, dtype=torch.uint8, device=dev), **kw), want)

@@ -324,3 +324,13 @@ def test_decreasing_group_starts(kernel, heads, starts, monkeypatch):
     got = mla_prefix_decode(kv, qa, qr, cfg, group_starts=torch.tensor(sorted(starts), dtype=torch.int32, device=DEV),
                             workspace=ws, **kw)
     assert torch.isfinite(got).all() and torch.equal(got, want)
+
+
+def test_workspaces_that_the_kernels_cannot_write_are_refused():
+    c = Case([2], [64], [5, 5], 16, torch.bfloat16, 64)
+    for ws in (torch.empty(64 << 20, dtype=torch.uint8), torch.empty(64 << 20, dtype=torch.uint8).pin_memory(),
+               torch.empty(1, dtype=torch.uint8, device=DEV).expand(64 << 20)):
+        for kernel in KERNELS:
+            with pytest.raises(RuntimeError, match="workspace must be"):
+                c.run(kernel, workspace=ws)
+    check(c.run(workspace=torch.empty(1, dtype=torch.uint8, device=DEV)), c.exact(), torch.bfloat16)
