@@ -742,7 +742,12 @@ def _cache(kv_cache: torch.Tensor, width: int):
     dt, index = kv_cache.dtype, kv_cache.get_device()
     if dt not in _DT or index < 0 or kv_cache.dim() != 2 or kv_cache.size(1) != width or kv_cache.stride(1) != 1:
         raise RuntimeError(f"kv_cache must be a CUDA fp16/bf16 (rows, {width}) tensor with unit inner stride")
-    return dt, index, kv_cache.stride(0)
+    rows, stride = kv_cache.size(0), kv_cache.stride(0)
+    if stride < width:   # (an expanded cache has a stride of 0, which means the default in the C structs)
+        if rows > 1:
+            raise RuntimeError(f"kv_cache's rows overlap: stride {stride} < {width}")
+        stride = width
+    return dt, index, stride
 
 
 def _current_stream(index: int) -> int:

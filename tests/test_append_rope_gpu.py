@@ -219,3 +219,16 @@ def test_refusals():
     refuses("norm_eps", kv, c, k, cu, lens, 64, norm_weight=torch.zeros(512, dtype=torch.bfloat16, device=DEV),
             norm_eps=-1.0)
     assert int(kv.abs().sum()) == 0
+
+
+def test_a_cache_whose_rows_overlap_is_refused():
+    cfg = MLAConfig(0, 512, 128, 64, 4, 128)
+    row = torch.zeros(1, 576, dtype=torch.bfloat16, device=DEV)
+    c, k = torch.ones(2, 512, dtype=torch.bfloat16, device=DEV), torch.ones(2, 64, dtype=torch.bfloat16, device=DEV)
+    cu, lens = torch.tensor([0, 2], dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    with pytest.raises(RuntimeError, match="overlap"):
+        mla_cache_append_rope(row.expand(64, 576), c, k, cu, lens, 64, cfg)
+    assert int(row.abs().sum()) == 0
+    one = row.view(-1).as_strided((1, 576), (0, 1))               # a single row has any stride
+    mla_cache_append_rope(one, c[:1], k[:1], cu - torch.tensor([0, 1], dtype=torch.int32, device=DEV), lens, 1, cfg)
+    assert torch.equal(row[0, :512], c[0])

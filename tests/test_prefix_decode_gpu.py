@@ -334,3 +334,18 @@ def test_workspaces_that_the_kernels_cannot_write_are_refused():
             with pytest.raises(RuntimeError, match="workspace must be"):
                 c.run(kernel, workspace=ws)
     check(c.run(workspace=torch.empty(1, dtype=torch.uint8, device=DEV)), c.exact(), torch.bfloat16)
+
+
+def test_a_cache_whose_rows_overlap_is_refused():
+    c = Case([2], [64], [5, 5], 16, torch.bfloat16, 64)
+    cfg = MLAConfig(0, 512, 128, 64, 16, 128)
+    row = torch.ones(1, 576, dtype=torch.bfloat16, device=DEV)
+    for kv in (row.expand(640, 576), row.view(-1).as_strided((2, 576), (0, 1)), row.expand(4, 576).reshape(-1).as_strided((4, 576), (570, 1))):
+        for kernel in KERNELS:
+            with pytest.raises(RuntimeError, match="overlap"):
+                mla_prefix_decode(kv, c.qa.to(DEV), c.qr.to(DEV), cfg, kernel=kernel, **c.args())
+    # a single row has any stride
+    one = Case([1], [0], [1], 16, torch.bfloat16, 0, gap=0)
+    kv = one.kv.to(DEV).as_strided((1, 576), (0, 1))
+    got = mla_prefix_decode(kv, one.qa.to(DEV), one.qr.to(DEV), cfg, **one.args())
+    check(got, one.exact(), torch.bfloat16)
