@@ -417,6 +417,10 @@ MLA_API mla_status_t mla_cache_append_rope(const mla_config_t* cfg, const mla_ap
  * in latent space (no W_UV), 0 for a request without rows. Each prefix is read once for all the
  * query rows of its group, not once a request; partial results are merged in fp32-weighted form.
  * No reference counterpart (its batched op, src/fused_mla_batched.cuh:5-11, shares the whole cache).
+ * Rounding: scores, maxima and sums in fp32; the weights exp(s - max) once to the type; with the tensor
+ * cores also partial results, to fp16 relative to the largest of 64 columns, and the two halves of a
+ * score (columns [0, 256) and [0, 32) of the rope key, and the rest) by 2^-22 of the largest half of 64
+ * positions, or to 16 significant bits where a half reaches 2^14 ln 2 = 11357.
  * Lengths are clamped to [0, max]. A page id or offset outside the cache reads nothing and makes
  * the outputs of the requests that use it NaN. */
 typedef struct mla_prefix_args {

@@ -23,9 +23,14 @@
 // two score buffers of 64 | Q latent 128 (two elements a column). (The alternatives: a whole score in
 // each CTA costs 1.53 times the MMAs; splitting the rows instead needs every value column twice in
 // shared memory, and those MMAs with both operands there ran at 1319 TFLOP/s alone, 868 with their
-// loads.) The two partial scores are exchanged in fp16 through distributed shared memory (in log2
-// units after scaling: 2^-11 of a partial), and both CTAs add the same two fp16 values, so their
-// softmax is the same bit for bit.
+// loads.) The partial scores cross through distributed shared memory, 24 bits each: a row of a tile as
+// integers of 23 bits under one power of two, 2^-22 to 2^-23 of the row's largest partial, where the sums
+// of products themselves are good to about 2^-23 of it. A row whose partials reach 2^14 (in log2 units; a
+// mask's lowest value, infinities and NaN among them) crosses as floats of 16 significant bits, so that one
+// such partial does not take the others' bits. Both CTAs add the same two values, so their softmax is the
+// same bit for bit. (32 bits: 40 percent more time with the three loading stages that leave room for them,
+// 29 with two exchange slots and P in a place of its own; 16 as fp16: 15 percent less, but then a weight is
+// off by 2^-11 of its score.)
 //
 // Warps (128 + 128 kSets threads): warp 0 loads, warp 1 issues the scores' MMAs and warp 2 the value
 // products' (two warps that sleep on their own barriers: one that polls both sees either 0.4 us later),
@@ -35,10 +40,10 @@
 // scores arrive in it, row by row in the layout of an MMA operand, and each thread replaces its row by
 // its row of P, from which the value product reads. The MMA that has read it tells the peer that the
 // slot is free.
-// Bound by that chain and the MMAs: a tile takes 1.13 us (0.78 at the measured tensor rate), a batch 16 us
+// Bound by that chain and the MMAs: a tile takes 1.35 us (0.78 at the measured tensor rate), a batch 16 us
 // beside its tiles (plan 4, first loads 3, last softmax and record 4, merge 3, launches), a group of its
 // own about 3. 64 requests of 128 heads
-// over a prefix of 8192: 157 us, 960 TFLOP/s; 32 of 16 heads over one of 131072: 154 us, 950 TFLOP/s.
+// over a prefix of 8192: 185 us, 811 TFLOP/s; 32 of 16 heads over one of 131072: 178 us, 822 TFLOP/s.
 // A parity wait may only start once the phase before the awaited one is known to be complete (it would
 // pass at once otherwise), so a barrier that a set waits on for its own tiles belongs to that set.
 #include <cfloat>
@@ -59,7 +64,7 @@ constexpr int kChunkBytes = kTile * 128;             // 64 rows x 64 latent colu
 constexpr int kRopeBoxBytes = kTile * 16;            // 64 rows x 8 rope columns, no swizzle
 constexpr int kRopeBytes = 4 * kRopeBoxBytes;
 constexpr int kStageBytes = kRopeBytes + 4 * kChunkBytes;
-constexpr int kXBytes = 128 * 128;                   // a slot: 128 rows x 64 fp16 partial scores, then P
+constexpr int kXBytes = 128 * 192;                   // a slot: 128 rows x 64 partial scores of 24 bits, then P in 16
 constexpr int kQRopeBoxBytes = 128 * 16;
 constexpr int kQRopeBytes = 4 * kQRopeBoxBytes;
 constexpr int kXUnit = 128 * 16;                     // 16-byte unit c of row t is at c * kXUnit + t * 16: a warp's stores
@@ -75,10 +80,12 @@ constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColO = 0, kColS = 256, kColQ = 384;
 constexpr int kMl = 12;
 constexpr float kRescale = 8.0f;                     // log2 units
-constexpr float kLowest = -1e37f;                    // reference of rows whose scores are all -inf
+constexpr float kLowest = -FLT_MAX;                  // reference of rows whose scores are all -inf
+constexpr float kMagic = 12582912.0f;                // 1.5 * 2^23: x + kMagic holds the integer nearest to x in its low 23 bits
+constexpr uint32_t kWideExp = 127 + 14;              // rows whose partials reach 2^14 cross as floats of 24 bits
 
 enum : int { kWaitLoad = 1, kWaitMma = 3, kWaitS = 7, kWaitX = 8, kWaitPV = 9, kWaitTeardown = 10, kWaitDrain = 11,
-             kWaitRef = 12, kWaitCredit = 13, kWaitEpi = 14 };
+             kWaitRef = 12, kWaitCredit = 13, kWaitEpi = 14, kAlignment = 15 };
 
 // A group of query rows with something to attend to.
 struct __align__(16) Group {
@@ -358,7 +365,7 @@ struct __align__(8) Barriers {
 };
 
 constexpr size_t kSmemBytes = static_cast<size_t>(kStages) * kStageBytes + static_cast<size_t>(kSlots) * kXBytes +
-                              kQRopeBytes + kMSlots * 128 * sizeof(float) + sizeof(Barriers) + 1024;
+                              kQRopeBytes + kMSlots * 128 * sizeof(float) + sizeof(Barriers) + kSlots * 128;
 static_assert(kSmemBytes <= 232448, "shared memory budget");
 
 // Walks a worker's tiles; every role walks an identical copy. A segment is the worker's run of tiles
@@ -434,6 +441,38 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
         : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
+        "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+// the largest magnitude of three (NaN if one is)
+__device__ __forceinline__ float maxabs3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// Three bytes of each of four words in three, and back (the top byte of each is then kMagic's).
+__device__ __forceinline__ void pack24(const float* x, uint32_t* w) {
+    const uint32_t a = __float_as_uint(x[0]), b = __float_as_uint(x[1]), c = __float_as_uint(x[2]), d = __float_as_uint(x[3]);
+    w[0] = __byte_perm(a, b, 0x4210);
+    w[1] = __byte_perm(b, c, 0x5421);
+    w[2] = __byte_perm(c, d, 0x6542);
+}
+__device__ __forceinline__ void unpack24(const uint32_t* w, float* x) {
+    constexpr uint32_t k = 0x4B000000u;
+    x[0] = __uint_as_float(__byte_perm(w[0], k, 0x7210));
+    x[1] = __uint_as_float((__byte_perm(w[0], w[1], 0x5543) & 0x00FFFFFFu) | k);
+    x[2] = __uint_as_float((__byte_perm(w[1], w[2], 0x4432) & 0x00FFFFFFu) | k);
+    x[3] = __uint_as_float(__byte_perm(w[2], k, 0x7321));
+}
+// A float rounded to 24 bits (16 significant ones), and back.
+__device__ __forceinline__ float to_wide24(float x) {
+    return __uint_as_float(x != x ? 0x7FC000u : (__float_as_uint(x) + 0x80u) >> 8);
+}
+__device__ __forceinline__ float from_wide24(float w) { return __uint_as_float(__float_as_uint(w) << 8); }
 // the largest of three (a NaN only if all are)
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
@@ -487,12 +526,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ CUtensorMap tmap_rope,
                      const __grid_constant__ PrefixArgs A, const __grid_constant__ Work wk) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    unsigned char* stages = smem;
+    unsigned char* stages = smem_raw;   // swizzled tiles want 1024 bytes; there is no room to align it by hand
     unsigned char* xbuf = stages + kStages * kStageBytes;
     unsigned char* qrope = xbuf + kSlots * kXBytes;
     float* m_pub = reinterpret_cast<float*>(qrope + kQRopeBytes);              // [kMSlots][128]
     Barriers* bars = reinterpret_cast<Barriers*>(m_pub + kMSlots * 128);
+    unsigned char* xexp = reinterpret_cast<unsigned char*>(bars + 1);          // [kSlots][128] exponents of a slot's rows
     // the row sums that one set hands to another at a segment's end: in global memory, where shared
     // memory has no room, and only for the segment's last tiles
     volatile float2* l_pub = wk.rowsum + static_cast<long long>(blockIdx.x) * kSums * 128;
@@ -501,6 +540,16 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
     const int w = blockIdx.x >> 1;
     volatile int* err = wk.status;
 
+    if (smem_u32(smem_raw) % 1024 != 0) {   // (all CTAs alike)
+        pdl_wait();
+        pdl_launch_dependents();
+        if (threadIdx.x == 0) {
+            record_timeout(err, code(kAlignment));
+            __threadfence();
+            atomicAdd(&wk.done[w], 1);
+        }
+        return;
+    }
     if (threadIdx.x == 0) {
         tma_prefetch_desc(&tmap);
         tma_prefetch_desc(&tmap_rope);
@@ -540,7 +589,7 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
     // identical in both CTAs of the pair; a pair without tiles goes straight to the teardown
     const Start start = wk.start[w];
     const int n = start.te - start.tb;
-    const uint32_t stages_u32 = smem_u32(stages), xbuf_u32 = smem_u32(xbuf), qrope_u32 = smem_u32(qrope);
+    const uint32_t stages_u32 = smem_u32(stages), xbuf_u32 = smem_u32(xbuf), qrope_u32 = smem_u32(qrope), xexp_u32 = smem_u32(xexp);
 
     if (warp < 4) {
         if (n > 0 && warp == 0 && lane == 0) {
@@ -716,12 +765,12 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
                 tc_fence_after();
                 load_q(it.d, 0, 1, &bars->q_ready);
             }
-            // ---- S_r(j) to registers, release S, send the fp16 partial
+            // ---- S_r(j) to registers, release S, put the partial in 24 bits
             got = mbar_wait(smem_u32(&bars->s_full[sid]), (j / kSets) & 1, err, code(kWaitS));
             if (!warp_ok(got)) break;
-            if (t == 0) mbar_arrive_expect_tx(x_full, kXBytes);
+            if (t == 0) mbar_arrive_expect_tx(x_full, kXBytes + 128);
             tc_fence_after();
-            uint32_t h[32];
+            float s[64];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 uint32_t sr[32];
@@ -731,20 +780,69 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
                     mbar_arrive(smem_u32(&bars->s_free[j & 1]));
                 }
 #pragma unroll
-                for (int q = 0; q < 16; ++q) {
-                    const float2 v = mul2(make_float2(__uint_as_float(sr[2 * q]), __uint_as_float(sr[2 * q + 1])),
-                                          make_float2(qscale, qscale));
-                    h[16 * c + q] = half2_of(v.x, v.y);
+                for (int q = 0; q < 32; ++q) s[32 * c + q] = __uint_as_float(sr[q]);
+            }
+            if (np < kTile) {   // what lies past the end must not set the row's exponent
+#pragma unroll
+                for (int k = 0; k < 64; ++k)
+                    if (k >= np) s[k] = 0.f;
+            }
+            uint32_t ex;
+            {
+                float mx[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < 64; k += 2) mx[(k / 2) & 3] = maxabs3(mx[(k / 2) & 3], s[k], s[k + 1]);
+                // (a little more than the largest, so that it stays below 2^22 after rounding)
+                ex = __float_as_uint(maxabs3(maxabs3(mx[0], mx[1], mx[2]), mx[3], 0.f) * qscale * 1.000001f) >> 23;
+            }
+            // (from 2^64 below 1 on, smaller rows are as good as zero; 255 says that the row crosses as floats)
+            const bool wide = ex >= kWideExp || !(qscale < 1e12f), some_wide = __any_sync(0xffffffffu, wide);
+            ex = wide ? 255u : max(ex, 64u);
+            const float sc = qscale * __uint_as_float((275u - ex) << 23);   // 2^21 to 2^22 for the largest
+            if (some_wide) {
+#pragma unroll
+                for (int k = 0; k < 64; ++k) s[k] = wide ? to_wide24(s[k] * qscale) : fmaf(s[k], sc, kMagic);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 32; ++q) {
+                    const float2 v = fma2(make_float2(s[2 * q], s[2 * q + 1]), make_float2(sc, sc), make_float2(kMagic, kMagic));
+                    s[2 * q] = v.x;
+                    s[2 * q + 1] = v.y;
                 }
             }
+            uint32_t ex4 = ex << (8 * (lane & 3));   // of four rows
+            ex4 |= __shfl_xor_sync(0xffffffffu, ex4, 1);
+            ex4 |= __shfl_xor_sync(0xffffffffu, ex4, 2);
             // the peer's value product of tile j - kSlots has read its slot
             got = j < kSlots || mbar_wait_cluster(smem_u32(&bars->x_empty[slot]), phase ^ 1, err, code(kWaitCredit));
             if (!warp_ok(got)) break;
             {
                 const uint32_t dst = mapa(x_row, peer), bar = mapa(x_full, peer);
 #pragma unroll
-                for (int c = 0; c < 8; ++c)
-                    st_async_v4(dst + c * kXUnit, h[4 * c], h[4 * c + 1], h[4 * c + 2], h[4 * c + 3], bar);
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t w[12];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) pack24(s + 16 * c + 4 * q, w + 3 * q);
+#pragma unroll
+                    for (int q = 0; q < 3; ++q)
+                        st_async_v4(dst + (3 * c + q) * kXUnit, w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3], bar);
+                }
+                if ((lane & 3) == 0) st_async(mapa(xexp_u32 + slot * 128 + t, peer), ex4, bar);
+            }
+            // this CTA's own values as the peer will see them
+            {
+                const float inv = __uint_as_float((ex - 21u) << 23), off = -kMagic * inv;
+                if (some_wide) {
+#pragma unroll
+                    for (int k = 0; k < 64; ++k) s[k] = wide ? from_wide24(s[k]) : fmaf(s[k], inv, off);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 32; ++q) {
+                        const float2 v = fma2(make_float2(s[2 * q], s[2 * q + 1]), make_float2(inv, inv), make_float2(off, off));
+                        s[2 * q] = v.x;
+                        s[2 * q + 1] = v.y;
+                    }
+                }
             }
             if (np < kTile) {
                 // rows past the end: their weights are zero, but zero times what lies there need not be
@@ -761,18 +859,41 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
             if (!warp_ok(got)) break;
             // (stage by stage over all columns: the warp issues in order, so column by column it would wait
             // for every step of every chain)
-            float s[64];
-            uint32_t pv[32];
+            {
+                uint32_t pe;
+                asm volatile("ld.shared.u8 %0, [%1];" : "=r"(pe) : "r"(xexp_u32 + slot * 128 + t));
+                const bool pwide = pe == 255u, some = __any_sync(0xffffffffu, pwide);
+                const float inv = __uint_as_float((pe - 21u) << 23), off = -kMagic * inv;
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-                asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                             : "=r"(pv[4 * c]), "=r"(pv[4 * c + 1]), "=r"(pv[4 * c + 2]), "=r"(pv[4 * c + 3])
-                             : "r"(x_row + c * kXUnit));
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t w[12];
 #pragma unroll
-            for (int q = 0; q < 32; ++q) {
-                const float2 r = add2(floats_of(h[q]), floats_of(pv[q]));
-                s[2 * q] = r.x;
-                s[2 * q + 1] = r.y;
+                    for (int q = 0; q < 3; ++q)
+                        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                                     : "=r"(w[4 * q]), "=r"(w[4 * q + 1]), "=r"(w[4 * q + 2]), "=r"(w[4 * q + 3])
+                                     : "r"(x_row + (3 * c + q) * kXUnit));
+                    float x[16];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) unpack24(w + 3 * q, x + 4 * q);
+                    if (some) {
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) x[q] = pwide ? from_wide24(x[q]) : fmaf(x[q], inv, off);
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) {
+                            const float2 v = fma2(make_float2(x[2 * q], x[2 * q + 1]), make_float2(inv, inv), make_float2(off, off));
+                            x[2 * q] = v.x;
+                            x[2 * q + 1] = v.y;
+                        }
+                    }
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        float* y = s + 16 * c + 2 * q;
+                        const float2 v = add2(make_float2(y[0], y[1]), make_float2(x[2 * q], x[2 * q + 1]));
+                        y[0] = v.x;
+                        y[1] = v.y;
+                    }
+                }
             }
             if (np < kTile) {
 #pragma unroll

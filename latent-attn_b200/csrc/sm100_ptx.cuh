@@ -380,7 +380,12 @@ __device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-// 16-byte store into another CTA's shared memory; counts 16 tx-bytes on its mbarrier.
+// 4- and 16-byte stores into another CTA's shared memory, which count their bytes on its mbarrier.
+__device__ __forceinline__ void st_async(uint32_t remote_addr, uint32_t a, uint32_t remote_bar) {
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(remote_addr), "r"(a),
+                 "r"(remote_bar)
+                 : "memory");
+}
 __device__ __forceinline__ void st_async_v4(uint32_t remote_addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d,
                                             uint32_t remote_bar) {
     asm volatile(

@@ -349,3 +349,82 @@ def test_a_cache_whose_rows_overlap_is_refused():
     kv = one.kv.to(DEV).as_strided((1, 576), (0, 1))
     got = mla_prefix_decode(kv, one.qa.to(DEV), one.qr.to(DEV), cfg, **one.args())
     check(got, one.exact(), torch.bfloat16)
+
+
+# Scores of any size. The tolerance does not grow with them: a score of up to 2^10 (log2 units) is a sum in
+# fp32, whose 18 steps of 16 products each round to 2^-14 at that size (a standard deviation below 2^-12), and
+# whose two halves may each be rounded by 2^-22 of the row's largest, 2^-12: together below 2^-11 in the
+# exponent as a standard deviation of several. P, the records and the result are rounded as above (u each):
+# bf16 sqrt(3 u^2 + 2^-22) = 6.8e-3 of a row's norm, fp16 9.8e-4, 8 times that for one element.
+def check_any_size(got, want, what=""):
+    u = 2.0 ** -8 if got.dtype == torch.bfloat16 else 2.0 ** -11
+    tol = math.sqrt(3 * u * u + 2.0 ** -22)
+    assert torch.isfinite(got).all(), what
+    d, norm = (got.double() - want).norm(dim=-1), want.norm(dim=-1)
+    assert bool((d <= tol * norm).all()), (what, float((d / norm.clamp(min=1e-30)).max()), tol)
+    big = (got.double() - want).abs().amax(-1)
+    assert bool((big <= 8 * tol * norm / math.sqrt(want.shape[-1])).all()), (what, "one element")
+
+
+def _sized(heads, dtype, seed):
+    return Case([6, 3], [700, 130], [0, 1, 65, 300, 40, 64, 5, 128, 200], heads, dtype, 64, seed=seed)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads", [16, 128])
+@pytest.mark.parametrize("size", [4.0, 30.0, 100.0])
+def test_sharp_scores(size, heads, dtype, kernel):
+    """Scores whose standard deviation is `size` / 3 (most within +-size), and so single keys that decide."""
+    c = _sized(heads, dtype, seed=21)
+    c.qa, c.qr = (c.qa.float() * size / 3).to(dtype), (c.qr.float() * size / 3).to(dtype)
+    check_any_size(c.run(kernel), c.exact(), (size, heads))
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads", [16, 128])
+@pytest.mark.parametrize("offset", [-600.0, -64.0, 64.0, 500.0])
+@pytest.mark.parametrize("column", [0, 40])
+def test_an_offset_common_to_all_keys(column, offset, heads, dtype, kernel):
+    """A large constant in every score (softmax does not see it), from either half of the columns."""
+    c = _sized(heads, dtype, seed=22)
+    c.kv[:, 512 + column] = 8.0
+    c.qr[..., column] = offset / (8.0 * SCALE)
+    check_any_size(c.run(kernel), c.exact(), (column, offset, heads))
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads", [16, 128])
+@pytest.mark.parametrize("size", [30.0, 100.0, 600.0])
+def test_halves_that_cancel(size, heads, dtype, kernel):
+    """Every key has a part of its score of up to +-size in one half of the columns and its opposite in the
+    other (the products are exact, so nothing of it is left in the sum)."""
+    c = _sized(heads, dtype, seed=23)
+    g = torch.Generator().manual_seed(24)
+    part = torch.randint(-8, 9, (c.kv.shape[0],), generator=g).to(dtype)
+    c.kv[:, 512 + 3], c.kv[:, 512 + 35] = part, part
+    c.qr[..., 3] = size / (8.0 * SCALE)
+    c.qr[..., 35] = -c.qr[..., 3]
+    check_any_size(c.run(kernel), c.exact(), (size, heads))
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("value", ["lowest", "-inf"])
+def test_keys_masked_by_the_lowest_value(value, dtype, kernel):
+    """Keys with the type's lowest value or -inf in a column where every query has 1: their weight is zero, the
+    others' as without them; and where all keys have the lowest value, none is preferred for it."""
+    c = _sized(16, dtype, seed=25)
+    c.qr[..., 7] = 1.0
+    c.kv[:, 512 + 7] = 0.0
+    masked = torch.zeros(c.kv.shape[0], dtype=torch.bool)
+    for r in c.rows_of:
+        masked[r[1::3]] = True
+    low = torch.finfo(dtype).min if value == "lowest" else -math.inf
+    c.kv[masked, 512 + 7] = low
+    check_any_size(c.run(kernel), c.exact(), value)
+    if value == "lowest" and dtype == torch.bfloat16:
+        c.kv[:, 512 + 7] = low                                   # (all scores are -2.4e37 in 64 bits too)
+        check_any_size(c.run(kernel), c.exact(), "all masked")
