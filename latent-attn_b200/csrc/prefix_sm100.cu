@@ -8,7 +8,7 @@
 //      (m, l, o) per group that it touches, at index group + worker (unique: walking the tiles in
 //      order, every step to the next (group, worker) piece advances one of the two).
 //   3. prefix_merge_kernel merges each output row's records by their maxima and sums, once the row's own
-//      workers have written them (they all run when it starts, so that its bounded wait ends).
+//      workers have written them.
 // Rounding: P is rounded to the cache's type for its MMA, and the row sums add the rounded values, so
 // that the weights of a row still add up to one; a record's o is stored in fp16 after an exact scaling
 // of each 64 columns by a power of two (2^-11 relative to their largest, at half of fp32's bytes); all sums, maxima and accumulators are fp32; the result is rounded once.
@@ -1031,21 +1031,25 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
 
 constexpr int kMergeWarps = 8;
 
-// Waits until the workers w0 .. w1 have written their records; false when one of them does not (warp-wide).
-// They all run: the kernel is let in by the last of them to start.
-__device__ __forceinline__ bool await_workers(const int* done, int w0, int w1, int lane) {
+constexpr uint64_t kPollNs = 1000000;   // 1 ms
+
+// Waits until the workers w0 .. w1 have written their records (warp-wide). They all run when this kernel does,
+// but how long they take goes by the lengths: after kPollNs it is the end of their kernel that is awaited.
+__device__ __forceinline__ void await_workers(const int* done, int w0, int w1, int lane) {
     const uint64_t t0 = globaltimer_ns();
     for (int w = w0 + lane; __any_sync(0xffffffffu, w <= w1); w += 32) {
         for (;;) {
             int n = 2;
             if (w <= w1) asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(n) : "l"(done + w) : "memory");
             if (__all_sync(0xffffffffu, n >= 2)) break;
-            if (__any_sync(0xffffffffu, globaltimer_ns() - t0 > kDefaultWaitNs)) return false;
+            if (__any_sync(0xffffffffu, globaltimer_ns() - t0 > kPollNs)) {
+                pdl_wait();
+                return;
+            }
             __nanosleep(64);
         }
     }
     __syncwarp();
-    return true;
 }
 
 // One output row per `kWarps` warps: each takes every kWarps-th record of the row's groups, keeping
@@ -1077,7 +1081,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) prefix_merge_kernel(const __
         for (int k = 0; k < 2; ++k) {
             if (piece[k].g < 0) continue;
             const int g = piece[k].g, w1 = piece[k].w1, r = k == 0 ? h % 128 : (f - rq.y) % 128;
-            bad = !await_workers(wk.done, piece[k].w0, w1, lane) || bad;
+            await_workers(wk.done, piece[k].w0, w1, lane);
             bad = bad || *static_cast<volatile int*>(wk.status) != 0 || __ldcg(wk.bad + g) != 0;
             constexpr int kAhead = 4;
             for (int w = piece[k].w0 + sub; w <= w1; w += kWarps * kAhead) {

@@ -428,3 +428,21 @@ def test_keys_masked_by_the_lowest_value(value, dtype, kernel):
     if value == "lowest" and dtype == torch.bfloat16:
         c.kv[:, 512 + 7] = low                                   # (all scores are -2.4e37 in 64 bits too)
         check_any_size(c.run(kernel), c.exact(), "all masked")
+
+
+def test_a_call_of_seconds():
+    """256 requests of one head over 35 million rows each (one page, over and over): 140 million tiles, some
+    2.5 seconds. All scores are 0 and all rows are equal, so the output is the row, to the bit: the sums of
+    powers of two are exact, and 2^-11 of a record is lost in the result's rounding to 8 bits."""
+    B, page, n = 256, 65536, 35_000_000
+    row = (2.0 ** torch.arange(512).remainder(7).sub(3) * (1 - 2 * torch.arange(512).remainder(2))).to(torch.bfloat16)
+    kv = torch.zeros(page, 576, dtype=torch.bfloat16, device=DEV)
+    kv[:, :512] = row.to(DEV)
+    zeros = torch.zeros(B, 1, 576, dtype=torch.bfloat16, device=DEV)
+    out = mla_prefix_decode(kv, zeros[..., :512].contiguous(), zeros[..., 512:].contiguous(), MLAConfig(0, 512, 128, 64, 1, 128),
+                            group_starts=torch.tensor([0, B], dtype=torch.int32, device=DEV),
+                            prefix_lens=torch.zeros(1, dtype=torch.int32, device=DEV), max_prefix_len=0,
+                            seq_lens=torch.full((B,), n, dtype=torch.int32, device=DEV), max_seq_len=n, page_rows=page,
+                            prefix_table=torch.zeros(1, 1, dtype=torch.int32, device=DEV),
+                            page_table=torch.zeros(B, -(-n // page), dtype=torch.int32, device=DEV), kernel=TC)
+    assert torch.equal(out, row.to(DEV).expand(B, 1, 512))
