@@ -1253,12 +1253,20 @@ cudaError_t launch(const PrefixArgs& A, unsigned char* ws, int sms, cudaStream_t
 
 }  // namespace
 
+// The most tiles and fixed costs of groups that the plan may count for these bounds of the lengths.
+static long long most_tiles(const PrefixArgs& A) {
+    const long long ptiles = (static_cast<long long>(A.max_plen) + kTile - 1) / kTile,
+                    otiles = (static_cast<long long>(A.max_len) + kTile - 1) / kTile;
+    const long long own = static_cast<long long>(A.B) * ceil_div(A.H, 128),
+                    shared = A.H % 128 == 0 ? own : static_cast<long long>(A.B) * A.H / 128 + (A.P < A.B ? A.P : A.B);
+    return own * (otiles + kGroupCost) + shared * (ptiles + kGroupCost);
+}
+
 bool prefix_sm100_supported(const PrefixArgs& A) {
     auto is16 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
     return A.dc == 512 && A.dR == 64 && A.stride % 8 == 0 && A.stride <= (1 << 30) && is16(A.kv) && is16(A.qa) &&
            is16(A.qr) && is16(A.out) && A.kv_rows < (1ll << 31) - 4 * kTile &&
-           // tiles are counted in 32 bits
-           static_cast<double>(A.B) * A.H / 64.0 * (static_cast<double>(A.max_plen) + A.max_len + 128) < 1e9;
+           most_tiles(A) < 0x7ff00000ll;   // counted in 32 bits, with the groups' fixed costs
 }
 
 size_t prefix_sm100_workspace(const PrefixArgs& A, int sms) { return layout(A, sms).total; }

@@ -446,3 +446,20 @@ def test_a_call_of_seconds():
                             prefix_table=torch.zeros(1, 1, dtype=torch.int32, device=DEV),
                             page_table=torch.zeros(B, -(-n // page), dtype=torch.int32, device=DEV), kernel=TC)
     assert torch.equal(out, row.to(DEV).expand(B, 1, 512))
+
+
+@pytest.mark.parametrize("heads,batch", [(128, 512), (16, 2048)])
+def test_wide_bounds_stay_on_the_tensor_cores(heads, batch):
+    """Bounds of the lengths far above the lengths: the tiles that they allow (8.4 million of 128 rows at 512
+    requests of 128 heads) can be counted, so the tensor-core kernel takes the call and gives the same bits as
+    with bounds that fit."""
+    own = [(5 * b) % 67 for b in range(batch)]
+    c = Case([batch - 3, 3], [100, 33], own, heads, torch.bfloat16, 0, seed=heads)
+    wide = c.run(TC, max_prefix_len=1 << 20, max_seq_len=1 << 18)
+    assert torch.equal(wide, c.run(TC))
+    pick = [0, 1, 13, batch // 2, batch - 4, batch - 1]
+    few = Case([6], [0], [0] * 6, heads, torch.bfloat16, 0)
+    few.kv, few.qa, few.qr = c.kv, c.qa[pick], c.qr[pick]
+    few.sizes = [1] * 6
+    few.rows_of = [c.rows_of[0] if b < batch - 3 else c.rows_of[1] for b in pick] + [c.rows_of[2 + b] for b in pick]
+    check(wide[pick], few.exact(), torch.bfloat16)
