@@ -114,7 +114,7 @@ struct Work {                 // workspace
     int2* request;            // per request: its prefix's first group among `pieces` (or -1) and first row
     int* gbase;               // per prefix group: its first row group (num_groups + 1)
     int* bad;                 // per group with tiles: it met a row outside the cache
-    int* done;                // per worker: its CTAs whose records are written
+    int* done;                // per worker: its CTAs that have begun, and those whose records are written
     float* rec_ml;            // per record row kMl floats: m, l, -, -, and 2^-f of each 64 columns of o
     uint16_t* rec_o;          // o 2^f in fp16
     float2* rowsum;           // per CTA: [kSums][128] row sums and references handed between its sets
@@ -542,12 +542,12 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
 
     if (smem_u32(smem_raw) % 1024 != 0) {   // (all CTAs alike)
         pdl_wait();
-        pdl_launch_dependents();
         if (threadIdx.x == 0) {
             record_timeout(err, code(kAlignment));
             __threadfence();
-            atomicAdd(&wk.done[w], 1);
+            atomicAdd(&wk.done[w], 2);
         }
+        pdl_launch_dependents();
         return;
     }
     if (threadIdx.x == 0) {
@@ -584,7 +584,9 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
     tc_fence_after();
     const uint32_t tbase = bars->tmem;
     pdl_wait();   // the plan
-    // the merge may start: the plan is complete for it too, and every CTA whose records it awaits runs
+    // passed on to the merge, which does not wait for the plan itself
+    if (threadIdx.x == 0) asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(wk.done + w) : "memory");
+    // the merge may start: every CTA whose records it awaits runs
     pdl_launch_dependents();
     // identical in both CTAs of the pair; a pair without tiles goes straight to the teardown
     const Start start = wk.start[w];
@@ -1033,15 +1035,26 @@ constexpr int kMergeWarps = 8;
 
 constexpr uint64_t kPollNs = 1000000;   // 1 ms
 
+__device__ __forceinline__ int load_done(const int* p) {
+    int n;
+    asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(n) : "l"(p) : "memory");
+    return n;
+}
+
+// The plan, which a CTA of any worker has seen, is seen by this warp too. (Both have begun when this kernel
+// runs, so this does not wait; the end of their kernel would say the same.)
+__device__ __forceinline__ void await_plan(const int* done) {
+    if (load_done(done) == 0) pdl_wait();
+}
+
 // Waits until the workers w0 .. w1 have written their records (warp-wide). They all run when this kernel does,
 // but how long they take goes by the lengths: after kPollNs it is the end of their kernel that is awaited.
 __device__ __forceinline__ void await_workers(const int* done, int w0, int w1, int lane) {
     const uint64_t t0 = globaltimer_ns();
     for (int w = w0 + lane; __any_sync(0xffffffffu, w <= w1); w += 32) {
         for (;;) {
-            int n = 2;
-            if (w <= w1) asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(n) : "l"(done + w) : "memory");
-            if (__all_sync(0xffffffffu, n >= 2)) break;
+            const int n = w <= w1 ? load_done(done + w) : 4;
+            if (__all_sync(0xffffffffu, n >= 4)) break;
             if (__any_sync(0xffffffffu, globaltimer_ns() - t0 > kPollNs)) {
                 pdl_wait();
                 return;
@@ -1068,6 +1081,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) prefix_merge_kernel(const __
     float o[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[i] = 0.f;
+    await_plan(wk.done + blockIdx.x % wk.W);
     bool bad = __ldcg(wk.unsorted) != 0;
     if (live && !bad) {
         const int b = f / A.H, h = f % A.H;
