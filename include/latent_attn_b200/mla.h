@@ -462,7 +462,8 @@ MLA_API mla_status_t mla_prefix_decode(const mla_config_t* cfg, const mla_prefix
  * (latent_attn/__init__.py:126, :128, :145), for requests with adapters; no reference counterpart.
  * tcgen05 kernel (CUDA cores for one or two tokens); the same call gives the same bits every time. The
  * workspace holds A_a X[m] per 256 tokens and adapter that may occur there. Products and sums in fp32,
- * A_a X[m] and Y rounded once to the operands' type. */
+ * scales[a] A_a X[m] rounded once to the operands' type (not for one or two tokens, nor where it passes the
+ * type's range: fp32 there), Y once. */
 typedef struct mla_lora_args {
   mla_dtype_t dtype;            /* of X, W, A, B, Y: F16 or BF16 */
   int M, N, K;                  /* tokens >= 1, outputs, inputs (a multiple of 8) */

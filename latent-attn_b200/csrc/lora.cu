@@ -30,8 +30,9 @@
 // that is not finite is computed again from its own operands alone (own_element): a broken adapter
 // stays with its requests, and only then costs more.
 //
-// Rounding: products and sums in fp32; U is rounded to the inputs' type once (it is an MMA operand)
-// and Y once.
+// Rounding: products and sums in fp32; U is rounded to the inputs' type once where it is an MMA operand
+// (fp16: in steps of 2^-24 below 2^-14; where it passes 65504, the outputs that use it are computed again
+// from U in fp32, as the CUDA-core kernel does for its few tokens), and Y once.
 #include "mla_internal.cuh"
 #include "ops.cuh"
 #include "sm100_ptx.cuh"
@@ -81,7 +82,7 @@ struct Plan {
     int width;                        // most columns of a piece
     int stages, stage_bytes;
     int ksplit, clusters, per_blk;    // CTAs of a shrink cluster, clusters in all and per token block
-    size_t off_status, off_count, off_meta, off_perm, off_x, off_u, off_part, total;
+    size_t off_status, off_count, off_meta, off_perm, off_x, off_u, off_u32, off_part, total;
 };
 
 int up(int a, int b) { return (a + b - 1) / b * b; }
@@ -144,6 +145,7 @@ Plan make_plan(int M, int N, int K, int adapters, int rank, int sms) {
     p.off_perm = take(sizeof(int) * kMaxTok);
     p.off_x = take(p.sorted ? static_cast<size_t>(p.tb) * K * 2 : 0);
     p.off_u = take(static_cast<size_t>(p.nb) * p.slots * p.rchunks * p.tb * p.kw * 2);
+    p.off_u32 = take(static_cast<size_t>(p.nb) * p.tb * p.rsteps * kStep * sizeof(float));
     p.off_part = take(p.slices == 0 && p.tail_pairs > rest ? static_cast<size_t>(p.tail_pairs) * 4 * kRows * p.tb * sizeof(float) : 0);
     p.total = off;
     return p;
@@ -157,6 +159,11 @@ __device__ __forceinline__ int2 pack_slot(int id, int slot, int lo, int n) {
 __device__ __forceinline__ int slot_of(int2 s) { return s.y >> 16; }
 __device__ __forceinline__ int slot_lo(int2 s) { return (s.y >> 8 & 255) * kColStep; }
 __device__ __forceinline__ int slot_n(int2 s) { return (s.y & 255) * kColStep; }
+
+// U in fp32, of the token in a block's column.
+__device__ __forceinline__ float* u32_row(const Plan& P, unsigned char* ws, int blk, int col) {
+    return reinterpret_cast<float*>(ws + P.off_u32) + (static_cast<size_t>(blk) * P.tb + col) * P.rsteps * kStep;
+}
 
 template <typename T> struct Fmt;
 template <> struct Fmt<__half> { static constexpr uint32_t v = 0; };
@@ -430,6 +437,7 @@ __global__ void __launch_bounds__(32 * kShrinkWarps, 2) lora_shrink_kernel(const
                         s += y;
                     }
                     u[o.col_of[m] * P.kw + k] = ElemTraits<T>::from_f(s * scale);
+                    u32_row(P, ws, blk, o.col_of[m])[q * kStep + k] = s * scale;
                 }
                 if (sub == 0 && kpart == P.ksplit - 1)
                     for (int i = tid; i < unit_n * 2; i += blockDim.x) {
@@ -536,25 +544,19 @@ __device__ __forceinline__ int load_slots(const Plan& P, const unsigned char* ws
     return kept;
 }
 
-// Output element (column c of the block, token m, weight row n) from the token's own operands: the rare
-// path of outputs that came out infinite or NaN.
+// Output element (column c of the block, token m, weight row n) from the token's own operands, U in fp32: the
+// rare path of outputs that came out infinite or NaN (also because U passed the type's range).
 template <typename T>
-__device__ __noinline__ float own_element(const LoraArgs& A, const Plan& P, const unsigned char* ws, int blk, int c, int m, int n) {
+__device__ __noinline__ float own_element(const LoraArgs& A, const Plan& P, unsigned char* ws, int blk, int c, int m, int n) {
     const T* x = static_cast<const T*>(A.x) + static_cast<long long>(m) * A.x_stride;
     const T* w = static_cast<const T*>(A.w) + static_cast<long long>(n) * P.K;
     float v = 0.f;
     for (int k = 0; k < P.K; ++k) v = fmaf(ElemTraits<T>::to_f(x[k]), ElemTraits<T>::to_f(w[k]), v);
     const int id = A.ids[m];
     if (id < 0 || id >= P.adapters) return v;
-    const int2* meta = reinterpret_cast<const int2*>(ws + P.off_meta) + static_cast<size_t>(blk) * (P.slots + 1);
-    int slot = 0;
-    while (slot < meta[0].x && meta[1 + slot].x != id) ++slot;
-    const T* u = reinterpret_cast<const T*>(ws + P.off_u);
+    const float* u = u32_row(P, ws, blk, c);
     const T* b = static_cast<const T*>(A.b) + (static_cast<long long>(id) * P.N + n) * P.r;
-    for (int k = 0; k < P.r; ++k) {
-        const size_t chunk = (static_cast<size_t>(blk) * P.slots + slot) * P.rchunks + k / P.kw;
-        v = fmaf(ElemTraits<T>::to_f(u[(chunk * P.tb + c) * P.kw + k % P.kw]), ElemTraits<T>::to_f(b[k]), v);
-    }
+    for (int k = 0; k < P.r; ++k) v = fmaf(u[k], ElemTraits<T>::to_f(b[k]), v);
     return v;
 }
 
@@ -957,10 +959,10 @@ __device__ __forceinline__ uint4 load_once(const void* p) {
 // the stream of W: 32 warps an SM keep 64 KB of it in flight (16 warps with four steps each: 20.3 us for
 // one token onto 8192 rows of 5120, 32 with two: 16.8; onto 65536 rows of 7168 139 us, 6.8 TB/s).
 template <typename T, int kM>
-__global__ void __launch_bounds__(32 * kGemvWarps, kGemvBlocks) lora_gemv_kernel(const LoraArgs A, const Plan P, const unsigned char* ws) {
+__global__ void __launch_bounds__(32 * kGemvWarps, kGemvBlocks) lora_gemv_kernel(const LoraArgs A, const Plan P, unsigned char* ws) {
     const int lane = threadIdx.x & 31, warps = gridDim.x * kGemvWarps;
     const T* x = static_cast<const T*>(A.x);
-    const T* u[kM];        // the token's row of U, or none
+    const float* u[kM];    // the token's row of U in fp32, or none
     long long b_row[kM];   // its adapter's first row of B
     bool ready = false;
     for (int pair = blockIdx.x * kGemvWarps + threadIdx.x / 32; pair * 2 < P.N; pair += warps) {
@@ -998,17 +1000,12 @@ __global__ void __launch_bounds__(32 * kGemvWarps, kGemvBlocks) lora_gemv_kernel
         if (!ready) {
             ready = true;
             pdl_wait();
-            const int2* meta = reinterpret_cast<const int2*>(ws + P.off_meta);
 #pragma unroll
             for (int m = 0; m < kM; ++m) {
-                u[m] = nullptr;
-                b_row[m] = 0;
                 const int id = m < P.M ? A.ids[m] : -1;
-                if (id < 0 || id >= P.adapters) continue;
-                int slot = 0;
-                while (slot < meta[0].x && meta[1 + slot].x != id) ++slot;
-                u[m] = reinterpret_cast<const T*>(ws + P.off_u) + (static_cast<size_t>(slot) * P.rchunks * P.tb + m) * P.kw;
-                b_row[m] = static_cast<long long>(id) * P.N;
+                const bool one = id >= 0 && id < P.adapters;
+                u[m] = one ? u32_row(P, ws, 0, m) : nullptr;
+                b_row[m] = one ? static_cast<long long>(id) * P.N : 0;
             }
         }
 #pragma unroll
@@ -1016,8 +1013,16 @@ __global__ void __launch_bounds__(32 * kGemvWarps, kGemvBlocks) lora_gemv_kernel
             if (u[m])
                 for (int k = 8 * lane; k < P.r; k += 256) {
                     const T* b = static_cast<const T*>(A.b);
-                    add(load_once(b + (b_row[m] + n0) * P.r + k), load_once(b + (b_row[m] + n1) * P.r + k),
-                        __ldcg(reinterpret_cast<const uint4*>(u[m] + static_cast<size_t>(k / P.kw) * P.tb * P.kw + k % P.kw)), m);
+                    const float4 u0 = __ldcg(reinterpret_cast<const float4*>(u[m] + k)), u1 = __ldcg(reinterpret_cast<const float4*>(u[m] + k + 4));
+                    const float y[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
+                    float f0[8], f1[8];
+                    to_float8<T>(load_once(b + (b_row[m] + n0) * P.r + k), f0);
+                    to_float8<T>(load_once(b + (b_row[m] + n1) * P.r + k), f1);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        acc[0][m] = fmaf(f0[i], y[i], acc[0][m]);
+                        acc[1][m] = fmaf(f1[i], y[i], acc[1][m]);
+                    }
                 }
 #pragma unroll
         for (int m = 0; m < kM; ++m)
@@ -1081,8 +1086,8 @@ cudaError_t launch(const LoraArgs& A, unsigned char* ws, int sms, cudaStream_t s
         const int blocks = ceil_div(ceil_div(P.N, 2), kGemvWarps);
         cfg.gridDim = dim3(blocks < kGemvBlocks * sms ? blocks : kGemvBlocks * sms);
         cfg.blockDim = dim3(32 * kGemvWarps);
-        e = A.M == 1 ? cudaLaunchKernelEx(&cfg, lora_gemv_kernel<T, 1>, A, P, static_cast<const unsigned char*>(ws))
-                     : cudaLaunchKernelEx(&cfg, lora_gemv_kernel<T, kFewTokens>, A, P, static_cast<const unsigned char*>(ws));
+        e = A.M == 1 ? cudaLaunchKernelEx(&cfg, lora_gemv_kernel<T, 1>, A, P, ws)
+                     : cudaLaunchKernelEx(&cfg, lora_gemv_kernel<T, kFewTokens>, A, P, ws);
         count_launches(2);
         return e != cudaSuccess ? e : cudaGetLastError();
     }

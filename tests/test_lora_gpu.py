@@ -177,3 +177,17 @@ def test_workspaces_that_the_kernels_cannot_write_are_refused():
             linear_lora(x, W, A, B, ids, scales=scales, workspace=ws)
     check(linear_lora(x, W, A, B, ids, scales=scales, workspace=torch.empty(1, dtype=torch.uint8, device=DEV)),
           exact(x, W, A, B, ids, scales))                        # too small: one is allocated
+
+
+@pytest.mark.parametrize("M", [1, 2, 3, 40, 200, 300])
+def test_intermediates_beyond_the_range_of_fp16(M):
+    """A x of up to some 10^6 before a small B: every output is finite, whichever tokens pass 65504."""
+    x, W, A, B, ids, scales = make(M, 300, 512, 24, 5, torch.float16, seed=M)
+    A = A * 512.0
+    x[::3] *= 800.0
+    W, B = W * 2.0 ** -4, B * 2.0 ** -13
+    t = (x.double() @ A[ids.clamp(min=0)[0]].double().T).abs()
+    ids[0] = 1
+    assert float((x[:1].double() @ A[1].double().T).abs().max() * scales[1]) > 65504 and float(t.max()) < 1e8
+    got = linear_lora(x, W, A, B, ids, scales=scales)
+    check(got, exact(x, W, A, B, ids, scales))
