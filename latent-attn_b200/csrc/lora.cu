@@ -603,7 +603,7 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
         // end on completion or on their own limit and do not look at it)
         Walk walk(P);
         Item it;
-        int i = 0, blk_slots = -1, lo_slots = -1, nslots = 0;
+        int i = 0, blk_slots = -1, lo_slots = -1, cols_slots = -1, nslots = 0;
         bool ok = true, waited = !P.sorted;   // X in adapter order comes from the shrink kernel
         bool meta_ready = false;
         int held = 0;                         // stages whose W is on its way while X is waited for
@@ -656,9 +656,11 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
                 pdl_wait();   // U and the adapters' list come from the shrink kernel
                 meta_ready = true;
             }
-            if (blk != blk_slots || it.lo != lo_slots) nslots = load_slots(P, ws, blk, it.lo, it.cols, bars->slots[0], lane);
+            if (blk != blk_slots || it.lo != lo_slots || it.cols != cols_slots)
+                nslots = load_slots(P, ws, blk, it.lo, it.cols, bars->slots[0], lane);
             blk_slots = blk;
             lo_slots = it.lo;
+            cols_slots = it.cols;
             const int chunks = nslots * P.rchunks;
             for (int s0 = 0; s0 < chunks; s0 += per_stage, ++i) {
                 const int s = i % P.stages;
@@ -694,7 +696,7 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
         if (rank == 0) {
             Walk walk(P);
             Item it;
-            int i = 0, n = 0, blk_slots = -1, lo_slots = -1, nslots = 0;
+            int i = 0, n = 0, blk_slots = -1, lo_slots = -1, cols_slots = -1, nslots = 0;
             bool ok = true, meta_ready = false;
             for (; ok && walk.next(P, &it); ++n) {
                 const int blk = it.tile % P.nb;
@@ -733,9 +735,11 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
                         pdl_wait();
                         meta_ready = true;
                     }
-                    if (blk != blk_slots || it.lo != lo_slots) nslots = load_slots(P, ws, blk, it.lo, it.cols, bars->slots[1], lane);
+                    if (blk != blk_slots || it.lo != lo_slots || it.cols != cols_slots)
+                        nslots = load_slots(P, ws, blk, it.lo, it.cols, bars->slots[1], lane);
                     blk_slots = blk;
                     lo_slots = it.lo;
+                    cols_slots = it.cols;
                     const int chunks = nslots * P.rchunks;
                     for (int s0 = 0; s0 < chunks; s0 += per_stage, ++i) {
                         const int s = i % P.stages;

@@ -191,3 +191,14 @@ def test_intermediates_beyond_the_range_of_fp16(M):
     assert float((x[:1].double() @ A[1].double().T).abs().max() * scales[1]) > 65504 and float(t.max()) < 1e8
     got = linear_lora(x, W, A, B, ids, scales=scales)
     check(got, exact(x, W, A, B, ids, scales))
+
+
+@pytest.mark.parametrize("M,N", [(256, 25600), (200, 38000), (600, 15400), (1100, 9000), (2051, 5120)])
+@pytest.mark.parametrize("mix", ["each its own", "runs", "random"])
+def test_whole_rounds_then_slices(mix, M, N):
+    """More tiles than CTA pairs, with one and several token blocks: pairs that go from whole tiles to a slice of
+    a tile's columns, where other adapters have tokens than in the whole."""
+    n = 24
+    ids = None if mix == "random" else [i % n if mix == "each its own" else i // 31 % n for i in range(M)]
+    a = make(M, N, 136, 24, n, torch.bfloat16, seed=M, ids=ids)
+    check(linear_lora(*a[:5], scales=a[5]), exact(*a))
