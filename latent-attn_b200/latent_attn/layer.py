@@ -50,7 +50,12 @@ class SharedPrefixBatch:
     ``prefix_offsets`` (groups) and ``own_offsets`` (B) on, or in pages of ``page_rows`` rows (a multiple
     of 64, of which every prefix length is a multiple) listed by ``prefix_table`` and ``own_table``.
     All are host sequences (tables: lists of lists); the tensors are built once, for as long as the
-    batch keeps its requests. The lengths advance on the device."""
+    batch keeps its requests.
+
+    The lengths advance on the device, in place, so a captured step advances with every replay. A step on
+    a batch with a full request is refused on the host, which counts the steps that it runs itself;
+    a replay drops the token of a full request (its lengths and rows stay, its output means nothing) and
+    sets bit 0 of ``status`` (int32, on the device)."""
 
     def __init__(self, cfg: MLAConfig, device, group_sizes, prefix_lens, own_lens, max_own_len: int, *,
                  prefix_offsets=None, own_offsets=None, prefix_table=None, own_table=None, page_rows: int = 0) -> None:
@@ -76,8 +81,12 @@ class SharedPrefixBatch:
             starts.append(starts[-1] + size)
         self.group_starts, self.prefix_lens, self.first = ints(starts), ints(prefix_lens), ints(first)
         self.own_lens = ints(own_lens)
-        self.positions = ints([f + n for f, n in zip(first, own_lens)])
+        # where each request's next token goes; max_positions, where the append drops it, once it is full
+        self.positions = ints([f + n if n < max_own_len else self.max_positions for f, n in zip(first, own_lens)])
+        self.status = torch.zeros(1, dtype=torch.int32, device=device)
         self._next = torch.empty_like(self.positions)
+        self._limits = ints([f + max_own_len for f in first])
+        self._full = torch.full_like(self.positions, self.max_positions)
         self._room = max_own_len - max(own_lens, default=0)   # steps until the longest request is full
         self.cu_tokens = ints(range(B + 1))
         self.prefix_offsets = self.own_offsets = self.row_offsets = None
@@ -97,9 +106,10 @@ class SharedPrefixBatch:
 
     def advance(self) -> None:
         """The appended tokens become part of the lengths."""
-        self._room -= 1
-        self.positions, self._next = self._next, self.positions
-        torch.sub(self.positions, self.first, out=self.own_lens)
+        if not (self.positions.is_cuda and torch.cuda.is_current_stream_capturing()):
+            self._room -= 1
+        torch.sub(self._next, self.first, out=self.own_lens).clamp_(max=self.max_own_len)
+        torch.where(self._next < self._limits, self._next, self._full, out=self.positions)
 
 
 class LatentAttentionLayer(nn.Module):
@@ -219,6 +229,7 @@ class LatentAttentionLayer(nn.Module):
         The tokens' latents ``c`` (B, d_c) and keys ``k_rope`` (B, d_R) are appended to the cache, normalised
         (with ``norm_weight``) and rotated to their positions, and ``batch``'s lengths advance. Each token then
         attends to its group's prefix, which is read once for the whole group, and to its request's own rows.
+        The step can be captured in a CUDA graph (after one that was not: it lays the weights out).
         ``kv_cache`` (rows, d_c + d_R) holds rows as ``mla_cache_append_rope`` writes them.
 
         ``adapters``: per projection ("W_Q_absorbed", "W_Q_rope", "W_O") a tuple of ``lora_a``, ``lora_b`` and
@@ -243,7 +254,7 @@ class LatentAttentionLayer(nn.Module):
         mla_cache_append_rope(kv_cache, c.to(dt), k_rope.to(dt), batch.cu_tokens, batch.positions, batch.max_positions, cfg,
                               norm_weight=norm_weight, norm_eps=norm_eps, kv_offsets=batch.row_offsets,
                               page_table=batch.row_table, page_rows=batch.page_rows, q_rope=q_r, q_out=q_r,
-                              new_lens=batch._next, **tables)
+                              new_lens=batch._next, status=batch.status, **tables)
         batch.advance()
         o = mla_prefix_decode(kv_cache, q_abs, q_r, cfg, group_starts=batch.group_starts, prefix_lens=batch.prefix_lens,
                               max_prefix_len=batch.max_prefix_len, seq_lens=batch.own_lens, max_seq_len=batch.max_own_len,

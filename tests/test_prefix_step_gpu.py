@@ -150,3 +150,64 @@ def test_refusals():
     layer.prefix_decode_step(x, c, k, kv, batch)
     with pytest.raises(RuntimeError, match="max_own_len"):
         layer.prefix_decode_step(x, c, k, kv, batch)
+
+
+@pytest.mark.parametrize("paged", [False, True])
+def test_a_captured_step_advances(paged):
+    """Replays of one captured step write the rows of eager steps to the bit, and give their outputs, until a
+    request is full; then its token is dropped, its lengths and every row stay, and the batch's status says so.
+
+    The outputs pass mla_linear, whose fp32 sums over a split K may differ in their last bits from call to call:
+    by 2^-18 of the largest output at most, and then by a step of bf16 (2^-7 of the value)."""
+    layer, cfg = _layer()
+    dt, B, steps = torch.bfloat16, sum(SIZES), 4
+    own = [0, 5, 64, 1, 63, 1]
+    cap = max(own) + steps
+    g = torch.Generator().manual_seed(31)
+
+    def batch_and_cache():
+        kv = torch.randn(64 * 40, DC + DR, generator=torch.Generator().manual_seed(32)).to(dt).cuda()
+        if paged:
+            order = torch.randperm(40, generator=torch.Generator().manual_seed(33)).tolist()
+            where = dict(prefix_table=[[order.pop() for _ in range(3)] for _ in PREFIX],
+                         own_table=[[order.pop() for _ in range(2)] for _ in range(B)], page_rows=64)
+        else:
+            where = dict(prefix_offsets=[3, 140, 200], own_offsets=[400 + cap * b for b in range(B)])
+        return SharedPrefixBatch(cfg, "cuda", SIZES, PREFIX, own, cap, **where), kv
+
+    data = [[torch.randn(B, n, generator=g).to(dt).cuda() for n in (DM, DC, DR)] for _ in range(steps)]
+    eager, kv = batch_and_cache()
+    want = []
+    for x, c, k in data:
+        y = layer.prefix_decode_step(x, c, k, kv, eager)
+        want.append((y, kv.clone(), eager.own_lens.tolist()))
+    assert int(eager.status) == 0
+    with pytest.raises(RuntimeError, match="max_own_len"):
+        layer.prefix_decode_step(*data[0], kv, eager)
+
+    batch, kv = batch_and_cache()
+    held = [t.clone() for t in data[0]]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer.prefix_decode_step(*held, kv, batch)
+    for i in range(steps):
+        for h, t in zip(held, data[i]):
+            h.copy_(t)
+        graph.replay()
+        y, rows, lens = want[i]
+        assert batch.own_lens.tolist() == lens
+        assert torch.equal(kv, rows), i
+        assert bool(((out - y).abs() <= 2.0 ** -7 * y.abs() + 2.0 ** -18 * y.abs().max()).all()), i
+    assert int(batch.status) == 0
+    # the third request is full: only its rows stay as they are
+    before, full = kv.clone(), batch.own_lens.tolist()
+    graph.replay()
+    graph.replay()
+    assert int(batch.status) & 1
+    assert batch.own_lens.tolist() == [min(n + 2, cap) for n in full]
+    changed = set((kv != before).any(1).nonzero()[:, 0].tolist())
+    expect = set()
+    for b, n in enumerate(full):
+        for i in range(n, min(n + 2, cap)):
+            expect.add(int(batch.own_table[b, i // 64]) * 64 + i % 64 if paged else int(batch.own_offsets[b]) + i)
+    assert changed == expect
