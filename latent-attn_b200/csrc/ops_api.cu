@@ -86,8 +86,13 @@ mla_status_t mla_cache_append_rope(const mla_config_t* cfg, const mla_append_rop
     if (A.stride < dc + dR) return api_fail(MLA_ERR_INVALID_ARGUMENT, "kv_row_stride %lld < d_c + d_R", A.stride);
     if (A.c_stride < 0 || A.k_stride < 0 || A.q_ts < 0 || A.q_hs < 0)
         return api_fail(MLA_ERR_INVALID_ARGUMENT, "strides must be >= 0");
-    // an output row must not overlap the next one
-    if (A.q && (A.qo_hs < dR || (a->tokens > 1 && A.qo_ts < (H - 1) * A.qo_hs + dR)))
+    // output rows must not overlap, whichever of tokens and heads is the outer dimension
+    auto apart = [dR](int64_t outer, int64_t inner, int n_inner) {
+        return (n_inner == 1 || inner >= dR) && outer >= (n_inner - 1) * (n_inner > 1 ? inner : 0) + dR;
+    };
+    const bool one_token = a->tokens <= 1;
+    if (A.q && !(one_token ? H == 1 || A.qo_hs >= dR
+                           : apart(A.qo_ts, A.qo_hs, H) || (H > 1 && apart(A.qo_hs, A.qo_ts, a->tokens))))
         return api_fail(MLA_ERR_INVALID_ARGUMENT, "q_out's rows overlap");
     if (!A.cos) {
         // as mla_decode: the double-precision power rounded once to fp32

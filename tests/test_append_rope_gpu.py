@@ -232,3 +232,29 @@ def test_a_cache_whose_rows_overlap_is_refused():
     one = row.view(-1).as_strided((1, 576), (0, 1))               # a single row has any stride
     mla_cache_append_rope(one, c[:1], k[:1], cu - torch.tensor([0, 1], dtype=torch.int32, device=DEV), lens, 1, cfg)
     assert torch.equal(row[0, :512], c[0])
+
+
+@pytest.mark.parametrize("T,H", [(5, 4), (1, 4), (5, 1), (1, 1)])
+def test_queries_with_heads_outside_tokens(T, H):
+    """Inputs and outputs laid out (H, T, d_R), with and without gaps, give the bits of the contiguous form."""
+    cfg = MLAConfig(0, 512, 128, 64, H, 128)
+    g = torch.Generator().manual_seed(T + H)
+    c, k, q = [torch.randn(*shape, generator=g).to(torch.bfloat16).to(DEV) for shape in ((T, 512), (T, 64), (T, H, 64))]
+    cu, lens = torch.tensor([0, T], dtype=torch.int32, device=DEV), torch.tensor([3], dtype=torch.int32, device=DEV)
+
+    def call(**kw):
+        kv = torch.zeros(64, 576, dtype=torch.bfloat16, device=DEV)
+        return mla_cache_append_rope(kv, c, k, cu, lens, 64, cfg, **kw)
+    want = call(q_rope=q)
+    for gap in (0, 8):
+        wide = torch.full((H, T, 64 + gap), 7.0, dtype=torch.bfloat16, device=DEV)
+        out = wide.permute(1, 0, 2)[..., :64]
+        src = torch.zeros(H, T, 64 + gap, dtype=torch.bfloat16, device=DEV).permute(1, 0, 2)[..., :64]
+        src.copy_(q)
+        assert torch.equal(call(q_rope=src, q_out=out), want) and (wide[..., 64:] == 7).all()
+        assert torch.equal(call(q_rope=src, q_out=src), want)      # in place
+    flat = torch.zeros(T * H * 64 + 64, dtype=torch.bfloat16, device=DEV)
+    for strides in ((64 * H, 63, 1), (63, 64 * T, 1), (64, 64, 1)):
+        if (H > 1 and strides[1] < 64) or (T > 1 and (strides[0] < 64 or (H > 1 and strides[0] == strides[1]))):
+            with pytest.raises(RuntimeError, match="overlap"):
+                call(q_rope=q, q_out=flat.as_strided((T, H, 64), strides))
