@@ -463,3 +463,23 @@ def test_wide_bounds_stay_on_the_tensor_cores(heads, batch):
     few.sizes = [1] * 6
     few.rows_of = [c.rows_of[0] if b < batch - 3 else c.rows_of[1] for b in pick] + [c.rows_of[2 + b] for b in pick]
     check(wide[pick], few.exact(), torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("own", [0, 300])
+@pytest.mark.parametrize("pattern", ["stairs", "zigzag", "single", "down"])
+def test_jumps_between_tiles(pattern, own, dtype):
+    """Every worker has ten tiles or so of one group, and the scores of whole tiles lie 8.25 to 40 log2 units a
+    step apart, up or down, each row with a step of its own (or none): the reference of a row moves past the
+    rescaling threshold between any two of the sets that take the tiles in turn, for some lanes of a warp."""
+    c = Case([8], [50000], [own] * 8, 16, dtype, 64, seed=41)
+    g = torch.Generator().manual_seed(42)
+    for r in c.rows_of:
+        tiles = -(-len(r) // 64)
+        t = torch.arange(tiles)
+        level = {"stairs": t % 11, "zigzag": torch.randint(-6, 7, (tiles,), generator=g),
+                 "single": 6 * (torch.randint(0, 4, (tiles,), generator=g) == 0), "down": 10 - t % 11}[pattern]
+        c.kv[r, 512 + 9] = level.repeat_interleave(64)[:len(r)].to(dtype)
+    step = torch.tensor([0.0, 8.25, -8.25, 10.0, -10.0, 16.0, -16.0, 40.0])[torch.randint(0, 8, (8, 16), generator=g)]
+    c.qr[..., 9] = (step * math.log(2.0) / SCALE).to(dtype)
+    check_any_size(c.run(TC), c.exact(), pattern)
