@@ -28,8 +28,8 @@
 // of products themselves are good to about 2^-23 of it. A row whose partials reach 2^14 (in log2 units; a
 // mask's lowest value, infinities and NaN among them) crosses as floats of 16 significant bits, so that one
 // such partial does not take the others' bits. Both CTAs add the same two values, so their softmax is the
-// same bit for bit. (32 bits: 40 percent more time with the three loading stages that leave room for them,
-// 29 with two exchange slots and P in a place of its own; 16 as fp16: 15 percent less, but then a weight is
+// same bit for bit. (32 bits: 20 percent more time with the three loading stages that leave room for them,
+// 14 with two exchange slots and P in a place of its own; 16 as fp16: 12 percent less, but then a weight is
 // off by 2^-11 of its score.)
 //
 // Warps (128 + 128 kSets threads): warp 0 loads, warp 1 issues the scores' MMAs and warp 2 the value
@@ -40,10 +40,10 @@
 // scores arrive in it, row by row in the layout of an MMA operand, and each thread replaces its row by
 // its row of P, from which the value product reads. The MMA that has read it tells the peer that the
 // slot is free.
-// Bound by that chain and the MMAs: a tile takes 1.35 us (0.78 at the measured tensor rate), a batch 16 us
+// Bound by that chain and the MMAs: a tile takes 1.30 us (0.78 at the measured tensor rate), a batch 16 us
 // beside its tiles (plan 4, first loads 3, last softmax and record 4, merge 3, launches), a group of its
 // own about 3. 64 requests of 128 heads
-// over a prefix of 8192: 185 us, 811 TFLOP/s; 32 of 16 heads over one of 131072: 178 us, 822 TFLOP/s.
+// over a prefix of 8192: 178 us, 843 TFLOP/s; 32 of 16 heads over one of 131072: 171 us, 853 TFLOP/s.
 // A parity wait may only start once the phase before the awaited one is known to be complete (it would
 // pass at once otherwise), so a barrier that a set waits on for its own tiles belongs to that set.
 #include <cfloat>
@@ -773,16 +773,13 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
             if (t == 0) mbar_arrive_expect_tx(x_full, kXBytes + 128);
             tc_fence_after();
             float s[64];
+            {
+                uint32_t sr[64];
+                tmem_ld64_sync(trow + kColS + 64 * (j & 1), sr);
+                tc_fence_before();
+                mbar_arrive(smem_u32(&bars->s_free[j & 1]));
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t sr[32];
-                tmem_ld32_sync(trow + kColS + 64 * (j & 1) + 32 * c, sr);
-                if (c == 2 - 1) {
-                    tc_fence_before();
-                    mbar_arrive(smem_u32(&bars->s_free[j & 1]));
-                }
-#pragma unroll
-                for (int q = 0; q < 32; ++q) s[32 * c + q] = __uint_as_float(sr[q]);
+                for (int q = 0; q < 64; ++q) s[q] = __uint_as_float(sr[q]);
             }
             if (np < kTile) {   // what lies past the end must not set the row's exponent
 #pragma unroll
@@ -864,36 +861,39 @@ prefix_attend_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_cons
             {
                 uint32_t pe;
                 asm volatile("ld.shared.u8 %0, [%1];" : "=r"(pe) : "r"(xexp_u32 + slot * 128 + t));
-                const bool pwide = pe == 255u, some = __any_sync(0xffffffffu, pwide);
+                const bool pwide = pe == 255u;
                 const float inv = __uint_as_float((pe - 21u) << 23), off = -kMagic * inv;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                auto load16 = [&](int c, float* x) {
                     uint32_t w[12];
 #pragma unroll
                     for (int q = 0; q < 3; ++q)
                         asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
                                      : "=r"(w[4 * q]), "=r"(w[4 * q + 1]), "=r"(w[4 * q + 2]), "=r"(w[4 * q + 3])
                                      : "r"(x_row + (3 * c + q) * kXUnit));
-                    float x[16];
 #pragma unroll
                     for (int q = 0; q < 4; ++q) unpack24(w + 3 * q, x + 4 * q);
-                    if (some) {
+                };
+                if (__any_sync(0xffffffffu, pwide)) {
 #pragma unroll
-                        for (int q = 0; q < 16; ++q) x[q] = pwide ? from_wide24(x[q]) : fmaf(x[q], inv, off);
-                    } else {
+                    for (int c = 0; c < 4; ++c) {
+                        float x[16];
+                        load16(c, x);
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) s[16 * c + q] += pwide ? from_wide24(x[q]) : fmaf(x[q], inv, off);
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        float x[16];
+                        load16(c, x);
 #pragma unroll
                         for (int q = 0; q < 8; ++q) {
-                            const float2 v = fma2(make_float2(x[2 * q], x[2 * q + 1]), make_float2(inv, inv), make_float2(off, off));
-                            x[2 * q] = v.x;
-                            x[2 * q + 1] = v.y;
+                            float* y = s + 16 * c + 2 * q;
+                            const float2 v = add2(make_float2(y[0], y[1]), fma2(make_float2(x[2 * q], x[2 * q + 1]),
+                                                                              make_float2(inv, inv), make_float2(off, off)));
+                            y[0] = v.x;
+                            y[1] = v.y;
                         }
-                    }
-#pragma unroll
-                    for (int q = 0; q < 8; ++q) {
-                        float* y = s + 16 * c + 2 * q;
-                        const float2 v = add2(make_float2(y[0], y[1]), make_float2(x[2 * q], x[2 * q + 1]));
-                        y[0] = v.x;
-                        y[1] = v.y;
                     }
                 }
             }
