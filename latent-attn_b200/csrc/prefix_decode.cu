@@ -4,7 +4,8 @@
 // One block attends one query row (b, h) to the concatenation of its group's prefix and the
 // request's own rows. Its warps take positions in turn, each with its own online softmax (running
 // maximum m, sum l and latent sum o, all fp32, rescaled when m moves), merged through shared memory
-// at the end. It reads a prefix once per query row, through L2: it serves the shapes outside the
+// at the end. It reads a prefix once per query row, through L2, and is bound by that and by its shuffles
+// (4 requests of 16 heads over 1000 rows: 474 us; 64 over 8192: 28 ms): it serves the shapes outside the
 // tensor-core kernel's, and checks that kernel.
 #include "mla_internal.cuh"
 #include "ops.cuh"
