@@ -28,7 +28,7 @@
 // results do not depend on who came last. No CTA waits for another pair's.
 //
 // A zero of U times an infinite or NaN value of another request's adapter would be NaN, so an output
-// that is not finite is computed again from its own operands alone (own_element): a broken adapter
+// that is not finite is computed again from its own operands alone (own_columns): a broken adapter
 // stays with its requests, and only then costs more.
 //
 // Rounding: products and sums in fp32; U is rounded to the inputs' type once where it is an MMA operand
@@ -161,6 +161,16 @@ __device__ __forceinline__ int slot_of(int2 s) { return s.y >> 16; }
 __device__ __forceinline__ int slot_lo(int2 s) { return (s.y >> 8 & 255) * kColStep; }
 __device__ __forceinline__ int slot_n(int2 s) { return (s.y & 255) * kColStep; }
 
+template <typename T>
+__device__ __forceinline__ void to_float8(const uint4& v, float (&f)[8]) {
+    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 p = ElemTraits<T>::to_f2(*reinterpret_cast<const typename ElemTraits<T>::T2*>(&x[i]));
+        f[2 * i] = p.x;
+        f[2 * i + 1] = p.y;
+    }
+}
 // U in fp32, of the token in a block's column.
 __device__ __forceinline__ float* u32_row(const Plan& P, unsigned char* ws, int blk, int col) {
     return reinterpret_cast<float*>(ws + P.off_u32) + (static_cast<size_t>(blk) * P.tb + col) * P.rsteps * kStep;
@@ -545,20 +555,83 @@ __device__ __forceinline__ int load_slots(const Plan& P, const unsigned char* ws
     return kept;
 }
 
-// Output element (column c of the block, token m, weight row n) from the token's own operands, U in fp32: the
-// rare path of outputs that came out infinite or NaN (also because U passed the type's range).
+// The infinite and NaN outputs among sixteen columns of a warp's 32 weight rows (lane = row n0 + lane) from the
+// tokens' own operands, U in fp32: the rare path of outputs that another token's adapter broke, or U where it
+// passed the type's range. perm: the columns' tokens where they are sorted. An output that its own adapter makes
+// NaN stays one; for the others W x is computed again, for the warp's rows and the columns at once, on
+// warp-level MMAs. (One NaN adapter of 12 in a batch of 67 tokens: 1.1 ms, element by element 153.) It works on
+// the outputs as they were stored, after all read-outs: called from there, it cost them registers (the same
+// batch without NaN 70 -> 75 us).
 template <typename T>
-__device__ __noinline__ float own_element(const LoraArgs& A, const Plan& P, unsigned char* ws, int blk, int c, int m, int n) {
-    const T* x = static_cast<const T*>(A.x) + static_cast<long long>(m) * A.x_stride;
-    const T* w = static_cast<const T*>(A.w) + static_cast<long long>(n) * P.K;
-    float v = 0.f;
-    for (int k = 0; k < P.K; ++k) v = fmaf(ElemTraits<T>::to_f(x[k]), ElemTraits<T>::to_f(w[k]), v);
-    const int id = A.ids[m];
-    if (id < 0 || id >= P.adapters) return v;
-    const float* u = u32_row(P, ws, blk, c);
-    const T* b = static_cast<const T*>(A.b) + (static_cast<long long>(id) * P.N + n) * P.r;
-    for (int k = 0; k < P.r; ++k) v = fmaf(u[k], ElemTraits<T>::to_f(b[k]), v);
-    return v;
+__device__ __noinline__ void own_columns(const LoraArgs& A, const Plan& P, unsigned char* ws, int blk, int c, int n0, int toks,
+                                         const int* perm) {
+    const int lane = threadIdx.x & 31, n = n0 + lane;
+    auto tok = [&](int k) { return P.sorted ? perm[c + k] : blk * P.tb + c + k; };
+    T* y = static_cast<T*>(A.y) + n;
+    uint32_t need = 0;
+    float w[16];   // the adapters' parts
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        w[k] = 0.f;
+        if (n < P.N && c + k < toks && !isfinite(ElemTraits<T>::to_f(y[static_cast<long long>(tok(k)) * P.N]))) {
+            const int id = A.ids[tok(k)];
+            float v = 0.f;
+            if (id >= 0 && id < P.adapters) {
+                const float* u = u32_row(P, ws, blk, c + k);
+                const uint4* b = reinterpret_cast<const uint4*>(static_cast<const T*>(A.b) + (static_cast<long long>(id) * P.N + n) * P.r);
+                for (int i = 0; i < P.r; i += 8) {
+                    float f[8];
+                    to_float8<T>(b[i / 8], f);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v = fmaf(u[i + e], f[e], v);
+                }
+            }
+            w[k] = v;
+            if (v == v) need |= 1u << k;
+        }
+    }
+    if (!__any_sync(0xffffffffu, need != 0)) return;
+    // W x: a quad's lane t takes columns 8 t .. 8 t + 7 of each 32 of K, for both operands alike
+    const int g = lane / 4, t = lane % 4;
+    const T *wr[4], *xr[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) wr[i] = static_cast<const T*>(A.w) + static_cast<long long>(min(n0 + 8 * i + g, P.N - 1)) * P.K + 8 * t;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) xr[i] = static_cast<const T*>(A.x) + static_cast<long long>(tok(min(8 * i + g, toks - c - 1))) * A.x_stride + 8 * t;
+    float acc[2][2][4] = {};
+    constexpr int kAhead = 4;
+    for (int k0 = 0; k0 < P.K; k0 += 32 * kAhead) {
+        uint4 vw[kAhead][4], vx[kAhead][2];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int k = k0 + 32 * j;
+            const bool in = k + 8 * t < P.K;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) vw[j][i] = in ? __ldg(reinterpret_cast<const uint4*>(wr[i] + k)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) vx[j][i] = in ? __ldg(reinterpret_cast<const uint4*>(xr[i] + k)) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint4 r0 = vw[j][2 * m], r1 = vw[j][2 * m + 1], v = vx[j][i];
+                    mma16816<T>(acc[m][i], r0.x, r1.x, r0.y, r1.y, v.x, v.y);
+                    mma16816<T>(acc[m][i], r0.z, r1.z, r0.w, r1.w, v.z, v.w);
+                }
+    }
+    // row 16 m + 8 h + g', column 8 i + 2 t' + e of the product is at lane 4 g' + t', acc[m][i][2 h + e]
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        const int src = lane % 8 * 4 + k % 8 / 2;
+        float z[4];   // by (m, h)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) z[q] = __shfl_sync(0xffffffffu, acc[q / 2][k / 8][2 * (q % 2) + k % 2], src);
+        const float v = w[k] + (lane & 16 ? (lane & 8 ? z[3] : z[2]) : (lane & 8 ? z[1] : z[0]));
+        if (need >> k & 1) y[static_cast<long long>(tok(k)) * P.N] = ElemTraits<T>::from_f(v);
+    }
 }
 
 template <typename T>
@@ -776,7 +849,13 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
         const uint32_t acc_empty0 = mapa(smem_u32(&bars->acc_empty[0]), 0), acc_empty1 = mapa(smem_u32(&bars->acc_empty[1]), 0);
         Walk walk(P);
         Item it;
-        bool ok = true;
+        bool ok = true, broken = false;   // (a broken output of this thread's)
+        // of the tiles cut along K, at most two: the columns that this CTA stored, in kJoinCols
+        uint32_t joined = 0;
+        auto joined_at = [&](int j) {
+            const long long c0 = static_cast<long long>(P.tiles - P.full) * P.kc * (blockIdx.x / 2) / P.tail_pairs;
+            return c0 / P.kc == j ? 0 : kJoins;
+        };
         pdl_wait();   // the counters are cleared and the columns' order is written by the shrink kernel
         if (P.sorted)
             for (int c = threadIdx.x - 64; c < P.M; c += 128) bars->perm[c] = reinterpret_cast<const int*>(ws + P.off_perm)[c];
@@ -791,7 +870,6 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
             const bool any = reinterpret_cast<const int2*>(ws + P.off_meta)[static_cast<size_t>(blk) * (P.slots + 1)].x > 0;
             // 16 columns from c on of this thread's weight row
             auto store16 = [&](int c, const float* v) {
-                if (col >= P.N) return;
                 int m[16];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -806,18 +884,16 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
 #pragma unroll
                 for (int k = 0; k < 16; ++k) finite = finite && isfinite(v[k]);
                 T* y = static_cast<T*>(A.y) + col;
-                if (c + 16 <= toks && ok && (finite || !any)) {
+                broken = broken || (!finite && any && ok && col < P.N);
+                if (col >= P.N) return;
+                if (c + 16 <= toks && ok) {
 #pragma unroll
                     for (int k = 0; k < 16; ++k) y[static_cast<long long>(m[k]) * P.N] = ElemTraits<T>::from_f(v[k]);
                     return;
                 }
 #pragma unroll
                 for (int k = 0; k < 16; ++k)
-                    if (c + k < toks) {
-                        float e = ok ? v[k] : NAN;
-                        if (!isfinite(e) && ok && any) e = own_element<T>(A, P, ws, blk, c + k, m[k], col);
-                        y[static_cast<long long>(m[k]) * P.N] = ElemTraits<T>::from_f(e);
-                    }
+                    if (c + k < toks) y[static_cast<long long>(m[k]) * P.N] = ElemTraits<T>::from_f(ok ? v[k] : NAN);
             };
             auto release = [&] {
                 tc_fence_before();
@@ -835,6 +911,7 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
                 w1 = static_cast<int>(((static_cast<long long>(it.j) + 1) * P.kc * P.tail_pairs - 1) / total);
             }
             if (w0 == w1) {
+                if (it.j >= 0) joined |= ((1u << kJoins) - 1) << joined_at(it.j);
                 for (int c = 0; c < min(it.cols, toks - it.lo); c += 16) {
                     uint32_t u[16];
                     tmem_ld16_sync(d + c, u);
@@ -843,87 +920,99 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
                     for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(u[k]);
                     store16(it.lo + c, v);
                 }
-                release();
-                continue;
-            }
-            // partials as float4 of 4 columns: column group g of row r at g * kRows + r
-            float4* parts = reinterpret_cast<float4*>(ws + P.off_part);
-            auto part = [&](int w) -> float4* {
-                // a pair touches at most two cut tiles: the first into its place 0, the second into place 1
-                const int first = static_cast<int>(total * w / P.tail_pairs / P.kc);
-                return parts + ((static_cast<size_t>(w) * 2 + (first == it.j ? 0 : 1)) * 2 + rank) * kRows * P.tb / 4 + row;
-            };
-            const int me = blockIdx.x / 2, joins = (toks + kJoinCols - 1) / kJoinCols;
-            float4* mine = part(me);
-            for (int c = 0; c < toks; c += 16) {
-                uint32_t v[16];
-                tmem_ld16_sync(d + c, v);
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    mine[(c / 4 + k) * kRows] = make_float4(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1]),
-                                                            __uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3]));
-            }
-            __threadfence();
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            if (threadIdx.x == 64) {
-                // the columns for which this CTA is the last of the tile's; the pairs begin at different
-                // ones, so that those which end together share the additions
-                int* count = reinterpret_cast<int*>(ws + P.off_count) + (2 * it.j + rank) * kJoins;
-                int seen[kJoins], last = 0;
-                const int at = (me - w0) * joins / (w1 - w0 + 1);
-#pragma unroll
-                for (int b = 0; b < kJoins; ++b)
-                    if (b < joins) seen[b] = atomicAdd(count + (at + b) % joins, 1);
-#pragma unroll
-                for (int b = 0; b < kJoins; ++b)
-                    if (b < joins && seen[b] == w1 - w0) last |= 1 << (at + b) % joins;
-                bars->last = last;
-            }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            const int last = bars->last;
-            if (last) __threadfence();
-            // add the partials in order, this CTA's own from the accumulator; the others' are requested three
-            // pairs at a time, one round trip each
-            for (int c = 0; c < toks; c += kJoinCols) {
-                if (!(last >> c / kJoinCols & 1)) continue;
-                uint32_t own[32];
-                tmem_ld32_sync(d + c, own);
-                float v[32] = {};
-                bool mine_in = false;
-                auto add_own = [&] {
-                    mine_in = true;
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) v[k] += __uint_as_float(own[k]);
+            } else {
+                // partials as float4 of 4 columns: column group g of row r at g * kRows + r
+                float4* parts = reinterpret_cast<float4*>(ws + P.off_part);
+                auto part = [&](int w) -> float4* {
+                    // a pair touches at most two cut tiles: the first into its place 0, the second into place 1
+                    const int first = static_cast<int>(total * w / P.tail_pairs / P.kc);
+                    return parts + ((static_cast<size_t>(w) * 2 + (first == it.j ? 0 : 1)) * 2 + rank) * kRows * P.tb / 4 + row;
                 };
-                for (int o = 0; o < w1 - w0; o += 3) {
-                    float4 y[3][8];
+                const int me = blockIdx.x / 2, joins = (toks + kJoinCols - 1) / kJoinCols;
+                float4* mine = part(me);
+                for (int c = 0; c < toks; c += 16) {
+                    uint32_t v[16];
+                    tmem_ld16_sync(d + c, v);
 #pragma unroll
-                    for (int i = 0; i < 3; ++i)
-                        if (o + i < w1 - w0) {
-                            const int wa = w0 + o + i + (w0 + o + i >= me);
-                            const float4* src = part(wa) + c / 4 * kRows;
-#pragma unroll
-                            for (int k = 0; k < 8; ++k)
-                                if (k < 4 || c + 16 < toks) y[i][k] = __ldcg(src + k * kRows);
-                        }
-#pragma unroll
-                    for (int i = 0; i < 3; ++i)
-                        if (o + i < w1 - w0) {
-                            if (!mine_in && w0 + o + i >= me) add_own();
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) {
-                                v[4 * k] += y[i][k].x;
-                                v[4 * k + 1] += y[i][k].y;
-                                v[4 * k + 2] += y[i][k].z;
-                                v[4 * k + 3] += y[i][k].w;
-                            }
-                        }
+                    for (int k = 0; k < 4; ++k)
+                        mine[(c / 4 + k) * kRows] = make_float4(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1]),
+                                                                __uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3]));
                 }
-                if (!mine_in) add_own();
-                store16(c, v);
-                if (c + 16 < toks) store16(c + 16, v + 16);
+                __threadfence();
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                if (threadIdx.x == 64) {
+                    // the columns for which this CTA is the last of the tile's; the pairs begin at different
+                    // ones, so that those which end together share the additions
+                    int* count = reinterpret_cast<int*>(ws + P.off_count) + (2 * it.j + rank) * kJoins;
+                    int seen[kJoins], last = 0;
+                    const int at = (me - w0) * joins / (w1 - w0 + 1);
+#pragma unroll
+                    for (int b = 0; b < kJoins; ++b)
+                        if (b < joins) seen[b] = atomicAdd(count + (at + b) % joins, 1);
+#pragma unroll
+                    for (int b = 0; b < kJoins; ++b)
+                        if (b < joins && seen[b] == w1 - w0) last |= 1 << (at + b) % joins;
+                    bars->last = last;
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                const int last = bars->last;
+                joined |= last << joined_at(it.j);
+                if (last) __threadfence();
+                // add the partials in order, this CTA's own from the accumulator; the others' are requested three
+                // pairs at a time, one round trip each
+                for (int c = 0; c < toks; c += kJoinCols) {
+                    if (!(last >> c / kJoinCols & 1)) continue;
+                    uint32_t own[32];
+                    tmem_ld32_sync(d + c, own);
+                    float v[32] = {};
+                    bool mine_in = false;
+                    auto add_own = [&] {
+                        mine_in = true;
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) v[k] += __uint_as_float(own[k]);
+                    };
+                    for (int o = 0; o < w1 - w0; o += 3) {
+                        float4 y[3][8];
+#pragma unroll
+                        for (int i = 0; i < 3; ++i)
+                            if (o + i < w1 - w0) {
+                                const int wa = w0 + o + i + (w0 + o + i >= me);
+                                const float4* src = part(wa) + c / 4 * kRows;
+#pragma unroll
+                                for (int k = 0; k < 8; ++k)
+                                    if (k < 4 || c + 16 < toks) y[i][k] = __ldcg(src + k * kRows);
+                            }
+#pragma unroll
+                        for (int i = 0; i < 3; ++i)
+                            if (o + i < w1 - w0) {
+                                if (!mine_in && w0 + o + i >= me) add_own();
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) {
+                                    v[4 * k] += y[i][k].x;
+                                    v[4 * k + 1] += y[i][k].y;
+                                    v[4 * k + 2] += y[i][k].z;
+                                    v[4 * k + 3] += y[i][k].w;
+                                }
+                            }
+                    }
+                    if (!mine_in) add_own();
+                    store16(c, v);
+                    if (c + 16 < toks) store16(c + 16, v + 16);
+                }
             }
             release();
+        }
+        if (__any_sync(0xffffffffu, broken)) {
+            // once more over what this CTA stored, for the outputs that are to be computed again
+            Walk again(P);
+            while (again.next(P, &it)) {
+                const int blk = it.tile % P.nb, toks = min(P.tb, P.M - blk * P.tb);
+                const uint32_t mine = it.j >= 0 ? joined >> joined_at(it.j) : ~0u;
+                if (reinterpret_cast<const int2*>(ws + P.off_meta)[static_cast<size_t>(blk) * (P.slots + 1)].x == 0) continue;
+                for (int c = it.lo; c < min(it.lo + it.cols, toks); c += 16)
+                    if (mine >> c / kJoinCols & 1)
+                        own_columns<T>(A, P, ws, blk, c, it.tile / P.nb * 2 * kRows + static_cast<int>(rank) * kRows + 32 * (warp & 3), toks, bars->perm);
+            }
         }
     }
     // ---- teardown
@@ -942,16 +1031,6 @@ lora_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan
 
 // ------------------------------------------------------------------------------------- a few tokens
 
-template <typename T>
-__device__ __forceinline__ void to_float8(const uint4& v, float (&f)[8]) {
-    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 p = ElemTraits<T>::to_f2(*reinterpret_cast<const typename ElemTraits<T>::T2*>(&x[i]));
-        f[2 * i] = p.x;
-        f[2 * i + 1] = p.y;
-    }
-}
 // 16 bytes that are used once (X, which every row of W meets, keeps its place in L1)
 __device__ __forceinline__ uint4 load_once(const void* p) {
     uint4 v;
