@@ -16,9 +16,9 @@
 // Small batches are bound by W's bytes (each read once for all tokens), prompts by the tensor pipe and
 // by what L2 delivers to the SMs (without multicast a pair needs 62 KB for 0.5 us of MMAs). Without
 // adapters the GEMM takes 212 us for 256 tokens onto 65536 rows of 7168 (1.14 PFLOP/s) and 266 us for
-// 2051 tokens onto 5120 rows of 16384; with 32 adapters of rank 64 and 4 of rank 32 it is 272 and 301 us,
+// 2051 tokens onto 5120 rows of 16384; with 32 adapters of rank 64 and 4 of rank 32 it is 267 and 298 us,
 // of which 23 and 49 us are the shrink kernel's (replayed graphs; in a stream of calls, at the clocks that
-// it settles at, 316 and 357).
+// it settles at, 313 and 351).
 //
 // Work split: whole tiles go round robin over the pairs, and the tiles that do not fill a last round are
 // cut. Blocks of 128 tokens and more are cut by columns (no sums to join: 256
