@@ -35,7 +35,7 @@
 // Warps (128 + 128 kSets threads): warp 0 loads, warp 1 issues the scores' MMAs and warp 2 the value
 // products' (two warps that sleep on their own barriers: one that polls both sees either 0.4 us later),
 // warp 3 rests; softmax set i takes the tiles j with j % kSets == i, thread = query row. A tile's way
-// through the softmax (read S, exchange, maximum, exponentials, write P) is about 3 us of latency with
+// through the softmax (read S, exchange, maximum, exponentials, write P) is about 3.5 us of latency with
 // little issue time, so kSets tiles are under way at once, each in a slot of its own: the peer's partial
 // scores arrive in it, row by row in the layout of an MMA operand, and each thread replaces its row by
 // its row of P, from which the value product reads. The MMA that has read it tells the peer that the
@@ -74,7 +74,7 @@ constexpr int kSets = 3;
 constexpr int kSlots = 3;                            // exchange and P slots, tile j in slot j % kSlots
 constexpr int kSums = 2 * kSlots;                    // row sums handed between the sets, tile j's in j % kSums
 constexpr int kGroupCost = 4;                        // a group's fixed cost, in tiles, for the split (a batch of
-                                                     // questions about a document of 131072: 2: 185 us, 4: 155, 6: 162)
+                                                     // questions about a document of 131072: 2: 178 us, 4: 171, 6: 176)
 constexpr int kThreads = 128 + 128 * kSets;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColO = 0, kColS = 256, kColQ = 384;
